@@ -70,6 +70,18 @@ SIGNATURES = {
                                _I, _I, _P, _I, _P, _SZ, _P]),
     "fl_attention_prefill_q8": (_I, [_P, _I, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _F, _I, _P,
                                      _I, _P]),
+    "fl_paged_kv_store": (_I, [_P, _P, _LL, _LL, _P, _P, _I, _I, _I, _P, _I, _LL, _P, _P, _I, _I, _I,
+                               _I, _P]),
+    "fl_paged_kv_load": (_I, [_P, _P, _I, _I, _I, _P, _I, _LL, _P, _P, _P, _P, _LL, _LL, _I, _I, _I,
+                              _I, _I, _P]),
+    "fl_attn_prep_paged": (_I, [_P, _I, _P, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _P, _I, _LL, _P,
+                                _P, _I, _I, _I, _I, _I, _I, _F, _F, _P]),
+    "fl_attention_prefill_paged_work_bytes": (_SZ, [_IP, _IP, _I, _I, _I, _I, _I, _I, _I]),
+    "fl_attention_prefill_paged": (_I, [_P, _I, _P, _P, _I, _I, _I, _P, _I, _LL, _IP, _IP, _I, _I, _I,
+                                        _I, _F, _I, _I, _I, _P, _I, _P, _SZ, _P]),
+    "fl_attn_decode_paged_work_bytes": (_SZ, [_I, _I, _I, _I, _I]),
+    "fl_attn_decode_paged": (_I, [_P, _I, _P, _P, _I, _I, _I, _P, _I, _LL, _P, _I, _I, _I, _I, _I, _F,
+                                  _I, _I, _I, _P, _I, _P, _SZ, _P]),
     "fl_conv1d_causal": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
     "fl_conv1d_causal_rows": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P]),
     "fl_l2norm_scaled": (_I, [_P, _P, _I, _I, _I, _F, _F, _I, _P]),

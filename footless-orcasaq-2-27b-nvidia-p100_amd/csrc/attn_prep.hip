@@ -29,9 +29,11 @@
 // by the in-lane pairs (c, c + 2) and (0, 1) -- the same additions in the same
 // order. The 8 warp sums are then combined as block_reduce_sum's second stage.
 #include "fl_common.hpp"
+#include "kv_pages.hpp"
 
 #include <cmath>
 #include <mutex>
+#include <type_traits>
 
 // Products and sums round separately (no fma contraction), as the oracle's
 // restatement does, so the two agree bit for bit.
@@ -59,26 +61,50 @@ struct PrepRows {
     int max_pos[FL_MAX_SEQS];
 };
 
+// The tokens of packed sequences (attn_prep_paged): token i of sequence b at
+// position pos0[b] + i - starts[b], its rows to that position's page (none where
+// the page is absent), q to rows qo_pitch apart; k is left as it was.
+struct PrepPaged {
+    fl::Pages pages;
+    const int* starts;
+    const int* pos0;
+    int B, qo_pitch;
+};
+
 // flags: bit 0 norm, bit 1 rope, bit 2 KV store (k rows and their v rows),
 // bit 3 the store in the int8 format (caches of capacity max_pos); RPW rows a
 // wavefront. ROWS: token t is row t of a batched decode step, its position,
-// cache and capacity from `rows` (pos0, kc, vc and max_pos unused).
-template <int FLAGS, int RPW, bool ROWS = false>
+// cache and capacity from `rows` (pos0, kc, vc and max_pos unused). PAGED: as
+// PrepPaged says, kc and vc the pools of capacity max_pos.
+template <int FLAGS, int RPW, bool ROWS = false, bool PAGED = false>
 __global__ void __launch_bounds__(64 * PR_WAVES)
 attn_prep_kernel(const f16* q, f16* qo, int q_pitch, f16* k, int k_pitch,
                  const f16* __restrict__ v, const float* __restrict__ wq,
                  const float* __restrict__ wk, void* __restrict__ kc_, void* __restrict__ vc_,
                  int n_q_heads, int n_kv_heads, int pos0, int max_pos_, int rope_dim,
-                 const RopeFreqs freqs, float eps, const PrepRows rows) {
+                 const RopeFreqs freqs, float eps,
+                 const typename std::conditional<PAGED, PrepPaged, PrepRows>::type rows) {
     __shared__ float scs[PR_MAXPAIRS], ssn[PR_MAXPAIRS];
     __shared__ __attribute__((aligned(16))) f16 srow[PR_WAVES][PR_HD];
     constexpr bool NORM = FLAGS & 1, ROPE = FLAGS & 2, STORE = FLAGS & 4, Q8 = FLAGS & 8;
     const int t = blockIdx.x, hd0 = blockIdx.y * PR_WAVES * RPW;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int pos = ROWS ? rows.pos[t] : pos0 + t;
-    void* const kc = ROWS ? rows.kc[t] : kc_;
-    void* const vc = ROWS ? rows.vc[t] : vc_;
-    const int max_pos = ROWS ? rows.max_pos[t] : max_pos_;
+    int pos = pos0 + t, max_pos = max_pos_;
+    void *kc = kc_, *vc = vc_;
+    long long cache_row = pos;   // < 0: not stored
+    if constexpr (ROWS) {
+        pos = rows.pos[t], max_pos = rows.max_pos[t];
+        kc = rows.kc[t], vc = rows.vc[t];
+        cache_row = pos;
+    }
+    if constexpr (PAGED) {
+        const int seq = fl::seq_of(rows.starts, rows.B, t);
+        if (seq >= rows.B || t < rows.starts[seq]) return;   // outside every sequence (the workgroup)
+        const long long at = (long long)rows.pos0[seq] + (t - rows.starts[seq]);
+        if (at < 0 || at > INT_MAX) return;
+        pos = (int)at;
+        cache_row = fl::page_row(rows.pages, seq, pos);
+    }
     const int half_r = rope_dim >> 1;
     if (ROPE) {
         for (int j = threadIdx.x; j < half_r; j += 64 * PR_WAVES) {
@@ -110,6 +136,8 @@ attn_prep_kernel(const f16* q, f16* qo, int q_pitch, f16* k, int k_pitch,
         const size_t roff = is_q ? ((size_t)t * n_q_heads + h) * q_pitch
                                  : ((size_t)t * n_kv_heads + h) * k_pitch;
         f16* orow = is_q ? qo + roff : k + roff;   // q rows may go elsewhere; k in place
+        if constexpr (PAGED)
+            if (is_q) orow = qo + ((size_t)t * n_q_heads + h) * rows.qo_pitch;
         f16x4 y = yin[r];
         if (NORM) {
             float x[4], sq[4];
@@ -156,10 +184,10 @@ attn_prep_kernel(const f16* q, f16* qo, int q_pitch, f16* k, int k_pitch,
             // the slice is rewritten by the wave's next row only after every
             // lane has read it back (in-order LDS within the wave)
         }
-        if (NORM || ROPE) *(f16x4*)(orow + 4 * lane) = y;
-        if (STORE && !is_q) {
+        if ((NORM || ROPE) && (is_q || !PAGED)) *(f16x4*)(orow + 4 * lane) = y;
+        if (STORE && !is_q && (!PAGED || cache_row >= 0)) {
             const f16x4 vin = *(const f16x4*)(v + ((size_t)t * n_kv_heads + h) * PR_HD + 4 * lane);
-            const size_t crow = (size_t)pos * n_kv_heads + h;
+            const size_t crow = (size_t)cache_row * n_kv_heads + h;
             if constexpr (Q8) {
                 const size_t vals = (size_t)max_pos * n_kv_heads * PR_HD;   // scales follow
                 q8_store_row(y, (signed char*)kc + crow * PR_HD,
@@ -330,6 +358,49 @@ int fl_attn_prep_rows(void* qg, int q_pitch, void* k, const void* v, const float
                            head_dim, (const f16*)v, wq, wk, nullptr, nullptr, n_q_heads,
                            n_kv_heads, 0, 0, rope_dim, freqs, eps, rows);
     return fl::check_launch("attn_prep_rows");
+}
+
+int fl_attn_prep_paged(void* qg, int q_pitch, const void* k, const void* v, const float* wq,
+                       const float* wk, void* q_out, int qo_pitch, void* kpool, void* vpool, int q8,
+                       int n_pages, int page_size, const int* pages, int max_pages,
+                       long long pages_stride, const int* starts, const int* pos0, int B, int N,
+                       int n_q_heads, int n_kv_heads, int head_dim, int rope_dim, float theta,
+                       float eps, fl_stream_t stream) {
+    PrepPaged pp = {};
+    int rc = fl::make_pages(kpool, vpool, q8, n_pages, page_size, pages, max_pages, pages_stride, B,
+                            n_kv_heads, head_dim, pp.pages);
+    if (rc) return rc;
+    FL_REQUIRE(N >= 0 && starts && pos0, "null pointer");
+    rc = check_prep(qg, k, v, wq, wk, kpool, vpool, q_pitch, n_q_heads, n_kv_heads, head_dim, 0, 1, 1,
+                    rope_dim, eps);
+    if (rc) return rc;
+    FL_REQUIRE(n_q_heads <= 4096, "n_q_heads <= 4096");
+    FL_REQUIRE(q_out == nullptr || (qo_pitch >= head_dim && qo_pitch % 4 == 0 && al(q_out, 8)),
+               "q_out: pitch >= head_dim, % 4, 8-byte aligned");
+    if (N == 0) return FL_OK;
+    pp.starts = starts;
+    pp.pos0 = pos0;
+    pp.B = B;
+    pp.qo_pitch = q_out ? qo_pitch : q_pitch;
+    f16* qo = (f16*)(q_out ? q_out : qg);
+    RopeFreqs freqs = {};
+    rope_freqs(theta, rope_dim, freqs);
+    const int heads = n_q_heads + n_kv_heads;
+    auto launch = [&](auto kernel, int rows_a_wave) {
+        hipLaunchKernelGGL(kernel,
+                           dim3(N, (heads + rows_a_wave * PR_WAVES - 1) / (rows_a_wave * PR_WAVES)),
+                           dim3(64 * PR_WAVES), 0, (hipStream_t)stream, (const f16*)qg, qo, q_pitch,
+                           (f16*)k, head_dim, (const f16*)v, wq, wk, kpool, vpool, n_q_heads,
+                           n_kv_heads, 0, n_pages << pp.pages.shift, rope_dim, freqs, eps, pp);
+    };
+    if (N < 256) {   // launch_prep's rule
+        if (q8) launch(attn_prep_kernel<15, 1, false, true>, 1);
+        else launch(attn_prep_kernel<7, 1, false, true>, 1);
+    } else {
+        if (q8) launch(attn_prep_kernel<15, 7, false, true>, 7);
+        else launch(attn_prep_kernel<7, 7, false, true>, 7);
+    }
+    return fl::check_launch("attn_prep_paged");
 }
 
 }  // extern "C"

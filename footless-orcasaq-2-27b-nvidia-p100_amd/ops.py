@@ -539,6 +539,251 @@ def attention_prefill_q8(q, kcache, vcache, *, pos0: int, max_pos: int, T: int |
 
 
 # ---------------------------------------------------------------------------
+# The paged KV cache (no reference counterpart: its caches are one buffer a
+# sequence). A layer's K or V pool holds the rows of all sequences in pages of
+# `page_size` positions (a power of two, 16 or more): fp16 [n_pages, page_size,
+# n_kv, 256], or a flat int8 buffer of kv8_nbytes(n_pages * page_size) bytes
+# (paged_pool makes either). pages [B, max_pages] int32 lists each sequence's
+# pages in order; an entry outside [0, n_pages) is an absent page, whose rows are
+# not written, read back as zeros and are not attended to. Packed tokens: sequence
+# b's are starts[b] .. starts[b + 1] - 1, the first at position pos0[b] (int32 [B +
+# 1] and [B] on the GPU: a captured call replays at whatever they hold then).
+# ---------------------------------------------------------------------------
+
+def paged_pool(n_pages: int, page_size: int, *, kv8: bool = False, n_kv_heads: int = N_KV,
+               head_dim: int = HEAD_DIM, device="cuda"):
+    """A zeroed pool of n_pages pages for one layer's K or V rows."""
+    if kv8:
+        return kv8_cache(n_pages * page_size, n_kv_heads, head_dim, device)
+    return torch.zeros((n_pages, page_size, n_kv_heads, head_dim), dtype=F16, device=device)
+
+
+def _paged(kpool, vpool, pages, page_size, B, n_kv_heads, head_dim):
+    """(kpool, vpool, q8, n_pages, page_size, pages, max_pages, pages_stride) of a
+    paged call after checking that the pools and the table are what it says."""
+    for name, c in (("kpool", kpool), ("vpool", vpool), ("pages", pages)):
+        if not isinstance(c, torch.Tensor):
+            raise TypeError(f"{name}: expected a torch.Tensor, got {type(c).__name__}")
+    if page_size < 1 or n_kv_heads < 1 or head_dim != HEAD_DIM:
+        raise ValueError("page_size and n_kv_heads must be positive, head_dim 256")
+    q8 = kpool.dtype == I8
+    if q8:
+        n_pages = kpool.numel() // kv8_nbytes(page_size, n_kv_heads, head_dim)
+        need = kv8_nbytes(n_pages * page_size, n_kv_heads, head_dim)
+        if kpool.numel() != need or vpool.numel() != need:
+            raise ValueError("kpool, vpool: not a whole number of pages, or not the same number")
+    else:
+        n_pages = kpool.shape[0]
+        shape = (n_pages, page_size, n_kv_heads, head_dim)
+        if tuple(kpool.shape) != shape or tuple(vpool.shape) != shape:
+            raise ValueError(f"kpool, vpool: shapes {tuple(kpool.shape)} and {tuple(vpool.shape)}, "
+                             f"expected [n_pages, {page_size}, {n_kv_heads}, {head_dim}]")
+        need = kpool.numel()
+    dtype = I8 if q8 else F16
+    kp, vp = _dense_ptr(kpool, dtype, "kpool", need), _dense_ptr(vpool, dtype, "vpool", need)
+    if pages.dim() != 2 or pages.shape[0] != B or (pages.stride(1) != 1 and pages.shape[1] > 1):
+        raise ValueError(f"pages: expected rows of page ids for {B} sequences")
+    stride = pages.stride(0) if B > 1 else pages.shape[1]
+    return (kp, vp, int(q8), n_pages, page_size,
+            _ptr(pages, torch.int32, "pages", (B - 1) * stride + pages.shape[1]), pages.shape[1],
+            stride)
+
+
+def _one_device(**tensors):
+    """Every tensor on the current device: the launches go on its stream."""
+    here = torch.cuda.current_device() if _device_index is None else _device_index()
+    for name, t in tensors.items():
+        if t is not None and t.is_cuda and t.device.index != here:
+            raise ValueError(f"{name}: on {t.device}, the current device is cuda:{here}")
+
+
+def _packed(starts, pos0):
+    """(starts, pos0, B) of packed tokens."""
+    if not isinstance(starts, torch.Tensor) or not isinstance(pos0, torch.Tensor):
+        raise TypeError("starts, pos0: expected torch tensors")
+    B = pos0.numel()
+    if pos0.dim() != 1 or starts.dim() != 1 or starts.numel() != B + 1:
+        raise ValueError("starts: one entry more than pos0, both one-dimensional")
+    return (_dense_ptr(starts, torch.int32, "starts", B + 1),
+            _dense_ptr(pos0, torch.int32, "pos0", B), B)
+
+
+def _token_rows(t, name, heads, width):
+    """Token stride of a [N, heads, width] tensor whose tokens are dense."""
+    if t.dim() != 3 or tuple(t.shape[1:]) != (heads, width):
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected [N, {heads}, {width}]")
+    if t.shape[0] and not t[0].is_contiguous():
+        raise ValueError(f"{name}: a token's rows must be contiguous")
+    return t.stride(0) if t.shape[0] > 1 else heads * width
+
+
+def paged_kv_store(k, v, kpool, vpool, pages, starts, pos0, *, page_size: int,
+                   n_kv_heads: int = N_KV, head_dim: int = HEAD_DIM):
+    """kv_store / kv_store_q8 into pages: the rows of packed tokens k, v [N, n_kv,
+    head_dim] fp16 (any token stride that is a multiple of 8) to their sequences'
+    positions. Tokens outside every sequence are not stored."""
+    sp, pp, B = _packed(starts, pos0)
+    N = k.shape[0]
+    if v.shape[0] != N:
+        raise ValueError("k and v: not the same number of tokens")
+    ks, vs = (_token_rows(t, n, n_kv_heads, head_dim) for t, n in ((k, "k"), (v, "v")))
+    row = n_kv_heads * head_dim
+    pg = _paged(kpool, vpool, pages, page_size, B, n_kv_heads, head_dim)
+    _one_device(k=k, v=v, kpool=kpool, vpool=vpool, pages=pages, starts=starts, pos0=pos0)
+    if N == 0:
+        return
+    _lib.call("fl_paged_kv_store", _ptr(k, F16, "k", (N - 1) * ks + row),
+              _ptr(v, F16, "v", (N - 1) * vs + row), ks, vs, *pg, sp, pp, B, N, n_kv_heads, head_dim,
+              _stream())
+
+
+def paged_kv_load(kpool, vpool, pages, starts, pos0, *, T: int, page_size: int, k=None, v=None,
+                  n_kv_heads: int = N_KV, head_dim: int = HEAD_DIM):
+    """Cached rows back from their pages: k, v [T, n_kv, head_dim] fp16 (new unless
+    given), int8 rows as fp16(byte * scale), rows of absent pages as zeros. Rows
+    outside every sequence are left as they are (zeros in new tensors)."""
+    sp, pp, B = _packed(starts, pos0)
+    if T < 0 or (k is None) != (v is None):
+        raise ValueError("T >= 0, k and v given both or neither")
+    pg = _paged(kpool, vpool, pages, page_size, B, n_kv_heads, head_dim)
+    new = k is None
+    if new:
+        k, v = (torch.empty((T, n_kv_heads, head_dim), dtype=F16, device=kpool.device)
+                for _ in range(2))
+    if k.shape[0] != T or v.shape[0] != T:
+        raise ValueError(f"k and v: expected {T} tokens")
+    ks, vs = (_token_rows(t, n, n_kv_heads, head_dim) for t, n in ((k, "k"), (v, "v")))
+    _one_device(k=k, v=v, kpool=kpool, vpool=vpool, pages=pages, starts=starts, pos0=pos0)
+    if T > 0:
+        row = n_kv_heads * head_dim
+        _lib.call("fl_paged_kv_load", *pg, sp, pp, _ptr(k, F16, "k", (T - 1) * ks + row),
+                  _ptr(v, F16, "v", (T - 1) * vs + row), ks, vs, int(new), B, T, n_kv_heads,
+                  head_dim, _stream())
+    return k, v
+
+
+def attn_prep_paged(qg, k, v, wq, wk, kpool, vpool, pages, starts, pos0, *, page_size: int,
+                    q_out=None, n_q_heads: int = N_HEADS, n_kv_heads: int = N_KV,
+                    head_dim: int = HEAD_DIM, rope_dim: int = ROPE_DIM, theta: float = ROPE_THETA,
+                    eps: float = NORM_EPS):
+    """attn_prep / attn_prep_q8 (runtime.py:2797-2815) of packed tokens, each at its
+    own sequence's position, into pages: rmsnorm1p and rope_partial of q (first in
+    the rows of qg [N, n_q_heads, q_pitch]) and k, and the store of the roped k
+    and v [N, n_kv, head_dim] -- those calls' values bit for bit. q is rewritten in
+    place, or goes to q_out [N, n_q_heads, pitch]; k is not rewritten. Returns
+    the tensor that holds q."""
+    sp, pp, B = _packed(starts, pos0)
+    N, heads, q_pitch = qg.shape
+    if heads != n_q_heads or tuple(k.shape) != (N, n_kv_heads, head_dim) or k.shape != v.shape:
+        raise ValueError("qg [N, n_q_heads, q_pitch], k and v [N, n_kv_heads, head_dim]")
+    for name, t in (("qg", qg), ("k", k), ("v", v)):
+        _contig(t, name)
+    qo, qo_pitch = None, 0
+    if q_out is not None:
+        _contig(q_out, "q_out")
+        if q_out.dim() != 3 or tuple(q_out.shape[:2]) != (N, n_q_heads):
+            raise ValueError(f"q_out: expected [{N}, {n_q_heads}, pitch]")
+        qo_pitch = q_out.shape[-1]
+    pg = _paged(kpool, vpool, pages, page_size, B, n_kv_heads, head_dim)
+    _one_device(qg=qg, k=k, v=v, wq=wq, wk=wk, q_out=q_out, kpool=kpool, vpool=vpool, pages=pages,
+                starts=starts, pos0=pos0)
+    if N > 0:
+        row = n_kv_heads * head_dim
+        if q_out is not None:
+            qo = _ptr(q_out, F16, "q_out", N * n_q_heads * qo_pitch)
+        _lib.call("fl_attn_prep_paged", _ptr(qg, F16, "qg", N * n_q_heads * q_pitch), q_pitch,
+                  _ptr(k, F16, "k", N * row), _ptr(v, F16, "v", N * row),
+                  _ptr(wq, F32, "wq", head_dim), _ptr(wk, F32, "wk", head_dim), qo, qo_pitch, *pg, sp,
+                  pp, B, N, n_q_heads, n_kv_heads, head_dim, rope_dim, float(theta), float(eps),
+                  _stream())
+    return qg if q_out is None else q_out
+
+
+def attention_prefill_paged_work_bytes(Ts, pos0s, n_q_heads: int = N_HEADS, n_kv_heads: int = N_KV,
+                                       head_dim: int = HEAD_DIM, window: int = 0, sinks: int = 0,
+                                       kv8: bool = False) -> int:
+    return int(_lib.lib().fl_attention_prefill_paged_work_bytes(
+        _lib.int_array(Ts), _lib.int_array(pos0s), len(Ts), n_q_heads, n_kv_heads, head_dim, window,
+        sinks, int(kv8)))
+
+
+def attention_prefill_paged(q, kpool, vpool, pages, Ts, pos0s, *, page_size: int, window: int = 0,
+                            sinks: int = 0, gated: bool = False, z=None, work=None,
+                            n_kv_heads: int = N_KV, scale: float = ATTN_SCALE):
+    """Causal attention of chunks of new tokens over pages: q [N, n_q_heads,
+    q_pitch] fp16 packs Ts[b] queries of each sequence behind each other, the
+    first at position pos0s[b] (host ints; up to 64 sequences), whose own rows are
+    in the pools already. A query at position p sees the rows r <= p with r > p -
+    window or r < sinks (window 0: all) on present pages; one that sees none gives
+    0. gated: attn_gate applied too, the gate the second half of each head's q row.
+    Returns z [N, n_q_heads, head_dim] fp16; rows behind the last chunk are left as
+    they are (zeros in a new tensor)."""
+    Ts, pos0s = [int(t) for t in Ts], [int(p) for p in pos0s]
+    B, total = len(Ts), sum(Ts)
+    if len(pos0s) != B or B == 0:
+        raise ValueError("one T and one pos0 per sequence, one sequence or more")
+    if min(Ts) < 0 or min(pos0s) < 0:
+        raise ValueError("T, pos0: negative")
+    N, n_q_heads, q_pitch = q.shape
+    _contig(q, "q")
+    if total > N:
+        raise ValueError(f"q: {N} tokens, the chunks have {total}")
+    pg = _paged(kpool, vpool, pages, page_size, B, n_kv_heads, HEAD_DIM)
+    if z is None:
+        make = torch.empty if total == N else torch.zeros
+        z = make((N, n_q_heads, HEAD_DIM), dtype=F16, device=q.device)
+    _contig(z, "z")
+    if z.dim() != 3 or z.shape[1] != n_q_heads or z.shape[0] < total:
+        raise ValueError(f"z: expected [{N}, {n_q_heads}, pitch]")
+    _one_device(q=q, z=z, kpool=kpool, vpool=vpool, pages=pages, work=work)
+    if total == 0:
+        return z
+    need = attention_prefill_paged_work_bytes(Ts, pos0s, n_q_heads, n_kv_heads, HEAD_DIM, window,
+                                              sinks, bool(pg[2]))
+    if work is None and need:
+        work = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _lib.call("fl_attention_prefill_paged", _ptr(q, F16, "q", N * n_q_heads * q_pitch), q_pitch, *pg,
+              _lib.int_array(Ts), _lib.int_array(pos0s), B, n_q_heads, n_kv_heads, HEAD_DIM,
+              float(scale), window, sinks, int(gated), _ptr(z, F16, "z", total * n_q_heads * z.shape[-1]),
+              z.shape[-1], *_prefill_work(work), _stream())
+    return z
+
+
+def attn_decode_paged_work_bytes(B: int, T: int, n_q_heads: int = N_HEADS, n_kv_heads: int = N_KV,
+                                 head_dim: int = HEAD_DIM) -> int:
+    return int(_lib.lib().fl_attn_decode_paged_work_bytes(B, T, n_q_heads, n_kv_heads, head_dim))
+
+
+def attn_decode_paged(qg, kpool, vpool, pages, pos0, *, page_size: int, window: int = 0,
+                      sinks: int = 0, gate: bool = True, z=None, work=None, n_kv_heads: int = N_KV,
+                      scale: float = ATTN_SCALE):
+    """attn_decode / attn_decode_q8 over pages: qg [B, T, n_q_heads, q_pitch] fp16 with
+    q | gate per head, pos0 [B] int32 on the GPU each sequence's first query
+    position (read when the call runs); up to 1024 sequences. What a query sees is
+    attention_prefill_paged's; one at a negative position (a padded batch's row)
+    sees nothing and gives 0. Returns z [B, T, n_q_heads, head_dim] fp16."""
+    B, T, n_q_heads, q_pitch = qg.shape
+    _contig(qg, "qg")
+    if pos0.dim() != 1 or pos0.numel() != B:
+        raise ValueError(f"pos0: expected {B} positions")
+    pg = _paged(kpool, vpool, pages, page_size, B, n_kv_heads, HEAD_DIM)
+    if z is None:
+        z = torch.empty((B, T, n_q_heads, HEAD_DIM), dtype=F16, device=qg.device)
+    _contig(z, "z")
+    if z.dim() != 4 or tuple(z.shape[:3]) != (B, T, n_q_heads):
+        raise ValueError(f"z: expected [{B}, {T}, {n_q_heads}, pitch]")
+    _one_device(qg=qg, z=z, kpool=kpool, vpool=vpool, pages=pages, pos0=pos0, work=work)
+    need = attn_decode_paged_work_bytes(B, T, n_q_heads, n_kv_heads)
+    if work is None and need:
+        work = torch.empty(need, dtype=torch.uint8, device=qg.device)
+    _lib.call("fl_attn_decode_paged", _ptr(qg, F16, "qg", B * T * n_q_heads * q_pitch), q_pitch, *pg,
+              _dense_ptr(pos0, torch.int32, "pos0", B), B, T, n_q_heads, n_kv_heads, HEAD_DIM,
+              float(scale), window, sinks, int(gate), _ptr(z, F16, "z", z.numel()), z.shape[-1],
+              *_prefill_work(work), _stream())
+    return z
+
+
+# ---------------------------------------------------------------------------
 # Gated DeltaNet
 # ---------------------------------------------------------------------------
 

@@ -34,6 +34,8 @@ typedef struct ihipStream_t* fl_stream_t; /* hipStream_t; NULL = default stream 
 #define FL_ESCRATCH 3 /* caller scratch smaller than *_work_bytes asked for */
 
 #define FL_MAX_SEQS 16 /* sequences one batched decode call carries */
+#define FL_PAGED_MAX_SEQS 1024       /* ... one call over a paged cache */
+#define FL_PAGED_MAX_SEQS_PREFILL 64 /* ... of chunks (fl_attention_prefill_paged) */
 
 int fl_abi_version(void);
 const char* fl_strerror(int status);
@@ -346,6 +348,83 @@ int fl_attention_prefill_q8(const void* q, int q_pitch, const void* k_new, const
                             void* kcache, void* vcache, int layer, int n_q_heads,
                             int n_kv_heads, int head_dim, int pos0, int max_pos, float scale,
                             int T, void* z, int z_pitch, fl_stream_t stream);
+
+/* ---- paged KV cache -------------------------------------------------------
+ * No counterpart in the reference, whose caches are one buffer a sequence.
+ * A pool holds a layer's K (or V) rows of all sequences: n_pages pages of
+ * page_size positions (a power of two, 16 or more), fp16 [n_pages * page_size]
+ * [n_kv_heads][256] or, q8, the int8 format above of capacity n_pages *
+ * page_size (all values, then all scales). Position p of sequence b is row
+ * p % page_size of page pages[b * pages_stride + p / page_size], pages a device
+ * array of max_pages entries a sequence. An entry outside [0, n_pages), and a
+ * position past max_pages pages, is an absent page: its rows are not written,
+ * read back as zeros and are not attended to (a window's freed pages, a padded
+ * batch's rows). Sequences may share pages that no call writes.
+ * Packed tokens: sequence b's are tokens starts[b] .. starts[b + 1] - 1 of N,
+ * the first at position pos0[b] (starts [B + 1] nondecreasing, pos0 [B]: device
+ * arrays, so that a captured call can be replayed at other positions). Tokens
+ * before starts[0], behind starts[B] or at a negative position are left as
+ * they are. head_dim 256, B <= FL_PAGED_MAX_SEQS; pools 16-byte aligned. */
+
+/* Store: k, v rows [n_kv_heads][256] f16, tokens k_stride / v_stride elements
+ * apart (multiples of 8, 16-byte aligned), into their positions; q8 quantised as
+ * fl_kv_store_q8 does. No two tokens of a call may have the same row. */
+int fl_paged_kv_store(const void* k, const void* v, long long k_stride, long long v_stride,
+                      void* kpool, void* vpool, int q8, int n_pages, int page_size,
+                      const int* pages, int max_pages, long long pages_stride, const int* starts,
+                      const int* pos0, int B, int N, int n_kv_heads, int head_dim,
+                      fl_stream_t stream);
+
+/* ... and back: the rows of each token's position into k, v (q8: f16(byte *
+ * scale), the value the attention entry points form). zero_rest: the rows of tokens
+ * outside every sequence are set to zero instead of left as they are. */
+int fl_paged_kv_load(const void* kpool, const void* vpool, int q8, int n_pages, int page_size,
+                     const int* pages, int max_pages, long long pages_stride, const int* starts,
+                     const int* pos0, void* k, void* v, long long k_stride, long long v_stride,
+                     int zero_rest, int B, int N, int n_kv_heads, int head_dim, fl_stream_t stream);
+
+/* fl_attn_prep / fl_attn_prep_q8 over packed tokens, each at its own sequence's
+ * position: q and k norms, rope, and the store of the roped k and v rows -- those
+ * calls' values bit for bit. k, v [N][n_kv_heads][256]; the q rows go to q_out
+ * [N][n_q_heads][qo_pitch], or in place where it is NULL. k is not rewritten. */
+int fl_attn_prep_paged(void* qg, int q_pitch, const void* k, const void* v, const float* wq,
+                       const float* wk, void* q_out, int qo_pitch, void* kpool, void* vpool, int q8,
+                       int n_pages, int page_size, const int* pages, int max_pages,
+                       long long pages_stride, const int* starts, const int* pos0, int B, int N,
+                       int n_q_heads, int n_kv_heads, int head_dim, int rope_dim, float theta,
+                       float eps, fl_stream_t stream);
+
+/* Causal GQA attention of chunks of new tokens over the pages: B sequences
+ * (host arrays; B <= FL_PAGED_MAX_SEQS_PREFILL), Ts[b] packed queries each (0:
+ * none), the first at position pos0s[b]; their own rows are in the pool
+ * already. The query at position p sees the rows r <= p with r > p - window or
+ * r < sinks (window 0: all of them) of the pages that are present; one that sees
+ * none gives 0. q [sum Ts][n_q_heads][q_pitch] f16; gated: then z = f16_sat(z *
+ * sigmoid(gate)), the gate the 256 halves after q in a head's row. z
+ * [sum Ts][n_q_heads][z_pitch]. work: fl_attention_prefill_paged_work_bytes of
+ * the same arguments, 16-byte aligned. pos0s[b] + Ts[b] <= max_pages *
+ * page_size. */
+size_t fl_attention_prefill_paged_work_bytes(const int* Ts, const int* pos0s, int B, int n_q_heads,
+                                             int n_kv_heads, int head_dim, int window, int sinks,
+                                             int q8);
+int fl_attention_prefill_paged(const void* q, int q_pitch, const void* kpool, const void* vpool,
+                               int q8, int n_pages, int page_size, const int* pages, int max_pages,
+                               long long pages_stride, const int* Ts, const int* pos0s, int B,
+                               int n_q_heads, int n_kv_heads, int head_dim, float scale, int window,
+                               int sinks, int gated, void* z, int z_pitch, void* work,
+                               size_t work_bytes, fl_stream_t stream);
+
+/* The decode / verify form: T queries of every sequence at positions pos0[b] ..
+ * (a device array), T * n_q_heads / n_kv_heads <= 32, the same visibility; a query
+ * at a negative position (a padded batch's row) sees nothing and gives 0. qg
+ * [B][T][n_q_heads][q_pitch], z [B][T][n_q_heads][z_pitch], work of
+ * fl_attn_decode_paged_work_bytes. Calls that overlap need a work buffer each. */
+size_t fl_attn_decode_paged_work_bytes(int B, int T, int n_q_heads, int n_kv_heads, int head_dim);
+int fl_attn_decode_paged(const void* qg, int q_pitch, const void* kpool, const void* vpool, int q8,
+                         int n_pages, int page_size, const int* pages, int max_pages,
+                         long long pages_stride, const int* pos0, int B, int T, int n_q_heads,
+                         int n_kv_heads, int head_dim, float scale, int window, int sinks, int gated,
+                         void* z, int z_pitch, void* work, size_t work_bytes, fl_stream_t stream);
 
 /* ---- causal conv ----------------------------------------------------------
  * conv1d_causal over `dim` channels of rows x [T][row_stride] f16: E =
