@@ -36,6 +36,7 @@ struct Chunks {
 struct Sight {
     int window, sinks;
 };
+typedef float f32x8 __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ float wave_sum(float v) {
     v += dpp_xor1(v);
@@ -123,20 +124,10 @@ prefill_rows_kernel(const f16* __restrict__ q, int q_pitch, const void* kpool, c
 // sequence's part of the run) and leaves each piece's partial in slot b + run:
 // from one piece to the next the sequence or the run steps on, so slots are
 // distinct. The merge weighs a sequence's partials and applies the gate.
-//
-// A tile: wave w takes kv rows 16 (w & 1) .. + 15 and dims 128 (w >> 1) .. + 127,
-// so that its 16 rows lie in one page and each row is read in whole lines. The
-// query rows are the N columns (32) of S^T = K Q^T on 16x16x32 MFMAs; the two
-// waves' partial scores are added through LDS; a lane pair then holds a column, the
-// softmax is in-lane and one exchange, and P is the B operand of O^T = V^T P^T
-// (V^T transposed through LDS into the slice of the wave that owns its 64 dims).
 // ---------------------------------------------------------------------------
 constexpr int DT = 32;              // rows a tile
-constexpr int D_THREADS = 256;
-constexpr int VTP = 36;             // halves a d row of the V^T slices (32 + pad)
+constexpr int D_WAVES = 4;
 constexpr float RESCALE_LOG2 = 8.f;
-constexpr int SEQ_COST = 2;         // a further piece's fixed cost in tiles (its q, its partial)
-constexpr int RUN_MIN = 2;          // tiles a run, at least
 
 struct DecPart {
     int2* meta;      // [B]: a sequence's first run and its number of partials
@@ -168,143 +159,165 @@ __device__ __forceinline__ DecSeq dec_seq(int pos0, int T, const Sight& sight, i
     return d;
 }
 
-// inclusive sum over the lanes 0 .. l
-__device__ __forceinline__ long long wave_scan(int v) {
-    const int lane = threadIdx.x & 63;
-    long long x = v;
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const long long y = __shfl_up(x, d, 64);
-        if (lane >= d) x += y;
-    }
+// inclusive sum over the lanes 0 .. l (DPP row shifts, then the rows' totals)
+__device__ __forceinline__ int wave_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);   // row_shr 1
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, true);   // row_bcast 15
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, true);   // row_bcast 31
     return x;
 }
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
-__device__ __forceinline__ long long uni64(long long x) {
-    return ((long long)uni((int)(x >> 32)) << 32) | (uint32_t)uni((int)x);
+// the low n bits (none for n <= 0, all from 32 up)
+__device__ __forceinline__ uint32_t low_bits(int n) {
+    return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u;
 }
 
-// One tile in flight: K[row 16 (w & 1) + (l & 15)][128 (w >> 1) + 32 (l / 16) + 8 ks
-// + 0..7] and V[row 16 (w & 1) + 4 (l & 3) + i][128 (w >> 1) + 8 (l / 4) + 0..7].
+// A workgroup's run of the stream: its kv head, and the pieces one after the other.
+struct Run {
+    int h, run, per;          // runs are `per` units long
+    int u, u_end;             // what is left of this one
+    int b, su, cost;          // the sequence that u lies in, where it starts, units ahead of its tiles
+    bool any;
+
+    // Workgroups go to the 8 XCDs round-robin: the kv heads of a run go to one of them
+    // (their rows share lines of scales), the runs to all.
+    __device__ __forceinline__ Run(const int* pos0, int B, int T, int n_kv, int runs, int run_min,
+                                   int seq_cost, const Sight& sight, int cap) {
+        const int id = blockIdx.x, lane = threadIdx.x & 63;
+        const bool even = runs % 8 == 0;
+        const int slot = even ? id >> 3 : id;
+        h = slot % n_kv;
+        run = even ? slot / n_kv * 8 + (id & 7) : slot / n_kv;
+        cost = B > 1 ? seq_cost : 1;   // (not 0: a sequence without rows has its place too)
+        auto units = [&](int s) { return dec_seq(pos0[s], T, sight, cap).n + cost; };
+        int total = 0, scan = 0, un = 0;   // (of the last 64 sequences: the first ones if B <= 64)
+        for (int b0 = 0; b0 < B; b0 += 64) {   // (the host has checked: under 2^31 tiles)
+            un = b0 + lane < B ? units(b0 + lane) : 0;
+            scan = wave_scan(un);
+            total += __builtin_amdgcn_readlane(scan, 63);
+        }
+        // (a little over total / runs: no run is left over)
+        per = max((int)((float)total * (1.0001f / (float)runs)) + 1, run_min);
+        any = (long long)run * per < total;
+        if (!any) return;
+        u = run * per;
+        u_end = (int)min((long long)u + per, (long long)total);
+        b = su = 0;
+        for (int b0 = 0; b0 < B; b0 += 64) {
+            if (B > 64) {
+                un = b0 + lane < B ? units(b0 + lane) : 0;
+                scan = wave_scan(un);
+            }
+            const int before = __popcll(__ballot(b0 + lane < B && scan <= u - su));
+            b = b0 + before;
+            if (before < 64) {
+                su += __builtin_amdgcn_readlane(scan - un, before);
+                break;
+            }
+            su += __builtin_amdgcn_readlane(scan, 63);
+        }
+    }
+    // The tiles [j0, j1) of sequence b that this run has, and the sequence's note for
+    // the merge from the run that it starts in.
+    __device__ __forceinline__ void piece(const DecSeq& d, const DecPart& out, int& j0, int& j1) const {
+        const int eu = su + d.n + cost;
+        if (u == su && h == 0 && threadIdx.x == 0) {
+            const int first = d.n > 0 ? (su + cost) / per : 0;
+            out.meta[b] = make_int2(first, d.n > 0 ? (eu - 1) / per - first + 1 : 0);
+        }
+        j0 = max(0, u - su - cost);
+        j1 = max(0, min(u_end, eu) - su - cost);
+    }
+    // on to the next sequence; false at the run's end
+    __device__ __forceinline__ bool next(const DecSeq& d) {
+        u = su = su + d.n + cost;
+        ++b;
+        return u < u_end;
+    }
+};
+
+// The masks of a tile at row r0 whose 16-row halves lie on pages id0 and id1, a bit
+// a row.
+struct TileMask {
+    int r0, sinks;
+    uint32_t here;   // rows on present pages
+    __device__ __forceinline__ TileMask(int r0, int id0, int id1, int sinks) : r0(r0), sinks(sinks) {
+        here = (id0 < 0 ? 0u : 0xFFFFu) | (id1 < 0 ? 0u : 0xFFFF0000u);
+    }
+    // of [lo, hi) and [0, min(sinks, hi))
+    __device__ __forceinline__ uint32_t rows(int lo, int hi) const {
+        return here & low_bits(hi - r0) & (~low_bits(lo - r0) | low_bits(sinks - r0));
+    }
+    // every token of the call sees every row
+    __device__ __forceinline__ bool whole(const DecSeq& d) const {
+        return here == ~0u && r0 + DT <= d.hi0 && (r0 >= d.lo1 || r0 + DT <= sinks);
+    }
+};
+
+// A wave-uniform address in global memory (scalar base, 32-bit lane offsets; a
+// generic pointer would make flat loads, whose wait the LDS barrier includes).
+typedef const __attribute__((address_space(1))) char* gptr;
+__device__ __forceinline__ gptr uni_global(const char* p) { return (gptr)uniform_ptr(p); }
+template <class V>
+__device__ __forceinline__ V load_g(gptr base, uint32_t off) {
+    return *(const __attribute__((address_space(1))) V*)(base + off);
+}
+template <class V>
+__device__ __forceinline__ V stream_g(gptr base, uint32_t off) {   // read once: non-temporal
+    return __builtin_nontemporal_load((const __attribute__((address_space(1))) V*)(base + off));
+}
+
+// ---------------------------------------------------------------------------
+// fp16 pools. The four waves share a tile: wave w takes kv rows 16 (w & 1) .. + 15 and
+// dims 128 (w >> 1) .. + 127, so that its 16 rows lie in one page and each row is read
+// in whole lines. The query rows are the N columns (32) of S^T = K Q^T on 16x16x32
+// MFMAs; the two waves' partial scores are added through LDS; a lane pair then holds a
+// column, the softmax is in-lane and one exchange, and P, rounded to fp16, is the B
+// operand of O^T = V^T P^T (V^T transposed through LDS into the slice of the wave that
+// owns its 64 dims).
+// ---------------------------------------------------------------------------
+constexpr int VTP = 36;             // halves a d row of the V^T slices (32 + pad)
+constexpr int RUN_MIN_F16 = 2;      // tiles a run, at least
+constexpr int SEQ_COST_F16 = 2;     // a further piece's fixed cost in tiles (its q, its partial)
+
+// A tile in flight: K[row 16 (w & 1) + (l & 15)][128 (w >> 1) + 32 (l / 16) + 8 s + 0..7]
+// and V[row 16 (w & 1) + 4 (l & 3) + e][128 (w >> 1) + 8 (l / 4) + 0..7].
 struct TileF16 {
     f16x8 k[4], v[4];
-};
-struct TileQ8 {
-    u32x4 k[2];
-    u32x2 v[4];
-    uint32_t sc;   // lanes < 32 K scales, above V scales: row (l & 15), blocks 4 (w >> 1)
-                   // + 2 ((l >> 4) & 1) + 0, 1
+    int id0, id1;   // the pages of its halves
 };
 
-// `at`: the pool row of the wave's first row (its 16 rows are consecutive)
-__device__ __forceinline__ void load_tile(TileF16& t, const char* kp, const char* vp, const Pages&,
-                                          long long at, int n_kv, int h, int lane, int w) {
-    const uint32_t rs = (uint32_t)n_kv * (2 * PAGED_HD);
-    const long long base = at * rs + (2 * PAGED_HD) * h + 256 * (w >> 1);
-    const f16x8* ks = (const f16x8*)(kp + base + ((lane & 15) * rs + 64 * (lane >> 4)));
-#pragma unroll
-    for (int i = 0; i < 4; ++i) t.k[i] = ks[i];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        t.v[i] = __builtin_nontemporal_load(
-            (const f16x8*)(vp + base + ((4 * (lane & 3) + i) * rs + 16 * (lane >> 2))));
-}
-__device__ __forceinline__ void load_tile(TileQ8& t, const char* kp, const char* vp, const Pages& pg,
-                                          long long at, int n_kv, int h, int lane, int w) {
-    const uint32_t rs = (uint32_t)n_kv * PAGED_HD;
-    const long long base = at * rs + PAGED_HD * h + 128 * (w >> 1);
-    const u32x4* ks = (const u32x4*)(kp + base + ((lane & 15) * rs + 32 * (lane >> 4)));
-    t.k[0] = ks[0];
-    t.k[1] = ks[1];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        t.v[i] = __builtin_nontemporal_load(
-            (const u32x2*)(vp + base + ((4 * (lane & 3) + i) * rs + 8 * (lane >> 2))));
-    const long long sc0 = (((long long)pg.n_pages << pg.shift) * n_kv) * PAGED_HD;
-    const char* sp = (lane < 32 ? kp : vp) + sc0 + (at * n_kv + h) * 16 + 8 * (w >> 1);
-    t.sc = *(const uint32_t*)(sp + ((lane & 15) * (16 * n_kv) + 4 * ((lane >> 4) & 1)));
-}
-
-__device__ __forceinline__ TileF16 expand(const TileF16& t, int) { return t; }
-__device__ __forceinline__ TileF16 expand(const TileQ8& q, int lane) {
-    TileF16 r;
-    // lane (l & 15) + 16 (l / 32)'s dword, half (l / 16) & 1; V 32 lanes above
-    auto of = [&](int from) {
-        const uint32_t p = (uint32_t)__builtin_amdgcn_ds_bpermute(from << 2, (int)q.sc);
-        const f16 s = __builtin_bit_cast(f16x2, p)[(lane >> 4) & 1];
-        return (f16x2){s, s};
-    };
-    const int bl = 16 * (lane >> 5);
-    const f16x2 ks2 = of((lane & 15) + bl);
-    auto eight = [](uint32_t a, uint32_t b, f16x2 s) {
-        const f16x4 lo = q8_deq4(a, s), hi = q8_deq4(b, s);
-        return (f16x8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-    };
-    r.k[0] = eight(q.k[0].x, q.k[0].y, ks2);
-    r.k[1] = eight(q.k[0].z, q.k[0].w, ks2);
-    r.k[2] = eight(q.k[1].x, q.k[1].y, ks2);
-    r.k[3] = eight(q.k[1].z, q.k[1].w, ks2);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) r.v[i] = eight(q.v[i].x, q.v[i].y, of(32 + bl + 4 * (lane & 3) + i));
-    return r;
-}
-
-template <bool Q8>
-__global__ void __launch_bounds__(D_THREADS, Q8 ? 2 : 1)
-paged_decode_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict__ kp,
-                    const char* __restrict__ vp, const Pages pg, const int* __restrict__ pos0, int B,
-                    int T, int n_q, int n_kv, int runs, float sl2, const Sight sight,
-                    const DecPart out) {
+__global__ void __launch_bounds__(64 * D_WAVES)
+paged_decode_f16_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict__ kp,
+                        const char* __restrict__ vp, const Pages pg, const int* __restrict__ pos0,
+                        int B, int T, int n_q, int n_kv, int runs, float sl2, const Sight sight,
+                        const DecPart out) {
     __shared__ __attribute__((aligned(16))) f32x4 s_part[2][2][4][64];
     __shared__ __attribute__((aligned(16))) f16 s_vt[2][4][64][VTP];
-    const int h = blockIdx.x % n_kv, run = blockIdx.x / n_kv;
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = uni(tid >> 6);
     const int hh = lane >> 5, ql = lane & 31;
     const int G = n_q / n_kv, R = T * G;
     const int cap = pg.max_pages << pg.shift;
-    const int seq_cost = B > 1 ? SEQ_COST : 1;   // (not 0: a sequence without rows has its place too)
-
-    // the whole stream, and this run's [u, u_end) of it
-    auto units = [&](int b) { return dec_seq(pos0[b], T, sight, cap).n + seq_cost; };
-    long long total = 0;
-    for (int b0 = 0; b0 < B; b0 += 64) {
-        const int b = b0 + lane;
-        total += uni64(__shfl(wave_scan(b < B ? units(b) : 0), 63, 64));
-    }
-    // (a little over total / runs: no run is left over)
-    const long long per =
-        max((long long)((float)total * (1.0001f / (float)runs)) + 1, (long long)RUN_MIN);
-    long long u = run * per;
-    const long long u_end = min(u + per, total);
-    if (u >= u_end) return;   // (the whole workgroup)
-    // the sequence that u lies in, and where it starts
-    int b = 0;
-    long long su = 0;
-    for (int b0 = 0; b0 < B; b0 += 64) {
-        const int bb = b0 + lane;
-        const int un = bb < B ? units(bb) : 0;
-        const long long incl = wave_scan(un) + su;
-        const int before = __popcll(__ballot(bb < B && incl <= u));
-        b = b0 + before;
-        if (before < 64) {
-            su = uni64(__shfl(incl - un, before, 64));
-            break;
-        }
-        su = uni64(__shfl(incl, 63, 64));
-    }
-    b = uni(b);
+    Run run(pos0, B, T, n_kv, runs, RUN_MIN_F16, SEQ_COST_F16, sight, cap);
+    if (!run.any) return;   // (the whole workgroup)
+    const int h = run.h;
+    // a lane's offsets from its wave's first row
+    const uint32_t rs = 2 * PAGED_HD * n_kv, col = 2 * PAGED_HD * h + 256 * (w >> 1);
+    const uint32_t ko = col + (lane & 15) * rs + 64 * (lane >> 4);
+    uint32_t vo[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) vo[e] = col + (4 * (lane & 3) + e) * rs + 16 * (lane >> 2);
 
     int tick = 0;   // tiles done: the LDS buffers' turn
     for (;;) {
+        const int b = uni(run.b);
         const DecSeq d = dec_seq(uni(pos0[b]), T, sight, cap);
-        const long long eu = su + d.n + seq_cost;
-        const long long pe = min(u_end, eu);
-        if (u == su && h == 0 && tid == 0) {
-            const long long first = d.n > 0 ? (su + seq_cost) / per : 0;
-            out.meta[b] = make_int2((int)first, d.n > 0 ? (int)((eu - 1) / per - first) + 1 : 0);
-        }
-        const int j0 = (int)max(0ll, u - su - seq_cost), j1 = (int)max(0ll, pe - su - seq_cost);
+        int j0, j1;
+        run.piece(d, out, j0, j1);
         if (j1 > j0) {
             // this lane's query column: token tq, q head h G + gq
             const bool qvalid = ql < R;
@@ -334,12 +347,7 @@ paged_decode_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restr
             f32x16 o0 = (f32x16)(0.f), o1 = (f32x16)(0.f);
             float m_run = -1e30f, l_run = 0.f;
 
-            typedef typename std::conditional<Q8, TileQ8, TileF16>::type Raw;
-            struct Slot {
-                Raw raw;
-                int id0, id1;
-            };
-            auto load = [&](Slot& t, int j) {
+            auto load = [&](TileF16& t, int j) {
                 if (j - jb >= 32) {
                     jb += 32;
                     ids = ids_next;
@@ -351,32 +359,30 @@ paged_decode_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restr
                 // the wave's half; an absent page reads page 0 (masked, and v taken as 0)
                 const int id = (w & 1) ? t.id1 : t.id0;
                 const int in_page = (d.row0(j) + 16 * (w & 1)) & ((1 << pg.shift) - 1);
-                load_tile(t.raw, kp, vp, pg, ((long long)max(id, 0) << pg.shift) + in_page, n_kv, h,
-                          lane, w);
+                const long long at = (((long long)max(id, 0) << pg.shift) + in_page) * rs;
+                const gptr kb = uni_global(kp + at), vb = uni_global(vp + at);
+#pragma unroll
+                for (int s = 0; s < 4; ++s) t.k[s] = load_g<f16x8>(kb, ko + 16 * s);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) t.v[e] = stream_g<f16x8>(vb, vo[e]);
             };
-            auto body = [&](const Slot& t, int j) {
+            auto body = [&](TileF16& t, int j) {
                 const int buf = tick & 1;
-                TileF16 r = expand(t.raw, lane);
                 const int r0 = d.row0(j);
-                // every token sees every row of the tile (uniform)
-                const bool whole = (t.id0 | t.id1) >= 0 && r0 + DT <= d.hi0 &&
-                                   (r0 >= d.lo1 || r0 + DT <= sight.sinks);
+                const TileMask mask(r0, t.id0, t.id1, sight.sinks);
+                const bool whole = mask.whole(d);   // uniform
                 if (!whole) {
                     // rows that no token sees may hold anything: their v must not
                     // meet the product, where 0 x NaN is a NaN
+                    const uint32_t any = mask.rows(d.lo0, d.hi1) >> (16 * (w & 1) + 4 * (lane & 3));
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int row = r0 + 16 * (w & 1) + 4 * (lane & 3) + i;
-                        const bool any = ((w & 1) ? t.id1 : t.id0) >= 0 && row < d.hi1 &&
-                                         (row >= d.lo0 || row < sight.sinks);
-                        r.v[i] = any ? r.v[i] : (f16x8)(0);
-                    }
+                    for (int i = 0; i < 4; ++i) t.v[i] = (any >> i) & 1 ? t.v[i] : (f16x8)(0);
                 }
                 f32x4 c0 = (f32x4)(0.f), c1 = (f32x4)(0.f);
 #pragma unroll
                 for (int ks = 0; ks < 4; ++ks) {
-                    c0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(r.k[ks], qreg[ks], c0, 0, 0, 0);
-                    c1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(r.k[ks], qreg[4 + ks], c1, 0, 0, 0);
+                    c0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(t.k[ks], qreg[ks], c0, 0, 0, 0);
+                    c1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(t.k[ks], qreg[4 + ks], c1, 0, 0, 0);
                 }
                 // 16x16x32: lane 16 g + i holds rows 4 g .. + 3 of column i; stored
                 // where the 32x32 layout reads rows 8 r4 + 4 hh .. + 3 of column ql
@@ -389,7 +395,7 @@ paged_decode_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restr
 #pragma unroll
                 for (int e = 0; e < 8; ++e)
                     *(f16x4*)&s_vt[buf][owner][d0 + e][kv0] =
-                        (f16x4){r.v[0][e], r.v[1][e], r.v[2][e], r.v[3][e]};
+                        (f16x4){t.v[0][e], t.v[1][e], t.v[2][e], t.v[3][e]};
                 // LDS written (the next tile's loads stay in flight across the barrier)
                 asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
                 float sc[16];
@@ -400,13 +406,10 @@ paged_decode_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restr
                     for (int e = 0; e < 4; ++e) sc[4 * r4 + e] = t4[e];
                 }
                 if (!whole) {
+                    const uint32_t see = mask.rows(qlo, qhi) >> (4 * hh);
 #pragma unroll
-                    for (int rr = 0; rr < 16; ++rr) {
-                        const int row = r0 + 8 * (rr >> 2) + 4 * hh + (rr & 3);
-                        const bool see = (rr < 8 ? t.id0 : t.id1) >= 0 && row < qhi &&
-                                         (row >= qlo || row < sight.sinks);
-                        sc[rr] = see ? sc[rr] : -INFINITY;
-                    }
+                    for (int rr = 0; rr < 16; ++rr)
+                        sc[rr] = see & (1u << (8 * (rr >> 2) + (rr & 3))) ? sc[rr] : -INFINITY;
                 }
                 float mt = sc[0];
 #pragma unroll
@@ -424,13 +427,17 @@ paged_decode_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restr
                     o1 *= corr;
                 }
                 float psum = 0.f;
-                f16x8 pk[2];
 #pragma unroll
                 for (int rr = 0; rr < 16; ++rr) {
-                    const float p = fast_exp2(fmaf(sc[rr], sl2, -m_run));
-                    psum += p;
-                    pk[rr >> 3][rr & 7] = (f16)p;
+                    sc[rr] = fast_exp2(fmaf(sc[rr], sl2, -m_run));
+                    psum += sc[rr];
                 }
+                f16x8 pk[2];
+#pragma unroll
+                for (int ks = 0; ks < 2; ++ks)
+                    pk[ks] = __builtin_convertvector(
+                        (f32x8){sc[8 * ks], sc[8 * ks + 1], sc[8 * ks + 2], sc[8 * ks + 3],
+                                sc[8 * ks + 4], sc[8 * ks + 5], sc[8 * ks + 6], sc[8 * ks + 7]}, f16x8);
                 l_run += pair32_sum(psum);
 #pragma unroll
                 for (int ks = 0; ks < 2; ++ks) {
@@ -444,18 +451,19 @@ paged_decode_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restr
                 }
                 ++tick;
             };
-            // two tiles in registers: the next one's loads are issued ahead of this one's math
-            Slot t[2];
+            // Two tiles in registers: the next one's loads are issued ahead of this
+            // one's math, and always (past the end the last tile's again): after a
+            // conditional load the compiler's wait for this tile would drain them all.
+            TileF16 t[2];
             load(t[0], j0);
             for (int j = j0; j < j1; j += 2) {
-                if (j + 1 < j1) load(t[1], j + 1);
+                load(t[1], min(j + 1, j1 - 1));
                 body(t[0], j);
-                if (j + 1 >= j1) break;
-                if (j + 2 < j1) load(t[0], j + 2);
-                body(t[1], j + 1);
+                load(t[0], min(j + 2, j1 - 1));
+                if (j + 1 < j1) body(t[1], j + 1);
             }
             if (qvalid) {
-                const size_t part = ((size_t)(b + run) * n_kv + h) * R + ql;
+                const size_t part = ((size_t)(b + run.run) * n_kv + h) * R + ql;
                 float* dst = out.pacc + part * PAGED_HD + 64 * w + 4 * hh;
 #pragma unroll
                 for (int r4 = 0; r4 < 4; ++r4) {
@@ -470,10 +478,347 @@ paged_decode_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restr
                 }
             }
         }
-        u = pe;
-        if (u >= u_end) return;
-        su = eu;
-        ++b;
+        if (!run.next(d)) return;
+    }
+}
+
+// ---------------------------------------------------------------------------
+// int8 pools. A wave takes every fourth tile of a piece alone, over all 256 dims: no
+// barrier and no exchange until the piece ends, where the four waves' O, maxima and
+// sums are combined through LDS.
+//   S^T (32 kv x 16 NB columns) = K Q^T   K from HBM in A operand order: lane (i, g)
+//                                         row 16 rb + i, dims 32 ks + 8 g .. + 7
+//   softmax                               a lane holds column i's rows 4 g + e of both
+//                                         halves; the maximum is exchanged only when
+//                                         it moves by more than RESCALE_LOG2
+//   O^T (256 dims) += V^T P^T             P as it lies: k slot (g, e) is row 4 g + e of
+//                                         half e / 4; V^T by transposed LDS reads
+// K of the next tile is requested once this one's scores are formed, V once this
+// one's is in LDS, so one of them is always in flight.
+//
+// Bytes are exact in fp16. A 32-dim block is one k step, so its scale is applied to
+// its fp32 partial score and K is not rounded at all; V is f16(byte scale), and P
+// goes in as two fp16 terms: V's rounding is the only one of the products, and the
+// error is that of fp16 pools, whose only one is P's. (With f16(byte scale) for K
+// and V and P in one term it is 1.5 times as large.)
+// ---------------------------------------------------------------------------
+constexpr int V_PITCH = 2 * PAGED_HD + 32;   // bytes a V row in LDS (the 32 spread rows over banks)
+constexpr int O_PITCH = PAGED_HD + 4;        // floats a column of O in LDS
+constexpr int PV_AHEAD = 4;                  // V^T fragments read ahead of their product
+constexpr int RUN_MIN_Q8 = 4;                // tiles a run, at least: one a wave
+constexpr int SEQ_COST_Q8 = 6;              // a further piece's fixed cost in tiles (its first loads)
+
+// A tile in flight: K bytes [row 16 rb + i][32 ks + 8 g .. + 7] and V bytes [row 4 n +
+// g][16 i .. + 15], and of each the scales of row l % 32, blocks 4 (l / 32) .. + 3.
+struct KTile {
+    u32x2 k[2][8];
+    f16x4 sc;
+};
+struct VTile {
+    u32x4 v[8];
+    f16x4 sc;
+};
+
+// Where a call's pools and a lane's part of a row lie.
+struct TileAt {
+    const char *kp, *vp, *ks, *vs;   // values and scales
+    uint32_t rs, ko, vo, so;         // bytes a row; a lane's offsets
+    bool upper;                      // its scales' half of the tile
+    __device__ __forceinline__ TileAt(const char* kp_, const char* vp_, const Pages& pg, int n_kv, int h,
+                                      int lane) {
+        const int i = lane & 15, g = lane >> 4;
+        kp = kp_, vp = vp_;
+        rs = PAGED_HD * n_kv;
+        const long long values = ((long long)pg.n_pages << pg.shift) * rs;
+        ks = kp + values, vs = vp + values;
+        ko = PAGED_HD * h + 8 * g + i * rs;
+        vo = PAGED_HD * h + 16 * i + g * rs;
+        so = 16 * h + 8 * (lane >> 5) + i * (rs / 16);
+        upper = g & 1;
+    }
+    __device__ __forceinline__ f16x4 scales(const char* of, const long long (&at)[2]) const {
+        const long long lo = at[0] * (rs / 16), hi = at[1] * (rs / 16);
+        return *(const __attribute__((address_space(1))) f16x4*)((gptr)of + ((upper ? hi : lo) + so));
+    }
+    // at[half]: the pool row of the tile's 16-row halves
+    __device__ __forceinline__ void load(KTile& t, const long long (&at)[2]) const {
+        t.sc = scales(ks, at);
+#pragma unroll
+        for (int rb = 0; rb < 2; ++rb) {
+            const gptr b = uni_global(kp + at[rb] * rs);
+#pragma unroll
+            for (int s = 0; s < 8; ++s) t.k[rb][s] = load_g<u32x2>(b, ko + 32 * s);
+        }
+        issued();
+    }
+    __device__ __forceinline__ void load(VTile& t, const long long (&at)[2]) const {
+        t.sc = scales(vs, at);
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            const gptr b = uni_global(vp + at[half] * rs);
+#pragma unroll
+            for (int n = 0; n < 4; ++n) t.v[4 * half + n] = stream_g<u32x4>(b + 4 * n * rs, vo);
+        }
+        issued();
+    }
+    // the compiler would sink the loads to where they are used
+    static __device__ __forceinline__ void issued() {
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    }
+};
+
+// 8 bytes as the integers they are, exact in fp16 (q8_deq4 without the scale)
+__device__ __forceinline__ f16x8 q8_ints(u32x2 b) {
+    const f16x2 off = {(f16)1152.f, (f16)1152.f};
+    f16x8 r;
+#pragma unroll
+    for (int d = 0; d < 2; ++d) {
+        const uint32_t u = b[d] ^ 0x80808080u;
+        const f16x2 lo = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - off;
+        const f16x2 hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - off;
+        r[4 * d] = lo[0], r[4 * d + 1] = lo[1], r[4 * d + 2] = hi[0], r[4 * d + 3] = hi[1];
+    }
+    return r;
+}
+__device__ __forceinline__ f16x8 q8_values(uint32_t a, uint32_t b, f16 s) {
+    const f16x4 lo = q8_deq4(a, (f16x2){s, s}), hi = q8_deq4(b, (f16x2){s, s});
+    return (f16x8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+}
+
+// NB: blocks of 16 query columns (2: one workgroup a CU)
+template <int NB>
+__global__ void __launch_bounds__(64 * D_WAVES, NB == 1 ? 2 : 1)
+paged_decode_q8_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict__ kp,
+                       const char* __restrict__ vp, const Pages pg, const int* __restrict__ pos0, int B,
+                       int T, int n_q, int n_kv, int runs, float sl2, const Sight sight,
+                       const DecPart out) {
+    // V of a wave's tile while it walks, O of the waves when a piece ends
+    constexpr int WAVE_B = std::max(DT * V_PITCH, 16 * NB * O_PITCH * 4);
+    __shared__ __attribute__((aligned(16))) char s_mem[D_WAVES * WAVE_B];
+    __shared__ float s_m[D_WAVES][16 * NB], s_l[D_WAVES][16 * NB];
+    // the scales of a wave's tile, [K, V][block][row], V's rows in the order 8 (r % 4) + r / 4
+    __shared__ __attribute__((aligned(16))) f16 s_sc[D_WAVES][2][8][DT + 8];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = uni(tid >> 6);
+    const int i = lane & 15, g = lane >> 4;
+    const int G = n_q / n_kv, R = T * G;
+    const int cap = pg.max_pages << pg.shift;
+    char* const mine = s_mem + w * WAVE_B;
+    Run run(pos0, B, T, n_kv, runs, RUN_MIN_Q8, SEQ_COST_Q8, sight, cap);
+    if (!run.any) return;   // (the whole workgroup)
+    const TileAt tiles(kp, vp, pg, n_kv, run.h, lane);
+
+    for (;;) {
+        const int b = uni(run.b);
+        const DecSeq d = dec_seq(uni(pos0[b]), T, sight, cap);
+        int j0, j1;
+        run.piece(d, out, j0, j1);
+        if (j1 > j0) {
+            f32x4 o[NB][16];
+            float m_run[NB], l_run[NB];   // l: of this lane's rows, summed when the piece ends
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                m_run[nb] = -1e30f, l_run[nb] = 0.f;
+#pragma unroll
+                for (int n = 0; n < 16; ++n) o[nb][n] = (f32x4)(0.f);
+            }
+            const int jw = j0 + w;   // this wave's tiles: jw, jw + 4, ... < j1
+            if (jw < j1) {
+                // page ids of 64 half tiles, a lane each: tile jb + 4 (l / 2), half l & 1
+                auto load_ids = [&](int jb) {
+                    const int j = jb + D_WAVES * (lane >> 1);
+                    return j < j1 ? fl::page_id(pg, b, (d.row0(j) + 16 * (lane & 1)) >> pg.shift) : -1;
+                };
+                int jb = jw, ids = load_ids(jb), ids_next = load_ids(jb + 32 * D_WAVES);
+                // B operand: Q[column 16 nb + i][32 ks + 8 g + 0..7]; the column's rows in sight
+                f16x8 q[NB][8];
+                int lo[NB], hi[NB];
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    const int c = 16 * nb + i;
+                    const bool ok = c < R;
+                    const int t = ok ? c / G : 0, gq = ok ? c - t * G : 0;
+                    const f16* row = qg + (((size_t)b * T + t) * n_q + run.h * G + gq) * q_pitch + 8 * g;
+#pragma unroll
+                    for (int s = 0; s < 8; ++s) q[nb][s] = ok ? *(const f16x8*)(row + 32 * s) : (f16x8)(0);
+                    token_range((long long)pos0[b] + t, sight.window, cap, lo[nb], hi[nb]);
+                }
+                struct Where {
+                    int id0, id1, r0;
+                    long long at[2];
+                };
+                auto where = [&](int j) {
+                    if (j - jb >= 32 * D_WAVES) {
+                        jb += 32 * D_WAVES;
+                        ids = ids_next;
+                        ids_next = load_ids(jb + 32 * D_WAVES);
+                    }
+                    const int l = 2 * ((j - jb) / D_WAVES);
+                    Where x;
+                    x.id0 = __builtin_amdgcn_readlane(ids, l);
+                    x.id1 = __builtin_amdgcn_readlane(ids, l + 1);
+                    x.r0 = d.row0(j);
+                    const int in_page = (1 << pg.shift) - 1;
+                    // (an absent page: page 0 is read, its scores masked and its v taken as 0)
+                    x.at[0] = ((long long)max(x.id0, 0) << pg.shift) + (x.r0 & in_page);
+                    x.at[1] = ((long long)max(x.id1, 0) << pg.shift) + ((x.r0 + 16) & in_page);
+                    return x;
+                };
+                Where x = where(jw);
+                KTile kt;
+                VTile vt;
+                tiles.load(kt, x.at);
+                tiles.load(vt, x.at);
+                const int j_last = jw + (j1 - 1 - jw) / D_WAVES * D_WAVES;
+                for (int j = jw; j < j1; j += D_WAVES) {
+                    const Where xn = where(min(j + D_WAVES, j_last));
+                    const TileMask mask(x.r0, x.id0, x.id1, sight.sinks);
+                    const bool whole = mask.whole(d);   // uniform
+                    // scores: s[nb][4 rb + e] of column i, row 16 rb + 4 g + e
+                    float s[NB][8];
+                    const int sc_row = lane & 31, sc_blk = 4 * (lane >> 5);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s_sc[w][0][sc_blk + e][sc_row] = kt.sc[e];
+#pragma unroll
+                    for (int rb = 0; rb < 2; ++rb) {
+                        f32x4 c[NB];
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) c[nb] = (f32x4)(0.f);
+#pragma unroll
+                        for (int ks = 0; ks < 8; ++ks) {
+                            const f16x8 a = q8_ints(kt.k[rb][ks]);
+                            const f16x4 sc = *(const f16x4*)&s_sc[w][0][ks][16 * rb + 4 * g];
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb) {
+                                const f32x4 p = __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                    a, q[nb][ks], (f32x4)(0.f), 0, 0, 0);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) c[nb][e] = fmaf((float)sc[e], p[e], c[nb][e]);
+                            }
+                        }
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) s[nb][4 * rb + e] = c[nb][e];
+                    }
+                    tiles.load(kt, xn.at);
+                    f16x8 p_hi[NB], p_lo[NB];
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb) {
+                        if (!whole) {
+                            const uint32_t see = mask.rows(lo[nb], hi[nb]) >> (4 * g);
+#pragma unroll
+                            for (int r = 0; r < 8; ++r)
+                                s[nb][r] = see & (1u << (16 * (r >> 2) + (r & 3))) ? s[nb][r] : -INFINITY;
+                        }
+                        float mt = s[nb][0];
+#pragma unroll
+                        for (int r = 1; r < 8; ++r) mt = __builtin_elementwise_maximum(mt, s[nb][r]);
+                        mt *= sl2;
+                        // the running maximum only moves when some score is more than
+                        // RESCALE_LOG2 above it: p <= 256 is exact enough in fp16, and O and
+                        // l are rescaled on few tiles
+                        if (__any(mt > m_run[nb] + RESCALE_LOG2)) {
+                            mt = fmaxf(mt, lane_xor(mt, 16));
+                            mt = pair32_max(mt);
+                            const float m_new = mt > m_run[nb] + RESCALE_LOG2 ? mt : m_run[nb];
+                            const float corr = fast_exp2(m_run[nb] - m_new);
+                            m_run[nb] = m_new;
+                            l_run[nb] *= corr;
+#pragma unroll
+                            for (int n = 0; n < 16; ++n) o[nb][n] *= corr;
+                        }
+                        f32x8 p;
+#pragma unroll
+                        for (int r = 0; r < 8; ++r) {
+                            p[r] = fast_exp2(fmaf(s[nb][r], sl2, -m_run[nb]));
+                            l_run[nb] += p[r];
+                        }
+                        p_hi[nb] = __builtin_convertvector(p, f16x8);
+                        p_lo[nb] =
+                            __builtin_convertvector(p - __builtin_convertvector(p_hi[nb], f32x8), f16x8);
+                    }
+                    // V to LDS as rows. Rows that no token sees may hold anything: their v
+                    // must not meet the product, where 0 x NaN is a NaN.
+                    const uint32_t any = whole ? ~0u : mask.rows(d.lo0, d.hi1);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s_sc[w][1][sc_blk + e][8 * (sc_row & 3) + (sc_row >> 2)] = vt.sc[e];
+                    const f16x8 sc = *(const f16x8*)&s_sc[w][1][i >> 1][8 * g];
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) {
+                        f16x8 a = q8_values(vt.v[n].x, vt.v[n].y, sc[n]);
+                        f16x8 c = q8_values(vt.v[n].z, vt.v[n].w, sc[n]);
+                        if (!whole) {
+                            const bool on = any >> (4 * n + g) & 1;
+                            a = on ? a : (f16x8)(0);
+                            c = on ? c : (f16x8)(0);
+                        }
+                        char* row = mine + (4 * n + g) * V_PITCH + 32 * i;
+                        *(f16x8*)row = a;
+                        *(f16x8*)(row + 16) = c;
+                    }
+                    tiles.load(vt, xn.at);
+                    // V^T: lane (i, g) of block n takes rows 4 g .. + 3 (and + 16) of dim 16 n
+                    // + i; it points at row 4 g + i / 4, dims 16 n + 4 (i % 4). PV_AHEAD
+                    // blocks are read ahead of the products.
+                    const char* vt0 = mine + (4 * g + (i >> 2)) * V_PITCH + 8 * (i & 3);
+                    auto frag = [&](int n) {
+                        const f16x4 va = __builtin_bit_cast(
+                            f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vt0 + 32 * n)));
+                        const f16x4 vb = __builtin_bit_cast(
+                            f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (lds_s16x4*)(vt0 + 16 * V_PITCH + 32 * n)));
+                        return (f16x8){va[0], va[1], va[2], va[3], vb[0], vb[1], vb[2], vb[3]};
+                    };
+                    f16x8 fr[PV_AHEAD];
+#pragma unroll
+                    for (int n = 0; n < PV_AHEAD; ++n) fr[n] = frag(n);
+#pragma unroll
+                    for (int n = 0; n < 16; ++n) {
+                        const f16x8 a = fr[n % PV_AHEAD];
+#pragma unroll
+                        for (int nb = 0; nb < NB; ++nb) {
+                            o[nb][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p_hi[nb], o[nb][n], 0, 0, 0);
+                            o[nb][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p_lo[nb], o[nb][n], 0, 0, 0);
+                        }
+                        if (n + PV_AHEAD < 16) fr[n % PV_AHEAD] = frag(n + PV_AHEAD);
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                    x = xn;
+                }
+            }
+            // the piece's partial: the waves' O weighed against their common maximum
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+                float l = l_run[nb];
+                l += lane_xor(l, 16);
+                l = pair32_sum(l);
+                if (g == 0) s_m[w][16 * nb + i] = m_run[nb], s_l[w][16 * nb + i] = l;
+#pragma unroll
+                for (int n = 0; n < 16; ++n)
+                    *(f32x4*)(mine + ((16 * nb + i) * O_PITCH + 16 * n + 4 * g) * 4) = o[nb][n];
+            }
+            __syncthreads();
+            for (int c = w; c < R; c += D_WAVES) {
+                float m = s_m[0][c], l = 0.f;
+#pragma unroll
+                for (int k = 1; k < D_WAVES; ++k) m = fmaxf(m, s_m[k][c]);
+                f32x4 a = (f32x4)(0.f);
+#pragma unroll
+                for (int k = 0; k < D_WAVES; ++k) {
+                    const float e = fast_exp2(s_m[k][c] - m);
+                    l = fmaf(e, s_l[k][c], l);
+                    a += e * *(const f32x4*)(s_mem + k * WAVE_B + (c * O_PITCH + 4 * lane) * 4);
+                }
+                const size_t part = ((size_t)(b + run.run) * n_kv + run.h) * R + c;
+                *(f32x4*)(out.pacc + part * PAGED_HD + 4 * lane) = a;
+                if (lane == 0) out.pm[part] = m, out.pd[part] = l;
+            }
+            __syncthreads();
+        }
+        if (!run.next(d)) return;
     }
 }
 
@@ -572,8 +917,11 @@ int cu_count() {
     return n;
 }
 
-// runs a kv head: one workgroup a CU over fp16 pools, two over int8 ones
-int dec_runs(int n_kv, bool q8) { return std::max(1, cu_count() * (q8 ? 2 : 1) / n_kv); }
+// runs a kv head: a workgroup a CU, two where the kernel's registers let a CU hold two
+// (int8 pools and at most 16 query rows)
+int dec_runs(int n_kv, bool q8, int rows) {
+    return std::max(1, cu_count() * (q8 && rows <= 16 ? 2 : 1) / n_kv);
+}
 
 size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 size_t dec_part(int B, int T, int n_q, int n_kv, int runs, char* work, DecPart& p) {
@@ -656,7 +1004,7 @@ size_t fl_attn_decode_paged_work_bytes(int B, int T, int n_q_heads, int n_kv_hea
         n_q_heads % n_kv_heads || (long long)T * (n_q_heads / n_kv_heads) > 32 || head_dim != PAGED_HD)
         return 0;
     DecPart p;
-    return dec_part(B, T, n_q_heads, n_kv_heads, dec_runs(n_kv_heads, true), nullptr, p);
+    return dec_part(B, T, n_q_heads, n_kv_heads, dec_runs(n_kv_heads, true, 1), nullptr, p);
 }
 
 int fl_attn_decode_paged(const void* qg, int q_pitch, const void* kpool, const void* vpool, int q8,
@@ -673,15 +1021,19 @@ int fl_attn_decode_paged(const void* qg, int q_pitch, const void* kpool, const v
     FL_REQUIRE(pos0, "null pointer");
     FL_REQUIRE(T >= 1 && (long long)T * (n_q_heads / n_kv_heads) <= 32,
                "T * n_q_heads / n_kv_heads <= 32");
+    FL_REQUIRE((((long long)max_pages << pg.shift) / DT + 8) * B < INT_MAX,
+               "B * max_pages * page_size < 2^36");
     DecPart part;
-    const int runs = dec_runs(n_kv_heads, q8);
+    const int rows = T * (n_q_heads / n_kv_heads);
+    const int runs = dec_runs(n_kv_heads, q8, rows);
     if (dec_part(B, T, n_q_heads, n_kv_heads, runs, (char*)work, part) > work_bytes || !work) {
         fl::set_error("work: smaller than fl_attn_decode_paged_work_bytes");
         return FL_ESCRATCH;
     }
     FL_REQUIRE(aligned16(work), "16-byte aligned work");
-    auto split = q8 ? paged_decode_kernel<true> : paged_decode_kernel<false>;
-    hipLaunchKernelGGL(split, dim3(runs * n_kv_heads), dim3(D_THREADS), 0, (hipStream_t)stream,
+    auto split = !q8 ? paged_decode_f16_kernel
+                     : rows > 16 ? paged_decode_q8_kernel<2> : paged_decode_q8_kernel<1>;
+    hipLaunchKernelGGL(split, dim3(runs * n_kv_heads), dim3(64 * D_WAVES), 0, (hipStream_t)stream,
                        (const f16*)qg, q_pitch, (const char*)kpool, (const char*)vpool, pg, pos0, B, T,
                        n_q_heads, n_kv_heads, runs, scale * FL_LOG2E, Sight{window, sinks}, part);
     rc = fl::check_launch("attn_decode_paged");
