@@ -45,6 +45,7 @@ FILE_FLAGS = {
     "attn_prefill": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-honor-nans", "-mno-amdgpu-ieee"],
     "attn_decode": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "attn_paged": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "attn_paged_prefill": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "gdn_chunk": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 

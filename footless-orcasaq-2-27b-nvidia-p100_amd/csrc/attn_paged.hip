@@ -1,117 +1,13 @@
-// Attention over the paged KV cache (kv_pages.hpp): chunks of new tokens of
-// several sequences, and one to a few tokens a sequence.
-//
-// The query of a token at position p sees the rows r <= p with r > p - window or
-// r < sinks (window 0: all r <= p) whose page is present:
-//   z = f16_sat(sum_r e^(scale q.k_r - m) v_r / sum_r e^(scale q.k_r - m)),
-// then z = f16_sat(z sigmoid(gate)) where a gate is given; a query that sees no
-// row gives 0. Sums, maxima and products are fp32; int8 rows enter as
-// f16(byte scale), like everywhere in this library.
-//
-// One wavefront a (token, q head): a lane holds 4 dims, the dot product is a
-// wave sum, the softmax runs along with one maximum and sum.
-#include "kv_pages.hpp"
+// Decode / verify attention over the paged KV cache: one to a few tokens a sequence
+// (attn_paged.hpp says what is computed).
+#include "attn_paged.hpp"
 
 #include <algorithm>
-#include <atomic>
-#include <type_traits>
-
-#include <math.h>
 
 using fl::Pages;
 using fl::PAGED_HD;
 
 namespace {
-
-constexpr int MAX_SEQS = FL_PAGED_MAX_SEQS_PREFILL;
-
-// Packed chunks: sequence b's tokens are start[b] .. start[b + 1] - 1, the first
-// at position pos0[b].
-struct Chunks {
-    int n;
-    int start[MAX_SEQS + 1];
-    int pos0[MAX_SEQS];
-};
-
-struct Sight {
-    int window, sinks;
-};
-typedef float f32x8 __attribute__((ext_vector_type(8)));
-
-__device__ __forceinline__ float wave_sum(float v) {
-    v += dpp_xor1(v);
-    v += dpp_xor2(v);
-    v += lane_xor(v, 4);
-    v += lane_xor(v, 8);
-    v += lane_xor(v, 16);
-    return pair32_sum(v);
-}
-
-template <bool Q8>
-__device__ __forceinline__ f16x4 row4(const void* pool, const Pages& pg, int n_kv, long long row, int h,
-                                      int lane) {
-    const size_t hr = (size_t)row * n_kv + h;
-    if constexpr (Q8) {
-        const f16* scales =
-            (const f16*)((const char*)pool + (((size_t)pg.n_pages << pg.shift) * n_kv) * PAGED_HD);
-        const f16 s = scales[hr * 8 + (lane >> 3)];
-        return q8_deq4(*(const uint32_t*)((const char*)pool + hr * PAGED_HD + 4 * lane), (f16x2){s, s});
-    } else {
-        return *(const f16x4*)((const f16*)pool + hr * PAGED_HD + 4 * lane);
-    }
-}
-
-// seq's query at position p, head `head` of q row `qrow`, to zrow
-template <bool Q8>
-__device__ void attend_row(const f16* qrow, const f16* gate, f16* zrow, const void* kpool,
-                           const void* vpool, const Pages& pg, long long seq, int p, int h, int n_kv,
-                           float sl2, Sight sight) {
-    const int lane = threadIdx.x & 63;
-    const f16x4 q = *(const f16x4*)(qrow + 4 * lane);
-    float m = -INFINITY, l = 0.f;
-    f32x4 o = (f32x4)(0.f);
-    auto walk = [&](int lo, int hi) {
-        for (int r = lo; r < hi; ++r) {
-            const long long row = fl::page_row(pg, seq, r);
-            if (row < 0) continue;
-            const f16x4 k = row4<Q8>(kpool, pg, n_kv, row, h, lane);
-            const f16x4 v = row4<Q8>(vpool, pg, n_kv, row, h, lane);
-            float s = 0.f;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s = fmaf((float)q[e], (float)k[e], s);
-            s = wave_sum(s) * sl2;
-            const float mn = fmaxf(m, s), c = fast_exp2(m - mn), e2 = fast_exp2(s - mn);
-            m = mn;
-            l = l * c + e2;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[e] = fmaf(e2, (float)v[e], o[e] * c);
-        }
-    };
-    const int lo = sight.window > 0 ? max(0, p - sight.window + 1) : 0;
-    if (lo > 0) walk(0, min(sight.sinks, lo));
-    walk(lo, p + 1);
-    f16x4 out;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        const float v = l == 0.f ? 0.f : o[e] / l;
-        out[e] = f16_sat(gate != nullptr ? v * sigmoid_f((float)gate[4 * lane + e]) : v);
-    }
-    *(f16x4*)(zrow + 4 * lane) = out;
-}
-
-template <bool Q8>
-__global__ void __launch_bounds__(64)
-prefill_rows_kernel(const f16* __restrict__ q, int q_pitch, const void* kpool, const void* vpool,
-                    const Pages pg, const Chunks ch, f16* __restrict__ z, int z_pitch, int gated,
-                    int n_q, int n_kv, float sl2, Sight sight) {
-    const int i = blockIdx.x, head = blockIdx.y;
-    int seq = 0;
-    while (i >= ch.start[seq + 1]) ++seq;
-    const size_t rh = (size_t)i * n_q + head;
-    const f16* qrow = q + rh * q_pitch;
-    attend_row<Q8>(qrow, gated ? qrow + PAGED_HD : nullptr, z + rh * z_pitch, kpool, vpool, pg, seq,
-                   ch.pos0[seq] + i - ch.start[seq], head / (n_q / n_kv), n_kv, sl2, sight);
-}
 
 // ---------------------------------------------------------------------------
 // Decode / verify: T rows a sequence, T G <= 32 query rows a kv head.
@@ -169,12 +65,6 @@ __device__ __forceinline__ int wave_scan(int x) {
     x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, true);   // row_bcast 31
     return x;
 }
-__device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }
-// the low n bits (none for n <= 0, all from 32 up)
-__device__ __forceinline__ uint32_t low_bits(int n) {
-    return n <= 0 ? 0u : n >= 32 ? ~0u : (1u << n) - 1u;
-}
-
 // A workgroup's run of the stream: its kv head, and the pieces one after the other.
 struct Run {
     int h, run, per;          // runs are `per` units long
@@ -238,37 +128,6 @@ struct Run {
         return u < u_end;
     }
 };
-
-// The masks of a tile at row r0 whose 16-row halves lie on pages id0 and id1, a bit
-// a row.
-struct TileMask {
-    int r0, sinks;
-    uint32_t here;   // rows on present pages
-    __device__ __forceinline__ TileMask(int r0, int id0, int id1, int sinks) : r0(r0), sinks(sinks) {
-        here = (id0 < 0 ? 0u : 0xFFFFu) | (id1 < 0 ? 0u : 0xFFFF0000u);
-    }
-    // of [lo, hi) and [0, min(sinks, hi))
-    __device__ __forceinline__ uint32_t rows(int lo, int hi) const {
-        return here & low_bits(hi - r0) & (~low_bits(lo - r0) | low_bits(sinks - r0));
-    }
-    // every token of the call sees every row
-    __device__ __forceinline__ bool whole(const DecSeq& d) const {
-        return here == ~0u && r0 + DT <= d.hi0 && (r0 >= d.lo1 || r0 + DT <= sinks);
-    }
-};
-
-// A wave-uniform address in global memory (scalar base, 32-bit lane offsets; a
-// generic pointer would make flat loads, whose wait the LDS barrier includes).
-typedef const __attribute__((address_space(1))) char* gptr;
-__device__ __forceinline__ gptr uni_global(const char* p) { return (gptr)uniform_ptr(p); }
-template <class V>
-__device__ __forceinline__ V load_g(gptr base, uint32_t off) {
-    return *(const __attribute__((address_space(1))) V*)(base + off);
-}
-template <class V>
-__device__ __forceinline__ V stream_g(gptr base, uint32_t off) {   // read once: non-temporal
-    return __builtin_nontemporal_load((const __attribute__((address_space(1))) V*)(base + off));
-}
 
 // ---------------------------------------------------------------------------
 // fp16 pools. The four waves share a tile: wave w takes kv rows 16 (w & 1) .. + 15 and
@@ -337,25 +196,13 @@ paged_decode_f16_kernel(const f16* __restrict__ qg, int q_pitch, const char* __r
                 for (int ks = 0; ks < 4; ++ks)
                     qreg[4 * nb + ks] = ok ? *(const f16x8*)(qrow + 8 * ks) : (f16x8)(0);
             }
-            // page ids of 64 half tiles, a lane each: list tile jb + l / 2, half l & 1
-            auto load_ids = [&](int jb) {
-                const int j = jb + (lane >> 1);
-                return j < j1 ? fl::page_id(pg, b, (d.row0(j) + 16 * (lane & 1)) >> pg.shift) : -1;
-            };
-            int jb = j0, ids = load_ids(jb), ids_next = load_ids(jb + 32);
+            auto ids = page_ids<1>(pg, b, j0, j1 - 1, [&](int j) { return d.row0(j); });
 
             f32x16 o0 = (f32x16)(0.f), o1 = (f32x16)(0.f);
             float m_run = -1e30f, l_run = 0.f;
 
             auto load = [&](TileF16& t, int j) {
-                if (j - jb >= 32) {
-                    jb += 32;
-                    ids = ids_next;
-                    ids_next = load_ids(jb + 32);
-                }
-                const int l = 2 * (j - jb);
-                t.id0 = __builtin_amdgcn_readlane(ids, l);
-                t.id1 = __builtin_amdgcn_readlane(ids, l + 1);
+                ids.at(j, t.id0, t.id1);
                 // the wave's half; an absent page reads page 0 (masked, and v taken as 0)
                 const int id = (w & 1) ? t.id1 : t.id0;
                 const int in_page = (d.row0(j) + 16 * (w & 1)) & ((1 << pg.shift) - 1);
@@ -370,7 +217,7 @@ paged_decode_f16_kernel(const f16* __restrict__ qg, int q_pitch, const char* __r
                 const int buf = tick & 1;
                 const int r0 = d.row0(j);
                 const TileMask mask(r0, t.id0, t.id1, sight.sinks);
-                const bool whole = mask.whole(d);   // uniform
+                const bool whole = mask.all(d.lo1, d.hi0);   // for every token (uniform)
                 if (!whole) {
                     // rows that no token sees may hold anything: their v must not
                     // meet the product, where 0 x NaN is a NaN
@@ -625,12 +472,7 @@ paged_decode_q8_kernel(const f16* __restrict__ qg, int q_pitch, const char* __re
             }
             const int jw = j0 + w;   // this wave's tiles: jw, jw + 4, ... < j1
             if (jw < j1) {
-                // page ids of 64 half tiles, a lane each: tile jb + 4 (l / 2), half l & 1
-                auto load_ids = [&](int jb) {
-                    const int j = jb + D_WAVES * (lane >> 1);
-                    return j < j1 ? fl::page_id(pg, b, (d.row0(j) + 16 * (lane & 1)) >> pg.shift) : -1;
-                };
-                int jb = jw, ids = load_ids(jb), ids_next = load_ids(jb + 32 * D_WAVES);
+                auto ids = page_ids<D_WAVES>(pg, b, jw, j1 - 1, [&](int j) { return d.row0(j); });
                 // B operand: Q[column 16 nb + i][32 ks + 8 g + 0..7]; the column's rows in sight
                 f16x8 q[NB][8];
                 int lo[NB], hi[NB];
@@ -649,15 +491,8 @@ paged_decode_q8_kernel(const f16* __restrict__ qg, int q_pitch, const char* __re
                     long long at[2];
                 };
                 auto where = [&](int j) {
-                    if (j - jb >= 32 * D_WAVES) {
-                        jb += 32 * D_WAVES;
-                        ids = ids_next;
-                        ids_next = load_ids(jb + 32 * D_WAVES);
-                    }
-                    const int l = 2 * ((j - jb) / D_WAVES);
                     Where x;
-                    x.id0 = __builtin_amdgcn_readlane(ids, l);
-                    x.id1 = __builtin_amdgcn_readlane(ids, l + 1);
+                    ids.at(j, x.id0, x.id1);
                     x.r0 = d.row0(j);
                     const int in_page = (1 << pg.shift) - 1;
                     // (an absent page: page 0 is read, its scores masked and its v taken as 0)
@@ -674,7 +509,7 @@ paged_decode_q8_kernel(const f16* __restrict__ qg, int q_pitch, const char* __re
                 for (int j = jw; j < j1; j += D_WAVES) {
                     const Where xn = where(min(j + D_WAVES, j_last));
                     const TileMask mask(x.r0, x.id0, x.id1, sight.sinks);
-                    const bool whole = mask.whole(d);   // uniform
+                    const bool whole = mask.all(d.lo1, d.hi0);   // for every token (uniform)
                     // scores: s[nb][4 rb + e] of column i, row 16 rb + 4 g + e
                     float s[NB][8];
                     const int sc_row = lane & 31, sc_blk = 4 * (lane >> 5);
@@ -905,25 +740,12 @@ paged_merge_kernel(const DecPart in, f16* __restrict__ z, int z_pitch, const f16
     *(f16x4*)(z + (size_t)rh * z_pitch + 4 * lane) = out;
 }
 
-// The current device's CU count, looked up once per device.
-int cu_count() {
-    static std::atomic<int> cached[64];
-    int dev = 0, n = 0;
-    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
-    if ((n = cached[dev].load()) > 0) return n;
-    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0)
-        n = 256;
-    cached[dev].store(n);
-    return n;
-}
-
 // runs a kv head: a workgroup a CU, two where the kernel's registers let a CU hold two
 // (int8 pools and at most 16 query rows)
 int dec_runs(int n_kv, bool q8, int rows) {
     return std::max(1, cu_count() * (q8 && rows <= 16 ? 2 : 1) / n_kv);
 }
 
-size_t up16(size_t n) { return (n + 15) & ~(size_t)15; }
 size_t dec_part(int B, int T, int n_q, int n_kv, int runs, char* work, DecPart& p) {
     const size_t rows = (size_t)(B + runs) * T * n_q;
     const size_t m = up16((size_t)B * sizeof(int2)), f = up16(rows * 4);
@@ -931,73 +753,9 @@ size_t dec_part(int B, int T, int n_q, int n_kv, int runs, char* work, DecPart& 
     return m + 2 * f + rows * PAGED_HD * 4;
 }
 
-bool aligned16(const void* p) { return ((uintptr_t)p & 15u) == 0; }
-
-int check_heads(const void* q, int q_pitch, const void* z, int z_pitch, int gated, int n_q_heads,
-                int n_kv_heads, float scale, int window, int sinks) {
-    FL_REQUIRE(q && z, "null pointer");
-    FL_REQUIRE(scale > 0.f && scale < INFINITY, "scale > 0");
-    FL_REQUIRE(n_q_heads >= 1 && n_q_heads <= 4096 && n_q_heads % n_kv_heads == 0,
-               "n_q_heads % n_kv_heads");
-    FL_REQUIRE(q_pitch >= (gated ? 2 : 1) * PAGED_HD && q_pitch % 8 == 0,
-               "q_pitch >= head_dim (2 head_dim with the gate), % 8");
-    FL_REQUIRE(z_pitch >= PAGED_HD && z_pitch % 4 == 0, "z_pitch >= head_dim, % 4");
-    FL_REQUIRE(aligned16(q) && ((uintptr_t)z & 7) == 0, "q 16-byte, z 8-byte aligned");
-    FL_REQUIRE(window >= 0 && sinks >= 0, "window, sinks >= 0");
-    return FL_OK;
-}
-
-// the chunks of a call; total tokens in ch.start[B]
-int make_chunks(const int* Ts, const int* pos0s, int B, int max_pages, int page_size, Chunks& ch) {
-    FL_REQUIRE(Ts && pos0s, "null pointer");
-    FL_REQUIRE(B >= 1 && B <= MAX_SEQS, "1 <= B <= FL_PAGED_MAX_SEQS_PREFILL");
-    ch.n = B;
-    long long at = 0;
-    for (int b = 0; b < B; ++b) {
-        FL_REQUIRE(Ts[b] >= 0 && pos0s[b] >= 0, "T, pos0 >= 0");
-        FL_REQUIRE((long long)pos0s[b] + Ts[b] <= (long long)max_pages * page_size,
-                   "pos0 + T <= max_pages * page_size");
-        ch.start[b] = (int)at;
-        ch.pos0[b] = pos0s[b];
-        at += Ts[b];
-        FL_REQUIRE(at <= (1 << 24), "at most 2^24 tokens a call");
-    }
-    ch.start[B] = (int)at;
-    return FL_OK;
-}
-
 }  // namespace
 
 extern "C" {
-
-size_t fl_attention_prefill_paged_work_bytes(const int* Ts, const int* pos0s, int B, int n_q_heads,
-                                             int n_kv_heads, int head_dim, int window, int sinks,
-                                             int q8) {
-    return 0;
-}
-
-int fl_attention_prefill_paged(const void* q, int q_pitch, const void* kpool, const void* vpool,
-                               int q8, int n_pages, int page_size, const int* pages, int max_pages,
-                               long long pages_stride, const int* Ts, const int* pos0s, int B,
-                               int n_q_heads, int n_kv_heads, int head_dim, float scale, int window,
-                               int sinks, int gated, void* z, int z_pitch, void* work,
-                               size_t work_bytes, fl_stream_t stream) {
-    Pages pg;
-    int rc = fl::make_pages(kpool, vpool, q8, n_pages, page_size, pages, max_pages, pages_stride, B,
-                            n_kv_heads, head_dim, pg);
-    if (rc) return rc;
-    rc = check_heads(q, q_pitch, z, z_pitch, gated, n_q_heads, n_kv_heads, scale, window, sinks);
-    if (rc) return rc;
-    Chunks ch;
-    rc = make_chunks(Ts, pos0s, B, max_pages, page_size, ch);
-    if (rc) return rc;
-    if (ch.start[B] == 0) return FL_OK;
-    auto kernel = q8 ? prefill_rows_kernel<true> : prefill_rows_kernel<false>;
-    hipLaunchKernelGGL(kernel, dim3(ch.start[B], n_q_heads), dim3(64), 0, (hipStream_t)stream,
-                       (const f16*)q, q_pitch, kpool, vpool, pg, ch, (f16*)z, z_pitch, gated,
-                       n_q_heads, n_kv_heads, scale * FL_LOG2E, Sight{window, sinks});
-    return fl::check_launch("attention_prefill_paged");
-}
 
 size_t fl_attn_decode_paged_work_bytes(int B, int T, int n_q_heads, int n_kv_heads, int head_dim) {
     if (B < 1 || B > FL_PAGED_MAX_SEQS || n_kv_heads < 1 || n_q_heads < 1 || T < 1 ||

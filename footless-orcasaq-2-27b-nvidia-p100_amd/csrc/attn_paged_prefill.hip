@@ -1,0 +1,819 @@
+// Causal attention of chunks of new tokens over the paged KV cache (attn_paged.hpp says
+// what is computed), several sequences a call.
+//
+// A row tile is 256 (token, q head) rows of one kv head of one sequence, token-major, 64
+// a wave; a wave's tile of 32 cache rows is attn_r64.hpp's: S^T = K Q^T with Q in
+// registers, the softmax with a query column a lane pair, O^T += V^T P^T in AGPRs, K and V
+// copied HBM -> LDS three tiles ahead. What is this file's own:
+//   * a tile's rows come from the pages of its two 16-row halves: a wave copies 8 rows of
+//     one half, so its copies have one scalar base. Rows that no query of the row tile
+//     sees (past its last token, before its window, on absent pages) are copied from a row
+//     of zeros: p is 0 there, and 0 times whatever a page holds must stay 0;
+//   * a row tile walks the tiles of the first `sinks` rows and those from its window on;
+//   * the masks are bits, formed only for tiles that some query does not see whole;
+//   * workgroups are persistent, one a CU, over a host-made plan for the whole batch:
+//     either a list of whole row tiles each (CUT false), or equal runs of all row tiles'
+//     walks laid end to end, cut wherever the cuts fall (CUT): an uncut row tile of a run
+//     goes to z, a cut one leaves partials that paged_piece_merge_kernel combines.
+// Over int8 pools the visible rows are first copied to fp16 (byte scale) in the work
+// buffer, absent and unwritten rows as zeros, and the same kernel walks that copy (DENSE).
+#include "attn_paged.hpp"
+#include "attn_r64.hpp"
+
+#include <algorithm>
+#include <mutex>
+#include <new>
+#include <queue>
+#include <string.h>
+#include <vector>
+
+using fl::R64_BQ;
+
+namespace {
+
+constexpr int MAX_SEQS = FL_PAGED_MAX_SEQS_PREFILL;
+constexpr int THREADS = 256;
+
+// Packed chunks: sequence b's tokens are start[b] .. start[b + 1] - 1, the first at
+// position pos0[b], its row tiles tile0[b] .. tile0[b + 1] - 1; dense[b]: its first row in
+// the fp16 copy (DENSE).
+struct Chunks {
+    int n;
+    int start[MAX_SEQS + 1];
+    int tile0[MAX_SEQS + 1];
+    int pos0[MAX_SEQS];
+    int dense[MAX_SEQS];
+};
+
+// What a row tile walks: the rows [lo, hi) and [0, min(sinks, hi)) of its sequence as
+// tiles, the first s ones, then those from a on, n in all.
+struct Walk {
+    int lo, hi, s, a, n;
+    __host__ __device__ __forceinline__ int row0(int j) const {
+        return R64_BK * (j < s ? j : a + j - s);
+    }
+};
+__host__ __device__ __forceinline__ Walk make_walk(int p_first, int p_last, const Sight& sight) {
+    Walk w;
+    w.hi = p_last + 1;
+    w.lo = sight.window > 0 && p_first >= sight.window ? p_first - sight.window + 1 : 0;
+    w.a = w.lo / R64_BK;
+    const int sk = sight.sinks < w.hi ? sight.sinks : w.hi;
+    const int st = (int)(((unsigned)sk + R64_BK - 1) / R64_BK);
+    w.s = st < w.a ? st : w.a;
+    w.n = w.s + (int)(((unsigned)w.hi + R64_BK - 1) / R64_BK) - w.a;
+    return w;
+}
+
+// The plan of a call, alike for every kv head. CUT: run r goes from row tile tile[r], tile
+// j[r] of its walk, to those of r + 1; its first partial's slot is slot[r]. Else run r has
+// the row tiles list[at[r]] .. list[at[r + 1] - 1].
+constexpr int MAX_RUNS = 256;
+constexpr int LIST_MAX = 1024;
+struct Plan {
+    int runs;
+    union {
+        struct {
+            uint32_t j[MAX_RUNS + 1];
+            uint16_t tile[MAX_RUNS + 1];
+            uint16_t slot[MAX_RUNS];
+        } cut;
+        struct {
+            uint16_t at[MAX_RUNS + 1];
+            uint16_t list[LIST_MAX];
+        } whole;
+    };
+};
+
+// The partials: O unnormalised [slot][256 rows][256], its maximum (log2 units) and sum
+// [slot][256]; kv head h's slots start at h n.
+struct Parts {
+    float* pacc;
+    float* pm;
+    float* pd;
+    int n;
+};
+
+__device__ const u32x4 zero_row[ROW_B / 16] = {};
+
+// Softmax of one 32-column block of a tile (a query column a lane pair, 16 of its 32
+// scores a lane: score r is row 8 (r / 4) + 4 hh + r % 4), `see` the column's visible rows
+// from 4 hh on; the lazy rescale of this block's O^T; P in fp16 as the PV operand.
+__device__ __forceinline__ void softmax_block(f32x16& s, bool whole, uint32_t see, float sl2,
+                                              float& m_run, float& l_run, f32x16 (&o)[8],
+                                              f16x8 (&pk)[2]) {
+    if (!whole) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            s[r] = see & (1u << (8 * (r >> 2) + (r & 3))) ? s[r] : -INFINITY;
+    }
+    float mt = s[0];
+#pragma unroll
+    for (int r = 1; r < 16; ++r) mt = __builtin_elementwise_maximum(mt, s[r]);
+    mt = pair32_max(mt) * sl2;
+    if (__any(mt > m_run + RESCALE_LOG2)) {   // always on a wave's first tile, rarely after
+        const float m_new = fmaxf(m_run, mt);
+        const float corr = fast_exp2(m_run - m_new);
+        m_run = m_new;
+        l_run *= corr;
+        acc_scale(o, corr);
+    }
+    float psum = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        s[r] = fast_exp2(fmaf(s[r], sl2, -m_run));
+        psum += s[r];
+    }
+#pragma unroll
+    for (int ks = 0; ks < 2; ++ks)
+        pk[ks] = __builtin_convertvector((f32x8){s[8 * ks], s[8 * ks + 1], s[8 * ks + 2], s[8 * ks + 3],
+                                                 s[8 * ks + 4], s[8 * ks + 5], s[8 * ks + 6],
+                                                 s[8 * ks + 7]}, f16x8);
+    l_run += pair32_sum(psum);
+}
+
+// Copy 8 rows of a tile's K and V (this wave's) into its stage: two rows an instruction,
+// loff[n] this lane's source offset, swizzled (attn_prefill's layout).
+__device__ __forceinline__ void copy_rows(uint32_t d0, const char* kr, const char* vr,
+                                          const uint32_t (&loff)[4]) {
+    copy16_at<0 * ROW_B>(kr, loff[0], d0);
+    copy16_at<2 * ROW_B>(kr, loff[1], d0);
+    copy16_at<4 * ROW_B>(kr, loff[2], d0);
+    copy16_at<6 * ROW_B>(kr, loff[3], d0);
+    copy16_at<R64_TILE + 0 * ROW_B>(vr, loff[0], d0);
+    copy16_at<R64_TILE + 2 * ROW_B>(vr, loff[1], d0);
+    copy16_at<R64_TILE + 4 * ROW_B>(vr, loff[2], d0);
+    copy16_at<R64_TILE + 6 * ROW_B>(vr, loff[3], d0);
+}
+
+// DENSE: kc and vc are the fp16 copy, [row][n_kv][256], else the pools.
+template <bool DENSE, bool CUT>
+__global__ void __launch_bounds__(THREADS)
+paged_prefill_kernel(const f16* __restrict__ q, int q_pitch, const char* __restrict__ kc,
+                     const char* __restrict__ vc, const Pages pg, const Chunks ch,
+                     f16* __restrict__ z, int z_pitch, int gated, int n_q_heads, int n_kv, float sl2,
+                     const Sight sight, const Plan plan, Parts parts) {
+    extern __shared__ __attribute__((aligned(16))) char smem[];
+    // Workgroups go to the 8 XCDs round-robin, each with an L2 of its own: where the kv
+    // heads divide 8, XCDs 8 / n_kv h .. take all of kv head h.
+    int h, run;
+    {
+        const int id = blockIdx.x;
+        if (8 % n_kv == 0 && gridDim.x % 8 == 0) {
+            const int xcd = id & 7, per = 8 / n_kv;
+            h = xcd / per;
+            run = (id >> 3) * per + xcd % per;
+        } else {
+            h = id % n_kv;
+            run = id / n_kv;
+        }
+    }
+    if (run >= plan.runs) return;
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = uni(tid >> 6);
+    const int ql = lane & 31, hh = lane >> 5;
+    const int G = n_q_heads / n_kv;
+    const uint32_t rsb = (uint32_t)n_kv * ROW_B;
+    const char* kb = uniform_ptr(kc + (size_t)h * ROW_B);
+    const char* vb = uniform_ptr(vc + (size_t)h * ROW_B);
+    uint32_t loff[4];
+#pragma unroll
+    for (int n = 0; n < 4; ++n) {
+        const int r = 2 * n + (lane >> 5);   // row from 8 w
+        loff[n] = r * rsb + 16 * ((lane & 31) ^ sw(8 * w + r));
+    }
+    const uint32_t lds_base = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)smem);
+    // K operand of k-step ks: tile row ql, chunk 16 hh + ks, at 16 hh + (ks ^ sw(ql))
+    const uint32_t koff = ql * ROW_B + 256 * hh + 16 * sw(ql);
+    const int tr_r = (lane & 15) >> 2;
+    const int tr_d = 16 * ((lane & 31) >> 4) + 4 * (lane & 3);
+    uint32_t troff[8];
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2)
+            troff[2 * u + s2] = (4 * hh + tr_r + 8 * s2) * ROW_B + 64 * (u ^ tr_r) +
+                                16 * ((tr_d >> 3) ^ (hh + 2 * s2)) + 2 * (tr_d & 7);
+
+    const int item0 = uni(CUT ? plan.cut.tile[run] : plan.whole.at[run]);
+    const int item1 = uni(CUT ? plan.cut.tile[run + 1] : plan.whole.at[run + 1]);
+    const int j_first = CUT ? uni(plan.cut.j[run]) : 0, j_last = CUT ? uni(plan.cut.j[run + 1]) : 0;
+    int slot = CUT ? uni(plan.cut.slot[run]) : 0;
+    const int n_items = item1 - item0 + (j_last > 0 ? 1 : 0);
+    int seq = 0;
+    for (int it = 0; it < n_items; ++it) {
+        const int tile = CUT ? item0 + it : uni(plan.whole.list[item0 + it]);
+        if (!CUT) seq = 0;
+        while (tile >= ch.tile0[seq + 1]) ++seq;   // (scalar)
+        if (it > 0) tile_done();   // every wave is done with the previous row tile's stages
+        const int pos0 = ch.pos0[seq], start = ch.start[seq];
+        const int RT = (ch.start[seq + 1] - start) * G;
+        const int R0 = (tile - ch.tile0[seq]) * R64_BQ;
+        // this lane's two query rows (columns of the two MFMA blocks)
+        int t[2], g[2], qpos[2];
+        bool rvalid[2];
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb) {
+            const int row = R0 + 64 * w + 32 * nb + ql;
+            rvalid[nb] = row < RT;
+            t[nb] = rvalid[nb] ? row / G : 0;
+            g[nb] = rvalid[nb] ? row - t[nb] * G : 0;
+            qpos[nb] = rvalid[nb] ? pos0 + t[nb] : -1;
+        }
+        const int wfirst = R0 + 64 * w, wlast = min(wfirst + 63, RT - 1);
+        const int wqmax = uni(wlast >= wfirst ? pos0 + wlast / G : -1);
+        const int wqmin = uni(pos0 + wfirst / G);
+        const Walk walk = make_walk(uni(pos0 + R0 / G), uni(pos0 + min(R0 + R64_BQ - 1, RT - 1) / G),
+                                    sight);
+        const int j_lo = CUT && it == 0 ? j_first : 0;
+        const int j_hi = CUT && it == n_items - 1 && j_last > 0 ? j_last : walk.n;
+        const int n_tiles = j_hi - j_lo;
+        if (CUT && n_tiles <= 0) continue;   // (uniform)
+
+        // in the copy a sequence's rows before its first window's are left out
+        int dense_cut = 0, dense_skip = 0;
+        if constexpr (DENSE) {
+            const Walk all = make_walk(pos0, pos0, sight);
+            dense_cut = R64_BK * all.s;
+            dense_skip = R64_BK * (all.a - all.s);
+        }
+        auto ids = page_ids<1>(pg, seq, j_lo, j_hi - 1, [&](int j) { return walk.row0(j); });
+        // copy tile j into the stage at dst; the pages of its halves
+        auto issue = [&](uint32_t dst, int j, int& id0, int& id1) {
+            const uint32_t d0 = uni(dst + 8 * w * ROW_B);
+            const int r0 = walk.row0(j);
+            ids.at(j, id0, id1);
+            if constexpr (DENSE) {
+                const long long at = ch.dense[seq] + (r0 < dense_cut ? r0 : r0 - dense_skip) + 8 * w;
+                copy_rows(d0, kb + at * rsb, vb + at * rsb, loff);
+                return;
+            }
+            const int id = w >> 1 ? id1 : id0, r = r0 + 8 * w;   // this wave's page, first row
+            const long long at = ((long long)max(id, 0) << pg.shift) + (r & ((1 << pg.shift) - 1));
+            const char* kr = kb + at * rsb;
+            const char* vr = vb + at * rsb;
+            if (id >= 0 && r + 8 <= walk.hi && (r >= walk.lo || r + 8 <= sight.sinks)) {
+                copy_rows(d0, kr, vr, loff);
+            } else {
+                const char* zero = (const char*)zero_row + 16 * (lane & 31);
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const int row = r + 2 * n + (lane >> 5);
+                    const bool on = id >= 0 && row < walk.hi && (row >= walk.lo || row < sight.sinks);
+                    copy16_v(on ? kr + loff[n] : zero, d0 + 2 * n * ROW_B);
+                    copy16_v(on ? vr + loff[n] : zero, d0 + R64_TILE + 2 * n * ROW_B);
+                }
+            }
+        };
+        // pages of the tiles in flight, tile j's at j % 4
+        int id0[R64_NST], id1[R64_NST];
+#pragma unroll
+        for (int d = 0; d < R64_DIST; ++d)
+            if (d < n_tiles) issue(lds_base + d * R64_STAGE, j_lo + d, id0[d], id1[d]);
+
+        // Q[row nb][128 hh + 8 ks + 0..7] (a lane past the rows reads token 0's; its
+        // column is never stored)
+        f16x8 qreg[2][16];
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb) {
+            const f16* qrow = q + ((size_t)(start + t[nb]) * n_q_heads + h * G + g[nb]) * q_pitch + 128 * hh;
+#pragma unroll
+            for (int ks = 0; ks < 16; ++ks) qreg[nb][ks] = *(const f16x8*)(qrow + 8 * ks);
+        }
+        WAIT_VMCNT(0);   // the first tiles, and Q, pinned here: a later wait would drain the copies
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+            for (int ks = 0; ks < 16; ++ks) asm volatile("" : "+v"(qreg[nb][ks]));
+
+        f32x16 o[2][8];
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb)
+#pragma unroll
+            for (int mb = 0; mb < 8; ++mb) acc_zero(o[nb][mb], (f16x8)(0));
+        float m_run[2] = {-1e30f, -1e30f}, l_run[2] = {0.f, 0.f};
+
+        typedef __attribute__((address_space(3))) const f16x8 lds_f16x8;
+        typedef __attribute__((address_space(3))) const char lds_char;
+        int st = 0;   // stage of tile j
+        for (int j = 0; j < n_tiles; ++j) {
+            // tile j landed: the copies of the min(DIST - 1, n_tiles - 1 - j) tiles issued
+            // after it may still be in flight
+            const int ahead = min(R64_DIST - 1, n_tiles - 1 - j);
+            if (ahead == 2) WAIT_VMCNT(2 * R64_COPIES);
+            else if (ahead == 1) WAIT_VMCNT(R64_COPIES);
+            else WAIT_VMCNT(0);
+            tile_done();   // every wave is past tile j - 1: its stage can be refilled
+            const int p0 = id0[0], p1 = id1[0];
+            id0[0] = id0[1], id1[0] = id1[1];
+            id0[1] = id0[2], id1[1] = id1[2];
+            if (j + R64_DIST < n_tiles) {
+                const int sn = st == 0 ? R64_NST - 1 : st - 1;   // (j + DIST) % NST == (j - 1) % NST
+                issue(lds_base + sn * R64_STAGE, j_lo + j + R64_DIST, id0[2], id1[2]);
+            }
+            const int kv0 = walk.row0(j_lo + j);
+            if (kv0 <= wqmax) {
+                const uint32_t kst = koff + st * R64_STAGE;
+                f32x16 s[2] = {(f32x16)(0.f), (f32x16)(0.f)};
+                constexpr int KPF = R64_KPF;
+                f16x8 ka[KPF];
+#pragma unroll
+                for (int ks = 0; ks < KPF; ++ks) ka[ks] = *(lds_f16x8*)((lds_char*)smem + (kst ^ (16 * ks)));
+#pragma unroll
+                for (int ks = 0; ks < 16; ++ks) {
+                    const f16x8 a = ka[ks % KPF];
+                    if (ks + KPF < 16)
+                        ka[ks % KPF] = *(lds_f16x8*)((lds_char*)smem + (kst ^ (16 * (ks + KPF))));
+                    s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qreg[0][ks], s[0], 0, 0, 0);
+                    s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qreg[1][ks], s[1], 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);   // keep the reads ahead
+                }
+                // whole: every query of the wave sees every row (uniform)
+                const TileMask mask(kv0, p0, p1, sight.sinks);
+                auto low = [&](int p) {
+                    return sight.window > 0 && p >= sight.window ? p - sight.window + 1 : 0;
+                };
+                const bool whole = mask.all(low(wqmax), wqmin + 1);
+                f16x8 pk[2][2];
+#pragma unroll
+                for (int nb = 0; nb < 2; ++nb) {
+                    uint32_t see = 0;
+                    if (!whole) see = mask.rows(low(qpos[nb]), qpos[nb] + 1) >> (4 * hh);
+                    softmax_block(s[nb], whole, see, sl2, m_run[nb], l_run[nb], o[nb], pk[nb]);
+                }
+                // O^T += V^T P^T: 4 steps (kq, dim half) of 4 fragments x 2 blocks, the next
+                // step's fragments read under this step's MFMAs
+                const char* vt = smem + st * R64_STAGE + R64_TILE;
+                s16x4 vf[2][8];
+                r64_vfrags(vf[0], vt, troff, 0);
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    if (n + 1 < 4) r64_vfrags(vf[(n + 1) & 1], vt, troff, n + 1);
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const f16x4 lf = __builtin_bit_cast(f16x4, vf[n & 1][2 * u]);
+                        const f16x4 hf = __builtin_bit_cast(f16x4, vf[n & 1][2 * u + 1]);
+                        const f16x8 av = {lf[0], lf[1], lf[2], lf[3], hf[0], hf[1], hf[2], hf[3]};
+                        acc_mfma(o[0][4 * (n & 1) + u], av, pk[0][n >> 1]);
+                        acc_mfma(o[1][4 * (n & 1) + u], av, pk[1][n >> 1]);
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            st = st == R64_NST - 1 ? 0 : st + 1;
+        }
+
+        acc_settle(o[0]);
+        acc_settle(o[1]);
+        // a cut row tile leaves its partial, a whole one z (one walk over O for both: with
+        // two the compiler spills the accumulators)
+        const bool part = CUT && n_tiles < walk.n;
+#pragma unroll
+        for (int nb = 0; nb < 2; ++nb) {
+            if (!rvalid[nb]) continue;
+            const size_t at = (size_t)(slot + h * parts.n) * R64_BQ + 64 * w + 32 * nb + ql;
+            float* acc = parts.pacc + at * PF_HD + 4 * hh;
+            const float inv = l_run[nb] == 0.f ? 0.f : 1.f / l_run[nb];   // (no row seen: 0)
+            const size_t rh = (size_t)(start + t[nb]) * n_q_heads + h * G + g[nb];
+            f16* zrow = z + rh * z_pitch + 4 * hh;
+            const f16* grow = q + rh * q_pitch + PF_HD + 4 * hh;
+            if (part && hh == 0) {
+                parts.pm[at] = m_run[nb];
+                parts.pd[at] = l_run[nb];
+            }
+#pragma unroll
+            for (int mb = 0; mb < 8; ++mb)
+#pragma unroll
+                for (int r4 = 0; r4 < 4; ++r4) {
+                    const f32x4 v = {o[nb][mb][4 * r4], o[nb][mb][4 * r4 + 1], o[nb][mb][4 * r4 + 2],
+                                     o[nb][mb][4 * r4 + 3]};
+                    if (part) {
+                        *(f32x4*)(acc + 32 * mb + 8 * r4) = v;
+                        continue;
+                    }
+                    float f[4] = {inv, inv, inv, inv};
+                    if (gated) {
+                        const f16x4 gv = *(const f16x4*)(grow + 32 * mb + 8 * r4);
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) f[e] *= fast_sigmoid((float)gv[e]);
+                    }
+                    f16x4 out;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) out[e] = f16_sat(v[e] * f[e]);
+                    *(f16x4*)(zrow + 32 * mb + 8 * r4) = out;
+                }
+        }
+        if (part) ++slot;
+    }
+}
+
+// The cut row tiles of a plan: row tile `tile`'s partials are slots first .. + n - 1.
+struct CutTiles {
+    int n;
+    uint16_t tile[MAX_RUNS], first[MAX_RUNS], count[MAX_RUNS];
+};
+
+// z of the cut row tiles: a wave a row, lane l holding dims 4 l .. + 3, the partials in
+// batches whose loads are all issued before any is used, against one running maximum.
+constexpr int PM_BATCH = 8;
+__global__ void __launch_bounds__(256)
+paged_piece_merge_kernel(const Parts in, const Chunks ch, const CutTiles cut, f16* __restrict__ z,
+                         int z_pitch, const f16* __restrict__ gate, int g_pitch, int n_q_heads, int n_kv) {
+    const int lane = threadIdx.x & 63, h = blockIdx.y, G = n_q_heads / n_kv;
+    const int c = uni(blockIdx.x / (R64_BQ / 4)), r = uni(4 * (blockIdx.x % (R64_BQ / 4)) + (threadIdx.x >> 6));
+    const int tile = cut.tile[c], ns = cut.count[c];
+    int seq = 0;
+    while (tile >= ch.tile0[seq + 1]) ++seq;
+    const int row = (tile - ch.tile0[seq]) * R64_BQ + r;
+    if (row >= (ch.start[seq + 1] - ch.start[seq]) * G) return;   // (wave-uniform)
+    const int t = row / G;
+    const size_t rh = (size_t)(ch.start[seq] + t) * n_q_heads + h * G + row - t * G;
+    f16x4 gv = (f16x4)(0);
+    if (gate != nullptr) gv = *(const f16x4*)(gate + rh * g_pitch + 4 * lane);
+    const size_t p0 = (size_t)(h * in.n + cut.first[c]) * R64_BQ + r;
+    f32x4 num = (f32x4)(0.f);
+    float den = 0.f, M = -1e30f;
+    for (int s = 0; s < ns; s += PM_BATCH) {
+        float mv[PM_BATCH], dv[PM_BATCH];
+        f32x4 av[PM_BATCH];
+#pragma unroll
+        for (int k = 0; k < PM_BATCH; ++k) {
+            if (s + k >= ns) break;   // uniform
+            const size_t at = p0 + (size_t)(s + k) * R64_BQ;
+            mv[k] = in.pm[at];
+            dv[k] = in.pd[at];
+            av[k] = *(const f32x4*)(in.pacc + at * PF_HD + 4 * lane);
+        }
+        float bm = M;
+#pragma unroll
+        for (int k = 0; k < PM_BATCH; ++k)
+            if (s + k < ns) bm = fmaxf(bm, mv[k]);
+        const float corr = fast_exp2(M - bm);
+        num *= corr;
+        den *= corr;
+        M = bm;
+#pragma unroll
+        for (int k = 0; k < PM_BATCH; ++k) {
+            if (s + k >= ns) break;
+            const float e = fast_exp2(mv[k] - M);
+            num += e * av[k];
+            den = fmaf(e, dv[k], den);
+        }
+    }
+    const float inv = den == 0.f ? 0.f : 1.f / den;
+    f16x4 out;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+        out[e] = f16_sat(num[e] * (gate != nullptr ? inv * fast_sigmoid((float)gv[e]) : inv));
+    *(f16x4*)(z + rh * z_pitch + 4 * lane) = out;
+}
+
+// ---------------------------------------------------------------------------
+// host: chunks, plan, launch
+// ---------------------------------------------------------------------------
+
+int make_chunks(const int* Ts, const int* pos0s, int B, int G, long long capacity, Chunks& ch) {
+    FL_REQUIRE(Ts && pos0s, "null pointer");
+    FL_REQUIRE(B >= 1 && B <= MAX_SEQS, "1 <= B <= FL_PAGED_MAX_SEQS_PREFILL");
+    memset(&ch, 0, sizeof(ch));
+    ch.n = B;
+    long long at = 0, tiles = 0;
+    for (int b = 0; b < B; ++b) {
+        FL_REQUIRE(Ts[b] >= 0 && pos0s[b] >= 0, "T, pos0 >= 0");
+        FL_REQUIRE((long long)pos0s[b] + Ts[b] <= capacity, "pos0 + T <= max_pages * page_size");
+        ch.pos0[b] = pos0s[b];
+        at += Ts[b];
+        tiles += ((long long)Ts[b] * G + R64_BQ - 1) / R64_BQ;
+        FL_REQUIRE(tiles < 65536, "sum of T n_q_heads / n_kv_heads under 2^24 a call");
+        ch.start[b + 1] = (int)at;
+        ch.tile0[b + 1] = (int)tiles;
+    }
+    return FL_OK;
+}
+
+// The rows of a sequence in the fp16 copy: those of the union of its row tiles' walks.
+int dense_rows(int T, int pos0, const Sight& sight) {
+    return T == 0 ? 0 : R64_BK * make_walk(pos0, pos0 + T - 1, sight).n;
+}
+
+constexpr int ITEM_COST = 5;    // a row tile's fixed cost in tiles (Q, pipeline fill, z)
+constexpr int PIECE_COST = 8;   // a piece's (its 256 KiB partial)
+constexpr int PIECE_MIN = 6;    // tiles a piece, at least
+constexpr int MERGE_COST = 2;         // the merge's launch, in tiles
+constexpr int SLOTS_PER_TILE = 40;    // partials the merge reads in a tile's time
+
+struct CallPlan {
+    bool cut;
+    int slots;
+    Plan plan;
+    CutTiles tiles;
+};
+
+void walks(const Chunks& ch, int G, const Sight& sight, std::vector<int>& n) {
+    n.clear();
+    for (int b = 0; b < ch.n; ++b) {
+        const int RT = (ch.start[b + 1] - ch.start[b]) * G;
+        for (int R0 = 0; R0 < RT; R0 += R64_BQ)
+            n.push_back(make_walk(ch.pos0[b] + R0 / G,
+                                  ch.pos0[b] + std::min(R0 + R64_BQ - 1, RT - 1) / G, sight).n);
+    }
+}
+
+// The cut plan over at most `most` runs, and its cost (the longest run and the merge).
+long long cut_plan(const std::vector<int>& n, int n_kv, int most, CallPlan& cp) {
+    const int N = (int)n.size();
+    long long total = 0;
+    for (int x : n) total += x + PIECE_COST;
+    const int runs = (int)std::max<long long>(
+        1, std::min<long long>(most, total / (PIECE_COST + 2 * PIECE_MIN)));
+    Plan& p = cp.plan;
+    p.runs = runs;
+    int tile = 0;
+    long long before = 0;   // cost of the row tiles ahead of `tile`
+    for (int r = 0; r <= runs; ++r) {
+        const long long u = r == runs ? total : total * r / runs;
+        while (tile < N && before + n[tile] + PIECE_COST <= u) before += n[tile++] + PIECE_COST;
+        int j = tile < N ? (int)std::max<long long>(0, u - before - PIECE_COST) : 0;
+        int t = tile;
+        if (j < PIECE_MIN) j = 0;
+        else if (n[t] - j < PIECE_MIN) ++t, j = 0;
+        p.cut.tile[r] = (uint16_t)t;
+        p.cut.j[r] = (uint32_t)j;
+    }
+    // slots of the cut row tiles' pieces, in stream order
+    cp.slots = 0;
+    cp.tiles.n = 0;
+    long long longest = 0;
+    int open = -1;   // the cut row tile that the last partial belongs to
+    for (int r = 0; r < runs; ++r) {
+        p.cut.slot[r] = (uint16_t)cp.slots;
+        const int t0 = p.cut.tile[r], t1 = p.cut.tile[r + 1];
+        const int j0 = (int)p.cut.j[r], j1 = (int)p.cut.j[r + 1];
+        long long cost = 0;
+        for (int t = t0; t < t1 + (j1 > 0 ? 1 : 0); ++t) {
+            const int lo = t == t0 ? j0 : 0, hi = t == t1 ? j1 : n[t];
+            if (hi == lo) continue;
+            const bool part = hi - lo < n[t];
+            cost += hi - lo + (part ? PIECE_COST : ITEM_COST);
+            if (!part) continue;
+            if (open != t) {
+                cp.tiles.tile[cp.tiles.n] = (uint16_t)t;
+                cp.tiles.first[cp.tiles.n] = (uint16_t)cp.slots;
+                cp.tiles.count[cp.tiles.n++] = 0;
+                open = t;
+            }
+            ++cp.tiles.count[cp.tiles.n - 1];
+            ++cp.slots;
+        }
+        longest = std::max(longest, cost);
+    }
+    return longest + (cp.slots ? MERGE_COST + cp.slots * n_kv / SLOTS_PER_TILE : 0);
+}
+
+// The plan of whole row tiles, the heaviest first to the lightest run, and its cost; 0
+// where its list does not fit.
+long long whole_plan(const std::vector<int>& n, int most, Plan& p) {
+    const int N = (int)n.size();
+    if (N > LIST_MAX) return 0;
+    const int runs = std::min(most, N);
+    std::vector<int> order(N), run_of(N);
+    for (int t = 0; t < N; ++t) order[t] = t;
+    std::stable_sort(order.begin(), order.end(), [&](int a, int b) { return n[a] > n[b]; });
+    typedef std::pair<long long, int> Load;
+    std::priority_queue<Load, std::vector<Load>, std::greater<Load>> light;
+    for (int r = 0; r < runs; ++r) light.push({0, r});
+    std::vector<std::vector<int>> list(runs);
+    long long longest = 0;
+    for (int t : order) {
+        Load l = light.top();
+        light.pop();
+        list[l.second].push_back(t);
+        l.first += n[t] + ITEM_COST;
+        longest = std::max(longest, l.first);
+        light.push(l);
+    }
+    p.runs = runs;
+    int k = 0;
+    for (int r = 0; r < runs; ++r) {
+        p.whole.at[r] = (uint16_t)k;
+        for (int t : list[r]) p.whole.list[k++] = (uint16_t)t;
+    }
+    p.whole.at[runs] = (uint16_t)k;
+    return longest;
+}
+
+void make_plan(const Chunks& ch, int G, int n_kv, const Sight& sight, int n_cu, CallPlan& cp) {
+    std::vector<int> n;
+    walks(ch, G, sight, n);
+    const int most = std::min(MAX_RUNS, std::max(1, n_cu / n_kv));
+    const long long cut = cut_plan(n, n_kv, most, cp);
+    Plan whole;
+    const long long w = whole_plan(n, most, whole);
+    cp.cut = w == 0 || cut < w;
+    if (!cp.cut) {
+        cp.plan = whole;
+        cp.slots = cp.tiles.n = 0;
+    }
+}
+
+// ... kept for the last few calls (the layers of a step ask the same)
+struct PlanEntry {
+    bool used;
+    Chunks ch;
+    int G, n_kv, n_cu;
+    Sight sight;
+    CallPlan cp;
+};
+constexpr int PLAN_CACHE = 8;
+std::mutex g_mu;
+PlanEntry g_plans[PLAN_CACHE];
+int g_next;
+
+// FL_OK, or FL_ELAUNCH without host memory
+int call_plan(const Chunks& ch, int G, int n_kv, const Sight& sight, int n_cu, CallPlan& cp) {
+    {
+        std::lock_guard<std::mutex> lock(g_mu);
+        for (const PlanEntry& e : g_plans)
+            if (e.used && e.G == G && e.n_kv == n_kv && e.n_cu == n_cu && e.sight.window == sight.window &&
+                e.sight.sinks == sight.sinks && memcmp(&e.ch, &ch, sizeof(ch)) == 0) {
+                cp = e.cp;
+                return FL_OK;
+            }
+    }
+    try {
+        make_plan(ch, G, n_kv, sight, n_cu, cp);
+    } catch (const std::bad_alloc&) {
+        fl::set_error("attention_prefill_paged: no host memory for the plan");
+        return FL_ELAUNCH;
+    }
+    std::lock_guard<std::mutex> lock(g_mu);
+    PlanEntry& e = g_plans[g_next];
+    e.used = true, e.ch = ch, e.G = G, e.n_kv = n_kv, e.n_cu = n_cu, e.sight = sight, e.cp = cp;
+    g_next = (g_next + 1) % PLAN_CACHE;
+    return FL_OK;
+}
+
+size_t parts_bytes(int slots, int n_kv) { return (size_t)slots * n_kv * R64_BQ * (PF_HD + 2) * 4; }
+
+// The rows of the fp16 copy of an int8 call; ch.dense[] set.
+long long lay_dense(Chunks& ch, const Sight& sight) {
+    long long at = 0;
+    for (int b = 0; b < ch.n; ++b) {
+        ch.dense[b] = (int)at;
+        at += dense_rows(ch.start[b + 1] - ch.start[b], ch.pos0[b], sight);
+        if (at > INT_MAX / 2) return -1;
+    }
+    return at;
+}
+size_t dense_bytes(long long rows, int n_kv) { return 2 * (size_t)rows * n_kv * ROW_B; }
+
+// Dynamic LDS above the default limit, raised once per device.
+int raise_lds() {
+    static std::atomic<bool> done[64];
+    int dev = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) {
+        fl::set_error("attention_prefill_paged: no current device below index 64");
+        return FL_ELAUNCH;
+    }
+    if (done[dev].load()) return FL_OK;
+    const void* fns[] = {(const void*)paged_prefill_kernel<false, false>,
+                         (const void*)paged_prefill_kernel<false, true>,
+                         (const void*)paged_prefill_kernel<true, false>,
+                         (const void*)paged_prefill_kernel<true, true>};
+    for (const void* f : fns)
+        if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, R64_LDS) != hipSuccess) {
+            fl::set_error("attention_prefill_paged: cannot raise the dynamic LDS limit to %d bytes",
+                          R64_LDS);
+            return FL_ELAUNCH;
+        }
+    done[dev].store(true);
+    return FL_OK;
+}
+
+// The fp16 copy: row i of sequence b's part is the row of the union of its walks; a
+// wave a row, 8 dims (both of K and V) a lane and step. Rows past the sequence and of
+// absent pages are zeros.
+__global__ void __launch_bounds__(256)
+paged_stage_kernel(const char* __restrict__ kp, const char* __restrict__ vp, const Pages pg,
+                   const Chunks ch, const Sight sight, f16x8* __restrict__ ko, f16x8* __restrict__ vo,
+                   long long rows, int n_kv) {
+    const long long i = (long long)blockIdx.x * 4 + uni(threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (i >= rows) return;   // (wave-uniform)
+    int seq = ch.n - 1;
+    while (seq > 0 && i < ch.dense[seq]) --seq;
+    const int p0 = ch.pos0[seq], end = p0 + ch.start[seq + 1] - ch.start[seq];
+    const Walk first = make_walk(p0, p0, sight);
+    const int k = (int)(i - ch.dense[seq]);
+    const int pos = k < R64_BK * first.s ? k : k + R64_BK * (first.a - first.s);
+    const bool seen = pos < end && (pos >= first.lo || pos < sight.sinks);
+    const long long row = seen ? fl::page_row(pg, seq, pos) : -1;
+    const int chunks = n_kv * (PF_HD / 8);
+    const size_t scales = (((size_t)pg.n_pages << pg.shift) * n_kv) * PF_HD;
+    for (int c = lane; c < chunks; c += 64) {
+        f16x8 kx = (f16x8)(0), vx = (f16x8)(0);
+        if (row >= 0) {
+            const size_t at = (size_t)row * chunks + c;
+            auto get = [&](const char* pool) {
+                const u32x2 b = *(const u32x2*)(pool + 8 * at);
+                const f16 s = ((const f16*)(pool + scales))[at >> 2];
+                const f16x4 lo = q8_deq4(b.x, (f16x2){s, s}), hi = q8_deq4(b.y, (f16x2){s, s});
+                return (f16x8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+            };
+            kx = get(kp);
+            vx = get(vp);
+        }
+        ko[(size_t)i * chunks + c] = kx;
+        vo[(size_t)i * chunks + c] = vx;
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t fl_attention_prefill_paged_work_bytes(const int* Ts, const int* pos0s, int B, int n_q_heads,
+                                             int n_kv_heads, int head_dim, int window, int sinks,
+                                             int q8) {
+    if (n_kv_heads < 1 || n_q_heads < 1 || n_q_heads % n_kv_heads || head_dim != PF_HD || window < 0 ||
+        sinks < 0)
+        return 0;
+    Chunks ch;
+    const int G = n_q_heads / n_kv_heads;
+    const Sight sight = {window, sinks};
+    if (make_chunks(Ts, pos0s, B, G, INT_MAX - 1024, ch) || ch.start[B] == 0) return 0;
+    CallPlan cp;
+    if (call_plan(ch, G, n_kv_heads, sight, cu_count(), cp)) return 0;
+    const long long rows = q8 ? lay_dense(ch, sight) : 0;
+    return up16(parts_bytes(cp.slots, n_kv_heads)) + (rows > 0 ? dense_bytes(rows, n_kv_heads) : 0);
+}
+
+int fl_attention_prefill_paged(const void* q, int q_pitch, const void* kpool, const void* vpool,
+                               int q8, int n_pages, int page_size, const int* pages, int max_pages,
+                               long long pages_stride, const int* Ts, const int* pos0s, int B,
+                               int n_q_heads, int n_kv_heads, int head_dim, float scale, int window,
+                               int sinks, int gated, void* z, int z_pitch, void* work,
+                               size_t work_bytes, fl_stream_t stream_) {
+    Pages pg;
+    int rc = fl::make_pages(kpool, vpool, q8, n_pages, page_size, pages, max_pages, pages_stride, B,
+                            n_kv_heads, head_dim, pg);
+    if (rc) return rc;
+    rc = check_heads(q, q_pitch, z, z_pitch, gated, n_q_heads, n_kv_heads, scale, window, sinks);
+    if (rc) return rc;
+    Chunks ch;
+    const int G = n_q_heads / n_kv_heads;
+    rc = make_chunks(Ts, pos0s, B, G, (long long)max_pages * page_size, ch);
+    if (rc) return rc;
+    if (ch.start[B] == 0) return FL_OK;
+    const Sight sight = {window, sinks};
+    const int n_cu = cu_count();
+    CallPlan cp;
+    rc = call_plan(ch, G, n_kv_heads, sight, n_cu, cp);
+    if (rc) return rc;
+    const long long rows = q8 ? lay_dense(ch, sight) : 0;
+    FL_REQUIRE(rows >= 0, "too many cached rows for one int8 call");
+    const size_t part_b = up16(parts_bytes(cp.slots, n_kv_heads));
+    const size_t need = part_b + dense_bytes(rows, n_kv_heads);
+    if (need > 0) {
+        if (work == nullptr || work_bytes < need) {
+            fl::set_error("work: %zu bytes, fl_attention_prefill_paged_work_bytes asks %zu", work_bytes,
+                          need);
+            return FL_ESCRATCH;
+        }
+        FL_REQUIRE(aligned16(work), "16-byte aligned work");
+    }
+    rc = raise_lds();
+    if (rc) return rc;
+    const hipStream_t stream = (hipStream_t)stream_;
+    const size_t part_rows = (size_t)cp.slots * n_kv_heads * R64_BQ;
+    Parts parts = {(float*)work, nullptr, nullptr, cp.slots};
+    parts.pm = parts.pacc + part_rows * PF_HD;
+    parts.pd = parts.pm + part_rows;
+    const char *kc = (const char*)kpool, *vc = (const char*)vpool;
+    if (q8) {
+        char* copy = (char*)work + part_b;
+        char* copy_v = copy + dense_bytes(rows, n_kv_heads) / 2;
+        hipLaunchKernelGGL(paged_stage_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, kc,
+                           vc, pg, ch, sight, (f16x8*)copy, (f16x8*)copy_v, rows, n_kv_heads);
+        rc = fl::check_launch("attention_prefill_paged int8 copy");
+        if (rc) return rc;
+        kc = copy;
+        vc = copy_v;
+    }
+    auto kernel = q8 ? (cp.cut ? paged_prefill_kernel<true, true> : paged_prefill_kernel<true, false>)
+                     : (cp.cut ? paged_prefill_kernel<false, true> : paged_prefill_kernel<false, false>);
+    // a whole number of workgroups an XCD, so that its kv head's rows stay in one L2
+    const int per = 8 % n_kv_heads == 0 ? 8 / n_kv_heads : 1;
+    const int runs = (cp.plan.runs + per - 1) / per * per;
+    hipLaunchKernelGGL(kernel, dim3(runs * n_kv_heads), dim3(THREADS), R64_LDS, stream, (const f16*)q,
+                       q_pitch, kc, vc, pg, ch, (f16*)z, z_pitch, gated, n_q_heads, n_kv_heads,
+                       scale * FL_LOG2E, sight, cp.plan, parts);
+    rc = fl::check_launch("attention_prefill_paged");
+    if (rc || cp.tiles.n == 0) return rc;
+    hipLaunchKernelGGL(paged_piece_merge_kernel, dim3(cp.tiles.n * (R64_BQ / 4), n_kv_heads), dim3(256), 0,
+                       stream, parts, ch, cp.tiles, (f16*)z, z_pitch,
+                       gated ? (const f16*)q + PF_HD : nullptr, q_pitch, n_q_heads, n_kv_heads);
+    return fl::check_launch("attention_prefill_paged merge");
+}
+
+}  // extern "C"

@@ -36,6 +36,7 @@
 // kernel's. The reference dequantizes V the same way; its K stays fp32
 // (byte * scale exact), here it is rounded to fp16 once.
 #include "attn_pieces.hpp"
+#include "attn_r64.hpp"
 #include "fl_common.hpp"
 
 #include <algorithm>
@@ -59,79 +60,12 @@ constexpr int PF_WAVES = 4;
 constexpr int PF_THREADS = 64 * PF_WAVES;
 constexpr int PF_BQ = 32 * PF_WAVES;   // rows a workgroup
 constexpr int PF_BK = 64;              // kv rows a tile
-constexpr int ROW_B = PF_HD * 2;       // bytes a K / V row
 constexpr int TILE_B = PF_BK * ROW_B;  // 32 KiB
 constexpr int LDS_B = 4 * TILE_B;      // K stage 0 | K stage 1 | V stage 0 | V stage 1
 constexpr int V_OFF = 2 * TILE_B;
-// A column's running max only moves when a tile's max exceeds it by more
-// than this (log2 units): P = 2^(s - m) stays <= 256, exact in fp16 range,
-// and the O / l rescale is skipped on almost every tile.
-constexpr float RESCALE_LOG2 = 8.f;
-
 // f16_sat for this file's NaN-free arithmetic (-fno-honor-nans): one median
 __device__ __forceinline__ f16 z_sat(float v) {
     return (f16)__builtin_amdgcn_fmed3f(v, -65504.f, 65504.f);
-}
-
-// the chunk swizzle of tile row r: chunk c is stored at c ^ sw(r)
-__device__ __forceinline__ int sw(int r) { return ((r & 3) << 2) | ((r >> 2) & 3); }
-
-// The O^T accumulators live in AGPRs and are touched only through the asm
-// below. With compiler-generated MFMAs O would be either in VGPRs (leaving no
-// registers to read LDS ahead) or, in AGPRs, given a VGPR home because of the
-// rare rescale and copied out of the accumulators on every tile. Hazards the
-// compiler cannot see inside asm are covered here: s_nop 2 before each MFMA
-// (a VALU write of an A / B operand needs two wait states before the MFMA
-// reads it; without them the MFMA reads the register's previous contents),
-// s_nop 2 between a VALU result and v_accvgpr_write of it, and acc_settle()
-// before the accumulators are read (an MFMA result must leave the pipeline
-// before v_accvgpr_read; 24 wait states cover the 8-pass MFMA). MFMAs that
-// accumulate into the same registers back to back need no wait states.
-__device__ __forceinline__ void acc_zero(f32x16& acc, const f16x8& zero) {
-    asm volatile("s_nop 2\n\tv_mfma_f32_32x32x16_f16 %0, %1, %1, 0" : "=a"(acc) : "v"(zero));
-}
-__device__ __forceinline__ void acc_mfma(f32x16& acc, const f16x8& a, const f16x8& b) {
-    asm("s_nop 2\n\tv_mfma_f32_32x32x16_f16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
-}
-__device__ __forceinline__ void acc_settle(f32x16 (&o)[8]) {
-    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7"
-                 : "+a"(o[0]), "+a"(o[1]), "+a"(o[2]), "+a"(o[3]), "+a"(o[4]), "+a"(o[5]),
-                   "+a"(o[6]), "+a"(o[7]));
-}
-// a0..a3 *= c, on accumulator registers
-__device__ __forceinline__ void scale4_acc(float& a0, float& a1, float& a2, float& a3, float c) {
-    float t0, t1;
-    asm volatile(
-        "v_accvgpr_read_b32 %4, %0\n\t"
-        "v_accvgpr_read_b32 %5, %1\n\t"
-        "v_mul_f32 %4, %4, %6\n\t"
-        "v_mul_f32 %5, %5, %6\n\t"
-        "s_nop 2\n\t"
-        "v_accvgpr_write_b32 %0, %4\n\t"
-        "v_accvgpr_write_b32 %1, %5\n\t"
-        "v_accvgpr_read_b32 %4, %2\n\t"
-        "v_accvgpr_read_b32 %5, %3\n\t"
-        "v_mul_f32 %4, %4, %6\n\t"
-        "v_mul_f32 %5, %5, %6\n\t"
-        "s_nop 2\n\t"
-        "v_accvgpr_write_b32 %2, %4\n\t"
-        "v_accvgpr_write_b32 %3, %5"
-        : "+a"(a0), "+a"(a1), "+a"(a2), "+a"(a3), "=&v"(t0), "=&v"(t1)
-        : "v"(c));
-}
-__device__ __forceinline__ void acc_scale(f32x16 (&o)[8], float c) {
-    acc_settle(o);
-#pragma unroll
-    for (int mb = 0; mb < 8; ++mb)
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            float x0 = o[mb][e], x1 = o[mb][e + 1], x2 = o[mb][e + 2], x3 = o[mb][e + 3];
-            scale4_acc(x0, x1, x2, x3, c);
-            o[mb][e] = x0;
-            o[mb][e + 1] = x1;
-            o[mb][e + 2] = x2;
-            o[mb][e + 3] = x3;
-        }
 }
 
 // O^T[mb] += V^T P^T for the 16 kv rows of step KQ, output blocks 4 HALF..+3.
@@ -505,23 +439,6 @@ attn_prefill_kernel(const f16* __restrict__ q, int q_pitch, const void* __restri
     }
 }
 
-// One HBM -> LDS copy of 16 bytes a lane to LDS dst + IMM (+ 16 lane). m0 is
-// set inside the asm from a wave-uniform base and an immediate, so the
-// compiler keeps no per-copy LDS addresses in SGPRs (it would otherwise hoist
-// all of them out of the tile loop); the asm declares m0 as its output, and that
-// the s_add overwrites SCC: without that the compiler put a copy between the two
-// halves of a 64-bit address add (s_add_u32 .. s_addc_u32) and the carry was
-// lost, so a V cache whose rows cross a 4 GiB boundary of the address space was
-// read 4 GiB below it (a memory fault, or another allocation's bytes).
-template <int IMM>
-__device__ __forceinline__ void copy16_at(const char* sbase, uint32_t voff, uint32_t dst) {
-    uint32_t m0v;
-    asm volatile("s_add_u32 m0, %3, %4\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2"
-                 : "={m0}"(m0v)
-                 : "v"(voff), "s"(sbase), "s"(dst), "i"(IMM)
-                 : "scc");
-}
-
 // ---------------------------------------------------------------------------
 // fp16 cache, long prompts: 64 query rows a wave. A workgroup owns 256 rows
 // (4 waves x 64) of one kv head and walks the causal KV range in 32-row
@@ -543,17 +460,6 @@ __device__ __forceinline__ void copy16_at(const char* sbase, uint32_t voff, uint
 // lazy rescale, P rounded to fp16); 32-row tiles move the rescale points,
 // so the two kernels agree to rounding, not bit for bit.
 // ---------------------------------------------------------------------------
-constexpr int R64_BK = 32;                  // kv rows a tile
-constexpr int R64_TILE = R64_BK * ROW_B;    // 16 KiB: K (or V) of a tile
-constexpr int R64_STAGE = 2 * R64_TILE;     // K | V
-// Tiles copied ahead and K fragments read ahead: 2, 3 and 4 tiles and 2, 3
-// and 4 k-steps measured the same within noise at 8k and 32k.
-constexpr int R64_DIST = 3;
-constexpr int R64_KPF = 3;
-constexpr int R64_NST = R64_DIST + 1;
-constexpr int R64_LDS = R64_NST * R64_STAGE;   // 128 KiB at R64_DIST 3
-static_assert(R64_LDS <= 160 * 1024, "R64_DIST: LDS <= 160 KiB");
-constexpr int R64_COPIES = 8;               // copy instructions a wave a tile (4 K + 4 V)
 // the r64 kernel from this many workgroups up (T >= 4096 at 24 / 4 heads).
 // Same-box A/B, r64 against the 128-row kernel: 192 workgroups (T = 2048)
 // 156 against 100 us, 384 (T = 4096) 289-299 against 297-315 us, 480 (T =
@@ -640,17 +546,6 @@ __device__ __forceinline__ void r64_softmax(f32x16& s, bool diag, int lim, float
         pk[r >> 3][r & 7] = (f16)p;
     }
     l_run += pair32_sum(psum);
-}
-
-// The 8 V^T fragments (ds_read_b64_tr_b16) of PV step n: k-step kq = n / 2
-// (kv rows 16 kq ..), dim blocks 4 (n % 2) .. + 3; b: this lane's offsets
-// (the troff of attn_prefill_kernel).
-__device__ __forceinline__ void r64_vfrags(s16x4 (&vb)[8], const char* vt,
-                                           const uint32_t (&b)[8], int n) {
-    const int imm = 16 * ROW_B * (n >> 1) + 256 * (n & 1);
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        vb[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vt + b[i] + imm));
 }
 
 // R64_ROWS: whole row tiles, bins > 0 the persistent plan's lists or bins == 0 a
