@@ -102,6 +102,12 @@ __device__ __forceinline__ V stream_g(gptr base, uint32_t off) {   // read once:
     return __builtin_nontemporal_load((const __attribute__((address_space(1))) V*)(base + off));
 }
 
+// four values with f16_sat's range and NaNs, converted in pairs
+__device__ __forceinline__ f16x4 f16_sat4(f32x4 v) {
+    return __builtin_elementwise_maximum(
+        __builtin_elementwise_minimum(__builtin_convertvector(v, f16x4), (f16x4)(f16)65504.f),
+        (f16x4)(f16)-65504.f);
+}
 // sigmoid on the transcendental unit (about 2 ulp; 1 / (1 + e^-x), a NaN stays one)
 __device__ __forceinline__ float fast_sigmoid(float x) {
     return __builtin_amdgcn_rcpf(1.f + fast_exp2(x * -FL_LOG2E));

@@ -33,6 +33,7 @@ namespace {
 
 constexpr int MAX_SEQS = FL_PAGED_MAX_SEQS_PREFILL;
 constexpr int THREADS = 256;
+constexpr int OUT_ROWS = 8;    // rows whose gates are in flight when a row tile ends
 
 // Packed chunks: sequence b's tokens are start[b] .. start[b + 1] - 1, the first at
 // position pos0[b], its row tiles tile0[b] .. tile0[b + 1] - 1; dense[b]: its first row in
@@ -363,45 +364,88 @@ paged_prefill_kernel(const f16* __restrict__ q, int q_pitch, const char* __restr
             st = st == R64_NST - 1 ? 0 : st + 1;
         }
 
+        // O leaves through LDS, a 32-row block at a time in this wave's quarter of the
+        // stages, so that rows are written (and gates read) whole: chunk c (4 dims) of row r
+        // at c ^ 2 r. A cut row tile's rows go to its partial, a whole one's to z.
         acc_settle(o[0]);
         acc_settle(o[1]);
-        // a cut row tile leaves its partial, a whole one z (one walk over O for both: with
-        // two the compiler spills the accumulators)
+        tile_done();   // every wave is past its last tile
         const bool part = CUT && n_tiles < walk.n;
+        char* ob = smem + w * (R64_LDS / 4);
+        int oq = ql, ol = lane;   // (opaque: the addresses below would be hoisted out of the tile
+        asm volatile("" : "+v"(oq), "+v"(ol));   // loop and held in registers that it needs)
+        const int first = R0 + 64 * w, rows = min(64, RT - first);   // this wave's rows (uniform)
+        // the (token, q head) row of its rows, one after the other; past the last the last
+        int tt = uni(first / G), gg = first - tt * G, left = rows;
+        auto next_row = [&] {
+            const size_t rh = (size_t)(start + tt) * n_q_heads + h * G + gg;
+            if (--left > 0 && ++gg == G) gg = 0, ++tt;
+            return rh;
+        };
+        const size_t slot0 = (size_t)(slot + h * parts.n) * R64_BQ + 64 * w;
+        // gates are requested OUT_ROWS rows ahead of their use (no gate: one that is open)
+        f16x4 g_next[OUT_ROWS];
+        size_t rh_next[OUT_ROWS];
+        auto request = [&] {
+#pragma unroll
+            for (int i = 0; i < OUT_ROWS; ++i) {
+                rh_next[i] = next_row();
+                g_next[i] = (f16x4)((f16)65504.f);
+            }
+            if (gated && !part) {
+#pragma unroll
+                for (int i = 0; i < OUT_ROWS; ++i)
+                    g_next[i] = *(const f16x4*)(q + rh_next[i] * q_pitch + PF_HD + 4 * ol);
+            }
+        };
+        if (rows > 0) request();
 #pragma unroll
         for (int nb = 0; nb < 2; ++nb) {
-            if (!rvalid[nb]) continue;
-            const size_t at = (size_t)(slot + h * parts.n) * R64_BQ + 64 * w + 32 * nb + ql;
-            float* acc = parts.pacc + at * PF_HD + 4 * hh;
-            const float inv = l_run[nb] == 0.f ? 0.f : 1.f / l_run[nb];   // (no row seen: 0)
-            const size_t rh = (size_t)(start + t[nb]) * n_q_heads + h * G + g[nb];
-            f16* zrow = z + rh * z_pitch + 4 * hh;
-            const f16* grow = q + rh * q_pitch + PF_HD + 4 * hh;
-            if (part && hh == 0) {
-                parts.pm[at] = m_run[nb];
-                parts.pd[at] = l_run[nb];
-            }
+            const int n = min(32, rows - 32 * nb);   // (uniform)
+            if (n <= 0) break;
 #pragma unroll
             for (int mb = 0; mb < 8; ++mb)
 #pragma unroll
-                for (int r4 = 0; r4 < 4; ++r4) {
-                    const f32x4 v = {o[nb][mb][4 * r4], o[nb][mb][4 * r4 + 1], o[nb][mb][4 * r4 + 2],
-                                     o[nb][mb][4 * r4 + 3]};
-                    if (part) {
-                        *(f32x4*)(acc + 32 * mb + 8 * r4) = v;
-                        continue;
-                    }
-                    float f[4] = {inv, inv, inv, inv};
-                    if (gated) {
-                        const f16x4 gv = *(const f16x4*)(grow + 32 * mb + 8 * r4);
+                for (int r4 = 0; r4 < 4; ++r4)
+                    *(f32x4*)(ob + 1024 * oq + 16 * ((8 * mb + 2 * r4 + hh) ^ (2 * oq))) =
+                        (f32x4){o[nb][mb][4 * r4], o[nb][mb][4 * r4 + 1], o[nb][mb][4 * r4 + 2],
+                                o[nb][mb][4 * r4 + 3]};
+            if (part && lane < n) {   // (lanes 0 .. 31 hold the columns)
+                parts.pm[slot0 + 32 * nb + lane] = m_run[nb];
+                parts.pd[slot0 + 32 * nb + lane] = l_run[nb];
+            }
+            const float den = l_run[nb] == 0.f ? 1.f : l_run[nb];   // (no row seen: O is 0)
+#pragma unroll 1
+            for (int r0 = 0; r0 < n; r0 += OUT_ROWS) {
+                f32x4 v[OUT_ROWS];
+                float l[OUT_ROWS];
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) f[e] *= fast_sigmoid((float)gv[e]);
-                    }
-                    f16x4 out;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) out[e] = f16_sat(v[e] * f[e]);
-                    *(f16x4*)(zrow + 32 * mb + 8 * r4) = out;
+                for (int i = 0; i < OUT_ROWS; ++i) {
+                    const int r = min(r0 + i, n - 1);   // (past the last row: the last once more)
+                    v[i] = *(const f32x4*)(ob + 1024 * r + 16 * (ol ^ (2 * r)));
+                    l[i] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(den), r));
                 }
+                if (part) {
+#pragma unroll
+                    for (int i = 0; i < OUT_ROWS; ++i)
+                        *(f32x4*)(parts.pacc + (slot0 + 32 * nb + min(r0 + i, n - 1)) * PF_HD + 4 * ol) = v[i];
+                    continue;
+                }
+                f16x4 gv[OUT_ROWS];
+                size_t rh[OUT_ROWS];
+#pragma unroll
+                for (int i = 0; i < OUT_ROWS; ++i) gv[i] = g_next[i], rh[i] = rh_next[i];
+                request();
+#pragma unroll
+                for (int i = 0; i < OUT_ROWS; ++i) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {   // O / l sigmoid(g) = O / (l + l e^-g)
+                        const float x = fast_exp2(fmaf((float)gv[i][e], -FL_LOG2E, 0.f));
+                        v[i][e] *= __builtin_amdgcn_rcpf(fmaf(l[i], x, l[i]));
+                    }
+                    *(f16x4*)(z + rh[i] * z_pitch + 4 * ol) = f16_sat4(v[i]);
+                }
+            }
         }
         if (part) ++slot;
     }
@@ -496,9 +540,10 @@ int dense_rows(int T, int pos0, const Sight& sight) {
     return T == 0 ? 0 : R64_BK * make_walk(pos0, pos0 + T - 1, sight).n;
 }
 
-constexpr int ITEM_COST = 5;    // a row tile's fixed cost in tiles (Q, pipeline fill, z)
-constexpr int PIECE_COST = 8;   // a piece's (its 256 KiB partial)
-constexpr int PIECE_MIN = 6;    // tiles a piece, at least
+constexpr int ITEM_COST = 12;   // a row tile's fixed cost in tiles (Q, pipeline fill, z)
+constexpr int PIECE_COST = 8;  // a piece's (its 256 KiB partial)
+constexpr int PIECE_MIN = 2;    // tiles a piece, at least
+constexpr int RUN_MIN = 6;      // a run's cost, at least
 constexpr int MERGE_COST = 2;         // the merge's launch, in tiles
 constexpr int SLOTS_PER_TILE = 40;    // partials the merge reads in a tile's time
 
@@ -523,17 +568,17 @@ void walks(const Chunks& ch, int G, const Sight& sight, std::vector<int>& n) {
 long long cut_plan(const std::vector<int>& n, int n_kv, int most, CallPlan& cp) {
     const int N = (int)n.size();
     long long total = 0;
-    for (int x : n) total += x + PIECE_COST;
+    for (int x : n) total += x + ITEM_COST;
     const int runs = (int)std::max<long long>(
-        1, std::min<long long>(most, total / (PIECE_COST + 2 * PIECE_MIN)));
+        1, std::min<long long>(most, total / RUN_MIN));
     Plan& p = cp.plan;
     p.runs = runs;
     int tile = 0;
     long long before = 0;   // cost of the row tiles ahead of `tile`
     for (int r = 0; r <= runs; ++r) {
         const long long u = r == runs ? total : total * r / runs;
-        while (tile < N && before + n[tile] + PIECE_COST <= u) before += n[tile++] + PIECE_COST;
-        int j = tile < N ? (int)std::max<long long>(0, u - before - PIECE_COST) : 0;
+        while (tile < N && before + n[tile] + ITEM_COST <= u) before += n[tile++] + ITEM_COST;
+        int j = tile < N ? (int)std::max<long long>(0, u - before - ITEM_COST) : 0;
         int t = tile;
         if (j < PIECE_MIN) j = 0;
         else if (n[t] - j < PIECE_MIN) ++t, j = 0;
