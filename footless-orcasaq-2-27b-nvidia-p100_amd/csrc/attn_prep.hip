@@ -45,6 +45,34 @@ constexpr int PR_HD = 256;
 constexpr int PR_WAVES = 4;
 constexpr int PR_MAXPAIRS = PR_HD / 2;
 
+// The sum of squares of a row (4 elements a lane), on every lane, in the reference's order
+// (the file's head): the trees of the four elements c of a warp's 8 lanes are folded into
+// one -- after the exchange at distance 4 a lane keeps two of them, after that at 2 one --
+// so 6 exchanges do where one tree an element takes 12; then the warps' sums as butterflies
+// at distance 32, 16 and 8. Every addition has the reference's two operands (+ is
+// commutative), so the sum has its bits.
+__device__ __forceinline__ float row_sum_sq(f16x4 y, int lane) {
+    auto xor4 = [](float v) {   // within 4 reversed, then within 8
+        return __int_as_float(__builtin_amdgcn_mov_dpp(
+            __builtin_amdgcn_mov_dpp(__float_as_int(v), 0x1B, 0xF, 0xF, true), 0x141, 0xF, 0xF, true));
+    };
+    float sq[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) sq[c] = fmaf((float)y[c], (float)y[c], 0.f);
+    const bool b4 = lane & 4, b2 = lane & 2;
+    const float a0 = (b4 ? sq[2] : sq[0]) + xor4(b4 ? sq[0] : sq[2]);   // offset 16
+    const float a1 = (b4 ? sq[3] : sq[1]) + xor4(b4 ? sq[1] : sq[3]);
+    float s = (b2 ? a1 : a0) + dpp_xor2(b2 ? a0 : a1);                   // offset 8
+    s += dpp_xor1(s);                                                    // offset 4
+    s += xor4(s);                                                        // offset 2: (0, 2), (1, 3)
+    s += dpp_xor2(s);                                                    // offset 1
+    s = pair32_sum(s);
+    const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(s), __float_as_uint(s), false, false);
+    s = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    s += __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(s), 0x128, 0xF, 0xF, true));   // row_ror 8
+    return s;
+}
+
 // The rotation's frequencies theta^(-2j / rope_dim), j < rope_dim / 2, in
 // fp64: they do not depend on the position, so the host forms them once per
 // (theta, rope_dim) and they ride in the kernel arguments.
@@ -84,7 +112,7 @@ attn_prep_kernel(const f16* q, f16* qo, int q_pitch, f16* k, int k_pitch,
                  int n_q_heads, int n_kv_heads, int pos0, int max_pos_, int rope_dim,
                  const RopeFreqs freqs, float eps,
                  const typename std::conditional<PAGED, PrepPaged, PrepRows>::type rows) {
-    __shared__ float scs[PR_MAXPAIRS], ssn[PR_MAXPAIRS];
+    __shared__ __attribute__((aligned(16))) float scs[PR_MAXPAIRS], ssn[PR_MAXPAIRS];
     __shared__ __attribute__((aligned(16))) f16 srow[PR_WAVES][PR_HD];
     constexpr bool NORM = FLAGS & 1, ROPE = FLAGS & 2, STORE = FLAGS & 4, Q8 = FLAGS & 8;
     const int t = blockIdx.x, hd0 = blockIdx.y * PR_WAVES * RPW;
@@ -117,56 +145,60 @@ attn_prep_kernel(const f16* q, f16* qo, int q_pitch, f16* k, int k_pitch,
         __syncthreads();
     }
     const int heads = n_q_heads + n_kv_heads;
-    f16x4 yin[RPW];
+    // the wave's rows (past the last head: the last one again, not stored)
+    auto head_of = [&](int r) { return min(hd0 + w + PR_WAVES * r, heads - 1); };
+    auto offset_of = [&](int hd) {
+        return hd < n_q_heads ? ((size_t)t * n_q_heads + hd) * q_pitch
+                              : ((size_t)t * n_kv_heads + hd - n_q_heads) * k_pitch;
+    };
+    if (hd0 + w >= heads) return;   // wave-uniform
+    f16x4 y[RPW];
 #pragma unroll
     for (int r = 0; r < RPW; ++r) {
-        const int hd = hd0 + w + PR_WAVES * r;
-        if (hd >= heads) break;
-        const bool is_q = hd < n_q_heads;
-        const size_t roff = is_q ? ((size_t)t * n_q_heads + hd) * q_pitch
-                                 : ((size_t)t * n_kv_heads + hd - n_q_heads) * k_pitch;
-        yin[r] = *(const f16x4*)((is_q ? q : k) + roff + 4 * lane);
+        const int hd = head_of(r);
+        y[r] = *(const f16x4*)((hd < n_q_heads ? q : k) + offset_of(hd) + 4 * lane);
     }
+    if (NORM) {
+        // every row's sum of squares on every lane; then the square roots and divides of
+        // all rows at once, row r's on lane r
+        float ss[RPW];
 #pragma unroll
-    for (int r = 0; r < RPW; ++r) {
-        const int hd = hd0 + w + PR_WAVES * r;
-        if (hd >= heads) break;
-        const bool is_q = hd < n_q_heads;
-        const int h = is_q ? hd : hd - n_q_heads;
-        const size_t roff = is_q ? ((size_t)t * n_q_heads + h) * q_pitch
-                                 : ((size_t)t * n_kv_heads + h) * k_pitch;
-        f16* orow = is_q ? qo + roff : k + roff;   // q rows may go elsewhere; k in place
-        if constexpr (PAGED)
-            if (is_q) orow = qo + ((size_t)t * n_q_heads + h) * rows.qo_pitch;
-        f16x4 y = yin[r];
-        if (NORM) {
-            float x[4], sq[4];
+        for (int r = 0; r < RPW; ++r) ss[r] = row_sum_sq(y[r], lane);
+        float mine = ss[0];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                x[c] = (float)y[c];
-                sq[c] = fmaf(x[c], x[c], 0.f);
-            }
+        for (int r = 1; r < RPW; ++r) mine = lane == r ? ss[r] : mine;
+        const float inv = 1.f / sqrtf(mine / (float)PR_HD + eps);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                sq[c] += lane_xor(sq[c], 4);   // offset 16
-                sq[c] += dpp_xor2(sq[c]);      // offset 8
-                sq[c] += dpp_xor1(sq[c]);      // offset 4
-            }
-            const float ws = (sq[0] + sq[2]) + (sq[1] + sq[3]);   // offsets 2, 1: lane 8 w' = warp w'
-            auto at = [](float val, int src) {
-                return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(val), src));
-            };
-            const float r0 = at(ws, 0), r1 = at(ws, 8), r2 = at(ws, 16), r3 = at(ws, 24);
-            const float r4 = at(ws, 32), r5 = at(ws, 40), r6 = at(ws, 48), r7 = at(ws, 56);
-            const float ss = ((r0 + r4) + (r2 + r6)) + ((r1 + r5) + (r3 + r7));
-            const float inv = 1.f / sqrtf(ss / (float)PR_HD + eps);
-            const f32x4 w4 = *(const f32x4*)((is_q ? wq : wk) + 4 * lane);
+        for (int r = 0; r < RPW; ++r) {
+            const float inv_r = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(inv), r));
+            const f32x4 w4 = *(const f32x4*)((head_of(r) < n_q_heads ? wq : wk) + 4 * lane);
 #pragma unroll
-            for (int c = 0; c < 4; ++c) y[c] = f16_sat(x[c] * inv * (1.f + w4[c]));
+            for (int c = 0; c < 4; ++c) y[r][c] = f16_sat((float)y[r][c] * inv_r * (1.f + w4[c]));
         }
-        if (ROPE) {
-            f16* sr = srow[w];
-            *(f16x4*)(sr + 4 * lane) = y;
+    }
+    if (ROPE && rope_dim == 64) {
+        // dims 4 l + c, l < 16: pair (j, j + 32) is lanes l and l ^ 8
+        const f32x4 cs = *(const f32x4*)(scs + 4 * (lane & 7)), sn = *(const f32x4*)(ssn + 4 * (lane & 7));
+#pragma unroll
+        for (int r = 0; r < RPW; ++r) {
+            const u32x2 own = __builtin_bit_cast(u32x2, y[r]);
+            u32x2 other;
+#pragma unroll
+            for (int d = 0; d < 2; ++d)   // row_ror 8
+                other[d] = (uint32_t)__builtin_amdgcn_mov_dpp((int)own[d], 0x128, 0xF, 0xF, true);
+            const f16x4 o = __builtin_bit_cast(f16x4, other);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const float xs = (float)o[c] * sn[c];
+                const float rot = (float)y[r][c] * cs[c] + (lane < 8 ? -xs : xs);
+                y[r][c] = lane < 16 ? f16_sat(rot) : y[r][c];
+            }
+        }
+    } else if (ROPE) {
+        f16* sr = srow[w];
+#pragma unroll
+        for (int r = 0; r < RPW; ++r) {
+            *(f16x4*)(sr + 4 * lane) = y[r];
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -180,22 +212,33 @@ attn_prep_kernel(const f16* q, f16* qo, int q_pitch, f16* k, int k_pitch,
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-            y = *(const f16x4*)(sr + 4 * lane);
+            y[r] = *(const f16x4*)(sr + 4 * lane);
             // the slice is rewritten by the wave's next row only after every
             // lane has read it back (in-order LDS within the wave)
         }
-        if ((NORM || ROPE) && (is_q || !PAGED)) *(f16x4*)(orow + 4 * lane) = y;
+    }
+#pragma unroll
+    for (int r = 0; r < RPW; ++r) {
+        const int hd = hd0 + w + PR_WAVES * r;
+        if (hd >= heads) break;
+        const bool is_q = hd < n_q_heads;
+        const int h = is_q ? hd : hd - n_q_heads;
+        // q rows may go elsewhere; k in place
+        f16* orow = is_q ? qo + offset_of(hd) : k + offset_of(hd);
+        if constexpr (PAGED)
+            if (is_q) orow = qo + ((size_t)t * n_q_heads + h) * rows.qo_pitch;
+        if ((NORM || ROPE) && (is_q || !PAGED)) *(f16x4*)(orow + 4 * lane) = y[r];
         if (STORE && !is_q && (!PAGED || cache_row >= 0)) {
             const f16x4 vin = *(const f16x4*)(v + ((size_t)t * n_kv_heads + h) * PR_HD + 4 * lane);
             const size_t crow = (size_t)cache_row * n_kv_heads + h;
             if constexpr (Q8) {
                 const size_t vals = (size_t)max_pos * n_kv_heads * PR_HD;   // scales follow
-                q8_store_row(y, (signed char*)kc + crow * PR_HD,
+                q8_store_row(y[r], (signed char*)kc + crow * PR_HD,
                              (f16*)((signed char*)kc + vals) + crow * 8, lane);
                 q8_store_row(vin, (signed char*)vc + crow * PR_HD,
                              (f16*)((signed char*)vc + vals) + crow * 8, lane);
             } else {
-                *(f16x4*)((f16*)kc + crow * PR_HD + 4 * lane) = y;
+                *(f16x4*)((f16*)kc + crow * PR_HD + 4 * lane) = y[r];
                 *(f16x4*)((f16*)vc + crow * PR_HD + 4 * lane) = vin;
             }
         }

@@ -10,6 +10,8 @@
 // 32-dim block is a quad of lanes and its absmax two DPP exchanges.
 #include "kv_pages.hpp"
 
+#include <math.h>
+
 using fl::Pages;
 using fl::PAGED_HD;
 
@@ -17,20 +19,39 @@ namespace {
 
 constexpr int PG_WAVES = 4;            // tokens a workgroup
 constexpr int CHUNKS = PAGED_HD / 8;   // 8-dim chunks a head row
+constexpr int STEP = 2;                // chunks of K and of V that a lane has in flight
 
-// 8 halves of a 32-dim block (4 lanes) in the int8 format
+// x / d for d > 0 with r about 1 / d: the product and one correction of it. An exact
+// quotient comes out exact, any other within 2 ulp.
+__device__ __forceinline__ float div_near(float x, float d, float r) {
+    const float q = x * r;
+    return fmaf(fmaf(-q, d, x), r, q);
+}
+
+// 8 halves of a 32-dim block (4 lanes) in the int8 format, q8_store_row's values. The
+// correctly rounded divisions there are most of a store's instructions and are not needed:
+// x and the scale s are fp16, so x / s (at most 127.1) is a half integer exactly or at
+// least 2^-13 away from one (|2x - (2n + 1) s| is a multiple of the smaller of their units,
+// and x >= s / 4 there), far more than div_near's error, and rint takes the same side. So
+// is absmax / 127, rounded to fp16: 127 t is no multiple of any unit near it unless exact.
 __device__ __forceinline__ void q8_put(f16x8 x, signed char* vals, f16* scale, bool first) {
-    float a = 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) a = fmaxf(a, fabsf((float)x[e]));
+    f16x8 m = __builtin_elementwise_abs(x);
+    f16x4 m4 = __builtin_elementwise_max((f16x4){m[0], m[1], m[2], m[3]}, (f16x4){m[4], m[5], m[6], m[7]});
+    float a = fmaxf(fmaxf((float)m4[0], (float)m4[1]), fmaxf((float)m4[2], (float)m4[3]));
     a = fmaxf(a, dpp_xor1(a));
     a = fmaxf(a, dpp_xor2(a));
-    const f16 sh = q8_scale(a);
+    const f16 sh = (f16)(a < INFINITY ? div_near(a, 127.f, 1.f / 127.f) : a);
+    const bool on = sh > (f16)0.f;
+    const float r = on ? __builtin_amdgcn_rcpf((float)sh) : 0.f;
+    const float s = (float)sh < INFINITY ? (float)sh : 0.f;   // (an infinite scale: x / inf = 0)
     u32x2 packed = {0, 0};
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-        packed[e >> 2] |= (uint32_t)(q8_value((float)x[e], (float)sh) & 0xff) << (8 * (e & 3));
-    *(u32x2*)vals = packed;
+    for (int e = 0; e < 8; ++e) {
+        const float v = (float)x[e];
+        const int n = (int)__builtin_amdgcn_fmed3f(rintf(div_near(v, s, r)), -127.f, 127.f);
+        packed[e >> 2] |= (uint32_t)(n & 0xff) << (8 * (e & 3));
+    }
+    *(u32x2*)vals = on ? packed : (u32x2){0, 0};
     if (first) *scale = sh;
 }
 
@@ -73,16 +94,33 @@ paged_store_kernel(const f16* __restrict__ k, const f16* __restrict__ v, long lo
                    int B, int N, int n_kv) {
     const int i = blockIdx.x * PG_WAVES + (threadIdx.x >> 6), lane = threadIdx.x & 63;
     if (i >= N) return;                                   // wave-uniform
+    // the first STEP chunks' loads run while the page is looked up
+    const int chunks = n_kv * CHUNKS;
+    const f16 *ki = k + i * k_stride, *vi = v + i * v_stride;
+    f16x8 kx[STEP], vx[STEP];
+    auto load = [&](int c0) {
+#pragma unroll
+        for (int u = 0; u < STEP; ++u) {
+            const int c = c0 + 64 * u;
+            if (c < chunks) kx[u] = *(const f16x8*)(ki + 8 * c), vx[u] = *(const f16x8*)(vi + 8 * c);
+        }
+    };
+    load(lane);
     const int seq = fl::seq_of(starts, B, i);
     if (seq >= B || i < starts[seq]) return;              // outside every sequence
     const long long pos = (long long)pos0[seq] + (i - starts[seq]);
     const long long row = pos < 0 || pos > INT_MAX ? -1 : fl::page_row(pg, seq, (int)pos);
     if (row < 0) return;
-    for (int c = lane; c < n_kv * CHUNKS; c += 64) {
-        const f16x8 kx = *(const f16x8*)(k + i * k_stride + 8 * c);
-        const f16x8 vx = *(const f16x8*)(v + i * v_stride + 8 * c);
-        put_chunk<Q8>(kpool, pg, n_kv, row, c, kx);
-        put_chunk<Q8>(vpool, pg, n_kv, row, c, vx);
+    for (int c0 = lane; c0 < chunks; c0 += 64 * STEP) {
+        if (c0 != lane) load(c0);
+#pragma unroll
+        for (int u = 0; u < STEP; ++u) {
+            const int c = c0 + 64 * u;
+            if (c < chunks) {
+                put_chunk<Q8>(kpool, pg, n_kv, row, c, kx[u]);
+                put_chunk<Q8>(vpool, pg, n_kv, row, c, vx[u]);
+            }
+        }
     }
 }
 

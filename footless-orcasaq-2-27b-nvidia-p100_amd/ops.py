@@ -23,10 +23,10 @@ import torch
 from . import _lib
 from .geometry import (ATTN_SCALE, DEC_SMAX, DEC_SPLIT_ROWS, DEC_TMIN, GATE_OFF, GDN_CHUNK,
                        GDN_GROUP, GDN_K, GDN_K_HEADS, GDN_NORM_EPS, GDN_V, GDN_V_HEADS, HEAD_DIM,
-                       L2_EPS, LOG2E, N_HEADS, N_KV, NORM_EPS, Q_PITCH, Q_SCALE, QKV_ROWS, ROPE_DIM,
+                       KV8_ROW, L2_EPS, LOG2E, N_HEADS, N_KV, NORM_EPS, Q_PITCH, Q_SCALE, QKV_ROWS, ROPE_DIM,
                        ROPE_THETA, SPLIT_MAX, SPLIT_ROWS, kv8_nbytes)
 
-F16, F32, I8 = torch.float16, torch.float32, torch.int8
+F16, F32, I8, I32 = torch.float16, torch.float32, torch.int8, torch.int32
 
 
 # The current stream's handle without building a torch.cuda.Stream around it
@@ -558,63 +558,109 @@ def paged_pool(n_pages: int, page_size: int, *, kv8: bool = False, n_kv_heads: i
     return torch.zeros((n_pages, page_size, n_kv_heads, head_dim), dtype=F16, device=device)
 
 
-def _paged(kpool, vpool, pages, page_size, B, n_kv_heads, head_dim):
+# The checks of a paged call are one expression a group of tensors where they hold
+# (a decode step makes three such calls a layer); what fails is looked for afterwards.
+
+def _here():
+    """The current device's index (-2 without a GPU: no tensor's)."""
+    try:
+        return torch.cuda.current_device() if _device_index is None else _device_index()
+    except (RuntimeError, AssertionError):
+        return -2
+
+
+def _paged(kpool, vpool, pages, page_size, B, n_kv_heads, head_dim, dev):
     """(kpool, vpool, q8, n_pages, page_size, pages, max_pages, pages_stride) of a
-    paged call after checking that the pools and the table are what it says."""
+    paged call after checking that the pools and the table are what it says, on
+    device `dev` (the current one: the launches go on its stream)."""
+    try:
+        q8 = kpool.dtype is I8
+        if q8:
+            unit, size = page_size * n_kv_heads * KV8_ROW, kpool.numel()
+            n_pages = size // unit
+            ok = n_pages * unit == size == vpool.numel() and vpool.dtype is I8
+        else:
+            shape = kpool.shape
+            n_pages = shape[0]
+            ok = (shape == (n_pages, page_size, n_kv_heads, head_dim) and vpool.shape == shape
+                  and kpool.dtype is F16 and vpool.dtype is F16)
+        rows, max_pages = pages.shape
+        stride, step = pages.stride()
+        if (ok and rows == B and (step == 1 or max_pages == 1) and pages.dtype is I32
+                and kpool.is_contiguous() and vpool.is_contiguous() and head_dim == HEAD_DIM
+                and kpool.get_device() == vpool.get_device() == pages.get_device() == dev):
+            return (kpool.data_ptr(), vpool.data_ptr(), int(q8), n_pages, page_size,
+                    pages.data_ptr(), max_pages, stride if B > 1 else max_pages)
+    except (AttributeError, ValueError, IndexError, TypeError, ZeroDivisionError):
+        pass
+    _refuse_paged(kpool, vpool, pages, page_size, B, n_kv_heads, head_dim, dev)
+
+
+def _refuse_paged(kpool, vpool, pages, page_size, B, n_kv_heads, head_dim, dev):
     for name, c in (("kpool", kpool), ("vpool", vpool), ("pages", pages)):
         if not isinstance(c, torch.Tensor):
             raise TypeError(f"{name}: expected a torch.Tensor, got {type(c).__name__}")
     if page_size < 1 or n_kv_heads < 1 or head_dim != HEAD_DIM:
         raise ValueError("page_size and n_kv_heads must be positive, head_dim 256")
-    q8 = kpool.dtype == I8
-    if q8:
-        n_pages = kpool.numel() // kv8_nbytes(page_size, n_kv_heads, head_dim)
-        need = kv8_nbytes(n_pages * page_size, n_kv_heads, head_dim)
-        if kpool.numel() != need or vpool.numel() != need:
-            raise ValueError("kpool, vpool: not a whole number of pages, or not the same number")
-    else:
-        n_pages = kpool.shape[0]
-        shape = (n_pages, page_size, n_kv_heads, head_dim)
-        if tuple(kpool.shape) != shape or tuple(vpool.shape) != shape:
-            raise ValueError(f"kpool, vpool: shapes {tuple(kpool.shape)} and {tuple(vpool.shape)}, "
-                             f"expected [n_pages, {page_size}, {n_kv_heads}, {head_dim}]")
-        need = kpool.numel()
-    dtype = I8 if q8 else F16
-    kp, vp = _dense_ptr(kpool, dtype, "kpool", need), _dense_ptr(vpool, dtype, "vpool", need)
+    for name, c in (("kpool", kpool), ("vpool", vpool)):
+        if c.dtype not in (F16, I8) or c.dtype != kpool.dtype:
+            raise TypeError(f"{name}: dtype {c.dtype}, the pools are both fp16 or both int8")
+        if c.dtype == F16 and (c.dim() != 4 or tuple(c.shape) != (kpool.shape[0], page_size, n_kv_heads,
+                                                                  head_dim)):
+            raise ValueError(f"{name}: shape {tuple(c.shape)}, expected [n_pages, {page_size}, "
+                             f"{n_kv_heads}, {head_dim}]")
+        if c.dtype == I8 and (c.numel() % (page_size * n_kv_heads * KV8_ROW)
+                              or c.numel() != kpool.numel()):
+            raise ValueError(f"{name}: not a whole number of pages, or not the same number")
+        _contig(c, name)
+    if pages.dtype != I32:
+        raise TypeError(f"pages: dtype {pages.dtype}, expected {I32}")
     if pages.dim() != 2 or pages.shape[0] != B or (pages.stride(1) != 1 and pages.shape[1] > 1):
         raise ValueError(f"pages: expected rows of page ids for {B} sequences")
-    stride = pages.stride(0) if B > 1 else pages.shape[1]
-    return (kp, vp, int(q8), n_pages, page_size,
-            _ptr(pages, torch.int32, "pages", (B - 1) * stride + pages.shape[1]), pages.shape[1],
-            stride)
+    _same_device(dev, kpool=kpool, vpool=vpool, pages=pages)
+    raise ValueError("kpool, vpool, pages: not a paged cache")
 
 
-def _one_device(**tensors):
-    """Every tensor on the current device: the launches go on its stream."""
-    here = torch.cuda.current_device() if _device_index is None else _device_index()
+def _same_device(dev, **tensors):
+    """Every tensor on the current device."""
     for name, t in tensors.items():
-        if t is not None and t.is_cuda and t.device.index != here:
-            raise ValueError(f"{name}: on {t.device}, the current device is cuda:{here}")
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise ValueError(f"{name}: must be a GPU tensor (got {t.device})")
+        if t.get_device() != dev:
+            raise ValueError(f"{name}: on {t.device}, the current device is cuda:{dev}")
 
 
-def _packed(starts, pos0):
+def _packed(starts, pos0, dev):
     """(starts, pos0, B) of packed tokens."""
     if not isinstance(starts, torch.Tensor) or not isinstance(pos0, torch.Tensor):
         raise TypeError("starts, pos0: expected torch tensors")
     B = pos0.numel()
+    if (starts.dtype is I32 and pos0.dtype is I32 and starts.dim() == pos0.dim() == 1
+            and starts.numel() == B + 1 and starts.is_contiguous() and pos0.is_contiguous()
+            and starts.get_device() == pos0.get_device() == dev):
+        return starts.data_ptr(), pos0.data_ptr(), B
     if pos0.dim() != 1 or starts.dim() != 1 or starts.numel() != B + 1:
         raise ValueError("starts: one entry more than pos0, both one-dimensional")
-    return (_dense_ptr(starts, torch.int32, "starts", B + 1),
-            _dense_ptr(pos0, torch.int32, "pos0", B), B)
+    _dense_ptr(starts, I32, "starts", B + 1), _dense_ptr(pos0, I32, "pos0", B)
+    _same_device(dev, starts=starts, pos0=pos0)
 
 
-def _token_rows(t, name, heads, width):
-    """Token stride of a [N, heads, width] tensor whose tokens are dense."""
-    if t.dim() != 3 or tuple(t.shape[1:]) != (heads, width):
-        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected [N, {heads}, {width}]")
-    if t.shape[0] and not t[0].is_contiguous():
+def _token_rows(t, name, N, heads, width, dev):
+    """(pointer, token stride) of a [N, heads, width] fp16 tensor whose tokens are
+    dense (any token stride)."""
+    if (t.shape == (N, heads, width) and t.dtype is F16 and t.is_contiguous()
+            and t.get_device() == dev):
+        return t.data_ptr(), heads * width
+    if t.dim() != 3 or tuple(t.shape) != (N, heads, width):
+        raise ValueError(f"{name}: shape {tuple(t.shape)}, expected [{N}, {heads}, {width}]")
+    if N and not t[0].is_contiguous():
         raise ValueError(f"{name}: a token's rows must be contiguous")
-    return t.stride(0) if t.shape[0] > 1 else heads * width
+    stride = t.stride(0) if N > 1 else heads * width
+    p = _ptr(t, F16, name, max(0, N - 1) * stride + heads * width if N else 0)
+    _same_device(dev, **{name: t})
+    return p, stride
 
 
 def paged_kv_store(k, v, kpool, vpool, pages, starts, pos0, *, page_size: int,
@@ -622,19 +668,15 @@ def paged_kv_store(k, v, kpool, vpool, pages, starts, pos0, *, page_size: int,
     """kv_store / kv_store_q8 into pages: the rows of packed tokens k, v [N, n_kv,
     head_dim] fp16 (any token stride that is a multiple of 8) to their sequences'
     positions. Tokens outside every sequence are not stored."""
-    sp, pp, B = _packed(starts, pos0)
+    dev = _here()
+    sp, pp, B = _packed(starts, pos0, dev)
     N = k.shape[0]
-    if v.shape[0] != N:
-        raise ValueError("k and v: not the same number of tokens")
-    ks, vs = (_token_rows(t, n, n_kv_heads, head_dim) for t, n in ((k, "k"), (v, "v")))
-    row = n_kv_heads * head_dim
-    pg = _paged(kpool, vpool, pages, page_size, B, n_kv_heads, head_dim)
-    _one_device(k=k, v=v, kpool=kpool, vpool=vpool, pages=pages, starts=starts, pos0=pos0)
-    if N == 0:
-        return
-    _lib.call("fl_paged_kv_store", _ptr(k, F16, "k", (N - 1) * ks + row),
-              _ptr(v, F16, "v", (N - 1) * vs + row), ks, vs, *pg, sp, pp, B, N, n_kv_heads, head_dim,
-              _stream())
+    kp, ks = _token_rows(k, "k", N, n_kv_heads, head_dim, dev)
+    vp, vs = _token_rows(v, "v", N, n_kv_heads, head_dim, dev)
+    pg = _paged(kpool, vpool, pages, page_size, B, n_kv_heads, head_dim, dev)
+    if N:
+        _lib.call("fl_paged_kv_store", kp, vp, ks, vs, *pg, sp, pp, B, N, n_kv_heads, head_dim,
+                  _stream())
 
 
 def paged_kv_load(kpool, vpool, pages, starts, pos0, *, T: int, page_size: int, k=None, v=None,
@@ -642,23 +684,22 @@ def paged_kv_load(kpool, vpool, pages, starts, pos0, *, T: int, page_size: int, 
     """Cached rows back from their pages: k, v [T, n_kv, head_dim] fp16 (new unless
     given), int8 rows as fp16(byte * scale), rows of absent pages as zeros. Rows
     outside every sequence are left as they are (zeros in new tensors)."""
-    sp, pp, B = _packed(starts, pos0)
+    dev = _here()
+    sp, pp, B = _packed(starts, pos0, dev)
     if T < 0 or (k is None) != (v is None):
         raise ValueError("T >= 0, k and v given both or neither")
-    pg = _paged(kpool, vpool, pages, page_size, B, n_kv_heads, head_dim)
-    new = k is None
-    if new:
-        k, v = (torch.empty((T, n_kv_heads, head_dim), dtype=F16, device=kpool.device)
-                for _ in range(2))
-    if k.shape[0] != T or v.shape[0] != T:
-        raise ValueError(f"k and v: expected {T} tokens")
-    ks, vs = (_token_rows(t, n, n_kv_heads, head_dim) for t, n in ((k, "k"), (v, "v")))
-    _one_device(k=k, v=v, kpool=kpool, vpool=vpool, pages=pages, starts=starts, pos0=pos0)
-    if T > 0:
-        row = n_kv_heads * head_dim
-        _lib.call("fl_paged_kv_load", *pg, sp, pp, _ptr(k, F16, "k", (T - 1) * ks + row),
-                  _ptr(v, F16, "v", (T - 1) * vs + row), ks, vs, int(new), B, T, n_kv_heads,
-                  head_dim, _stream())
+    pg = _paged(kpool, vpool, pages, page_size, B, n_kv_heads, head_dim, dev)
+    if k is None:
+        k, v = torch.empty((2, T, n_kv_heads, head_dim), dtype=F16, device=kpool.device).unbind(0)
+        ks = vs = n_kv_heads * head_dim
+        kp, vp, new = k.data_ptr(), v.data_ptr(), 1
+    else:
+        kp, ks = _token_rows(k, "k", T, n_kv_heads, head_dim, dev)
+        vp, vs = _token_rows(v, "v", T, n_kv_heads, head_dim, dev)
+        new = 0
+    if T:
+        _lib.call("fl_paged_kv_load", *pg, sp, pp, kp, vp, ks, vs, new, B, T, n_kv_heads, head_dim,
+                  _stream())
     return k, v
 
 
@@ -672,39 +713,36 @@ def attn_prep_paged(qg, k, v, wq, wk, kpool, vpool, pages, starts, pos0, *, page
     and v [N, n_kv, head_dim] -- those calls' values bit for bit. q is rewritten in
     place, or goes to q_out [N, n_q_heads, pitch]; k is not rewritten. Returns
     the tensor that holds q."""
-    sp, pp, B = _packed(starts, pos0)
+    dev = _here()
+    sp, pp, B = _packed(starts, pos0, dev)
     N, heads, q_pitch = qg.shape
-    if heads != n_q_heads or tuple(k.shape) != (N, n_kv_heads, head_dim) or k.shape != v.shape:
+    if heads != n_q_heads or k.shape != (N, n_kv_heads, head_dim) or v.shape != k.shape:
         raise ValueError("qg [N, n_q_heads, q_pitch], k and v [N, n_kv_heads, head_dim]")
-    for name, t in (("qg", qg), ("k", k), ("v", v)):
-        _contig(t, name)
     qo, qo_pitch = None, 0
     if q_out is not None:
-        _contig(q_out, "q_out")
-        if q_out.dim() != 3 or tuple(q_out.shape[:2]) != (N, n_q_heads):
+        if q_out.dim() != 3 or q_out.shape[0] != N or q_out.shape[1] != n_q_heads:
             raise ValueError(f"q_out: expected [{N}, {n_q_heads}, pitch]")
-        qo_pitch = q_out.shape[-1]
-    pg = _paged(kpool, vpool, pages, page_size, B, n_kv_heads, head_dim)
-    _one_device(qg=qg, k=k, v=v, wq=wq, wk=wk, q_out=q_out, kpool=kpool, vpool=vpool, pages=pages,
-                starts=starts, pos0=pos0)
-    if N > 0:
-        row = n_kv_heads * head_dim
-        if q_out is not None:
-            qo = _ptr(q_out, F16, "q_out", N * n_q_heads * qo_pitch)
-        _lib.call("fl_attn_prep_paged", _ptr(qg, F16, "qg", N * n_q_heads * q_pitch), q_pitch,
-                  _ptr(k, F16, "k", N * row), _ptr(v, F16, "v", N * row),
-                  _ptr(wq, F32, "wq", head_dim), _ptr(wk, F32, "wk", head_dim), qo, qo_pitch, *pg, sp,
-                  pp, B, N, n_q_heads, n_kv_heads, head_dim, rope_dim, float(theta), float(eps),
-                  _stream())
+        qo_pitch = q_out.shape[2]
+        qo = _dense_ptr(q_out, F16, "q_out", N * n_q_heads * qo_pitch)
+    ptrs = (_dense_ptr(qg, F16, "qg"), q_pitch, _dense_ptr(k, F16, "k"), _dense_ptr(v, F16, "v"),
+            _dense_ptr(wq, F32, "wq", head_dim), _dense_ptr(wk, F32, "wk", head_dim), qo, qo_pitch)
+    pg = _paged(kpool, vpool, pages, page_size, B, n_kv_heads, head_dim, dev)
+    if not (qg.get_device() == k.get_device() == v.get_device() == wq.get_device()
+            == wk.get_device() == dev) or (q_out is not None and q_out.get_device() != dev):
+        _same_device(dev, qg=qg, k=k, v=v, wq=wq, wk=wk, q_out=q_out)
+    if N:
+        _lib.call("fl_attn_prep_paged", *ptrs, *pg, sp, pp, B, N, n_q_heads, n_kv_heads, head_dim,
+                  rope_dim, theta, eps, _stream())
     return qg if q_out is None else q_out
 
 
 def attention_prefill_paged_work_bytes(Ts, pos0s, n_q_heads: int = N_HEADS, n_kv_heads: int = N_KV,
                                        head_dim: int = HEAD_DIM, window: int = 0, sinks: int = 0,
                                        kv8: bool = False) -> int:
-    return int(_lib.lib().fl_attention_prefill_paged_work_bytes(
+    """The `work` bytes of attention_prefill_paged of these chunks."""
+    return _lib.lib().fl_attention_prefill_paged_work_bytes(
         _lib.int_array(Ts), _lib.int_array(pos0s), len(Ts), n_q_heads, n_kv_heads, head_dim, window,
-        sinks, int(kv8)))
+        sinks, int(kv8))
 
 
 def attention_prefill_paged(q, kpool, vpool, pages, Ts, pos0s, *, page_size: int, window: int = 0,
@@ -716,42 +754,46 @@ def attention_prefill_paged(q, kpool, vpool, pages, Ts, pos0s, *, page_size: int
     in the pools already. A query at position p sees the rows r <= p with r > p -
     window or r < sinks (window 0: all) on present pages; one that sees none gives
     0. gated: attn_gate applied too, the gate the second half of each head's q row.
+    work: uint8 of attention_prefill_paged_work_bytes (allocated here unless given).
     Returns z [N, n_q_heads, head_dim] fp16; rows behind the last chunk are left as
     they are (zeros in a new tensor)."""
-    Ts, pos0s = [int(t) for t in Ts], [int(p) for p in pos0s]
+    dev = _here()
     B, total = len(Ts), sum(Ts)
     if len(pos0s) != B or B == 0:
         raise ValueError("one T and one pos0 per sequence, one sequence or more")
     if min(Ts) < 0 or min(pos0s) < 0:
         raise ValueError("T, pos0: negative")
     N, n_q_heads, q_pitch = q.shape
-    _contig(q, "q")
     if total > N:
         raise ValueError(f"q: {N} tokens, the chunks have {total}")
-    pg = _paged(kpool, vpool, pages, page_size, B, n_kv_heads, HEAD_DIM)
+    pg = _paged(kpool, vpool, pages, page_size, B, n_kv_heads, HEAD_DIM, dev)
+    qp = _dense_ptr(q, F16, "q")
     if z is None:
         make = torch.empty if total == N else torch.zeros
         z = make((N, n_q_heads, HEAD_DIM), dtype=F16, device=q.device)
-    _contig(z, "z")
-    if z.dim() != 3 or z.shape[1] != n_q_heads or z.shape[0] < total:
+    elif z.dim() != 3 or z.shape[1] != n_q_heads or z.shape[0] < total:
         raise ValueError(f"z: expected [{N}, {n_q_heads}, pitch]")
-    _one_device(q=q, z=z, kpool=kpool, vpool=vpool, pages=pages, work=work)
+    zp = _dense_ptr(z, F16, "z")
+    if not (q.get_device() == z.get_device() == dev) or work is not None:
+        _same_device(dev, q=q, z=z, work=work)
     if total == 0:
         return z
-    need = attention_prefill_paged_work_bytes(Ts, pos0s, n_q_heads, n_kv_heads, HEAD_DIM, window,
-                                              sinks, bool(pg[2]))
-    if work is None and need:
-        work = torch.empty(need, dtype=torch.uint8, device=q.device)
-    _lib.call("fl_attention_prefill_paged", _ptr(q, F16, "q", N * n_q_heads * q_pitch), q_pitch, *pg,
-              _lib.int_array(Ts), _lib.int_array(pos0s), B, n_q_heads, n_kv_heads, HEAD_DIM,
-              float(scale), window, sinks, int(gated), _ptr(z, F16, "z", total * n_q_heads * z.shape[-1]),
-              z.shape[-1], *_prefill_work(work), _stream())
+    ts, ps = _lib.int_array(Ts), _lib.int_array(pos0s)
+    if work is None:
+        need = _lib.lib().fl_attention_prefill_paged_work_bytes(
+            ts, ps, B, n_q_heads, n_kv_heads, HEAD_DIM, window, sinks, pg[2])
+        if need:
+            work = torch.empty(need, dtype=torch.uint8, device=q.device)
+    _lib.call("fl_attention_prefill_paged", qp, q_pitch, *pg, ts, ps, B, n_q_heads, n_kv_heads,
+              HEAD_DIM, scale, window, sinks, int(gated), zp, z.shape[2], *_prefill_work(work),
+              _stream())
     return z
 
 
 def attn_decode_paged_work_bytes(B: int, T: int, n_q_heads: int = N_HEADS, n_kv_heads: int = N_KV,
                                  head_dim: int = HEAD_DIM) -> int:
-    return int(_lib.lib().fl_attn_decode_paged_work_bytes(B, T, n_q_heads, n_kv_heads, head_dim))
+    """The `work` bytes of attn_decode_paged."""
+    return _lib.lib().fl_attn_decode_paged_work_bytes(B, T, n_q_heads, n_kv_heads, head_dim)
 
 
 def attn_decode_paged(qg, kpool, vpool, pages, pos0, *, page_size: int, window: int = 0,
@@ -761,25 +803,26 @@ def attn_decode_paged(qg, kpool, vpool, pages, pos0, *, page_size: int, window: 
     q | gate per head, pos0 [B] int32 on the GPU each sequence's first query
     position (read when the call runs); up to 1024 sequences. What a query sees is
     attention_prefill_paged's; one at a negative position (a padded batch's row)
-    sees nothing and gives 0. Returns z [B, T, n_q_heads, head_dim] fp16."""
+    sees nothing and gives 0. work: uint8 of attn_decode_paged_work_bytes (allocated
+    here unless given). Returns z [B, T, n_q_heads, head_dim] fp16."""
+    dev = _here()
     B, T, n_q_heads, q_pitch = qg.shape
-    _contig(qg, "qg")
     if pos0.dim() != 1 or pos0.numel() != B:
         raise ValueError(f"pos0: expected {B} positions")
-    pg = _paged(kpool, vpool, pages, page_size, B, n_kv_heads, HEAD_DIM)
+    pg = _paged(kpool, vpool, pages, page_size, B, n_kv_heads, HEAD_DIM, dev)
+    qp, pp = _dense_ptr(qg, F16, "qg"), _dense_ptr(pos0, I32, "pos0")
     if z is None:
         z = torch.empty((B, T, n_q_heads, HEAD_DIM), dtype=F16, device=qg.device)
-    _contig(z, "z")
-    if z.dim() != 4 or tuple(z.shape[:3]) != (B, T, n_q_heads):
+    elif z.dim() != 4 or z.shape[0] != B or z.shape[1] != T or z.shape[2] != n_q_heads:
         raise ValueError(f"z: expected [{B}, {T}, {n_q_heads}, pitch]")
-    _one_device(qg=qg, z=z, kpool=kpool, vpool=vpool, pages=pages, pos0=pos0, work=work)
-    need = attn_decode_paged_work_bytes(B, T, n_q_heads, n_kv_heads)
-    if work is None and need:
-        work = torch.empty(need, dtype=torch.uint8, device=qg.device)
-    _lib.call("fl_attn_decode_paged", _ptr(qg, F16, "qg", B * T * n_q_heads * q_pitch), q_pitch, *pg,
-              _dense_ptr(pos0, torch.int32, "pos0", B), B, T, n_q_heads, n_kv_heads, HEAD_DIM,
-              float(scale), window, sinks, int(gate), _ptr(z, F16, "z", z.numel()), z.shape[-1],
-              *_prefill_work(work), _stream())
+    zp = _dense_ptr(z, F16, "z")
+    if not (qg.get_device() == z.get_device() == pos0.get_device() == dev) or work is not None:
+        _same_device(dev, qg=qg, z=z, pos0=pos0, work=work)
+    if work is None:
+        work = torch.empty(attn_decode_paged_work_bytes(B, T, n_q_heads, n_kv_heads),
+                           dtype=torch.uint8, device=qg.device)
+    _lib.call("fl_attn_decode_paged", qp, q_pitch, *pg, pp, B, T, n_q_heads, n_kv_heads, HEAD_DIM,
+              scale, window, sinks, int(gate), zp, z.shape[3], *_prefill_work(work), _stream())
     return z
 
 

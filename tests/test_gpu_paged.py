@@ -135,6 +135,30 @@ def test_store_and_load(fl, dev, kv8, page_size, spans, n_kv):
     assert torch.equal(ko[:N], k2[:N]) and bool((ko[N:] == 7).all()) and bool((vo[N:] == 7).all())
 
 
+def test_int8_store_at_ties_and_non_finite_values(fl, dev):
+    """The bytes and scales of kv_store_q8 where x / scale is a half integer, next to one,
+    or not a number: blocks whose scale is a power of two (ties exact), every fp16 scale
+    magnitude, subnormal blocks, infinities and NaN."""
+    g, ops = gen(7), fl.ops
+    N = 64
+    x = torch.randn((N, 4, 8, 32), generator=g)
+    for n in range(N):                                       # scale 2^(n % 24 - 20), ties below
+        s = 2.0 ** (n % 24 - 20)
+        if 127 * s <= 65504:
+            x[n, 0] = (torch.randint(-127, 127, (8, 32), generator=g) + 0.5) * s
+            x[n, 0, :, 0] = 127 * s
+    x[:, 1] *= 10.0 ** (torch.rand((N, 8, 1), generator=g) * 9 - 6)
+    x[0, 2, 0, 3], x[1, 2, 1, 4], x[2, 2, 2, 5] = float("inf"), float("nan"), -float("inf")
+    x[3, 2, 3] = float("nan")
+    x[4, 2, 4], x[5, 2, 5] = 0.0, 2.0 ** -24
+    x = x.view(N, 4, 256).to(F16).cuda()
+    kp, vp = (ops.paged_pool(4, 16, kv8=True) for _ in range(2))
+    ops.paged_kv_store(x, x, kp, vp, i32(0, 1, 2, 3).view(1, 4), i32(0, N), i32(0), page_size=16)
+    kc, vc = ops.kv8_cache(N), ops.kv8_cache(N)
+    ops.kv_store_q8(x, x, kc, vc, pos0=0, max_pos=N)
+    assert torch.equal(kp, kc) and torch.equal(vp, vc)
+
+
 @pytest.mark.parametrize("kv8", [False, True])
 def test_store_and_load_strided_absent_and_negative(fl, dev, kv8):
     """Token strides of a wider row, pages that are absent (negative, past the pool,
