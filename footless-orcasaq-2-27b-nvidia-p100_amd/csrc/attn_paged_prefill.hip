@@ -615,8 +615,8 @@ long long cut_plan(const std::vector<int>& n, int n_kv, int most, CallPlan& cp) 
     return longest + (cp.slots ? MERGE_COST + cp.slots * n_kv / SLOTS_PER_TILE : 0);
 }
 
-// The plan of whole row tiles, the heaviest first to the lightest run, and its cost; 0
-// where its list does not fit.
+// The plan of whole row tiles, the heaviest first to the lightest run, then moves and swaps
+// off the heaviest run while they shorten it; and its cost, 0 where its list does not fit.
 long long whole_plan(const std::vector<int>& n, int most, Plan& p) {
     const int N = (int)n.size();
     if (N > LIST_MAX) return 0;
@@ -628,15 +628,44 @@ long long whole_plan(const std::vector<int>& n, int most, Plan& p) {
     std::priority_queue<Load, std::vector<Load>, std::greater<Load>> light;
     for (int r = 0; r < runs; ++r) light.push({0, r});
     std::vector<std::vector<int>> list(runs);
-    long long longest = 0;
+    std::vector<long long> load(runs, 0);
+    long long total = 0;
     for (int t : order) {
         Load l = light.top();
         light.pop();
         list[l.second].push_back(t);
-        l.first += n[t] + ITEM_COST;
-        longest = std::max(longest, l.first);
+        load[l.second] = l.first += n[t] + ITEM_COST;
+        total += n[t] + ITEM_COST;
         light.push(l);
     }
+    for (int round = 0; round < 4 * N; ++round) {
+        const int hi = (int)(std::max_element(load.begin(), load.end()) - load.begin());
+        if (load[hi] * runs <= total + total / 256) break;   // even to 0.4 %
+        long long best = load[hi];
+        int bx = -1, by = -1, bl = -1;   // list[hi][bx] to run bl, for list[bl][by] (by < 0: for none)
+        for (int lo = 0; lo < runs; ++lo) {
+            if (lo == hi) continue;
+            for (int x = 0; x < (int)list[hi].size(); ++x)
+                for (int y = -1; y < (int)list[lo].size(); ++y) {
+                    const long long d =
+                        n[list[hi][x]] - (y < 0 ? -ITEM_COST : n[list[lo][y]]);
+                    const long long m = std::max(load[hi] - d, load[lo] + d);
+                    if (d > 0 && m < best) best = m, bx = x, by = y, bl = lo;
+                }
+        }
+        if (bl < 0) break;
+        const int t = list[hi][bx];
+        const long long d = n[t] - (by < 0 ? -ITEM_COST : n[list[bl][by]]);
+        load[hi] -= d;
+        load[bl] += d;
+        if (by < 0) {
+            list[hi].erase(list[hi].begin() + bx);
+            list[bl].push_back(t);
+        } else {
+            std::swap(list[hi][bx], list[bl][by]);
+        }
+    }
+    const long long longest = *std::max_element(load.begin(), load.end());
     p.runs = runs;
     int k = 0;
     for (int r = 0; r < runs; ++r) {
