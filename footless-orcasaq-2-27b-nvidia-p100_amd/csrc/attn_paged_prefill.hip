@@ -741,6 +741,21 @@ long long lay_dense(Chunks& ch, const Sight& sight) {
 }
 size_t dense_bytes(long long rows, int n_kv) { return 2 * (size_t)rows * n_kv * ROW_B; }
 
+// The sequences of an int8 call whose copies fit GROUP_BYTES together, from `b` on (one at
+// least): the call runs a group after the other over the same work, so that a batch of long
+// contexts does not ask for tens of GB (4 KiB a row at 4 kv heads).
+constexpr size_t GROUP_BYTES = (size_t)1 << 30;
+int group_end(const int* Ts, const int* pos0s, int B, int b, int n_kv, const Sight& sight) {
+    size_t bytes = 0;
+    int e = b;
+    for (; e < B; ++e) {
+        const long long rows = dense_rows(Ts[e], pos0s[e], sight);
+        bytes += dense_bytes(rows, n_kv);
+        if (e > b && bytes > GROUP_BYTES) break;
+    }
+    return e;
+}
+
 // Dynamic LDS above the default limit, raised once per device.
 int raise_lds() {
     static std::atomic<bool> done[64];
@@ -762,6 +777,11 @@ int raise_lds() {
         }
     done[dev].store(true);
     return FL_OK;
+}
+
+int too_little_work(size_t have, size_t need) {
+    fl::set_error("work: %zu bytes, fl_attention_prefill_paged_work_bytes asks %zu", have, need);
+    return FL_ESCRATCH;
 }
 
 // The fp16 copy: row i of sequence b's part is the row of the union of its walks; a
@@ -812,14 +832,22 @@ size_t fl_attention_prefill_paged_work_bytes(const int* Ts, const int* pos0s, in
     if (n_kv_heads < 1 || n_q_heads < 1 || n_q_heads % n_kv_heads || head_dim != PF_HD || window < 0 ||
         sinks < 0)
         return 0;
-    Chunks ch;
     const int G = n_q_heads / n_kv_heads;
     const Sight sight = {window, sinks};
-    if (make_chunks(Ts, pos0s, B, G, INT_MAX - 1024, ch) || ch.start[B] == 0) return 0;
-    CallPlan cp;
-    if (call_plan(ch, G, n_kv_heads, sight, cu_count(), cp)) return 0;
-    const long long rows = q8 ? lay_dense(ch, sight) : 0;
-    return up16(parts_bytes(cp.slots, n_kv_heads)) + (rows > 0 ? dense_bytes(rows, n_kv_heads) : 0);
+    Chunks ch;
+    if (make_chunks(Ts, pos0s, B, G, INT_MAX - 1024, ch)) return 0;
+    size_t most = 0;
+    for (int b = 0, e; b < B; b = e) {
+        e = q8 ? group_end(Ts, pos0s, B, b, n_kv_heads, sight) : B;
+        CallPlan cp;
+        if (make_chunks(Ts + b, pos0s + b, e - b, G, INT_MAX - 1024, ch)) return 0;
+        if (ch.start[e - b] == 0) continue;
+        if (call_plan(ch, G, n_kv_heads, sight, cu_count(), cp)) return 0;
+        const long long rows = q8 ? lay_dense(ch, sight) : 0;
+        if (rows < 0) return 0;
+        most = std::max(most, up16(parts_bytes(cp.slots, n_kv_heads)) + dense_bytes(rows, n_kv_heads));
+    }
+    return most;
 }
 
 int fl_attention_prefill_paged(const void* q, int q_pitch, const void* kpool, const void* vpool,
@@ -840,6 +868,22 @@ int fl_attention_prefill_paged(const void* q, int q_pitch, const void* kpool, co
     if (rc) return rc;
     if (ch.start[B] == 0) return FL_OK;
     const Sight sight = {window, sinks};
+    if (q8 && group_end(Ts, pos0s, B, 0, n_kv_heads, sight) < B) {
+        const size_t need = fl_attention_prefill_paged_work_bytes(Ts, pos0s, B, n_q_heads, n_kv_heads,
+                                                                  head_dim, window, sinks, q8);
+        if (work == nullptr || work_bytes < need) return too_little_work(work_bytes, need);
+        for (int b = 0, e; b < B; b = e) {
+            e = group_end(Ts, pos0s, B, b, n_kv_heads, sight);
+            const size_t row = (size_t)ch.start[b] * n_q_heads;
+            rc = fl_attention_prefill_paged((const f16*)q + row * q_pitch, q_pitch, kpool, vpool, q8,
+                                            n_pages, page_size, pages + b * pages_stride, max_pages,
+                                            pages_stride, Ts + b, pos0s + b, e - b, n_q_heads,
+                                            n_kv_heads, head_dim, scale, window, sinks, gated,
+                                            (f16*)z + row * z_pitch, z_pitch, work, work_bytes, stream_);
+            if (rc) return rc;
+        }
+        return FL_OK;
+    }
     const int n_cu = cu_count();
     CallPlan cp;
     rc = call_plan(ch, G, n_kv_heads, sight, n_cu, cp);
@@ -849,11 +893,7 @@ int fl_attention_prefill_paged(const void* q, int q_pitch, const void* kpool, co
     const size_t part_b = up16(parts_bytes(cp.slots, n_kv_heads));
     const size_t need = part_b + dense_bytes(rows, n_kv_heads);
     if (need > 0) {
-        if (work == nullptr || work_bytes < need) {
-            fl::set_error("work: %zu bytes, fl_attention_prefill_paged_work_bytes asks %zu", work_bytes,
-                          need);
-            return FL_ESCRATCH;
-        }
+        if (work == nullptr || work_bytes < need) return too_little_work(work_bytes, need);
         FL_REQUIRE(aligned16(work), "16-byte aligned work");
     }
     rc = raise_lds();

@@ -17,6 +17,7 @@ will touch.
 from __future__ import annotations
 
 import ctypes
+import functools
 
 import torch
 
@@ -792,7 +793,12 @@ def attention_prefill_paged(q, kpool, vpool, pages, Ts, pos0s, *, page_size: int
 
 def attn_decode_paged_work_bytes(B: int, T: int, n_q_heads: int = N_HEADS, n_kv_heads: int = N_KV,
                                  head_dim: int = HEAD_DIM) -> int:
-    """The `work` bytes of attn_decode_paged."""
+    """The `work` bytes of attn_decode_paged on the current device."""
+    return _decode_paged_bytes(B, T, n_q_heads, n_kv_heads, head_dim, _here())
+
+
+@functools.lru_cache(maxsize=256)
+def _decode_paged_bytes(B, T, n_q_heads, n_kv_heads, head_dim, dev):
     return _lib.lib().fl_attn_decode_paged_work_bytes(B, T, n_q_heads, n_kv_heads, head_dim)
 
 
@@ -819,7 +825,7 @@ def attn_decode_paged(qg, kpool, vpool, pages, pos0, *, page_size: int, window: 
     if not (qg.get_device() == z.get_device() == pos0.get_device() == dev) or work is not None:
         _same_device(dev, qg=qg, z=z, pos0=pos0, work=work)
     if work is None:
-        work = torch.empty(attn_decode_paged_work_bytes(B, T, n_q_heads, n_kv_heads),
+        work = torch.empty(_decode_paged_bytes(B, T, n_q_heads, n_kv_heads, HEAD_DIM, dev),
                            dtype=torch.uint8, device=qg.device)
     _lib.call("fl_attn_decode_paged", qp, q_pitch, *pg, pp, B, T, n_q_heads, n_kv_heads, HEAD_DIM,
               scale, window, sinks, int(gate), zp, z.shape[3], *_prefill_work(work), _stream())

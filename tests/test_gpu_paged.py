@@ -242,6 +242,29 @@ def test_prep_equals_the_contiguous_prep(fl, dev, kv8, spans):
         at += t
 
 
+@pytest.mark.parametrize("heads,rope_dim,N", [((6, 2), 32, 5), ((1, 1), 256, 3), ((24, 4), 128, 300),
+                                              ((9, 3), 64, 270), ((40, 8), 2, 2)])
+def test_prep_heads_and_rotations(fl, dev, heads, rope_dim, N):
+    """Other head counts and rotary widths, one sequence: attn_prep's bits."""
+    g, ops, P = gen(rope_dim), fl.ops, 16
+    nq, nkv = heads
+    p = 37
+    pages, n_pages = ref.make_pages(g, [p + N], P)
+    kp, vp = (ops.paged_pool(n_pages, P, n_kv_heads=nkv) for _ in range(2))
+    qg, k, v = randn(g, N, nq, 264), randn(g, N, nkv, 256), randn(g, N, nkv, 256)
+    wq, wk = randn(g, 256, dtype=F32, scale=0.1), randn(g, 256, dtype=F32, scale=0.1)
+    q1, k1 = qg.clone(), k.clone()
+    kc, vc = (torch.zeros((p + N, nkv, 256), dtype=F16, device="cuda") for _ in range(2))
+    ops.attn_prep(q1, k1, v, wq, wk, kc, vc, pos0=p, n_q_heads=nq, n_kv_heads=nkv, q_pitch=264,
+                  rope_dim=rope_dim)
+    ops.attn_prep_paged(qg, k, v, wq, wk, kp, vp, pages, i32(0, N), i32(p), page_size=P, n_q_heads=nq,
+                        n_kv_heads=nkv, rope_dim=rope_dim)
+    rows = ref.rows_of(pages.cpu(), 0, P, torch.arange(p, p + N)).cuda()
+    assert torch.equal(qg, q1)
+    for pool, c in ((kp, kc), (vp, vc)):
+        assert torch.equal(values(pool, n_pages * P, nkv)[rows], c[p:])
+
+
 # ---------------------------------------------------------------------------
 # attention
 # ---------------------------------------------------------------------------
@@ -320,6 +343,52 @@ def test_prefill_absent_pages(fl, dev, kv8, page_size):
     absent = [a for a in absent if a[1] * page_size < [300, 23, 134][a[0]]]
     run_prefill(fl, 21, spans, page_size, kv8, absent=absent)
     run_prefill(fl, 22, spans, page_size, kv8, 40, 5, absent=absent)
+
+
+def test_prefill_int8_copies_in_groups(fl, dev):
+    """int8 contexts whose fp16 copies pass 1 GiB together: the call runs them in groups
+    over one work buffer of that size."""
+    lens, P = [100000, 99000, 98500, 70], 256
+    g, ops = gen(23), fl.ops
+    pages, n_pages = ref.make_pages(g, lens, P)
+    kp, vp = (ops.paged_pool(n_pages, P, kv8=True) for _ in range(2))
+    cut = n_pages * P * 1024
+    for pool in (kp, vp):
+        pool[:cut].random_(-127, 128)
+        pool[cut:].view(F16).fill_(0.01).mul_(1 + torch.rand(1, device="cuda").half())
+    Ts = [3, 1, 20, 70]
+    p0s = [L - t for L, t in zip(lens, Ts)]
+    need = ops.attention_prefill_paged_work_bytes(Ts, p0s, kv8=True)
+    assert (1 << 29) < need < (1 << 30) + (200 << 20)
+    qg = randn(g, sum(Ts), 24, 512)
+    z = ops.attention_prefill_paged(qg, kp, vp, pages, Ts, p0s, page_size=P, gated=True)
+    K, V = (ref.dequant(pool, n_pages * P, 4) for pool in (kp, vp))
+    at = 0
+    for b, (t, L) in enumerate(zip(Ts, lens)):
+        rows = ref.rows_of(pages.cpu(), b, P, torch.arange(L)).cuda()
+        want, bound = ref.attention(qg[at:at + t, :, :256], K[rows], V[rows], L - t,
+                                    seen_mask(t, L - t, L, 0, 0), SCALE, True, qg[at:at + t, :, 256:])
+        check(z[at:at + t], want, bound, f"sequence {b}")
+        at += t
+
+
+def test_table_of_a_wider_one(fl, dev):
+    """A column slice of a wider table: its row stride is taken."""
+    g = gen(24)
+    kp, vp, pages, caches = filled(fl, g, [100, 40], 16, False)
+    wide = torch.full((2, pages.shape[1] + 5), 10 ** 6, dtype=I32, device="cuda")
+    wide[:, 2:2 + pages.shape[1]] = pages
+    part = wide[:, 2:2 + pages.shape[1]]
+    qg = randn(g, 2, 1, 24, 512)
+    pos = i32(99, 39)
+    assert torch.equal(fl.ops.attn_decode_paged(qg, kp, vp, part, pos, page_size=16),
+                       fl.ops.attn_decode_paged(qg, kp, vp, pages, pos, page_size=16))
+    args = dict(page_size=16, gated=True)
+    assert torch.equal(fl.ops.attention_prefill_paged(qg[:, 0], kp, vp, part, [1, 1], [99, 39], **args),
+                       fl.ops.attention_prefill_paged(qg[:, 0], kp, vp, pages, [1, 1], [99, 39], **args))
+    for a, b in zip(fl.ops.paged_kv_load(kp, vp, part, i32(0, 9, 12), i32(5, 30), T=12, page_size=16),
+                    fl.ops.paged_kv_load(kp, vp, pages, i32(0, 9, 12), i32(5, 30), T=12, page_size=16)):
+        assert torch.equal(a, b)
 
 
 def run_decode(fl, seed, lens, page_size, kv8, T=1, window=0, sinks=0, heads=(24, 4), gate=True, q_scale=1.0,

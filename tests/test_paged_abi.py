@@ -117,3 +117,24 @@ def test_op_layer_refuses_what_is_not_a_pool(fl):
     odd = torch.zeros(fl.geometry.kv8_nbytes(16) + 272, dtype=torch.int8)
     with pytest.raises(ValueError, match="pages"):
         ops.attn_decode_paged(qg, odd, odd, pages, pos0, page_size=16)
+
+
+def test_int8_work_is_bounded_by_groups(fl):
+    """Many long int8 contexts: the fp16 copies are made in groups of 1 GiB; fp16 pools need
+    none, and work that is too small is refused."""
+    f = fl.ops.attention_prefill_paged_work_bytes
+    many = f([1] * 40, [100000] * 40, kv8=True)
+    assert f([1], [100000], kv8=True) < many < (1 << 30) + (200 << 20)
+    assert f([1] * 40, [100000] * 40) < 200 << 20
+    assert f([0], [5], kv8=True) == 0 and f([1], [0]) == 0
+    # a window's copy holds the window, not the context: 32-row tiles 2997 (row 95905 - 1)
+    # .. 3126 and the first tokens' one, 4 KiB a row, beside an fp16 call's partials
+    args = dict(window=4096, sinks=4)
+    assert f([64], [100000], kv8=True, **args) - f([64], [100000], **args) == 131 * 32 * 4096
+    for T, pos in (([1024], [30000]), ([1] * 40, [3000] * 40)):
+        rc = call(fl, "fl_attention_prefill_paged",
+                  dict(B=len(T), Ts=ints(*T), pos0s=ints(*pos), q8=1, max_pages=1 << 16, stride=1 << 16,
+                       work=FAKE, wb=1024))
+        assert rc == 3 and b"work" in fl._lib.lib().fl_last_error()
+    assert call(fl, "fl_attn_decode_paged", dict(work=FAKE, wb=64)) == 3
+    assert call(fl, "fl_attn_decode_paged", dict(work=FAKE + 8, wb=1 << 30)) == 1
