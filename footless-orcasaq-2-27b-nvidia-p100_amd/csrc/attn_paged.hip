@@ -65,23 +65,28 @@ __device__ __forceinline__ int wave_scan(int x) {
     x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, true);   // row_bcast 31
     return x;
 }
-// A workgroup's run of the stream: its kv head, and the pieces one after the other.
+// How a stream is cut: runs a kv head, tiles a run at least, and what a sequence costs
+// ahead of its tiles, in tiles. A workgroup may take 2, .. 2^heads_lg kv heads, and runs are
+// that much shorter then (Run).
+struct Cut {
+    int runs, run_min, seq_cost, heads_lg;
+};
+constexpr int LONG_RUN = 64;    // tiles a run of one head
+constexpr int SHORT_SEQ = 16;   // tiles a sequence, with its cost
+// A workgroup's run of the stream: its kv heads, and the pieces one after the other.
 struct Run {
-    int h, run, per;          // runs are `per` units long
+    int h, heads_lg;          // kv heads h << heads_lg .. + 2^heads_lg - 1
+    int run, per;             // runs are `per` units long
     int u, u_end;             // what is left of this one
     int b, su, cost;          // the sequence that u lies in, where it starts, units ahead of its tiles
     bool any;
 
     // Workgroups go to the 8 XCDs round-robin: the kv heads of a run go to one of them
     // (their rows share lines of scales), the runs to all.
-    __device__ __forceinline__ Run(const int* pos0, int B, int T, int n_kv, int runs, int run_min,
-                                   int seq_cost, const Sight& sight, int cap) {
+    __device__ __forceinline__ Run(const int* pos0, int B, int T, int n_kv, const Cut& cut,
+                                   const Sight& sight, int cap) {
         const int id = blockIdx.x, lane = threadIdx.x & 63;
-        const bool even = runs % 8 == 0;
-        const int slot = even ? id >> 3 : id;
-        h = slot % n_kv;
-        run = even ? slot / n_kv * 8 + (id & 7) : slot / n_kv;
-        cost = B > 1 ? seq_cost : 1;   // (not 0: a sequence without rows has its place too)
+        cost = B > 1 ? cut.seq_cost : 1;   // (not 0: a sequence without rows has its place too)
         auto units = [&](int s) { return dec_seq(pos0[s], T, sight, cap).n + cost; };
         int total = 0, scan = 0, un = 0;   // (of the last 64 sequences: the first ones if B <= 64)
         for (int b0 = 0; b0 < B; b0 += 64) {   // (the host has checked: under 2^31 tiles)
@@ -89,8 +94,21 @@ struct Run {
             scan = wave_scan(un);
             total += __builtin_amdgcn_readlane(scan, 63);
         }
+        // Waves of a workgroup that take all kv heads of a row read it whole: 64 contexts of
+        // 30 - 50k 869 us against 937 with a head a workgroup, 64 of 100 - 32k 145 against 159,
+        // 16 of 8k 58.4 against 60.2. With shorter runs the waves of a head rather go
+        // through its tiles together (fewer partials): one context of 32k 27.9 against 42.0, 4
+        // of 8k 24.7 against 29.7. Sequences shorter than their waves: 96 of 50 17.2 with two
+        // heads, 19.2 with one, 22.1 with four.
+        const int lg = total / LONG_RUN >= cut.runs ? 2 : total < SHORT_SEQ * B ? 1 : 0;
+        heads_lg = min(lg, cut.heads_lg);
+        const int runs = cut.runs << heads_lg, groups = n_kv >> heads_lg;
+        const bool even = runs % 8 == 0;
+        const int slot = even ? id >> 3 : id;
+        h = slot % groups;
+        run = even ? slot / groups * 8 + (id & 7) : slot / groups;
         // (a little over total / runs: no run is left over)
-        per = max((int)((float)total * (1.0001f / (float)runs)) + 1, run_min);
+        per = max((int)((float)total * (1.0001f / (float)runs)) + 1, cut.run_min >> heads_lg);
         any = (long long)run * per < total;
         if (!any) return;
         u = run * per;
@@ -152,7 +170,7 @@ struct TileF16 {
 __global__ void __launch_bounds__(64 * D_WAVES)
 paged_decode_f16_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict__ kp,
                         const char* __restrict__ vp, const Pages pg, const int* __restrict__ pos0,
-                        int B, int T, int n_q, int n_kv, int runs, float sl2, const Sight sight,
+                        int B, int T, int n_q, int n_kv, const Cut cut, float sl2, const Sight sight,
                         const DecPart out) {
     __shared__ __attribute__((aligned(16))) f32x4 s_part[2][2][4][64];
     __shared__ __attribute__((aligned(16))) f16 s_vt[2][4][64][VTP];
@@ -161,7 +179,7 @@ paged_decode_f16_kernel(const f16* __restrict__ qg, int q_pitch, const char* __r
     const int hh = lane >> 5, ql = lane & 31;
     const int G = n_q / n_kv, R = T * G;
     const int cap = pg.max_pages << pg.shift;
-    Run run(pos0, B, T, n_kv, runs, RUN_MIN_F16, SEQ_COST_F16, sight, cap);
+    Run run(pos0, B, T, n_kv, cut, sight, cap);
     if (!run.any) return;   // (the whole workgroup)
     const int h = run.h;
     // a lane's offsets from its wave's first row
@@ -196,7 +214,7 @@ paged_decode_f16_kernel(const f16* __restrict__ qg, int q_pitch, const char* __r
                 for (int ks = 0; ks < 4; ++ks)
                     qreg[4 * nb + ks] = ok ? *(const f16x8*)(qrow + 8 * ks) : (f16x8)(0);
             }
-            auto ids = page_ids<1>(pg, b, j0, j1 - 1, [&](int j) { return d.row0(j); });
+            auto ids = page_ids(pg, b, j0, j1 - 1, 0, [&](int j) { return d.row0(j); });
 
             f32x16 o0 = (f32x16)(0.f), o1 = (f32x16)(0.f);
             float m_run = -1e30f, l_run = 0.f;
@@ -330,46 +348,51 @@ paged_decode_f16_kernel(const f16* __restrict__ qg, int q_pitch, const char* __r
 }
 
 // ---------------------------------------------------------------------------
-// int8 pools. A wave takes every fourth tile of a piece alone, over all 256 dims: no
-// barrier and no exchange until the piece ends, where the four waves' O, maxima and
-// sums are combined through LDS.
-//   S^T (32 kv x 16 NB columns) = K Q^T   K from HBM in A operand order: lane (i, g)
-//                                         row 16 rb + i, dims 32 ks + 8 g .. + 7
+// int8 pools. A wave takes tiles alone, over all 256 dims: no barrier and no exchange until
+// the piece ends, where the O, maxima and sums of a head's waves are combined through LDS.
+//   S^T (32 kv x 16 NB columns) = K Q^T   A operand: lane (i, g) row 16 rb + i, dims 32 ks
+//                                         + 8 g .. + 7
 //   softmax                               a lane holds column i's rows 4 g + e of both
 //                                         halves; the maximum is exchanged only when
 //                                         it moves by more than RESCALE_LOG2
 //   O^T (256 dims) += V^T P^T             P as it lies: k slot (g, e) is row 4 g + e of
 //                                         half e / 4; V^T by transposed LDS reads
-// K of the next tile is requested once this one's scores are formed, V once this
-// one's is in LDS, so one of them is always in flight.
+// K and V come as whole rows, 16 bytes a lane, non-temporal, and are turned into operands
+// through LDS: K as bytes, V as fp16. K of the next tile is requested once this one's is in
+// LDS, V likewise, so one of them is always in flight.
 //
-// Bytes are exact in fp16. A 32-dim block is one k step, so its scale is applied to
-// its fp32 partial score and K is not rounded at all; V is f16(byte scale), and P
-// goes in as two fp16 terms: V's rounding is the only one of the products, and the
-// error is that of fp16 pools, whose only one is P's. (With f16(byte scale) for K
-// and V and P in one term it is 1.5 times as large.)
+// Bytes are exact in fp16. A 32-dim block is one k step, so its scale is applied to its fp32
+// partial score and K is not rounded at all; V is f16(byte scale), and P goes in as two fp16
+// terms: V's rounding is the only one of the products, and the error is that of fp16 pools,
+// whose only one is P's. (With f16(byte scale) for K and V and P in one term it is 1.5 times
+// as large.)
+//
+// What it reaches: 64 contexts of 100 - 32k 145 us (812 MB, 5.6 TB/s), 64 of 30 - 50k 869
+// (6.3), 4 of 100k with 18 rows 178 (4.6). With 16 rows it is bound by the memory: without its
+// products it takes as long, and what a workgroup's waves read at a time counts. K in operand
+// order from memory (8 bytes a lane, 32 of a row an instruction), a head a workgroup and two
+// workgroups of 4 waves a CU: 165; 8 waves with K through LDS 159; four heads a workgroup 145.
+// With 17 - 32 rows O and Q leave registers for one wave a SIMD, whose chain of products and
+// conversions shows: 151 us without them. Its columns shared out to two waves, with 8 a CU,
+// each converting all of K and V: 229.
 // ---------------------------------------------------------------------------
+constexpr int K_PITCH = PAGED_HD + 16;       // bytes a K row in LDS (a b64 of 16 rows meets all banks)
 constexpr int V_PITCH = 2 * PAGED_HD + 32;   // bytes a V row in LDS (the 32 spread rows over banks)
 constexpr int O_PITCH = PAGED_HD + 4;        // floats a column of O in LDS
 constexpr int PV_AHEAD = 4;                  // V^T fragments read ahead of their product
-constexpr int RUN_MIN_Q8 = 4;                // tiles a run, at least: one a wave
-constexpr int SEQ_COST_Q8 = 6;              // a further piece's fixed cost in tiles (its first loads)
+constexpr int SEQ_COST_Q8 = 6;               // a further piece's fixed cost in tiles (its first loads)
 
-// A tile in flight: K bytes [row 16 rb + i][32 ks + 8 g .. + 7] and V bytes [row 4 n +
-// g][16 i .. + 15], and of each the scales of row l % 32, blocks 4 (l / 32) .. + 3.
-struct KTile {
-    u32x2 k[2][8];
-    f16x4 sc;
-};
-struct VTile {
-    u32x4 v[8];
+// A tile of K or V in flight: bytes [row 4 n + g][16 i .. + 15] and the scales of row l % 32,
+// blocks 4 (l / 32) .. + 3.
+struct Tile8 {
+    u32x4 x[8];
     f16x4 sc;
 };
 
 // Where a call's pools and a lane's part of a row lie.
 struct TileAt {
     const char *kp, *vp, *ks, *vs;   // values and scales
-    uint32_t rs, ko, vo, so;         // bytes a row; a lane's offsets
+    uint32_t rs, vo, so;             // bytes a row; a lane's offsets
     bool upper;                      // its scales' half of the tile
     __device__ __forceinline__ TileAt(const char* kp_, const char* vp_, const Pages& pg, int n_kv, int h,
                                       int lane) {
@@ -378,7 +401,6 @@ struct TileAt {
         rs = PAGED_HD * n_kv;
         const long long values = ((long long)pg.n_pages << pg.shift) * rs;
         ks = kp + values, vs = vp + values;
-        ko = PAGED_HD * h + 8 * g + i * rs;
         vo = PAGED_HD * h + 16 * i + g * rs;
         so = 16 * h + 8 * (lane >> 5) + i * (rs / 16);
         upper = g & 1;
@@ -388,26 +410,19 @@ struct TileAt {
         return *(const __attribute__((address_space(1))) f16x4*)((gptr)of + ((upper ? hi : lo) + so));
     }
     // at[half]: the pool row of the tile's 16-row halves
-    __device__ __forceinline__ void load(KTile& t, const long long (&at)[2]) const {
-        t.sc = scales(ks, at);
-#pragma unroll
-        for (int rb = 0; rb < 2; ++rb) {
-            const gptr b = uni_global(kp + at[rb] * rs);
-#pragma unroll
-            for (int s = 0; s < 8; ++s) t.k[rb][s] = load_g<u32x2>(b, ko + 32 * s);
-        }
-        issued();
-    }
-    __device__ __forceinline__ void load(VTile& t, const long long (&at)[2]) const {
-        t.sc = scales(vs, at);
+    __device__ __forceinline__ void load(Tile8& t, const char* rows, const char* sc,
+                                         const long long (&at)[2]) const {
+        t.sc = scales(sc, at);
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const gptr b = uni_global(vp + at[half] * rs);
+            const gptr b = uni_global(rows + at[half] * rs);
 #pragma unroll
-            for (int n = 0; n < 4; ++n) t.v[4 * half + n] = stream_g<u32x4>(b + 4 * n * rs, vo);
+            for (int n = 0; n < 4; ++n) t.x[4 * half + n] = stream_g<u32x4>(b + 4 * n * rs, vo);
         }
         issued();
     }
+    __device__ __forceinline__ void load_k(Tile8& t, const long long (&at)[2]) const { load(t, kp, ks, at); }
+    __device__ __forceinline__ void load_v(Tile8& t, const long long (&at)[2]) const { load(t, vp, vs, at); }
     // the compiler would sink the loads to where they are used
     static __device__ __forceinline__ void issued() {
         asm volatile("" ::: "memory");
@@ -417,44 +432,50 @@ struct TileAt {
 
 // 8 bytes as the integers they are, exact in fp16 (q8_deq4 without the scale)
 __device__ __forceinline__ f16x8 q8_ints(u32x2 b) {
-    const f16x2 off = {(f16)1152.f, (f16)1152.f};
-    f16x8 r;
+    u32x4 r;
 #pragma unroll
     for (int d = 0; d < 2; ++d) {
-        const uint32_t u = b[d] ^ 0x80808080u;
-        const f16x2 lo = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u)) - off;
-        const f16x2 hi = __builtin_bit_cast(f16x2, __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u)) - off;
-        r[4 * d] = lo[0], r[4 * d + 1] = lo[1], r[4 * d + 2] = hi[0], r[4 * d + 3] = hi[1];
+        const uint32_t u = b[d] ^ 0x80808080u;   // 1024 + (byte + 128), less 1152
+        r[2 * d] = __builtin_amdgcn_perm(0x64646464u, u, 0x04010400u);
+        r[2 * d + 1] = __builtin_amdgcn_perm(0x64646464u, u, 0x04030402u);
     }
-    return r;
+    return __builtin_bit_cast(f16x8, r) - (f16x8)((f16)1152.f);
 }
 __device__ __forceinline__ f16x8 q8_values(uint32_t a, uint32_t b, f16 s) {
     const f16x4 lo = q8_deq4(a, (f16x2){s, s}), hi = q8_deq4(b, (f16x2){s, s});
     return (f16x8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 
-// NB: blocks of 16 query columns (2: one workgroup a CU)
+// waves a workgroup, one a CU, by the blocks of 16 query columns: what its registers hold
+constexpr int q8_waves(int NB) { return NB == 1 ? 8 : 4; }
+
+// NB: blocks of 16 query columns
 template <int NB>
-__global__ void __launch_bounds__(64 * D_WAVES, NB == 1 ? 2 : 1)
+__global__ void __launch_bounds__(64 * q8_waves(NB))
 paged_decode_q8_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict__ kp,
                        const char* __restrict__ vp, const Pages pg, const int* __restrict__ pos0, int B,
-                       int T, int n_q, int n_kv, int runs, float sl2, const Sight sight,
+                       int T, int n_q, int n_kv, const Cut cut, float sl2, const Sight sight,
                        const DecPart out) {
-    // V of a wave's tile while it walks, O of the waves when a piece ends
-    constexpr int WAVE_B = std::max(DT * V_PITCH, 16 * NB * O_PITCH * 4);
-    __shared__ __attribute__((aligned(16))) char s_mem[D_WAVES * WAVE_B];
-    __shared__ float s_m[D_WAVES][16 * NB], s_l[D_WAVES][16 * NB];
+    constexpr int W = q8_waves(NB), W_LG = W == 8 ? 3 : 2;
+    // K and V of a wave's tile while it walks, O of the waves when a piece ends
+    constexpr int WAVE_B = std::max(DT * V_PITCH, 16 * O_PITCH * 4);
+    __shared__ __attribute__((aligned(16))) char s_mem[W * WAVE_B];
+    __shared__ float s_m[W][16], s_l[W][16];
     // the scales of a wave's tile, [K, V][block][row], V's rows in the order 8 (r % 4) + r / 4
-    __shared__ __attribute__((aligned(16))) f16 s_sc[D_WAVES][2][8][DT + 8];
+    __shared__ __attribute__((aligned(16))) f16 s_sc[W][2][8][DT + 8];
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = uni(tid >> 6);
     const int i = lane & 15, g = lane >> 4;
     const int G = n_q / n_kv, R = T * G;
     const int cap = pg.max_pages << pg.shift;
     char* const mine = s_mem + w * WAVE_B;
-    Run run(pos0, B, T, n_kv, runs, RUN_MIN_Q8, SEQ_COST_Q8, sight, cap);
+    Run run(pos0, B, T, n_kv, cut, sight, cap);
     if (!run.any) return;   // (the whole workgroup)
-    const TileAt tiles(kp, vp, pg, n_kv, run.h, lane);
+    // this wave's kv head; its tiles: the turn-th, and every step-th after it; w0 .. + step - 1
+    // are the head's waves
+    const int step_lg = W_LG - run.heads_lg, step = 1 << step_lg;
+    const int h = (run.h << run.heads_lg) + (w >> step_lg), turn = w & (step - 1), w0 = w - turn;
+    const TileAt tiles(kp, vp, pg, n_kv, h, lane);
 
     for (;;) {
         const int b = uni(run.b);
@@ -470,9 +491,9 @@ paged_decode_q8_kernel(const f16* __restrict__ qg, int q_pitch, const char* __re
 #pragma unroll
                 for (int n = 0; n < 16; ++n) o[nb][n] = (f32x4)(0.f);
             }
-            const int jw = j0 + w;   // this wave's tiles: jw, jw + 4, ... < j1
+            const int jw = j0 + turn;
             if (jw < j1) {
-                auto ids = page_ids<D_WAVES>(pg, b, jw, j1 - 1, [&](int j) { return d.row0(j); });
+                auto ids = page_ids(pg, b, jw, j1 - 1, step_lg, [&](int j) { return d.row0(j); });
                 // B operand: Q[column 16 nb + i][32 ks + 8 g + 0..7]; the column's rows in sight
                 f16x8 q[NB][8];
                 int lo[NB], hi[NB];
@@ -481,7 +502,7 @@ paged_decode_q8_kernel(const f16* __restrict__ qg, int q_pitch, const char* __re
                     const int c = 16 * nb + i;
                     const bool ok = c < R;
                     const int t = ok ? c / G : 0, gq = ok ? c - t * G : 0;
-                    const f16* row = qg + (((size_t)b * T + t) * n_q + run.h * G + gq) * q_pitch + 8 * g;
+                    const f16* row = qg + (((size_t)b * T + t) * n_q + h * G + gq) * q_pitch + 8 * g;
 #pragma unroll
                     for (int s = 0; s < 8; ++s) q[nb][s] = ok ? *(const f16x8*)(row + 32 * s) : (f16x8)(0);
                     token_range((long long)pos0[b] + t, sight.window, cap, lo[nb], hi[nb]);
@@ -501,35 +522,46 @@ paged_decode_q8_kernel(const f16* __restrict__ qg, int q_pitch, const char* __re
                     return x;
                 };
                 Where x = where(jw);
-                KTile kt;
-                VTile vt;
-                tiles.load(kt, x.at);
-                tiles.load(vt, x.at);
-                const int j_last = jw + (j1 - 1 - jw) / D_WAVES * D_WAVES;
-                for (int j = jw; j < j1; j += D_WAVES) {
-                    const Where xn = where(min(j + D_WAVES, j_last));
+                Tile8 kt, vt;
+                tiles.load_k(kt, x.at);
+                tiles.load_v(vt, x.at);
+                const int j_last = jw + ((j1 - 1 - jw) & -step);
+                for (int j = jw; j < j1; j += step) {
+                    const Where xn = where(min(j + step, j_last));
                     const TileMask mask(x.r0, x.id0, x.id1, sight.sinks);
                     const bool whole = mask.all(d.lo1, d.hi0);   // for every token (uniform)
-                    // scores: s[nb][4 rb + e] of column i, row 16 rb + 4 g + e
-                    float s[NB][8];
                     const int sc_row = lane & 31, sc_blk = 4 * (lane >> 5);
 #pragma unroll
                     for (int e = 0; e < 4; ++e) s_sc[w][0][sc_blk + e][sc_row] = kt.sc[e];
 #pragma unroll
+                    for (int n = 0; n < 8; ++n) *(u32x4*)(mine + (4 * n + g) * K_PITCH + 16 * i) = kt.x[n];
+                    tiles.load_k(kt, xn.at);
+                    // scores: s[nb][4 rb + e] of column i, row 16 rb + 4 g + e
+                    float s[NB][8];
+                    const char* krow = mine + i * K_PITCH + 8 * g;
+#pragma unroll
                     for (int rb = 0; rb < 2; ++rb) {
-                        f32x4 c[NB];
+                        f32x4 c[NB], p[NB], pn[NB];
+                        auto product = [&](int ks, f32x4 (&d)[NB]) {
+                            const f16x8 a = q8_ints(*(const u32x2*)(krow + 16 * rb * K_PITCH + 32 * ks));
+#pragma unroll
+                            for (int nb = 0; nb < NB; ++nb)
+                                d[nb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q[nb][ks], (f32x4)(0.f),
+                                                                               0, 0, 0);
+                        };
+                        product(0, p);
 #pragma unroll
                         for (int nb = 0; nb < NB; ++nb) c[nb] = (f32x4)(0.f);
 #pragma unroll
                         for (int ks = 0; ks < 8; ++ks) {
-                            const f16x8 a = q8_ints(kt.k[rb][ks]);
+                            // (the next block's product runs while this one's scale is applied)
+                            if (ks < 7) product(ks + 1, pn);
                             const f16x4 sc = *(const f16x4*)&s_sc[w][0][ks][16 * rb + 4 * g];
 #pragma unroll
                             for (int nb = 0; nb < NB; ++nb) {
-                                const f32x4 p = __builtin_amdgcn_mfma_f32_16x16x32_f16(
-                                    a, q[nb][ks], (f32x4)(0.f), 0, 0, 0);
 #pragma unroll
-                                for (int e = 0; e < 4; ++e) c[nb][e] = fmaf((float)sc[e], p[e], c[nb][e]);
+                                for (int e = 0; e < 4; ++e) c[nb][e] = fmaf((float)sc[e], p[nb][e], c[nb][e]);
+                                p[nb] = pn[nb];
                             }
                         }
 #pragma unroll
@@ -537,7 +569,6 @@ paged_decode_q8_kernel(const f16* __restrict__ qg, int q_pitch, const char* __re
 #pragma unroll
                             for (int e = 0; e < 4; ++e) s[nb][4 * rb + e] = c[nb][e];
                     }
-                    tiles.load(kt, xn.at);
                     f16x8 p_hi[NB], p_lo[NB];
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
@@ -574,27 +605,20 @@ paged_decode_q8_kernel(const f16* __restrict__ qg, int q_pitch, const char* __re
                         p_lo[nb] =
                             __builtin_convertvector(p - __builtin_convertvector(p_hi[nb], f32x8), f16x8);
                     }
-                    // V to LDS as rows. Rows that no token sees may hold anything: their v
-                    // must not meet the product, where 0 x NaN is a NaN.
-                    const uint32_t any = whole ? ~0u : mask.rows(d.lo0, d.hi1);
+                    // V to LDS as rows. Rows that no token sees may hold any scale: theirs is
+                    // 0, since their v meets the product, where 0 x NaN is a NaN.
+                    const bool on = whole || (mask.rows(d.lo0, d.hi1) >> sc_row & 1);
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        s_sc[w][1][sc_blk + e][8 * (sc_row & 3) + (sc_row >> 2)] = vt.sc[e];
+                        s_sc[w][1][sc_blk + e][8 * (sc_row & 3) + (sc_row >> 2)] = on ? vt.sc[e] : (f16)0;
                     const f16x8 sc = *(const f16x8*)&s_sc[w][1][i >> 1][8 * g];
 #pragma unroll
                     for (int n = 0; n < 8; ++n) {
-                        f16x8 a = q8_values(vt.v[n].x, vt.v[n].y, sc[n]);
-                        f16x8 c = q8_values(vt.v[n].z, vt.v[n].w, sc[n]);
-                        if (!whole) {
-                            const bool on = any >> (4 * n + g) & 1;
-                            a = on ? a : (f16x8)(0);
-                            c = on ? c : (f16x8)(0);
-                        }
                         char* row = mine + (4 * n + g) * V_PITCH + 32 * i;
-                        *(f16x8*)row = a;
-                        *(f16x8*)(row + 16) = c;
+                        *(f16x8*)row = q8_values(vt.x[n].x, vt.x[n].y, sc[n]);
+                        *(f16x8*)(row + 16) = q8_values(vt.x[n].z, vt.x[n].w, sc[n]);
                     }
-                    tiles.load(vt, xn.at);
+                    tiles.load_v(vt, xn.at);
                     // V^T: lane (i, g) of block n takes rows 4 g .. + 3 (and + 16) of dim 16 n
                     // + i; it points at row 4 g + i / 4, dims 16 n + 4 (i % 4). PV_AHEAD
                     // blocks are read ahead of the products.
@@ -624,34 +648,36 @@ paged_decode_q8_kernel(const f16* __restrict__ qg, int q_pitch, const char* __re
                     x = xn;
                 }
             }
-            // the piece's partial: the waves' O weighed against their common maximum
+            // the piece's partial: the O of a head's waves weighed against their common
+            // maximum, 16 columns at a time
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
                 float l = l_run[nb];
                 l += lane_xor(l, 16);
                 l = pair32_sum(l);
-                if (g == 0) s_m[w][16 * nb + i] = m_run[nb], s_l[w][16 * nb + i] = l;
+                if (g == 0) s_m[w][i] = m_run[nb], s_l[w][i] = l;
 #pragma unroll
                 for (int n = 0; n < 16; ++n)
-                    *(f32x4*)(mine + ((16 * nb + i) * O_PITCH + 16 * n + 4 * g) * 4) = o[nb][n];
-            }
-            __syncthreads();
-            for (int c = w; c < R; c += D_WAVES) {
-                float m = s_m[0][c], l = 0.f;
+                    *(f32x4*)(mine + (i * O_PITCH + 16 * n + 4 * g) * 4) = o[nb][n];
+                __syncthreads();
+                for (int c = turn; c < min(R - 16 * nb, 16); c += step) {
+                    float m = -1e30f, l = 0.f;
+                    f32x4 a = (f32x4)(0.f);
 #pragma unroll
-                for (int k = 1; k < D_WAVES; ++k) m = fmaxf(m, s_m[k][c]);
-                f32x4 a = (f32x4)(0.f);
+                    for (int k = 0; k < W; ++k) m = fmaxf(m, s_m[w0 + min(k, step - 1)][c]);
 #pragma unroll
-                for (int k = 0; k < D_WAVES; ++k) {
-                    const float e = fast_exp2(s_m[k][c] - m);
-                    l = fmaf(e, s_l[k][c], l);
-                    a += e * *(const f32x4*)(s_mem + k * WAVE_B + (c * O_PITCH + 4 * lane) * 4);
+                    for (int k = 0; k < W; ++k) {   // (past the head's waves: its last one's, weighed 0)
+                        const int wk = w0 + min(k, step - 1);
+                        const float e = k < step ? fast_exp2(s_m[wk][c] - m) : 0.f;
+                        l = fmaf(e, s_l[wk][c], l);
+                        a += e * *(const f32x4*)(s_mem + wk * WAVE_B + (c * O_PITCH + 4 * lane) * 4);
+                    }
+                    const size_t part = ((size_t)(b + run.run) * n_kv + h) * R + 16 * nb + c;
+                    *(f32x4*)(out.pacc + part * PAGED_HD + 4 * lane) = a;
+                    if (lane == 0) out.pm[part] = m, out.pd[part] = l;
                 }
-                const size_t part = ((size_t)(b + run.run) * n_kv + run.h) * R + c;
-                *(f32x4*)(out.pacc + part * PAGED_HD + 4 * lane) = a;
-                if (lane == 0) out.pm[part] = m, out.pd[part] = l;
+                __syncthreads();
             }
-            __syncthreads();
         }
         if (!run.next(d)) return;
     }
@@ -740,11 +766,16 @@ paged_merge_kernel(const DecPart in, f16* __restrict__ z, int z_pitch, const f16
     *(f16x4*)(z + (size_t)rh * z_pitch + 4 * lane) = out;
 }
 
-// runs a kv head: a workgroup a CU, two where the kernel's registers let a CU hold two
-// (int8 pools and at most 16 query rows)
-int dec_runs(int n_kv, bool q8, int rows) {
-    return std::max(1, cu_count() * (q8 && rows <= 16 ? 2 : 1) / n_kv);
+// A workgroup a CU.
+Cut dec_cut(int n_kv, bool q8, int rows) {
+    Cut c = {std::max(1, cu_count() / n_kv), RUN_MIN_F16, SEQ_COST_F16, 0};
+    if (q8) {
+        c.run_min = q8_waves(rows > 16 ? 2 : 1), c.seq_cost = SEQ_COST_Q8;
+        if (rows <= 16) c.heads_lg = std::min(2, __builtin_ctz((unsigned)n_kv));
+    }
+    return c;
 }
+int most_runs(const Cut& c) { return c.runs << c.heads_lg; }
 
 size_t dec_part(int B, int T, int n_q, int n_kv, int runs, char* work, DecPart& p) {
     const size_t rows = (size_t)(B + runs) * T * n_q;
@@ -762,7 +793,7 @@ size_t fl_attn_decode_paged_work_bytes(int B, int T, int n_q_heads, int n_kv_hea
         n_q_heads % n_kv_heads || (long long)T * (n_q_heads / n_kv_heads) > 32 || head_dim != PAGED_HD)
         return 0;
     DecPart p;
-    return dec_part(B, T, n_q_heads, n_kv_heads, dec_runs(n_kv_heads, true, 1), nullptr, p);
+    return dec_part(B, T, n_q_heads, n_kv_heads, most_runs(dec_cut(n_kv_heads, true, 1)), nullptr, p);
 }
 
 int fl_attn_decode_paged(const void* qg, int q_pitch, const void* kpool, const void* vpool, int q8,
@@ -783,22 +814,33 @@ int fl_attn_decode_paged(const void* qg, int q_pitch, const void* kpool, const v
                "B * max_pages * page_size < 2^36");
     DecPart part;
     const int rows = T * (n_q_heads / n_kv_heads);
-    const int runs = dec_runs(n_kv_heads, q8, rows);
+    const Cut cut = dec_cut(n_kv_heads, q8, rows);
+    const int runs = most_runs(cut);
     if (dec_part(B, T, n_q_heads, n_kv_heads, runs, (char*)work, part) > work_bytes || !work) {
         fl::set_error("work: smaller than fl_attn_decode_paged_work_bytes");
         return FL_ESCRATCH;
     }
     FL_REQUIRE(aligned16(work), "16-byte aligned work");
-    auto split = !q8 ? paged_decode_f16_kernel
-                     : rows > 16 ? paged_decode_q8_kernel<2> : paged_decode_q8_kernel<1>;
-    hipLaunchKernelGGL(split, dim3(runs * n_kv_heads), dim3(64 * D_WAVES), 0, (hipStream_t)stream,
-                       (const f16*)qg, q_pitch, (const char*)kpool, (const char*)vpool, pg, pos0, B, T,
-                       n_q_heads, n_kv_heads, runs, scale * FL_LOG2E, Sight{window, sinks}, part);
+    const dim3 grid(cut.runs * n_kv_heads);
+    const float sl2 = scale * FL_LOG2E;
+    const Sight sight = {window, sinks};
+    if (!q8)
+        hipLaunchKernelGGL(paged_decode_f16_kernel, grid, dim3(64 * D_WAVES), 0, (hipStream_t)stream,
+                           (const f16*)qg, q_pitch, (const char*)kpool, (const char*)vpool, pg, pos0, B, T,
+                           n_q_heads, n_kv_heads, cut, sl2, sight, part);
+    else
+        hipLaunchKernelGGL(rows > 16 ? paged_decode_q8_kernel<2> : paged_decode_q8_kernel<1>, grid,
+                           dim3(64 * q8_waves(rows > 16 ? 2 : 1)), 0, (hipStream_t)stream,
+                           (const f16*)qg, q_pitch, (const char*)kpool, (const char*)vpool, pg, pos0, B, T,
+                           n_q_heads, n_kv_heads, cut, sl2, sight, part);
     rc = fl::check_launch("attn_decode_paged");
     if (rc) return rc;
     const int pairs = B * T * n_q_heads;
     const f16* gate = gated ? (const f16*)qg + PAGED_HD : nullptr;
-    const bool wide = runs >= 2 * B;
+    // four waves a pair where a sequence has 4 partials or more: one context of 500 10.5 us
+    // against 12.3, 4 of 8k 30.0 against 33.2; one wave where it has fewer: 40 of 2k 54.2
+    // against 55.6, 96 of 50 18.5 against 20.6
+    const bool wide = runs >= 4 * B;
     auto merge = wide ? paged_merge_kernel<4> : paged_merge_kernel<1>;
     hipLaunchKernelGGL(merge, dim3(wide ? pairs : (pairs + 3) / 4), dim3(256), 0, (hipStream_t)stream,
                        part, (f16*)z, z_pitch, gate, q_pitch, T, n_q_heads, n_kv_heads, pairs);

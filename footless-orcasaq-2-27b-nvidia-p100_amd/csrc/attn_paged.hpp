@@ -48,45 +48,45 @@ struct TileMask {
     }
 };
 
-// The pages of a sequence's tiles first, first + STEP, ... <= last, asked for in that
+// The pages of a sequence's tiles first, first + 2^lg, ... <= last, asked for in that
 // order: lane l of a wave holds the table's entry for half l & 1 of the (l / 2)-th of 32
 // tiles, and the next 32 tiles' are loaded while those are used (a table entry a tile
 // would put its latency in front of every tile's loads). The entries are checked when
 // they are taken, on the scalar unit, so that nothing waits for the loads before.
-template <int STEP, class Row0>
+template <class Row0>
 struct PageIdsOf {
     const int* row;
     const Pages& pg;
     Row0 row0;
-    int last, base, now, next;
+    int last, lg, base, now, next;
     __device__ __forceinline__ int load(int j) const {
         const int lane = threadIdx.x & 63;
-        const int r = row0(min(j + STEP * (lane >> 1), last)) + 16 * (lane & 1);
+        const int r = row0(min(j + ((lane >> 1) << lg), last)) + 16 * (lane & 1);
         return row[min(r >> pg.shift, pg.max_pages - 1)];   // (rows past the table are masked)
     }
-    __device__ __forceinline__ PageIdsOf(const Pages& pg, int seq, int first, int last, Row0 row0)
-        : row(pg.table + seq * pg.stride), pg(pg), row0(row0), last(last), base(first) {
+    __device__ __forceinline__ PageIdsOf(const Pages& pg, int seq, int first, int last, int lg, Row0 row0)
+        : row(pg.table + seq * pg.stride), pg(pg), row0(row0), last(last), lg(lg), base(first) {
         now = load(first);
-        next = load(first + 32 * STEP);
+        next = load(first + (32 << lg));
     }
     // the pages of tile j's halves, -1 where absent
     __device__ __forceinline__ void at(int j, int& id0, int& id1) {
-        if (j - base >= 32 * STEP) {
-            base += 32 * STEP;
+        if (j - base >= 32 << lg) {
+            base += 32 << lg;
             now = next;
-            next = load(base + 32 * STEP);
+            next = load(base + (32 << lg));
         }
-        const int l = 2 * ((j - base) / STEP);
+        const int l = 2 * ((j - base) >> lg);
         id0 = __builtin_amdgcn_readlane(now, l);
         id1 = __builtin_amdgcn_readlane(now, l + 1);
         id0 = (unsigned)id0 < (unsigned)pg.n_pages ? id0 : -1;
         id1 = (unsigned)id1 < (unsigned)pg.n_pages ? id1 : -1;
     }
 };
-template <int STEP, class Row0>
-__device__ __forceinline__ PageIdsOf<STEP, Row0> page_ids(const Pages& pg, int seq, int first, int last,
-                                                          Row0 row0) {
-    return PageIdsOf<STEP, Row0>(pg, seq, first, last, row0);
+template <class Row0>
+__device__ __forceinline__ PageIdsOf<Row0> page_ids(const Pages& pg, int seq, int first, int last, int lg,
+                                                    Row0 row0) {
+    return PageIdsOf<Row0>(pg, seq, first, last, lg, row0);
 }
 
 // A wave-uniform address in global memory (scalar base, 32-bit lane offsets; a

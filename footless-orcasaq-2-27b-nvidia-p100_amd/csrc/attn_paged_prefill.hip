@@ -238,7 +238,7 @@ paged_prefill_kernel(const f16* __restrict__ q, int q_pitch, const char* __restr
             dense_cut = R64_BK * all.s;
             dense_skip = R64_BK * (all.a - all.s);
         }
-        auto ids = page_ids<1>(pg, seq, j_lo, j_hi - 1, [&](int j) { return walk.row0(j); });
+        auto ids = page_ids(pg, seq, j_lo, j_hi - 1, 0, [&](int j) { return walk.row0(j); });
         // copy tile j into the stage at dst; the pages of its halves
         auto issue = [&](uint32_t dst, int j, int& id0, int& id1) {
             const uint32_t d0 = uni(dst + 8 * w * ROW_B);
