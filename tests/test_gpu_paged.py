@@ -440,6 +440,26 @@ def test_decode_heads(fl, dev, heads, T):
 
 
 @pytest.mark.parametrize("kv8", [False, True])
+@pytest.mark.parametrize("heads,T,B,window", [((24, 4), 1, 64, 0), ((8, 8), 2, 40, 0), ((4, 2), 1, 150, 0),
+                                              ((3, 3), 1, 90, 0), ((24, 4), 3, 64, 0), ((8, 4), 1, 130, 1500)])
+def test_decode_many_long_contexts(fl, dev, heads, T, B, window, kv8):
+    """Batches that give every run many tiles: sequences of unlike lengths over shared
+    pages (one prefix of all, as long as the longest)."""
+    g = gen(65 + B)
+    L, page_size, (n_q, n_kv) = 2200, 32, heads
+    kp, vp, pages, [(K, V)] = filled(fl, g, [L], page_size, kv8, n_kv)
+    lens = [int(x) for x in torch.randint(1900, L + 1, (B,), generator=g)]
+    qg = randn(g, B, T, n_q, 512)
+    z = fl.ops.attn_decode_paged(qg, kp, vp, pages.repeat(B, 1), i32(*[n - T for n in lens]),
+                                 page_size=page_size, n_kv_heads=n_kv, window=window)
+    for b in range(0, B, 7):
+        n = lens[b]
+        want, bound = ref.attention(qg[b, :, :, :256], K[:n], V[:n], None,
+                                    seen_mask(T, n - T, n, window, 0), SCALE, kv8, qg[b, :, :, 256:])
+        check(z[b], want, bound, f"sequence {b}")
+
+
+@pytest.mark.parametrize("kv8", [False, True])
 def test_decode_peaked_scores(fl, dev, kv8):
     run_decode(fl, 61, [2000, 300], 32, kv8, 2, q_scale=4.0)
 
