@@ -155,6 +155,14 @@ struct Run {
 // column, the softmax is in-lane and one exchange, and P, rounded to fp16, is the B
 // operand of O^T = V^T P^T (V^T transposed through LDS into the slice of the wave that
 // owns its 64 dims).
+//
+// Bound by the memory: 6 contexts of 60 - 100k with 18 rows 345 us (2.33 GB, 6.7 TB/s), 64
+// of 100 - 32k with 6 rows 230 (6.6). A wave a tile alone, as over int8 pools, takes 364 and
+// 257: its 16 KiB of K and 16 of V a tile leave registers for one wave a SIMD. Two
+// workgroups a CU: 358, and 4 contexts of 8k 33.7 against 29.5. V is read once by one
+// workgroup, non-temporal; K as well, but its lines by four instructions each.
+// A small call is two launches and their chains of loads (positions, table, rows;
+// partials): one context of 500 7.2 + 4.5 us by the trace, 10.5 in a graph.
 // ---------------------------------------------------------------------------
 constexpr int VTP = 36;             // halves a d row of the V^T slices (32 + pad)
 constexpr int RUN_MIN_F16 = 2;      // tiles a run, at least

@@ -16,7 +16,18 @@
 //     walks laid end to end, cut wherever the cuts fall (CUT): an uncut row tile of a run
 //     goes to z, a cut one leaves partials that paged_piece_merge_kernel combines.
 // Over int8 pools the visible rows are first copied to fp16 (byte scale) in the work
-// buffer, absent and unwritten rows as zeros, and the same kernel walks that copy (DENSE).
+// buffer, absent and unwritten rows as zeros, and the same kernel walks that copy (DENSE):
+// K, V and P are each rounded once, so z is off by about twice the rounding of z itself
+// (1.4 times over fp16 pools, where P's is the only one).
+//
+// Bound by the matrix cores: 8192 fresh tokens at 24 q and 4 kv heads 830 us, 1.0 PFLOP/s of
+// the 1.3 that a large fp16 product reaches; the softmax between the two products of a tile
+// and a row tile's start and end (ITEM_COST) are the difference. Four chunks of 1024 with
+// a window 450 - 470 us (0.8: short walks), six of 1 - 1024 tokens at 0 - 60k over int8 1.25
+// ms, 117 us of it the copy (6.3 TB/s).
+// The wave's registers are all taken. A spill is not only slow but wrong here: the O
+// accumulators are written by inline-asm MFMAs, whose hazards the compiler does not see
+// when it stores them. Its resource report has to say 0 spilled VGPRs.
 #include "attn_paged.hpp"
 #include "attn_r64.hpp"
 
@@ -33,7 +44,8 @@ namespace {
 
 constexpr int MAX_SEQS = FL_PAGED_MAX_SEQS_PREFILL;
 constexpr int THREADS = 256;
-constexpr int OUT_ROWS = 8;    // rows whose gates are in flight when a row tile ends
+constexpr int OUT_ROWS = 8;    // rows whose gates are in flight when a row tile ends (4, 8, 16:
+                               // 1075, 1006, 1003 us for 8192 fresh tokens)
 
 // Packed chunks: sequence b's tokens are start[b] .. start[b + 1] - 1, the first at
 // position pos0[b], its row tiles tile0[b] .. tile0[b + 1] - 1; dense[b]: its first row in
@@ -540,12 +552,15 @@ int dense_rows(int T, int pos0, const Sight& sight) {
     return T == 0 ? 0 : R64_BK * make_walk(pos0, pos0 + T - 1, sight).n;
 }
 
-constexpr int ITEM_COST = 12;   // a row tile's fixed cost in tiles (Q, pipeline fill, z)
-constexpr int PIECE_COST = 8;  // a piece's (its 256 KiB partial)
+// The plan's costs, in tiles' time (about 1.3 us).
+constexpr int ITEM_COST = 12;   // a row tile's (Q, pipeline fill, z); 5, 8, 10, 12, 14: 1006,
+                                // 1007, 945, 926, 931 us for 8192 fresh tokens
+constexpr int PIECE_COST = 8;   // a piece's (its 256 KiB partial)
 constexpr int PIECE_MIN = 2;    // tiles a piece, at least
-constexpr int RUN_MIN = 6;      // a run's cost, at least
-constexpr int MERGE_COST = 2;         // the merge's launch, in tiles
-constexpr int SLOTS_PER_TILE = 40;    // partials the merge reads in a tile's time
+constexpr int RUN_MIN = 6;      // a run's cost, at least; 20, 8, 6, 3: 80, 57, 57, 56 us for 1024
+                                // fresh tokens, 62, 41, 40, 38 for 37 at 3001
+constexpr int MERGE_COST = 2;        // the merge's launch
+constexpr int SLOTS_PER_TILE = 40;   // partials the merge reads in a tile's time
 
 struct CallPlan {
     bool cut;
@@ -616,7 +631,9 @@ long long cut_plan(const std::vector<int>& n, int n_kv, int most, CallPlan& cp) 
 }
 
 // The plan of whole row tiles, the heaviest first to the lightest run, then moves and swaps
-// off the heaviest run while they shorten it; and its cost, 0 where its list does not fit.
+// off the heaviest run while they shorten it (8192 fresh tokens 0.89 -> 0.83 ms; 0.1 ms of
+// host time for their 192 row tiles, up to 2.4 for a thousand unlike ones, once for the layers
+// of a step); and its cost, 0 where its list does not fit.
 long long whole_plan(const std::vector<int>& n, int most, Plan& p) {
     const int N = (int)n.size();
     if (N > LIST_MAX) return 0;
@@ -683,6 +700,8 @@ void make_plan(const Chunks& ch, int G, int n_kv, const Sight& sight, int n_cu, 
     const long long cut = cut_plan(n, n_kv, most, cp);
     Plan whole;
     const long long w = whole_plan(n, most, whole);
+    // (whole / cut, us: 8192 fresh tokens 826 / 895, 130 fresh 30.9 / 32.2, four chunks of 1024
+    // with a window 549 / 449, 1024 at 30000 1871 / 786, 37 at 3001 200 / 40)
     cp.cut = w == 0 || cut < w;
     if (!cp.cut) {
         cp.plan = whole;
