@@ -140,24 +140,17 @@ attn_prep_kernel(const f16* q, f16* qo, int q_pitch, f16* k, int k_pitch,
         return hd < n_q_heads ? ((size_t)t * n_q_heads + hd) * q_pitch
                               : ((size_t)t * n_kv_heads + hd - n_q_heads) * k_pitch;
     };
-    f16x4 y[RPW], v_row;
-    f32x4 weight;
-    auto load_rows = [&] {
-#pragma unroll
-        for (int r = 0; r < RPW; ++r) {
-            const int hd = head_of(r);
-            y[r] = *(const f16x4*)((hd < n_q_heads ? q : k) + offset_of(hd) + 4 * lane);
-        }
-    };
-    auto load_v = [&](int h) { return *(const f16x4*)(v + ((size_t)t * n_kv_heads + h) * PR_HD + 4 * lane); };
     // One row a wave: few tokens, a chain of latencies, so all that the row needs is asked
     // for ahead of the table. (With 7 the registers cost a wave a SIMD.)
     constexpr bool EARLY = RPW == 1;
-    if (EARLY) {
-        load_rows();
+    f16x4 y[RPW], v_row;
+    f32x4 weight;
+    if constexpr (EARLY) {
         const int hd = head_of(0);
+        y[0] = *(const f16x4*)((hd < n_q_heads ? q : k) + offset_of(hd) + 4 * lane);
         if (NORM) weight = *(const f32x4*)((hd < n_q_heads ? wq : wk) + 4 * lane);
-        if (STORE && hd >= n_q_heads) v_row = load_v(hd - n_q_heads);
+        if (STORE && hd >= n_q_heads)
+            v_row = *(const f16x4*)(v + ((size_t)t * n_kv_heads + hd - n_q_heads) * PR_HD + 4 * lane);
     }
     const int half_r = rope_dim >> 1;
     if (ROPE) {
@@ -171,7 +164,13 @@ attn_prep_kernel(const f16* q, f16* qo, int q_pitch, f16* k, int k_pitch,
         __syncthreads();
     }
     if (hd0 + w >= heads) return;   // wave-uniform
-    if (!EARLY) load_rows();
+    if constexpr (!EARLY) {
+#pragma unroll
+        for (int r = 0; r < RPW; ++r) {
+            const int hd = head_of(r);
+            y[r] = *(const f16x4*)((hd < n_q_heads ? q : k) + offset_of(hd) + 4 * lane);
+        }
+    }
     if (NORM) {
         // every row's sum of squares on every lane; then the square roots and divides of
         // all rows at once, row r's on lane r
@@ -243,7 +242,8 @@ attn_prep_kernel(const f16* q, f16* qo, int q_pitch, f16* k, int k_pitch,
             if (is_q) orow = qo + ((size_t)t * n_q_heads + h) * rows.qo_pitch;
         if ((NORM || ROPE) && (is_q || !PAGED)) *(f16x4*)(orow + 4 * lane) = y[r];
         if (STORE && !is_q && (!PAGED || cache_row >= 0)) {
-            const f16x4 vin = EARLY ? v_row : load_v(h);
+            const f16x4 vin =
+                EARLY ? v_row : *(const f16x4*)(v + ((size_t)t * n_kv_heads + h) * PR_HD + 4 * lane);
             const size_t crow = (size_t)cache_row * n_kv_heads + h;
             if constexpr (Q8) {
                 const size_t vals = (size_t)max_pos * n_kv_heads * PR_HD;   // scales follow
