@@ -364,7 +364,10 @@ int fl_attention_prefill_q8(const void* q, int q_pitch, const void* k_new, const
  * the first at position pos0[b] (starts [B + 1] nondecreasing, pos0 [B]: device
  * arrays, so that a captured call can be replayed at other positions). Tokens
  * before starts[0], behind starts[B] or at a negative position are left as
- * they are. head_dim 256, B <= FL_PAGED_MAX_SEQS; pools 16-byte aligned. */
+ * they are. head_dim 256, B <= FL_PAGED_MAX_SEQS; pools 16-byte aligned.
+ * A NaN or infinity in a v row reaches the queries that see the row, and may
+ * reach others computed with them (of a sequence's call: rows that none of its
+ * queries sees never do). */
 
 /* Store: k, v rows [n_kv_heads][256] f16, tokens k_stride / v_stride elements
  * apart (multiples of 8, 16-byte aligned), into their positions; q8 quantised as
@@ -402,8 +405,8 @@ int fl_attn_prep_paged(void* qg, int q_pitch, const void* k, const void* v, cons
  * none gives 0. q [sum Ts][n_q_heads][q_pitch] f16; gated: then z = f16_sat(z *
  * sigmoid(gate)), the gate the 256 halves after q in a head's row. z
  * [sum Ts][n_q_heads][z_pitch]. work: fl_attention_prefill_paged_work_bytes of
- * the same arguments, 16-byte aligned. pos0s[b] + Ts[b] <= max_pages *
- * page_size. */
+ * the same arguments, 16-byte aligned, one for each call that may overlap with
+ * another. pos0s[b] + Ts[b] <= max_pages * page_size. */
 size_t fl_attention_prefill_paged_work_bytes(const int* Ts, const int* pos0s, int B, int n_q_heads,
                                              int n_kv_heads, int head_dim, int window, int sinks,
                                              int q8);
