@@ -320,7 +320,8 @@ def test_prefill_window_and_sinks(fl, dev, window, sinks, kv8):
     run_prefill(fl, window, [(260, 0), (70, 777), (1, 900), (130, 100)], 32, kv8, window, sinks)
 
 
-@pytest.mark.parametrize("heads", [(1, 1), (4, 4), (8, 1), (32, 8), (6, 2), (64, 2), (3, 3), (40, 1), (16, 16)])
+@pytest.mark.parametrize("heads", [(1, 1), (4, 4), (8, 1), (32, 8), (6, 2), (64, 2), (3, 3), (40, 1), (16, 16),
+                                   (300, 1)])
 def test_prefill_heads(fl, dev, heads):
     run_prefill(fl, 5, [(70, 130), (9, 0)], 16, False, heads=heads)
     run_prefill(fl, 6, [(33, 300)], 64, True, 50, 2, heads=heads, gated=False)
@@ -587,6 +588,63 @@ def test_a_captured_step_replays_at_new_positions(fl, dev, kv8):
             got[1][0], got[2][0], want[1][0], want[2][0] = 0, 0, 0, 0
         for a, b in zip(got, want):
             assert torch.equal(a, b), i
+
+
+@pytest.mark.parametrize("kv8", [False, True])
+def test_captured_chunks_replay_over_new_rows(fl, dev, kv8):
+    """Chunks of three sequences, some cut between workgroups, captured once; replays
+    after the queries, the cached rows and the table changed equal the eager calls."""
+    g, ops, P = gen(105), fl.ops, 32
+    Ts, p0s = [200, 3, 70], [1500, 700, 0]
+    lens = [t + p for t, p in zip(Ts, p0s)]
+    kp, vp, pages, _ = filled(fl, g, lens, P, kv8)
+    qg = randn(g, sum(Ts), 24, 512)
+    tables = [pages.clone(), pages.clone()]
+    tables[1][0, 3] = -1
+    tables[1][0, 5:9] = pages[0, 5:9].flip(0)
+    call = lambda: ops.attention_prefill_paged(qg, kp, vp, pages, Ts, p0s, page_size=P, gated=True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        out = call()
+    for i in range(4):
+        qg.copy_(randn(g, sum(Ts), 24, 512))
+        pages.copy_(tables[i % 2])
+        rows = randn(g, lens[1], 4, 256)
+        ops.paged_kv_store(rows, rows, kp, vp, pages[1:2], i32(0, lens[1]), i32(0), page_size=P)
+        gr.replay()
+        torch.cuda.synchronize()
+        got, want = out.clone(), call()
+        torch.cuda.synchronize()
+        assert torch.isfinite(got).all() and torch.equal(got, want), i
+
+
+@pytest.mark.parametrize("kv8", [False, True])
+def test_decode_of_as_many_sequences_as_a_call_takes(fl, dev, kv8):
+    """1024 sequences, a few rows each and some without any; then none with a row."""
+    g, P, B = gen(106), 16, 1024
+    lens = [int(x) for x in torch.randint(0, 60, (B,), generator=g)]
+    kp, vp, pages, caches = filled(fl, g, lens, P, kv8)
+    qg = randn(g, B, 1, 24, 512)
+    z = fl.ops.attn_decode_paged(qg, kp, vp, pages, i32(*[n - 1 for n in lens]), page_size=P)
+    for b in range(0, B, 31):
+        if lens[b] == 0:
+            assert not z[b].any()
+            continue
+        want, bound = ref.attention(qg[b, :, :, :256], *caches[b], None, seen_mask(1, lens[b] - 1, lens[b], 0, 0),
+                                    SCALE, kv8, qg[b, :, :, 256:])
+        check(z[b], want, bound, f"sequence {b} of {lens[b]} rows")
+    empty = torch.tensor([n == 0 for n in lens], device="cuda")
+    assert empty.any() and not z[empty].any()
+    z = fl.ops.attn_decode_paged(qg, kp, vp, pages, i32(*([-1] * B)), page_size=P)
+    assert not z.any()
+    with pytest.raises((ValueError, fl._lib.FlError)):
+        fl.ops.attn_decode_paged(torch.cat([qg, qg[:1]]), kp, vp, torch.cat([pages, pages[:1]]),
+                                 i32(*([0] * (B + 1))), page_size=P)
 
 
 def test_calls_on_two_streams(fl, dev):
