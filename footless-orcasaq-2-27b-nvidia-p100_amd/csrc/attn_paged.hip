@@ -358,7 +358,7 @@ paged_decode_f16_kernel(const f16* __restrict__ qg, int q_pitch, const char* __r
 // ---------------------------------------------------------------------------
 // int8 pools. A wave takes tiles alone, over all 256 dims: no barrier and no exchange until
 // the piece ends, where the O, maxima and sums of a head's waves are combined through LDS.
-//   S^T (32 kv x 16 NB columns) = K Q^T   A operand: lane (i, g) row 16 rb + i, dims 32 ks
+//   S^T (32 kv x 16 columns) = K Q^T      A operand: lane (i, g) row 16 rb + i, dims 32 ks
 //                                         + 8 g .. + 7
 //   softmax                               a lane holds column i's rows 4 g + e of both
 //                                         halves; the maximum is exchanged only when
@@ -375,14 +375,15 @@ paged_decode_f16_kernel(const f16* __restrict__ qg, int q_pitch, const char* __r
 // whose only one is P's. (With f16(byte scale) for K and V and P in one term it is 1.5 times
 // as large.)
 //
-// What it reaches: 64 contexts of 100 - 32k 145 us (812 MB, 5.6 TB/s), 64 of 30 - 50k 869
-// (6.3), 4 of 100k with 18 rows 178 (4.6). With 16 rows it is bound by the memory: without its
+// What it reaches: 64 contexts of 100 - 32k 144 us (812 MB, 5.7 TB/s), 64 of 30 - 50k 865
+// (6.3), 4 of 100k with 18 rows 169 (4.9). With 16 rows it is bound by the memory: without its
 // products it takes as long, and what a workgroup's waves read at a time counts. K in operand
 // order from memory (8 bytes a lane, 32 of a row an instruction), a head a workgroup and two
 // workgroups of 4 waves a CU: 165; 8 waves with K through LDS 159; four heads a workgroup 145.
-// With 17 - 32 rows O and Q leave registers for one wave a SIMD, whose chain of products and
-// conversions shows: 151 us without them. Its columns shared out to two waves, with 8 a CU,
-// each converting all of K and V: 229.
+// With 17 - 32 rows O and Q leave a wave alone registers for one a SIMD, whose chain of
+// products and conversions shows (4 of 100k 184 us, 151 without them; 4 of 8k 31), so a pair
+// of waves shares a tile there: 169, 28.7. The columns shared out to two waves instead, each
+// converting all of K and V: 229.
 // ---------------------------------------------------------------------------
 constexpr int K_PITCH = PAGED_HD + 16;       // bytes a K row in LDS (a b64 of 16 rows meets all banks)
 constexpr int V_PITCH = 2 * PAGED_HD + 32;   // bytes a V row in LDS (the 32 spread rows over banks)
@@ -454,17 +455,45 @@ __device__ __forceinline__ f16x8 q8_values(uint32_t a, uint32_t b, f16 s) {
     return (f16x8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
 }
 
-// waves a workgroup, one a CU, by the blocks of 16 query columns: what its registers hold
-constexpr int q8_waves(int NB) { return NB == 1 ? 8 : 4; }
+// A V^T operand of 16 dims: lane (i, g) takes rows 4 g .. + 3 (and + 16) of dim i; it points
+// at row 4 g + i / 4, dims 4 (i % 4) ..
+__device__ __forceinline__ f16x8 v_frag(const char* at) {
+    const f16x4 va =
+        __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at));
+    const f16x4 vb = __builtin_bit_cast(
+        f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 16 * V_PITCH)));
+    return (f16x8){va[0], va[1], va[2], va[3], vb[0], vb[1], vb[2], vb[3]};
+}
 
-// NB: blocks of 16 query columns
-template <int NB>
-__global__ void __launch_bounds__(64 * q8_waves(NB))
+// Column c of the O's that the holders w0 .. w0 + step - 1 (of W) left in LDS, O_PITCH floats
+// a column and `bytes` a holder, weighed against their common maximum, to partial `part`.
+template <int W>
+__device__ __forceinline__ void store_partial(const DecPart& out, size_t part, const float (*s_m)[16],
+                                              const float (*s_l)[16], const char* s_o, int bytes, int w0,
+                                              int step, int c, int lane) {
+    float m = -1e30f, l = 0.f;
+    f32x4 a = (f32x4)(0.f);
+#pragma unroll
+    for (int k = 0; k < W; ++k) m = fmaxf(m, s_m[w0 + min(k, step - 1)][c]);
+#pragma unroll
+    for (int k = 0; k < W; ++k) {   // (past the last holder: it once more, weighed 0)
+        const int wk = w0 + min(k, step - 1);
+        const float e = k < step ? fast_exp2(s_m[wk][c] - m) : 0.f;
+        l = fmaf(e, s_l[wk][c], l);
+        a += e * *(const f32x4*)(s_o + wk * bytes + (c * O_PITCH + 4 * lane) * 4);
+    }
+    *(f32x4*)(out.pacc + part * PAGED_HD + 4 * lane) = a;
+    if (lane == 0) out.pm[part] = m, out.pd[part] = l;
+}
+
+// Up to 16 query rows.
+constexpr int Q8_WAVES = 8;
+__global__ void __launch_bounds__(64 * Q8_WAVES)
 paged_decode_q8_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict__ kp,
                        const char* __restrict__ vp, const Pages pg, const int* __restrict__ pos0, int B,
                        int T, int n_q, int n_kv, const Cut cut, float sl2, const Sight sight,
                        const DecPart out) {
-    constexpr int W = q8_waves(NB), W_LG = W == 8 ? 3 : 2;
+    constexpr int W = Q8_WAVES;
     // K and V of a wave's tile while it walks, O of the waves when a piece ends
     constexpr int WAVE_B = std::max(DT * V_PITCH, 16 * O_PITCH * 4);
     __shared__ __attribute__((aligned(16))) char s_mem[W * WAVE_B];
@@ -481,7 +510,7 @@ paged_decode_q8_kernel(const f16* __restrict__ qg, int q_pitch, const char* __re
     if (!run.any) return;   // (the whole workgroup)
     // this wave's kv head; its tiles: the turn-th, and every step-th after it; w0 .. + step - 1
     // are the head's waves
-    const int step_lg = W_LG - run.heads_lg, step = 1 << step_lg;
+    const int step_lg = 3 - run.heads_lg, step = 1 << step_lg;
     const int h = (run.h << run.heads_lg) + (w >> step_lg), turn = w & (step - 1), w0 = w - turn;
     const TileAt tiles(kp, vp, pg, n_kv, h, lane);
 
@@ -491,30 +520,22 @@ paged_decode_q8_kernel(const f16* __restrict__ qg, int q_pitch, const char* __re
         int j0, j1;
         run.piece(d, out, j0, j1);
         if (j1 > j0) {
-            f32x4 o[NB][16];
-            float m_run[NB], l_run[NB];   // l: of this lane's rows, summed when the piece ends
+            f32x4 o[16];
+            float m_run = -1e30f, l_run = 0.f;   // l: of this lane's rows, summed when the piece ends
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-                m_run[nb] = -1e30f, l_run[nb] = 0.f;
-#pragma unroll
-                for (int n = 0; n < 16; ++n) o[nb][n] = (f32x4)(0.f);
-            }
+            for (int n = 0; n < 16; ++n) o[n] = (f32x4)(0.f);
             const int jw = j0 + turn;
             if (jw < j1) {
                 auto ids = page_ids(pg, b, jw, j1 - 1, step_lg, [&](int j) { return d.row0(j); });
-                // B operand: Q[column 16 nb + i][32 ks + 8 g + 0..7]; the column's rows in sight
-                f16x8 q[NB][8];
-                int lo[NB], hi[NB];
+                // B operand: Q[column i][32 ks + 8 g + 0..7]; the column's rows in sight
+                const bool ok = i < R;
+                const int t = ok ? i / G : 0, gq = ok ? i - t * G : 0;
+                const f16* qrow = qg + (((size_t)b * T + t) * n_q + h * G + gq) * q_pitch + 8 * g;
+                f16x8 q[8];
 #pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                    const int c = 16 * nb + i;
-                    const bool ok = c < R;
-                    const int t = ok ? c / G : 0, gq = ok ? c - t * G : 0;
-                    const f16* row = qg + (((size_t)b * T + t) * n_q + h * G + gq) * q_pitch + 8 * g;
-#pragma unroll
-                    for (int s = 0; s < 8; ++s) q[nb][s] = ok ? *(const f16x8*)(row + 32 * s) : (f16x8)(0);
-                    token_range((long long)pos0[b] + t, sight.window, cap, lo[nb], hi[nb]);
-                }
+                for (int s = 0; s < 8; ++s) q[s] = ok ? *(const f16x8*)(qrow + 32 * s) : (f16x8)(0);
+                int lo, hi;
+                token_range((long long)pos0[b] + t, sight.window, cap, lo, hi);
                 struct Where {
                     int id0, id1, r0;
                     long long at[2];
@@ -544,75 +565,61 @@ paged_decode_q8_kernel(const f16* __restrict__ qg, int q_pitch, const char* __re
 #pragma unroll
                     for (int n = 0; n < 8; ++n) *(u32x4*)(mine + (4 * n + g) * K_PITCH + 16 * i) = kt.x[n];
                     tiles.load_k(kt, xn.at);
-                    // scores: s[nb][4 rb + e] of column i, row 16 rb + 4 g + e
-                    float s[NB][8];
+                    // scores: s[4 rb + e] of column i, row 16 rb + 4 g + e
+                    float s[8];
                     const char* krow = mine + i * K_PITCH + 8 * g;
 #pragma unroll
                     for (int rb = 0; rb < 2; ++rb) {
-                        f32x4 c[NB], p[NB], pn[NB];
-                        auto product = [&](int ks, f32x4 (&d)[NB]) {
-                            const f16x8 a = q8_ints(*(const u32x2*)(krow + 16 * rb * K_PITCH + 32 * ks));
-#pragma unroll
-                            for (int nb = 0; nb < NB; ++nb)
-                                d[nb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q[nb][ks], (f32x4)(0.f),
-                                                                               0, 0, 0);
+                        auto product = [&](int ks) {
+                            return __builtin_amdgcn_mfma_f32_16x16x32_f16(
+                                q8_ints(*(const u32x2*)(krow + 16 * rb * K_PITCH + 32 * ks)), q[ks],
+                                (f32x4)(0.f), 0, 0, 0);
                         };
-                        product(0, p);
-#pragma unroll
-                        for (int nb = 0; nb < NB; ++nb) c[nb] = (f32x4)(0.f);
+                        f32x4 c = (f32x4)(0.f), p = product(0);
 #pragma unroll
                         for (int ks = 0; ks < 8; ++ks) {
                             // (the next block's product runs while this one's scale is applied)
-                            if (ks < 7) product(ks + 1, pn);
+                            const f32x4 pn = ks < 7 ? product(ks + 1) : p;
                             const f16x4 sc = *(const f16x4*)&s_sc[w][0][ks][16 * rb + 4 * g];
 #pragma unroll
-                            for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) c[nb][e] = fmaf((float)sc[e], p[nb][e], c[nb][e]);
-                                p[nb] = pn[nb];
-                            }
+                            for (int e = 0; e < 4; ++e) c[e] = fmaf((float)sc[e], p[e], c[e]);
+                            p = pn;
                         }
 #pragma unroll
-                        for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                            for (int e = 0; e < 4; ++e) s[nb][4 * rb + e] = c[nb][e];
+                        for (int e = 0; e < 4; ++e) s[4 * rb + e] = c[e];
                     }
-                    f16x8 p_hi[NB], p_lo[NB];
+                    if (!whole) {
+                        const uint32_t see = mask.rows(lo, hi) >> (4 * g);
 #pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) {
-                        if (!whole) {
-                            const uint32_t see = mask.rows(lo[nb], hi[nb]) >> (4 * g);
-#pragma unroll
-                            for (int r = 0; r < 8; ++r)
-                                s[nb][r] = see & (1u << (16 * (r >> 2) + (r & 3))) ? s[nb][r] : -INFINITY;
-                        }
-                        float mt = s[nb][0];
-#pragma unroll
-                        for (int r = 1; r < 8; ++r) mt = __builtin_elementwise_maximum(mt, s[nb][r]);
-                        mt *= sl2;
-                        // the running maximum only moves when some score is more than
-                        // RESCALE_LOG2 above it: p <= 256 is exact enough in fp16, and O and
-                        // l are rescaled on few tiles
-                        if (__any(mt > m_run[nb] + RESCALE_LOG2)) {
-                            mt = fmaxf(mt, lane_xor(mt, 16));
-                            mt = pair32_max(mt);
-                            const float m_new = mt > m_run[nb] + RESCALE_LOG2 ? mt : m_run[nb];
-                            const float corr = fast_exp2(m_run[nb] - m_new);
-                            m_run[nb] = m_new;
-                            l_run[nb] *= corr;
-#pragma unroll
-                            for (int n = 0; n < 16; ++n) o[nb][n] *= corr;
-                        }
-                        f32x8 p;
-#pragma unroll
-                        for (int r = 0; r < 8; ++r) {
-                            p[r] = fast_exp2(fmaf(s[nb][r], sl2, -m_run[nb]));
-                            l_run[nb] += p[r];
-                        }
-                        p_hi[nb] = __builtin_convertvector(p, f16x8);
-                        p_lo[nb] =
-                            __builtin_convertvector(p - __builtin_convertvector(p_hi[nb], f32x8), f16x8);
+                        for (int r = 0; r < 8; ++r)
+                            s[r] = see & (1u << (16 * (r >> 2) + (r & 3))) ? s[r] : -INFINITY;
                     }
+                    float mt = s[0];
+#pragma unroll
+                    for (int r = 1; r < 8; ++r) mt = __builtin_elementwise_maximum(mt, s[r]);
+                    mt *= sl2;
+                    // the running maximum only moves when some score is more than
+                    // RESCALE_LOG2 above it: p <= 256 is exact enough in fp16, and O and l
+                    // are rescaled on few tiles
+                    if (__any(mt > m_run + RESCALE_LOG2)) {
+                        mt = fmaxf(mt, lane_xor(mt, 16));
+                        mt = pair32_max(mt);
+                        const float m_new = mt > m_run + RESCALE_LOG2 ? mt : m_run;
+                        const float corr = fast_exp2(m_run - m_new);
+                        m_run = m_new;
+                        l_run *= corr;
+#pragma unroll
+                        for (int n = 0; n < 16; ++n) o[n] *= corr;
+                    }
+                    f32x8 p;
+#pragma unroll
+                    for (int r = 0; r < 8; ++r) {
+                        p[r] = fast_exp2(fmaf(s[r], sl2, -m_run));
+                        l_run += p[r];
+                    }
+                    const f16x8 p_hi = __builtin_convertvector(p, f16x8);
+                    const f16x8 p_lo =
+                        __builtin_convertvector(p - __builtin_convertvector(p_hi, f32x8), f16x8);
                     // V to LDS as rows. Rows that no token sees may hold any scale: theirs is
                     // 0, since their v meets the product, where 0 x NaN is a NaN.
                     const bool on = whole || (mask.rows(d.lo0, d.hi1) >> sc_row & 1);
@@ -627,63 +634,262 @@ paged_decode_q8_kernel(const f16* __restrict__ qg, int q_pitch, const char* __re
                         *(f16x8*)(row + 16) = q8_values(vt.x[n].z, vt.x[n].w, sc[n]);
                     }
                     tiles.load_v(vt, xn.at);
-                    // V^T: lane (i, g) of block n takes rows 4 g .. + 3 (and + 16) of dim 16 n
-                    // + i; it points at row 4 g + i / 4, dims 16 n + 4 (i % 4). PV_AHEAD
-                    // blocks are read ahead of the products.
+                    // PV_AHEAD blocks of V^T are read ahead of their products
                     const char* vt0 = mine + (4 * g + (i >> 2)) * V_PITCH + 8 * (i & 3);
-                    auto frag = [&](int n) {
-                        const f16x4 va = __builtin_bit_cast(
-                            f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(vt0 + 32 * n)));
-                        const f16x4 vb = __builtin_bit_cast(
-                            f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                       (lds_s16x4*)(vt0 + 16 * V_PITCH + 32 * n)));
-                        return (f16x8){va[0], va[1], va[2], va[3], vb[0], vb[1], vb[2], vb[3]};
-                    };
                     f16x8 fr[PV_AHEAD];
 #pragma unroll
-                    for (int n = 0; n < PV_AHEAD; ++n) fr[n] = frag(n);
+                    for (int n = 0; n < PV_AHEAD; ++n) fr[n] = v_frag(vt0 + 32 * n);
 #pragma unroll
                     for (int n = 0; n < 16; ++n) {
                         const f16x8 a = fr[n % PV_AHEAD];
-#pragma unroll
-                        for (int nb = 0; nb < NB; ++nb) {
-                            o[nb][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p_hi[nb], o[nb][n], 0, 0, 0);
-                            o[nb][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p_lo[nb], o[nb][n], 0, 0, 0);
-                        }
-                        if (n + PV_AHEAD < 16) fr[n % PV_AHEAD] = frag(n + PV_AHEAD);
+                        o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p_hi, o[n], 0, 0, 0);
+                        o[n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p_lo, o[n], 0, 0, 0);
+                        if (n + PV_AHEAD < 16) fr[n % PV_AHEAD] = v_frag(vt0 + 32 * (n + PV_AHEAD));
                         __builtin_amdgcn_sched_barrier(0);
                     }
                     x = xn;
                 }
             }
-            // the piece's partial: the O of a head's waves weighed against their common
+            // the piece's partial: the O of a head's waves weighed against their common maximum
+            l_run += lane_xor(l_run, 16);
+            l_run = pair32_sum(l_run);
+            if (g == 0) s_m[w][i] = m_run, s_l[w][i] = l_run;
+#pragma unroll
+            for (int n = 0; n < 16; ++n) *(f32x4*)(mine + (i * O_PITCH + 16 * n + 4 * g) * 4) = o[n];
+            __syncthreads();
+            for (int c = turn; c < R; c += step)
+                store_partial<W>(out, ((size_t)(b + run.run) * n_kv + h) * R + c, s_m, s_l, s_mem, WAVE_B, w0,
+                                 step, c, lane);
+            __syncthreads();
+        }
+        if (!run.next(d)) return;
+    }
+}
+
+// 17 - 32 query rows: a pair of waves shares a tile, each converting 16 of its rows and
+// holding 128 dims of O for all columns. Scores go through LDS, so both know every
+// maximum; two barriers a round, in which each pair takes a tile. (Half of the pairs half a
+// round later: 172; two workgroups of two pairs a CU 173, and 4 of 8k 31.7; the kv heads of
+// a row in one workgroup, as below 17 rows: 175.)
+constexpr int PAIRS = 4;
+constexpr int PAIR_PV_AHEAD = 2;             // (4: spills)
+constexpr int S_PITCH = DT + 4;              // floats a column of scores in LDS
+
+// half a tile of K or V in flight: bytes [row 4 n + g][16 i .. + 15] and the scales of row
+// l % 16, blocks 4 (l / 16 % 2) .. + 3
+struct HalfTile8 {
+    u32x4 x[4];
+    f16x4 sc;
+};
+
+__global__ void __launch_bounds__(128 * PAIRS)
+paged_decode_q8_pairs_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict__ kp,
+                             const char* __restrict__ vp, const Pages pg, const int* __restrict__ pos0,
+                             int B, int T, int n_q, int n_kv, const Cut cut, float sl2, const Sight sight,
+                             const DecPart out) {
+    // a pair's V while it walks, its O when a piece ends
+    constexpr int PAIR_B = std::max(DT * V_PITCH, 16 * O_PITCH * 4);
+    __shared__ __attribute__((aligned(16))) char s_v[PAIRS][PAIR_B];
+    __shared__ __attribute__((aligned(16))) char s_k[2 * PAIRS][DT / 2 * K_PITCH];
+    __shared__ __attribute__((aligned(16))) float s_s[PAIRS][32 * S_PITCH];
+    __shared__ float s_m[PAIRS][16], s_l[PAIRS][16];
+    // the scales of a wave's half, [K, V][block][row], V's rows in the order 4 (r % 4) + r / 4
+    __shared__ __attribute__((aligned(16))) f16 s_sc[2 * PAIRS][2][8][DT / 2 + 8];
+    const int tid = threadIdx.x, lane = tid & 63;
+    const int w = uni(tid >> 6), pair = w >> 1, sub = w & 1;
+    const int i = lane & 15, g = lane >> 4;
+    const int G = n_q / n_kv, R = T * G;
+    const int cap = pg.max_pages << pg.shift;
+    Run run(pos0, B, T, n_kv, cut, sight, cap);
+    if (!run.any) return;   // (the whole workgroup)
+    const int h = run.h;
+    const uint32_t rs = PAGED_HD * n_kv;   // bytes a row
+    const long long values = ((long long)pg.n_pages << pg.shift) * rs;
+    const uint32_t xo = PAGED_HD * h + 16 * i + g * rs;
+    const uint32_t so = 16 * h + 8 * (g & 1) + i * (rs / 16);
+    const int sc_row = i, sc_blk = 4 * (g & 1);
+    auto load = [&](HalfTile8& t, const char* pool, long long at) {
+        t.sc = load_g<f16x4>(uni_global(pool + values + at * (rs / 16)), so);
+        const gptr b = uni_global(pool + at * rs);
+#pragma unroll
+        for (int n = 0; n < 4; ++n) t.x[n] = stream_g<u32x4>(b + 4 * n * rs, xo);
+        asm volatile("" ::: "memory");   // (the compiler would sink the loads to where they are used)
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // LDS written; the next tile's loads stay in flight across the barrier
+    auto barrier = [] { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); };
+
+    for (;;) {
+        const int b = uni(run.b);
+        const DecSeq d = dec_seq(uni(pos0[b]), T, sight, cap);
+        int j0, j1;
+        run.piece(d, out, j0, j1);
+        if (j1 > j0) {
+            f32x4 o[2][8];   // O^T of dims 128 sub + 16 n + 4 g .. + 3, columns 16 nb + i
+            float m_run[2], l_run[2];   // l: of this lane's rows, summed when the piece ends
+            // B operand: Q[column 16 nb + i][32 ks + 8 g + 0..7]; the column's rows in sight
+            f16x8 q[2][8];
+            int lo[2], hi[2];
+#pragma unroll
+            for (int nb = 0; nb < 2; ++nb) {
+                m_run[nb] = -1e30f, l_run[nb] = 0.f;
+#pragma unroll
+                for (int n = 0; n < 8; ++n) o[nb][n] = (f32x4)(0.f);
+                const int c = 16 * nb + i;
+                const bool ok = c < R;
+                const int t = ok ? c / G : 0, gq = ok ? c - t * G : 0;
+                const f16* row = qg + (((size_t)b * T + t) * n_q + h * G + gq) * q_pitch + 8 * g;
+#pragma unroll
+                for (int s = 0; s < 8; ++s) q[nb][s] = ok ? *(const f16x8*)(row + 32 * s) : (f16x8)(0);
+                token_range((long long)pos0[b] + t, sight.window, cap, lo[nb], hi[nb]);
+            }
+            auto ids = page_ids(pg, b, min(j0 + pair, j1 - 1), j1 - 1, 2,
+                                [&](int j) { return d.row0(j); });
+            struct Where {
+                int id0, id1, r0;
+                long long at;   // the pool row of this wave's half
+            };
+            auto where = [&](int j) {
+                Where x;
+                ids.at(j, x.id0, x.id1);
+                x.r0 = d.row0(j);
+                // (an absent page: page 0 is read, its scores masked and its v taken as 0)
+                x.at = ((long long)max(sub ? x.id1 : x.id0, 0) << pg.shift) +
+                       ((x.r0 + 16 * sub) & ((1 << pg.shift) - 1));
+                return x;
+            };
+            // a pair without a tile in the last round (or in any) has its last tile's loads again
+            const int jw = min(j0 + pair, j1 - 1), j_last = jw + ((j1 - 1 - jw) & -PAIRS);
+            Where x = where(jw);
+            HalfTile8 kt, vt;
+            load(kt, kp, x.at);
+            load(vt, vp, x.at);
+            for (int j = j0; j < j1; j += PAIRS) {   // (the workgroup's rounds: uniform)
+                const bool mine = j + pair < j1;
+                const Where xn = where(min(j + pair + PAIRS, j_last));
+                const TileMask mask(x.r0, x.id0, x.id1, sight.sinks);
+                const bool whole = mask.all(d.lo1, d.hi0);   // for every token (uniform)
+                if (mine) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s_sc[w][0][sc_blk + e][sc_row] = kt.sc[e];
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) *(u32x4*)(s_k[w] + (4 * n + g) * K_PITCH + 16 * i) = kt.x[n];
+                }
+                load(kt, kp, xn.at);
+                if (mine) {
+                    // scores of column 16 nb + i, rows 16 sub + 4 g .. + 3
+                    const char* krow = s_k[w] + i * K_PITCH + 8 * g;
+                    f32x4 c[2], p[2], pn[2];
+                    auto product = [&](int ks, f32x4 (&r)[2]) {
+                        const f16x8 a = q8_ints(*(const u32x2*)(krow + 32 * ks));
+#pragma unroll
+                        for (int nb = 0; nb < 2; ++nb)
+                            r[nb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q[nb][ks], (f32x4)(0.f), 0, 0, 0);
+                    };
+                    product(0, p);
+                    c[0] = c[1] = (f32x4)(0.f);
+#pragma unroll
+                    for (int ks = 0; ks < 8; ++ks) {
+                        // (the next block's product runs while this one's scale is applied)
+                        if (ks < 7) product(ks + 1, pn);
+                        const f16x4 sc = *(const f16x4*)&s_sc[w][0][ks][4 * g];
+#pragma unroll
+                        for (int nb = 0; nb < 2; ++nb) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) c[nb][e] = fmaf((float)sc[e], p[nb][e], c[nb][e]);
+                            p[nb] = pn[nb];
+                        }
+                    }
+#pragma unroll
+                    for (int nb = 0; nb < 2; ++nb)
+                        *(f32x4*)&s_s[pair][(16 * nb + i) * S_PITCH + 16 * sub + 4 * g] = c[nb];
+                    // V to LDS as rows. Rows that no token sees may hold any scale: theirs is
+                    // 0, since their v meets the product, where 0 x NaN is a NaN.
+                    const bool on = whole || (mask.rows(d.lo0, d.hi1) >> (16 * sub + sc_row) & 1);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s_sc[w][1][sc_blk + e][4 * (sc_row & 3) + (sc_row >> 2)] = on ? vt.sc[e] : (f16)0;
+                    const f16x4 sc = *(const f16x4*)&s_sc[w][1][i >> 1][4 * g];
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        char* row = s_v[pair] + (16 * sub + 4 * n + g) * V_PITCH + 32 * i;
+                        *(f16x8*)row = q8_values(vt.x[n].x, vt.x[n].y, sc[n]);
+                        *(f16x8*)(row + 16) = q8_values(vt.x[n].z, vt.x[n].w, sc[n]);
+                    }
+                }
+                load(vt, vp, xn.at);
+                barrier();
+                if (mine) {
+                    f16x8 p_hi[2], p_lo[2];
+#pragma unroll
+                    for (int nb = 0; nb < 2; ++nb) {
+                        const float* sr = &s_s[pair][(16 * nb + i) * S_PITCH + 4 * g];
+                        const f32x4 s0 = *(const f32x4*)sr, s1 = *(const f32x4*)(sr + 16);
+                        f32x8 s = {s0[0], s0[1], s0[2], s0[3], s1[0], s1[1], s1[2], s1[3]};
+                        if (!whole) {
+                            const uint32_t see = mask.rows(lo[nb], hi[nb]) >> (4 * g);
+#pragma unroll
+                            for (int r = 0; r < 8; ++r)
+                                s[r] = see & (1u << (16 * (r >> 2) + (r & 3))) ? s[r] : -INFINITY;
+                        }
+                        float mt = s[0];
+#pragma unroll
+                        for (int r = 1; r < 8; ++r) mt = __builtin_elementwise_maximum(mt, s[r]);
+                        mt *= sl2;
+                        if (__any(mt > m_run[nb] + RESCALE_LOG2)) {   // (as above; both waves alike)
+                            mt = fmaxf(mt, lane_xor(mt, 16));
+                            mt = pair32_max(mt);
+                            const float m_new = mt > m_run[nb] + RESCALE_LOG2 ? mt : m_run[nb];
+                            const float corr = fast_exp2(m_run[nb] - m_new);
+                            m_run[nb] = m_new;
+                            l_run[nb] *= corr;
+#pragma unroll
+                            for (int n = 0; n < 8; ++n) o[nb][n] *= corr;
+                        }
+                        f32x8 p;
+#pragma unroll
+                        for (int r = 0; r < 8; ++r) {
+                            p[r] = fast_exp2(fmaf(s[r], sl2, -m_run[nb]));
+                            l_run[nb] += p[r];
+                        }
+                        p_hi[nb] = __builtin_convertvector(p, f16x8);
+                        p_lo[nb] =
+                            __builtin_convertvector(p - __builtin_convertvector(p_hi[nb], f32x8), f16x8);
+                    }
+                    const char* vt0 = s_v[pair] + (4 * g + (i >> 2)) * V_PITCH + 256 * sub + 8 * (i & 3);
+                    f16x8 fr[PAIR_PV_AHEAD];
+#pragma unroll
+                    for (int n = 0; n < PAIR_PV_AHEAD; ++n) fr[n] = v_frag(vt0 + 32 * n);
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) {
+                        const f16x8 a = fr[n % PAIR_PV_AHEAD];
+#pragma unroll
+                        for (int nb = 0; nb < 2; ++nb) {
+                            o[nb][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p_hi[nb], o[nb][n], 0, 0, 0);
+                            o[nb][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p_lo[nb], o[nb][n], 0, 0, 0);
+                        }
+                        if (n + PAIR_PV_AHEAD < 8) fr[n % PAIR_PV_AHEAD] = v_frag(vt0 + 32 * (n + PAIR_PV_AHEAD));
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                }
+                barrier();   // scores and V may be overwritten
+                x = xn;
+            }
+            // the piece's partial: the O of the pairs weighed against their common
             // maximum, 16 columns at a time
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
+            for (int nb = 0; nb < 2; ++nb) {
                 float l = l_run[nb];
                 l += lane_xor(l, 16);
                 l = pair32_sum(l);
-                if (g == 0) s_m[w][i] = m_run[nb], s_l[w][i] = l;
+                if (g == 0 && sub == 0) s_m[pair][i] = m_run[nb], s_l[pair][i] = l;
 #pragma unroll
-                for (int n = 0; n < 16; ++n)
-                    *(f32x4*)(mine + (i * O_PITCH + 16 * n + 4 * g) * 4) = o[nb][n];
+                for (int n = 0; n < 8; ++n)
+                    *(f32x4*)(s_v[pair] + (i * O_PITCH + 128 * sub + 16 * n + 4 * g) * 4) = o[nb][n];
                 __syncthreads();
-                for (int c = turn; c < min(R - 16 * nb, 16); c += step) {
-                    float m = -1e30f, l = 0.f;
-                    f32x4 a = (f32x4)(0.f);
-#pragma unroll
-                    for (int k = 0; k < W; ++k) m = fmaxf(m, s_m[w0 + min(k, step - 1)][c]);
-#pragma unroll
-                    for (int k = 0; k < W; ++k) {   // (past the head's waves: its last one's, weighed 0)
-                        const int wk = w0 + min(k, step - 1);
-                        const float e = k < step ? fast_exp2(s_m[wk][c] - m) : 0.f;
-                        l = fmaf(e, s_l[wk][c], l);
-                        a += e * *(const f32x4*)(s_mem + wk * WAVE_B + (c * O_PITCH + 4 * lane) * 4);
-                    }
-                    const size_t part = ((size_t)(b + run.run) * n_kv + h) * R + 16 * nb + c;
-                    *(f32x4*)(out.pacc + part * PAGED_HD + 4 * lane) = a;
-                    if (lane == 0) out.pm[part] = m, out.pd[part] = l;
-                }
+                for (int c = 2 * pair + sub; c < min(R - 16 * nb, 16); c += 2 * PAIRS)
+                    store_partial<PAIRS>(out, ((size_t)(b + run.run) * n_kv + h) * R + 16 * nb + c, s_m, s_l,
+                                         s_v[0], PAIR_B, 0, PAIRS, c, lane);
                 __syncthreads();
             }
         }
@@ -778,7 +984,7 @@ paged_merge_kernel(const DecPart in, f16* __restrict__ z, int z_pitch, const f16
 Cut dec_cut(int n_kv, bool q8, int rows) {
     Cut c = {std::max(1, cu_count() / n_kv), RUN_MIN_F16, SEQ_COST_F16, 0};
     if (q8) {
-        c.run_min = q8_waves(rows > 16 ? 2 : 1), c.seq_cost = SEQ_COST_Q8;
+        c.run_min = rows > 16 ? PAIRS : Q8_WAVES, c.seq_cost = SEQ_COST_Q8;
         if (rows <= 16) c.heads_lg = std::min(2, __builtin_ctz((unsigned)n_kv));
     }
     return c;
@@ -801,7 +1007,8 @@ size_t fl_attn_decode_paged_work_bytes(int B, int T, int n_q_heads, int n_kv_hea
         n_q_heads % n_kv_heads || (long long)T * (n_q_heads / n_kv_heads) > 32 || head_dim != PAGED_HD)
         return 0;
     DecPart p;
-    return dec_part(B, T, n_q_heads, n_kv_heads, most_runs(dec_cut(n_kv_heads, true, 1)), nullptr, p);
+    const Cut cut = dec_cut(n_kv_heads, true, T * (n_q_heads / n_kv_heads));   // (fp16: as many or fewer)
+    return dec_part(B, T, n_q_heads, n_kv_heads, most_runs(cut), nullptr, p);
 }
 
 int fl_attn_decode_paged(const void* qg, int q_pitch, const void* kpool, const void* vpool, int q8,
@@ -837,8 +1044,8 @@ int fl_attn_decode_paged(const void* qg, int q_pitch, const void* kpool, const v
                            (const f16*)qg, q_pitch, (const char*)kpool, (const char*)vpool, pg, pos0, B, T,
                            n_q_heads, n_kv_heads, cut, sl2, sight, part);
     else
-        hipLaunchKernelGGL(rows > 16 ? paged_decode_q8_kernel<2> : paged_decode_q8_kernel<1>, grid,
-                           dim3(64 * q8_waves(rows > 16 ? 2 : 1)), 0, (hipStream_t)stream,
+        hipLaunchKernelGGL(rows > 16 ? paged_decode_q8_pairs_kernel : paged_decode_q8_kernel, grid,
+                           dim3(64 * Q8_WAVES), 0, (hipStream_t)stream,
                            (const f16*)qg, q_pitch, (const char*)kpool, (const char*)vpool, pg, pos0, B, T,
                            n_q_heads, n_kv_heads, cut, sl2, sight, part);
     rc = fl::check_launch("attn_decode_paged");
