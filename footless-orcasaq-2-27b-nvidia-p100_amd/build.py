@@ -38,7 +38,8 @@ HIPCC_FLAGS = [
 # accumulators are AGPRs held by inline asm); no NaNs and IEEE mode off, so
 # the score max is plain v_max / v_max3 without NaN-quieting canonicalisation
 # (scores are finite or -inf). attn_decode: its accumulators (scores read by the
-# softmax, O rescaled in place) in VGPRs as well. gdn_chunk: the products'
+# softmax, O rescaled in place) in VGPRs as well; so attn_paged and, for its scores,
+# attn_paged_prefill. gdn_chunk: the products'
 # results are split, scaled and fed back as operands by VALU code; in AGPRs
 # each would be copied out first.
 FILE_FLAGS = {
