@@ -2,11 +2,15 @@
 
 The library is loaded once, from this package directory. There is no
 fallback: if it is missing or does not load, importing the op layer raises,
-so nothing can silently run another implementation.
+so nothing can silently run another implementation. The paged entry points
+have a compiled binding as well (fl355_paged.so), which calls the same
+library with less work on the host.
 """
 from __future__ import annotations
 
 import ctypes
+import importlib.machinery
+import importlib.util
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libfl355.so"
@@ -117,11 +121,32 @@ class FlError(RuntimeError):
 
 
 _lib = None
+# the compiled binding of the paged entry points (csrc/paged_binding.cpp), once the library is
+# loaded; None where it has not been built: ops.py then makes the same calls through ctypes
+lane = None
+BINDING_PATH = LIB_PATH.with_name("fl355_paged.so")
+BOUND = ("fl_paged_kv_store", "fl_paged_kv_load", "fl_attn_prep_paged",
+         "fl_attention_prefill_paged_work_bytes", "fl_attention_prefill_paged",
+         "fl_attn_decode_paged_work_bytes", "fl_attn_decode_paged")
+
+
+def _load_binding(L: ctypes.CDLL):
+    if not BINDING_PATH.exists():
+        return None
+    loader = importlib.machinery.ExtensionFileLoader("fl355_paged", str(BINDING_PATH))
+    try:
+        module = importlib.util.module_from_spec(
+            importlib.util.spec_from_file_location("fl355_paged", BINDING_PATH, loader=loader))
+        loader.exec_module(module)
+    except ImportError:   # (built for another torch)
+        return None
+    module.bind(*(ctypes.cast(getattr(L, name), ctypes.c_void_p).value for name in BOUND))
+    return module
 
 
 def lib() -> ctypes.CDLL:
     """The loaded library (raises if it has not been built)."""
-    global _lib
+    global _lib, lane
     if _lib is None:
         if not LIB_PATH.exists():
             raise ImportError(
@@ -132,6 +157,7 @@ def lib() -> ctypes.CDLL:
             fn = getattr(L, name)
             fn.restype = res
             fn.argtypes = args
+        lane = _load_binding(L)
         _lib = L
     return _lib
 
@@ -140,10 +166,15 @@ def call(name: str, *args) -> None:
     """Call an int-returning entry point; raise FlError on a non-zero status."""
     rc = getattr(_lib or lib(), name)(*args)
     if rc != FL_OK:
-        detail = lib().fl_last_error().decode(errors="replace")
-        if rc == FL_EINVAL:
-            raise ValueError(f"{name}: {detail}")
-        raise FlError(name, rc, detail)
+        fail(name, rc)
+
+
+def fail(name: str, rc: int) -> None:
+    """Raise what an entry point's non-zero status says."""
+    detail = lib().fl_last_error().decode(errors="replace")
+    if rc == FL_EINVAL:
+        raise ValueError(f"{name}: {detail}")
+    raise FlError(name, rc, detail)
 
 
 # array types by length: making one costs more than filling it

@@ -19,6 +19,7 @@ CSRC = PKG_DIR / "csrc"
 INCLUDE = REPO / "include"
 BUILD_DIR = REPO / "_build" / "fl355"
 LIB_PATH = PKG_DIR / "libfl355.so"
+BINDING_PATH = PKG_DIR / "fl355_paged.so"
 ARCH = "gfx950"
 
 HIPCC_FLAGS = [
@@ -67,15 +68,45 @@ def _compile(src: Path) -> Path:
     return obj
 
 
+def build_binding(verbose: bool = False) -> Path:
+    """Compile the Python binding of the paged entry points (host code over torch's headers)."""
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension
+
+    cxx = shutil.which("g++") or shutil.which("c++")
+    if cxx is None:
+        raise RuntimeError("no C++ compiler for csrc/paged_binding.cpp")
+    torch_lib = Path(torch.__file__).parent / "lib"
+    tmp = BINDING_PATH.with_suffix(".so.tmp")
+    cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           *(f"-I{p}" for p in cpp_extension.include_paths()),
+           f"-I{sysconfig.get_paths()['include']}", f"-I{INCLUDE}",
+           str(CSRC / "paged_binding.cpp"), "-o", str(tmp),
+           f"-L{torch_lib}", "-ltorch_python", "-ltorch_cpu", "-lc10"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"paged_binding.cpp failed:\n{res.stderr}")
+    os.replace(tmp, BINDING_PATH)
+    if verbose:
+        print(f"built {BINDING_PATH}")
+    return BINDING_PATH
+
+
 def build(verbose: bool = False) -> Path:
-    """Compile every csrc/*.hip for gfx950 and link libfl355.so; returns its path."""
+    """Compile every csrc/*.hip for gfx950 and link libfl355.so, and the binding beside it;
+    returns the library's path."""
     BUILD_DIR.mkdir(parents=True, exist_ok=True)
     sources = sorted(CSRC.glob("*.hip"))
     if not sources:
         raise RuntimeError(f"no HIP sources under {CSRC}")
     workers = min(len(sources), max(1, (os.cpu_count() or 4) // 2), 8)
-    with cf.ThreadPoolExecutor(max_workers=workers) as ex:
+    with cf.ThreadPoolExecutor(max_workers=workers + 1) as ex:
+        binding = ex.submit(build_binding, verbose)
         objs = list(ex.map(_compile, sources))
+        binding.result()
     tmp = LIB_PATH.with_suffix(".so.tmp")
     cmd = [hipcc(), f"--offload-arch={ARCH}", "-shared", "-o", str(tmp), *map(str, objs)]
     res = subprocess.run(cmd, capture_output=True, text=True)

@@ -559,8 +559,10 @@ def paged_pool(n_pages: int, page_size: int, *, kv8: bool = False, n_kv_heads: i
     return torch.zeros((n_pages, page_size, n_kv_heads, head_dim), dtype=F16, device=device)
 
 
-# The checks of a paged call are one expression a group of tensors where they hold
-# (a decode step makes three such calls a layer); what fails is looked for afterwards.
+# A decode step makes three such calls a layer, so a call whose tensors are plain (dense, of
+# the right types and shapes, on the current device) is checked and made by the compiled
+# binding (_lib.lane). What it does not take comes here: the checks are one expression a
+# group of tensors where they hold, and what fails is looked for afterwards.
 
 def _here():
     """The current device's index (-2 without a GPU: no tensor's)."""
@@ -568,6 +570,13 @@ def _here():
         return torch.cuda.current_device() if _device_index is None else _device_index()
     except (RuntimeError, AssertionError):
         return -2
+
+
+def _made(name, r, out):
+    """`out` of a call that the binding made: r is its result, or its status."""
+    if type(r) is int:
+        _lib.fail(name, r)
+    return out
 
 
 def _paged(kpool, vpool, pages, page_size, B, n_kv_heads, head_dim, dev):
@@ -670,6 +679,11 @@ def paged_kv_store(k, v, kpool, vpool, pages, starts, pos0, *, page_size: int,
     head_dim] fp16 (any token stride that is a multiple of 8) to their sequences'
     positions. Tokens outside every sequence are not stored."""
     dev = _here()
+    if dev >= 0 and _lib.lane is not None:
+        r = _lib.lane.kv_store(dev, _stream(), k, v, starts, pos0, kpool, vpool, pages, page_size,
+                               n_kv_heads, head_dim)
+        if r is not None:
+            return _made("fl_paged_kv_store", r, None)
     sp, pp, B = _packed(starts, pos0, dev)
     N = k.shape[0]
     kp, ks = _token_rows(k, "k", N, n_kv_heads, head_dim, dev)
@@ -686,6 +700,11 @@ def paged_kv_load(kpool, vpool, pages, starts, pos0, *, T: int, page_size: int, 
     given), int8 rows as fp16(byte * scale), rows of absent pages as zeros. Rows
     outside every sequence are left as they are (zeros in new tensors)."""
     dev = _here()
+    if k is None and v is None and dev >= 0 and _lib.lane is not None:
+        r = _lib.lane.kv_load(dev, _stream(), starts, pos0, kpool, vpool, pages, T, page_size,
+                              n_kv_heads, head_dim)
+        if r is not None:
+            return _made("fl_paged_kv_load", r, r)
     sp, pp, B = _packed(starts, pos0, dev)
     if T < 0 or (k is None) != (v is None):
         raise ValueError("T >= 0, k and v given both or neither")
@@ -715,6 +734,11 @@ def attn_prep_paged(qg, k, v, wq, wk, kpool, vpool, pages, starts, pos0, *, page
     place, or goes to q_out [N, n_q_heads, pitch]; k is not rewritten. Returns
     the tensor that holds q."""
     dev = _here()
+    if dev >= 0 and _lib.lane is not None:
+        r = _lib.lane.prep(dev, _stream(), qg, k, v, wq, wk, q_out, starts, pos0, kpool, vpool, pages,
+                           page_size, n_q_heads, n_kv_heads, head_dim, rope_dim, theta, eps)
+        if r is not None:
+            return _made("fl_attn_prep_paged", r, qg if q_out is None else q_out)
     sp, pp, B = _packed(starts, pos0, dev)
     N, heads, q_pitch = qg.shape
     if heads != n_q_heads or k.shape != (N, n_kv_heads, head_dim) or v.shape != k.shape:
@@ -759,6 +783,11 @@ def attention_prefill_paged(q, kpool, vpool, pages, Ts, pos0s, *, page_size: int
     Returns z [N, n_q_heads, head_dim] fp16; rows behind the last chunk are left as
     they are (zeros in a new tensor)."""
     dev = _here()
+    if dev >= 0 and _lib.lane is not None:
+        r = _lib.lane.prefill(dev, _stream(), q, kpool, vpool, pages, Ts, pos0s, page_size, window, sinks,
+                              gated, z, work, n_kv_heads, scale)
+        if r is not None:
+            return _made("fl_attention_prefill_paged", r, r)
     B, total = len(Ts), sum(Ts)
     if len(pos0s) != B or B == 0:
         raise ValueError("one T and one pos0 per sequence, one sequence or more")
@@ -812,6 +841,11 @@ def attn_decode_paged(qg, kpool, vpool, pages, pos0, *, page_size: int, window: 
     sees nothing and gives 0. work: uint8 of attn_decode_paged_work_bytes (allocated
     here unless given). Returns z [B, T, n_q_heads, head_dim] fp16."""
     dev = _here()
+    if dev >= 0 and _lib.lane is not None:
+        r = _lib.lane.decode(dev, _stream(), qg, kpool, vpool, pages, pos0, page_size, window, sinks, gate,
+                             z, work, n_kv_heads, scale)
+        if r is not None:
+            return _made("fl_attn_decode_paged", r, r)
     B, T, n_q_heads, q_pitch = qg.shape
     if pos0.dim() != 1 or pos0.numel() != B:
         raise ValueError(f"pos0: expected {B} positions")

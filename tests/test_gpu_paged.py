@@ -717,3 +717,93 @@ def test_refusals_on_the_gpu(fl, dev):
         ops.attention_prefill_paged(qg[0], kp, kp, pages, [1], [64], page_size=16)
     with pytest.raises(ValueError):
         ops.attn_decode_paged(qg, kp, kp, pages, pos0, page_size=16, window=-1)
+
+
+@pytest.mark.parametrize("kv8", [False, True])
+def test_binding_and_ctypes_make_the_same_calls(fl, dev, kv8, monkeypatch):
+    """Every operator through the compiled binding and, with it out of the way, through
+    the Python checks and ctypes: the same bits, given and new outputs, and the same
+    refusals."""
+    ops, P = fl.ops, 32
+    fl._lib.lib()
+    assert fl._lib.lane is not None, "fl355_paged.so is not built"
+    g = gen(141)
+    lens = [100, 1, 333]
+    Ts = [3, 1, 5]
+    p0 = [n - t for n, t in zip(lens, Ts)]
+    pages, n_pages = ref.make_pages(g, lens, P)
+    x = {n: randn(g, 9, h, w) for n, h, w in (("k", 4, 256), ("v", 4, 256), ("qg", 24, 512))}
+    wq, wk = randn(g, 256, dtype=F32, scale=0.1), randn(g, 256, dtype=F32, scale=0.1)
+    rows = randn(g, sum(lens), 4, 256)
+    starts, pos0 = starts_of(Ts), i32(*p0)
+
+    def calls():
+        kp, vp = (ops.paged_pool(n_pages, P, kv8=kv8) for _ in range(2))
+        ops.paged_kv_store(rows, rows, kp, vp, pages, starts_of(lens), i32(0, 0, 0), page_size=P)
+        q = x["qg"].clone()
+        out = torch.zeros(9, 24, 512, dtype=F16, device="cuda")
+        same = ops.attn_prep_paged(q, x["k"], x["v"], wq, wk, kp, vp, pages, starts, pos0, page_size=P)
+        other = ops.attn_prep_paged(x["qg"], x["k"], x["v"], wq, wk, kp, vp, pages, starts, pos0, page_size=P,
+                                    q_out=out)
+        assert same is q and other is out
+        got = list(ops.paged_kv_load(kp, vp, pages, starts_of(lens), i32(0, 0, 0), T=sum(lens) + 1, page_size=P))
+        z = torch.full((9, 24, 300), 5.0, dtype=F16, device="cuda")
+        work = torch.empty(ops.attention_prefill_paged_work_bytes(Ts, p0, kv8=kv8), dtype=torch.uint8,
+                           device="cuda")
+        assert ops.attention_prefill_paged(q, kp, vp, pages, Ts, p0, page_size=P, gated=True, z=z,
+                                           work=work) is z
+        got += [q, out, z, ops.attention_prefill_paged(q, kp, vp, pages, tuple(Ts), p0, page_size=P, window=20,
+                                                       sinks=2),
+                ops.attention_prefill_paged(q, kp, vp, pages, [3, 0, 5], p0, page_size=P)]
+        qd = x["qg"][:6].view(3, 2, 24, 512)
+        zd = torch.full((3, 2, 24, 256), 5.0, dtype=F16, device="cuda")
+        work = torch.empty(ops.attn_decode_paged_work_bytes(3, 2), dtype=torch.uint8, device="cuda")
+        assert ops.attn_decode_paged(qd, kp, vp, pages, pos0, page_size=P, z=zd, work=work) is zd
+        return got + [zd, ops.attn_decode_paged(qd, kp, vp, pages, pos0, page_size=P, window=9, gate=False), kp, vp]
+
+    def refused():
+        """What each call says of arguments that it does not take."""
+        kp, vp = (ops.paged_pool(n_pages, P, kv8=kv8) for _ in range(2))
+        said = []
+        bad = [
+            lambda: ops.paged_kv_store(x["k"], x["v"], kp, vp, pages[:2], starts, pos0, page_size=P),
+            lambda: ops.paged_kv_store(x["k"].float(), x["v"], kp, vp, pages, starts, pos0, page_size=P),
+            lambda: ops.paged_kv_store(x["k"].cpu(), x["v"], kp, vp, pages, starts, pos0, page_size=P),
+            lambda: ops.paged_kv_store(x["k"], x["v"][:8], kp, vp, pages, starts, pos0, page_size=P),
+            lambda: ops.paged_kv_load(kp, vp, pages.long(), starts, pos0, T=9, page_size=P),
+            lambda: ops.paged_kv_load(kp, vp, pages, starts, pos0, T=-1, page_size=P),
+            lambda: ops.paged_kv_load(kp, vp, pages, starts[:3], pos0, T=9, page_size=P),
+            lambda: ops.attn_prep_paged(x["qg"], x["k"], x["v"], wq[:100].clone(), wk, kp, vp, pages, starts, pos0, page_size=P),
+            lambda: ops.attn_prep_paged(x["qg"], x["k"], x["v"], wq, wk, kp, vp, pages, starts, pos0, page_size=P,
+                                        rope_dim=33),
+            lambda: ops.attention_prefill_paged(x["qg"], kp, vp, pages, Ts, [1, 2], page_size=P),
+            lambda: ops.attention_prefill_paged(x["qg"], kp, vp, pages, [3, -1, 5], p0, page_size=P),
+            lambda: ops.attention_prefill_paged(x["qg"], kp, vp, pages, [30, 1, 5], p0, page_size=P),
+            lambda: ops.attention_prefill_paged(x["qg"], kp, vp, pages, Ts, [10000, 1, 5], page_size=P),
+            lambda: ops.attention_prefill_paged(x["qg"], kp, vp, pages, Ts, p0, page_size=P, window=-1),
+            lambda: ops.attn_decode_paged(x["qg"][:3, None], kp, vp, pages, i32(1, 2), page_size=P),
+            lambda: ops.attn_decode_paged(x["qg"].view(3, 3, 24, 512), kp, vp, pages, pos0, page_size=17),
+            lambda: ops.attn_decode_paged(x["qg"][:3, None], kp, vp, pages, pos0, page_size=P, scale=0.0),
+            lambda: ops.attn_decode_paged(torch.zeros(3, 6, 24, 512, dtype=F16, device="cuda"), kp, vp, pages, pos0,
+                                          page_size=P),
+            lambda: ops.attn_decode_paged(x["qg"][:3, None], kp, vp, pages, pos0, page_size=P,
+                                          work=torch.empty(64, dtype=torch.uint8, device="cuda")),
+        ]
+        for i, call in enumerate(bad):
+            try:
+                call()
+            except (TypeError, ValueError, fl._lib.FlError) as e:
+                said.append((type(e), str(e)))
+            else:
+                pytest.fail(f"call {i} was taken")
+        return said
+
+    got, said = calls(), refused()
+    monkeypatch.setattr(fl._lib, "lane", None)
+    want, says = calls(), refused()
+    torch.cuda.synchronize()
+    for i, (a, b) in enumerate(zip(got, want)):
+        assert a.dtype == b.dtype and a.shape == b.shape, i
+        assert torch.equal(a.view(torch.int8) if a.dtype != torch.int8 else a,
+                           b.view(torch.int8) if b.dtype != torch.int8 else b), i
+    assert said == says

@@ -138,3 +138,32 @@ def test_int8_work_is_bounded_by_groups(fl):
         assert rc == 3 and b"work" in fl._lib.lib().fl_last_error()
     assert call(fl, "fl_attn_decode_paged", dict(work=FAKE, wb=64)) == 3
     assert call(fl, "fl_attn_decode_paged", dict(work=FAKE + 8, wb=1 << 30)) == 1
+
+
+def test_binding_is_built_and_declines_what_is_not_plain(fl):
+    """The compiled binding loads with the library and leaves everything that is not a dense
+    tensor on the current GPU (here: nothing is) to the checks in Python."""
+    fl._lib.lib()
+    lane = fl._lib.lane
+    assert lane is not None, "fl355_paged.so is not built"
+    F16, I32 = torch.float16, torch.int32
+    k = torch.zeros(2, 4, 256, dtype=F16)
+    pool, pages = torch.zeros(3, 16, 4, 256, dtype=F16), torch.zeros(1, 2, dtype=I32)
+    starts, pos0 = torch.tensor([0, 2], dtype=I32), torch.zeros(1, dtype=I32)
+    q, w = torch.zeros(2, 24, 512, dtype=F16), torch.zeros(256)
+    calls = {
+        "kv_store": (0, 0, k, k, starts, pos0, pool, pool, pages, 16, 4, 256),
+        "kv_load": (0, 0, starts, pos0, pool, pool, pages, 2, 16, 4, 256),
+        "prep": (0, 0, q, k, k, w, w, None, starts, pos0, pool, pool, pages, 16, 24, 4, 256, 64, 1e7, 1e-6),
+        "prefill": (0, 0, q, pool, pool, pages, [2], [0], 16, 0, 0, True, None, None, 4, 0.0625),
+        "decode": (0, 0, q[:, None], pool, pool, pages.expand(2, 2), pos0.expand(2), 16, 0, 0, True, None, None,
+                   4, 0.0625),
+    }
+    for name, args in calls.items():
+        call = getattr(lane, name)
+        assert call(*args) is None and call(*args[:-1]) is None and call() is None
+        for i in range(len(args)):          # any argument of another kind
+            for other in (None, "x", 1 << 70, 0.5, [1], object()):
+                assert call(*args[:i], other, *args[i + 1:]) is None, (name, i, other)
+    with pytest.raises(TypeError):
+        lane.bind(1, 2)
