@@ -39,14 +39,16 @@ struct DecSeq {
     int s, a, n;
     __device__ __forceinline__ int row0(int j) const { return DT * (j < s ? j : a + j - s); }
 };
-__device__ __forceinline__ void token_range(long long p, int window, int cap, int& lo, int& hi) {
-    hi = (int)max(0ll, min(p + 1, (long long)cap));
-    lo = window > 0 ? (int)max(0ll, min(p - window + 1, (long long)INT_MAX)) : 0;
+// (p saturates at 2^31 - 1, past any row)
+__device__ __forceinline__ void token_range(int p0, int t, int window, int cap, int& lo, int& hi) {
+    const int p = __builtin_elementwise_add_sat(p0, t);
+    hi = max(0, min(p, cap - 1) + 1);
+    lo = window > 0 ? max(0, __builtin_elementwise_sub_sat(p, window - 1)) : 0;
 }
 __device__ __forceinline__ DecSeq dec_seq(int pos0, int T, const Sight& sight, int cap) {
     DecSeq d;
-    token_range(pos0, sight.window, cap, d.lo0, d.hi0);
-    token_range((long long)pos0 + T - 1, sight.window, cap, d.lo1, d.hi1);
+    token_range(pos0, 0, sight.window, cap, d.lo0, d.hi0);
+    token_range(pos0, T - 1, sight.window, cap, d.lo1, d.hi1);
     d.a = d.lo0 / DT;
     const int e = (d.hi1 + DT - 1) / DT;
     const int sk = min(sight.sinks, d.hi1);
@@ -54,6 +56,12 @@ __device__ __forceinline__ DecSeq dec_seq(int pos0, int T, const Sight& sight, i
     d.n = d.s + max(0, e - d.a);
     return d;
 }
+
+// Query heads a kv head, and the token of a query row (rows under 32): r / G by a product.
+struct QHeads {
+    int G, inv;
+    __device__ __forceinline__ int token(int r) const { return r * inv >> 16; }
+};
 
 // inclusive sum over the lanes 0 .. l (DPP row shifts, then the rows' totals)
 __device__ __forceinline__ int wave_scan(int x) {
@@ -162,7 +170,7 @@ struct Run {
 // workgroups a CU: 358, and 4 contexts of 8k 33.7 against 29.5. V is read once by one
 // workgroup, non-temporal; K as well, but its lines by four instructions each.
 // A small call is two launches and their chains of loads (positions, table, rows;
-// partials): one context of 500 7.2 + 4.5 us by the trace, 10.5 in a graph.
+// partials): one context of 500 9.7 us in a graph, where two empty ones take 3.1.
 // ---------------------------------------------------------------------------
 constexpr int VTP = 36;             // halves a d row of the V^T slices (32 + pad)
 constexpr int RUN_MIN_F16 = 2;      // tiles a run, at least
@@ -178,14 +186,14 @@ struct TileF16 {
 __global__ void __launch_bounds__(64 * D_WAVES)
 paged_decode_f16_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict__ kp,
                         const char* __restrict__ vp, const Pages pg, const int* __restrict__ pos0,
-                        int B, int T, int n_q, int n_kv, const Cut cut, float sl2, const Sight sight,
+                        int B, int T, int n_q, int n_kv, const QHeads heads, const Cut cut, float sl2, const Sight sight,
                         const DecPart out) {
     __shared__ __attribute__((aligned(16))) f32x4 s_part[2][2][4][64];
     __shared__ __attribute__((aligned(16))) f16 s_vt[2][4][64][VTP];
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = uni(tid >> 6);
     const int hh = lane >> 5, ql = lane & 31;
-    const int G = n_q / n_kv, R = T * G;
+    const int G = heads.G, R = T * G;
     const int cap = pg.max_pages << pg.shift;
     Run run(pos0, B, T, n_kv, cut, sight, cap);
     if (!run.any) return;   // (the whole workgroup)
@@ -206,16 +214,16 @@ paged_decode_f16_kernel(const f16* __restrict__ qg, int q_pitch, const char* __r
         if (j1 > j0) {
             // this lane's query column: token tq, q head h G + gq
             const bool qvalid = ql < R;
-            const int tq = qvalid ? ql / G : 0, gq = qvalid ? ql - tq * G : 0;
+            const int tq = qvalid ? heads.token(ql) : 0, gq = qvalid ? ql - tq * G : 0;
             int qlo, qhi;
-            token_range((long long)pos0[b] + tq, sight.window, cap, qlo, qhi);
+            token_range(pos0[b], tq, sight.window, cap, qlo, qhi);
             // Q[column 16 nb + (l & 15)][128 (w >> 1) + 32 (l / 16) + 8 ks + 0..7]
             f16x8 qreg[8];
 #pragma unroll
             for (int nb = 0; nb < 2; ++nb) {
                 const int c = 16 * nb + (lane & 15);
                 const bool ok = c < R;
-                const int t = ok ? c / G : 0, g = ok ? c - t * G : 0;
+                const int t = ok ? heads.token(c) : 0, g = ok ? c - t * G : 0;
                 const f16* qrow = qg + (((size_t)b * T + t) * n_q + h * G + g) * q_pitch +
                                   128 * (w >> 1) + 32 * (lane >> 4);
 #pragma unroll
@@ -388,7 +396,7 @@ paged_decode_f16_kernel(const f16* __restrict__ qg, int q_pitch, const char* __r
 constexpr int K_PITCH = PAGED_HD + 16;       // bytes a K row in LDS (a b64 of 16 rows meets all banks)
 constexpr int V_PITCH = 2 * PAGED_HD + 32;   // bytes a V row in LDS (the 32 spread rows over banks)
 constexpr int O_PITCH = PAGED_HD + 4;        // floats a column of O in LDS
-constexpr int PV_AHEAD = 4;                  // V^T fragments read ahead of their product
+constexpr int PV_AHEAD = 2;                  // V^T fragments read ahead of their product
 constexpr int SEQ_COST_Q8 = 6;               // a further piece's fixed cost in tiles (its first loads)
 
 // A tile of K or V in flight: bytes [row 4 n + g][16 i .. + 15] and the scales of row l % 32,
@@ -491,7 +499,7 @@ constexpr int Q8_WAVES = 8;
 __global__ void __launch_bounds__(64 * Q8_WAVES)
 paged_decode_q8_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict__ kp,
                        const char* __restrict__ vp, const Pages pg, const int* __restrict__ pos0, int B,
-                       int T, int n_q, int n_kv, const Cut cut, float sl2, const Sight sight,
+                       int T, int n_q, int n_kv, const QHeads heads, const Cut cut, float sl2, const Sight sight,
                        const DecPart out) {
     constexpr int W = Q8_WAVES;
     // K and V of a wave's tile while it walks, O of the waves when a piece ends
@@ -503,7 +511,7 @@ paged_decode_q8_kernel(const f16* __restrict__ qg, int q_pitch, const char* __re
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = uni(tid >> 6);
     const int i = lane & 15, g = lane >> 4;
-    const int G = n_q / n_kv, R = T * G;
+    const int G = heads.G, R = T * G;
     const int cap = pg.max_pages << pg.shift;
     char* const mine = s_mem + w * WAVE_B;
     Run run(pos0, B, T, n_kv, cut, sight, cap);
@@ -529,13 +537,13 @@ paged_decode_q8_kernel(const f16* __restrict__ qg, int q_pitch, const char* __re
                 auto ids = page_ids(pg, b, jw, j1 - 1, step_lg, [&](int j) { return d.row0(j); });
                 // B operand: Q[column i][32 ks + 8 g + 0..7]; the column's rows in sight
                 const bool ok = i < R;
-                const int t = ok ? i / G : 0, gq = ok ? i - t * G : 0;
+                const int t = ok ? heads.token(i) : 0, gq = ok ? i - t * G : 0;
                 const f16* qrow = qg + (((size_t)b * T + t) * n_q + h * G + gq) * q_pitch + 8 * g;
                 f16x8 q[8];
 #pragma unroll
                 for (int s = 0; s < 8; ++s) q[s] = ok ? *(const f16x8*)(qrow + 32 * s) : (f16x8)(0);
                 int lo, hi;
-                token_range((long long)pos0[b] + t, sight.window, cap, lo, hi);
+                token_range(pos0[b], t, sight.window, cap, lo, hi);
                 struct Where {
                     int id0, id1, r0;
                     long long at[2];
@@ -672,7 +680,6 @@ paged_decode_q8_kernel(const f16* __restrict__ qg, int q_pitch, const char* __re
 // round later: 172; two workgroups of two pairs a CU 173, and 4 of 8k 31.7; the kv heads of
 // a row in one workgroup, as below 17 rows: 175.)
 constexpr int PAIRS = 4;
-constexpr int PAIR_PV_AHEAD = 2;             // (4: spills)
 constexpr int S_PITCH = DT + 4;              // floats a column of scores in LDS
 
 // half a tile of K or V in flight: bytes [row 4 n + g][16 i .. + 15] and the scales of row
@@ -685,7 +692,7 @@ struct HalfTile8 {
 __global__ void __launch_bounds__(128 * PAIRS)
 paged_decode_q8_pairs_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict__ kp,
                              const char* __restrict__ vp, const Pages pg, const int* __restrict__ pos0,
-                             int B, int T, int n_q, int n_kv, const Cut cut, float sl2, const Sight sight,
+                             int B, int T, int n_q, int n_kv, const QHeads heads, const Cut cut, float sl2, const Sight sight,
                              const DecPart out) {
     // a pair's V while it walks, its O when a piece ends
     constexpr int PAIR_B = std::max(DT * V_PITCH, 16 * O_PITCH * 4);
@@ -698,7 +705,7 @@ paged_decode_q8_pairs_kernel(const f16* __restrict__ qg, int q_pitch, const char
     const int tid = threadIdx.x, lane = tid & 63;
     const int w = uni(tid >> 6), pair = w >> 1, sub = w & 1;
     const int i = lane & 15, g = lane >> 4;
-    const int G = n_q / n_kv, R = T * G;
+    const int G = heads.G, R = T * G;
     const int cap = pg.max_pages << pg.shift;
     Run run(pos0, B, T, n_kv, cut, sight, cap);
     if (!run.any) return;   // (the whole workgroup)
@@ -737,11 +744,11 @@ paged_decode_q8_pairs_kernel(const f16* __restrict__ qg, int q_pitch, const char
                 for (int n = 0; n < 8; ++n) o[nb][n] = (f32x4)(0.f);
                 const int c = 16 * nb + i;
                 const bool ok = c < R;
-                const int t = ok ? c / G : 0, gq = ok ? c - t * G : 0;
+                const int t = ok ? heads.token(c) : 0, gq = ok ? c - t * G : 0;
                 const f16* row = qg + (((size_t)b * T + t) * n_q + h * G + gq) * q_pitch + 8 * g;
 #pragma unroll
                 for (int s = 0; s < 8; ++s) q[nb][s] = ok ? *(const f16x8*)(row + 32 * s) : (f16x8)(0);
-                token_range((long long)pos0[b] + t, sight.window, cap, lo[nb], hi[nb]);
+                token_range(pos0[b], t, sight.window, cap, lo[nb], hi[nb]);
             }
             auto ids = page_ids(pg, b, min(j0 + pair, j1 - 1), j1 - 1, 2,
                                 [&](int j) { return d.row0(j); });
@@ -857,18 +864,18 @@ paged_decode_q8_pairs_kernel(const f16* __restrict__ qg, int q_pitch, const char
                             __builtin_convertvector(p - __builtin_convertvector(p_hi[nb], f32x8), f16x8);
                     }
                     const char* vt0 = s_v[pair] + (4 * g + (i >> 2)) * V_PITCH + 256 * sub + 8 * (i & 3);
-                    f16x8 fr[PAIR_PV_AHEAD];
+                    f16x8 fr[PV_AHEAD];
 #pragma unroll
-                    for (int n = 0; n < PAIR_PV_AHEAD; ++n) fr[n] = v_frag(vt0 + 32 * n);
+                    for (int n = 0; n < PV_AHEAD; ++n) fr[n] = v_frag(vt0 + 32 * n);
 #pragma unroll
                     for (int n = 0; n < 8; ++n) {
-                        const f16x8 a = fr[n % PAIR_PV_AHEAD];
+                        const f16x8 a = fr[n % PV_AHEAD];
 #pragma unroll
                         for (int nb = 0; nb < 2; ++nb) {
                             o[nb][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p_hi[nb], o[nb][n], 0, 0, 0);
                             o[nb][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p_lo[nb], o[nb][n], 0, 0, 0);
                         }
-                        if (n + PAIR_PV_AHEAD < 8) fr[n % PAIR_PV_AHEAD] = v_frag(vt0 + 32 * (n + PAIR_PV_AHEAD));
+                        if (n + PV_AHEAD < 8) fr[n % PV_AHEAD] = v_frag(vt0 + 32 * (n + PV_AHEAD));
                         __builtin_amdgcn_sched_barrier(0);
                     }
                 }
@@ -902,7 +909,9 @@ paged_decode_q8_pairs_kernel(const f16* __restrict__ qg, int q_pitch, const char
 // pair (4: few sequences, many partials each; 1: many sequences), lane l holding
 // dims 4 l .. + 3, each wave's partials s = j, j + J, ... in batches whose loads are
 // all issued before any is used, the J sums added in order through LDS.
-constexpr int MG_BATCH = 8;
+// (a small call runs its code once, and fetching it shows: with batches of 2, 4, 8, 16 one
+// context of 500 10.0, 10.0, 10.65, 11.1 us, one of 4k 14.0, 13.9, 15.2, 15.1)
+constexpr int MG_BATCH = 4;
 template <int J>
 __global__ void __launch_bounds__(256)
 paged_merge_kernel(const DecPart in, f16* __restrict__ z, int z_pitch, const f16* __restrict__ gate,
@@ -975,7 +984,7 @@ paged_merge_kernel(const DecPart in, f16* __restrict__ z, int z_pitch, const f16
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         const float v = num[c] * inv;
-        out[c] = f16_sat(gate != nullptr ? v * sigmoid_f((float)gv[c]) : v);
+        out[c] = f16_sat(gate != nullptr ? v * fast_sigmoid((float)gv[c]) : v);
     }
     *(f16x4*)(z + (size_t)rh * z_pitch + 4 * lane) = out;
 }
@@ -1037,24 +1046,26 @@ int fl_attn_decode_paged(const void* qg, int q_pitch, const void* kpool, const v
     }
     FL_REQUIRE(aligned16(work), "16-byte aligned work");
     const dim3 grid(cut.runs * n_kv_heads);
+    const int G = n_q_heads / n_kv_heads;
+    const QHeads heads = {G, 65536 / G + 1};   // exact for rows up to 32
     const float sl2 = scale * FL_LOG2E;
     const Sight sight = {window, sinks};
     if (!q8)
         hipLaunchKernelGGL(paged_decode_f16_kernel, grid, dim3(64 * D_WAVES), 0, (hipStream_t)stream,
                            (const f16*)qg, q_pitch, (const char*)kpool, (const char*)vpool, pg, pos0, B, T,
-                           n_q_heads, n_kv_heads, cut, sl2, sight, part);
+                           n_q_heads, n_kv_heads, heads, cut, sl2, sight, part);
     else
         hipLaunchKernelGGL(rows > 16 ? paged_decode_q8_pairs_kernel : paged_decode_q8_kernel, grid,
                            dim3(64 * Q8_WAVES), 0, (hipStream_t)stream,
                            (const f16*)qg, q_pitch, (const char*)kpool, (const char*)vpool, pg, pos0, B, T,
-                           n_q_heads, n_kv_heads, cut, sl2, sight, part);
+                           n_q_heads, n_kv_heads, heads, cut, sl2, sight, part);
     rc = fl::check_launch("attn_decode_paged");
     if (rc) return rc;
     const int pairs = B * T * n_q_heads;
     const f16* gate = gated ? (const f16*)qg + PAGED_HD : nullptr;
     // four waves a pair where a sequence has 4 partials or more: one context of 500 10.5 us
     // against 12.3, 4 of 8k 30.0 against 33.2; one wave where it has fewer: 40 of 2k 54.2
-    // against 55.6, 96 of 50 18.5 against 20.6
+    // against 55.6, 96 of 50 18.5 against 20.6 (measured with batches of 8)
     const bool wide = runs >= 4 * B;
     auto merge = wide ? paged_merge_kernel<4> : paged_merge_kernel<1>;
     hipLaunchKernelGGL(merge, dim3(wide ? pairs : (pairs + 3) / 4), dim3(256), 0, (hipStream_t)stream,
