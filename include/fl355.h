@@ -406,7 +406,9 @@ int fl_attn_prep_paged(void* qg, int q_pitch, const void* k, const void* v, cons
  * sigmoid(gate)), the gate the 256 halves after q in a head's row. z
  * [sum Ts][n_q_heads][z_pitch]. work: fl_attention_prefill_paged_work_bytes of
  * the same arguments, 16-byte aligned, one for each call that may overlap with
- * another. pos0s[b] + Ts[b] <= max_pages * page_size. */
+ * another. pos0s[b] + Ts[b] <= max_pages * page_size. q8: the rows in sight are
+ * first copied into work as f16(byte * scale), 1 KiB a row and kv head, in
+ * groups of sequences that take 1 GiB together (a sequence alone: what it takes). */
 size_t fl_attention_prefill_paged_work_bytes(const int* Ts, const int* pos0s, int B, int n_q_heads,
                                              int n_kv_heads, int head_dim, int window, int sinks,
                                              int q8);
@@ -421,7 +423,8 @@ int fl_attention_prefill_paged(const void* q, int q_pitch, const void* kpool, co
  * (a device array), T * n_q_heads / n_kv_heads <= 32, the same visibility; a query
  * at a negative position (a padded batch's row) sees nothing and gives 0. qg
  * [B][T][n_q_heads][q_pitch], z [B][T][n_q_heads][z_pitch], work of
- * fl_attn_decode_paged_work_bytes. Calls that overlap need a work buffer each. */
+ * fl_attn_decode_paged_work_bytes. Calls that overlap need a work buffer each.
+ * q8: reads the bytes themselves, k with its exact scale, v as f16(byte * scale). */
 size_t fl_attn_decode_paged_work_bytes(int B, int T, int n_q_heads, int n_kv_heads, int head_dim);
 int fl_attn_decode_paged(const void* qg, int q_pitch, const void* kpool, const void* vpool, int q8,
                          int n_pages, int page_size, const int* pages, int max_pages,
