@@ -670,6 +670,46 @@ def test_calls_on_two_streams(fl, dev):
             assert torch.equal(w[0], x[0]) and torch.equal(w[1], x[1])
 
 
+def test_calls_from_two_threads(fl, dev):
+    """Two threads, each on a stream of its own, with chunks whose plans replace each
+    other's in the library's cache."""
+    import threading
+    g = gen(113)
+    sets = [filled(fl, g, [900, 120], 32, bool(i)) for i in range(2)]
+    qg = [randn(g, 2, 1, 24, 512) for _ in range(2)]
+    qc = [randn(g, 120, 24, 512) for _ in range(2)]
+    pos = i32(899, 119)
+
+    def once(i, n):
+        kp, vp, pages, _ = sets[i]
+        t = 60 + n % 11
+        return (fl.ops.attn_decode_paged(qg[i], kp, vp, pages, pos, page_size=32),
+                fl.ops.attention_prefill_paged(qc[i][:t + 20], kp, vp, pages, [t, 20], [800, 100], page_size=32))
+
+    want = [[once(i, n) for n in range(11)] for i in range(2)]
+    torch.cuda.synchronize()
+    wrong = []
+
+    def work(i):
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for n in range(44):
+                    got = once(i, n)
+                    torch.cuda.current_stream().synchronize()
+                    if not all(torch.equal(a, b) for a, b in zip(got, want[i][n % 11])):
+                        wrong.append((i, n))
+        except Exception as e:
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not wrong, wrong
+
+
 @pytest.mark.parametrize("kv8", [False, True])
 def test_rows_past_4_gib(fl, dev, kv8):
     """Pages whose rows lie past 2^32 bytes of the pool."""
