@@ -11,6 +11,7 @@ from __future__ import annotations
 import ctypes
 import importlib.machinery
 import importlib.util
+import warnings
 from pathlib import Path
 
 LIB_PATH = Path(__file__).resolve().parent / "libfl355.so"
@@ -29,6 +30,7 @@ _IP = ctypes.POINTER(ctypes.c_int)
 # name -> (restype, argtypes); the order is the header's
 SIGNATURES = {
     "fl_abi_version": (_I, []),
+    "fl_header_digest": (ctypes.c_char_p, []),
     "fl_strerror": (ctypes.c_char_p, [_I]),
     "fl_last_error": (ctypes.c_char_p, []),
     "fl_kv_store": (_I, [_P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P]),
@@ -122,7 +124,8 @@ class FlError(RuntimeError):
 
 _lib = None
 # the compiled binding of the paged entry points (csrc/paged_binding.cpp), once the library is
-# loaded; None where it has not been built: ops.py then makes the same calls through ctypes
+# loaded; None where it has not been built, or for another library or torch: ops.py then makes
+# the same calls through ctypes
 lane = None
 BINDING_PATH = LIB_PATH.with_name("fl355_paged.so")
 BOUND = ("fl_paged_kv_store", "fl_paged_kv_load", "fl_attn_prep_paged",
@@ -130,15 +133,22 @@ BOUND = ("fl_paged_kv_store", "fl_paged_kv_load", "fl_attn_prep_paged",
          "fl_attn_decode_paged_work_bytes", "fl_attn_decode_paged")
 
 
-def _load_binding(L: ctypes.CDLL):
-    if not BINDING_PATH.exists():
+def _load_binding(L: ctypes.CDLL, path: Path | None = None):
+    path = path or BINDING_PATH
+    if not path.exists():
         return None
-    loader = importlib.machinery.ExtensionFileLoader("fl355_paged", str(BINDING_PATH))
+    loader = importlib.machinery.ExtensionFileLoader("fl355_paged", str(path))
     try:
         module = importlib.util.module_from_spec(
-            importlib.util.spec_from_file_location("fl355_paged", BINDING_PATH, loader=loader))
+            importlib.util.spec_from_file_location("fl355_paged", path, loader=loader))
         loader.exec_module(module)
     except ImportError:   # (built for another torch)
+        return None
+    import torch
+    built_for, here = getattr(module, "built_for", None), (L.fl_header_digest().decode(), torch.__version__)
+    if built_for != here:   # its calls' arguments, or its tensors, may be laid out differently
+        warnings.warn(f"{path.name} is not used: built for (header, torch) {built_for}, here are "
+                      f"{here}; build again", RuntimeWarning, stacklevel=2)
         return None
     module.bind(*(ctypes.cast(getattr(L, name), ctypes.c_void_p).value for name in BOUND))
     return module

@@ -8,6 +8,7 @@ instructions are kept out of the generated code.
 from __future__ import annotations
 
 import concurrent.futures as cf
+import hashlib
 import os
 import shutil
 import subprocess
@@ -59,9 +60,16 @@ def hipcc() -> str:
     return path
 
 
+def digest_flag() -> str:
+    """Which fl355.h a build is of: fl_header_digest() of the library, and the binding's, so
+    that a binding left from another build is not used with it."""
+    return f'-DFL_HEADER_DIGEST="{hashlib.sha256((INCLUDE / "fl355.h").read_bytes()).hexdigest()[:16]}"'
+
+
 def _compile(src: Path) -> Path:
     obj = BUILD_DIR / (src.stem + ".o")
-    cmd = [hipcc(), *HIPCC_FLAGS, *FILE_FLAGS.get(src.stem, []), "-c", str(src), "-o", str(obj)]
+    extra = [digest_flag()] if src.stem == "abi" else FILE_FLAGS.get(src.stem, [])
+    cmd = [hipcc(), *HIPCC_FLAGS, *extra, "-c", str(src), "-o", str(obj)]
     res = subprocess.run(cmd, capture_output=True, text=True)
     if res.returncode != 0:
         raise RuntimeError(f"hipcc failed on {src.name}:\n{res.stderr}")
@@ -82,6 +90,7 @@ def build_binding(verbose: bool = False) -> Path:
     tmp = BINDING_PATH.with_suffix(".so.tmp")
     cmd = [cxx, "-O2", "-std=c++17", "-fPIC", "-shared",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           digest_flag(), f'-DBUILT_WITH_TORCH="{torch.__version__}"',
            *(f"-I{p}" for p in cpp_extension.include_paths()),
            f"-I{sysconfig.get_paths()['include']}", f"-I{INCLUDE}",
            str(CSRC / "paged_binding.cpp"), "-o", str(tmp),

@@ -27,6 +27,11 @@ extern "C" {
 
 int fl_abi_version(void) { return 1; }
 
+#ifndef FL_HEADER_DIGEST   // (build.py)
+#define FL_HEADER_DIGEST ""
+#endif
+const char* fl_header_digest(void) { return FL_HEADER_DIGEST; }
+
 const char* fl_strerror(int status) {
     switch (status) {
     case FL_OK: return "ok";

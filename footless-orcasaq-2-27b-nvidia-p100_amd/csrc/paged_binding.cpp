@@ -6,6 +6,8 @@
 // that is made gives its result, or its status where it is not FL_OK.
 //
 // The entry points' addresses come from bind(): the library is whichever the package loaded.
+// built_for says which fl355.h and which torch this was compiled with; with any others it must
+// not be bound.
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -390,4 +392,11 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "fl355_paged", nullptr, -1, methods
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_fl355_paged() { return PyModule_Create(&module); }
+PyMODINIT_FUNC PyInit_fl355_paged() {
+    PyObject* m = PyModule_Create(&module);
+    PyObject* built_for = m ? Py_BuildValue("(ss)", FL_HEADER_DIGEST, BUILT_WITH_TORCH) : nullptr;
+    if (built_for && PyModule_AddObject(m, "built_for", built_for) == 0) return m;
+    Py_XDECREF(built_for);
+    Py_XDECREF(m);
+    return nullptr;
+}

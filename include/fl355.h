@@ -38,6 +38,10 @@ typedef struct ihipStream_t* fl_stream_t; /* hipStream_t; NULL = default stream 
 #define FL_PAGED_MAX_SEQS_PREFILL 64 /* ... of chunks (fl_attention_prefill_paged) */
 
 int fl_abi_version(void);
+/* Of the fl355.h that the library was built with: the first 16 hex digits of its SHA-256
+ * ("" if the build did not say). A caller compiled against another header passes its
+ * arguments in another layout. */
+const char* fl_header_digest(void);
 const char* fl_strerror(int status);
 /* Detail of the last failure on the calling thread ("" if none). */
 const char* fl_last_error(void);
