@@ -189,7 +189,10 @@ attn_prep_kernel(const f16* q, f16* qo, int q_pitch, f16* k, int k_pitch,
             for (int c = 0; c < 4; ++c) y[r][c] = f16_sat((float)y[r][c] * inv_r * (1.f + w4[c]));
         }
     }
-    if (ROPE && rope_dim == 64) {
+    // (One row a wave: a launch's code runs once, so its length counts, and the way through
+    // LDS is there for every width anyhow: T = 1 2.40 us with it alone, 2.54 with both, 64
+    // rows 3.21 and 3.35.)
+    if (ROPE && RPW > 1 && rope_dim == 64) {
         // dims 4 l + c, l < 16: pair (j, j + 32) is lanes l and l ^ 8
         const f32x4 cs = *(const f32x4*)(scs + 4 * (lane & 7)), sn = *(const f32x4*)(ssn + 4 * (lane & 7));
 #pragma unroll
