@@ -146,11 +146,12 @@ bool work_of(PyObject* o, Args& a, size_t need, at::Tensor& made, void*& p, size
     return true;
 }
 
+// f() while other Python threads run
 template <class F>
-int released(F f) {
-    int rc;
-    Py_BEGIN_ALLOW_THREADS rc = f();
-    Py_END_ALLOW_THREADS return rc;
+auto released(F f) {
+    decltype(f()) r;
+    Py_BEGIN_ALLOW_THREADS r = f();
+    Py_END_ALLOW_THREADS return r;
 }
 
 #define PLAIN(x) \
@@ -297,8 +298,10 @@ PyObject* prefill(PyObject*, PyObject* const* args, Py_ssize_t n) {
         PLAIN(t && t->size(0) >= total && t->size(1) == n_q && t->size(2) <= INT_MAX);
         z = *t;
     }
-    const size_t need = wo != Py_None ? 0 : p_prefill_bytes(Ts, p0s, (int)B, (int)n_q, (int)n_kv,
-                                                            (int)HEAD_DIM, window, sinks, c.q8);
+    // (this makes the call's plan, up to milliseconds of host work)
+    const size_t need = wo != Py_None ? 0 : released([&] {
+        return p_prefill_bytes(Ts, p0s, (int)B, (int)n_q, (int)n_kv, (int)HEAD_DIM, window, sinks, c.q8);
+    });
     at::Tensor made;
     void* work;
     size_t bytes;
