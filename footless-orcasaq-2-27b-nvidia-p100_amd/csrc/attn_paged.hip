@@ -979,12 +979,13 @@ paged_merge_kernel(const DecPart in, f16* __restrict__ z, int z_pitch, const f16
             den = fmaf(e, s_den[k], den);
         }
     }
-    const float inv = den == 0.f ? 0.f : 1.f / den;   // (no row seen: 0)
+    const float inv = 1.f / den;
     f16x4 out;
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
         const float v = num[c] * inv;
-        out[c] = f16_sat(gate != nullptr ? v * fast_sigmoid((float)gv[c]) : v);
+        // (no row seen: 0, whatever the gate and the rows that other tokens see hold)
+        out[c] = den == 0.f ? (f16)0.f : f16_sat(gate != nullptr ? v * fast_sigmoid((float)gv[c]) : v);
     }
     *(f16x4*)(z + (size_t)rh * z_pitch + 4 * lane) = out;
 }

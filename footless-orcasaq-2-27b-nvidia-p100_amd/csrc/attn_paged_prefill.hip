@@ -426,7 +426,6 @@ paged_prefill_kernel(const f16* __restrict__ q, int q_pitch, const char* __restr
                 parts.pm[slot0 + 32 * nb + lane] = m_run[nb];
                 parts.pd[slot0 + 32 * nb + lane] = l_run[nb];
             }
-            const float den = l_run[nb] == 0.f ? 1.f : l_run[nb];   // (no row seen: O is 0)
 #pragma unroll 1
             for (int r0 = 0; r0 < n; r0 += OUT_ROWS) {
                 f32x4 v[OUT_ROWS];
@@ -435,7 +434,7 @@ paged_prefill_kernel(const f16* __restrict__ q, int q_pitch, const char* __restr
                 for (int i = 0; i < OUT_ROWS; ++i) {
                     const int r = min(r0 + i, n - 1);   // (past the last row: the last once more)
                     v[i] = *(const f32x4*)(ob + 1024 * r + 16 * (ol ^ (2 * r)));
-                    l[i] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(den), r));
+                    l[i] = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(l_run[nb]), r));
                 }
                 if (part) {
 #pragma unroll
@@ -458,6 +457,15 @@ paged_prefill_kernel(const f16* __restrict__ q, int q_pitch, const char* __restr
                     *(f16x4*)(z + rh[i] * z_pitch + 4 * ol) = f16_sat4(v[i]);
                 }
             }
+            // queries that see no row give 0, whatever their gates and the rows that others
+            // see hold: rare, so written over what was formed above
+            if (!part)
+                for (uint32_t blind = (uint32_t)__ballot(lane < n && l_run[nb] == 0.f); blind;
+                     blind &= blind - 1) {
+                    const int row = first + 32 * nb + __builtin_ctz(blind), tb = row / G;
+                    const size_t at = (size_t)(start + tb) * n_q_heads + h * G + row - tb * G;
+                    *(f16x4*)(z + at * z_pitch + 4 * ol) = (f16x4)(0);
+                }
         }
         if (part) ++slot;
     }
@@ -516,11 +524,12 @@ paged_piece_merge_kernel(const Parts in, const Chunks ch, const CutTiles cut, f1
             den = fmaf(e, dv[k], den);
         }
     }
-    const float inv = den == 0.f ? 0.f : 1.f / den;
+    const float inv = 1.f / den;
     f16x4 out;
 #pragma unroll
-    for (int e = 0; e < 4; ++e)
-        out[e] = f16_sat(num[e] * (gate != nullptr ? inv * fast_sigmoid((float)gv[e]) : inv));
+    for (int e = 0; e < 4; ++e)   // (no row seen: 0)
+        out[e] = den == 0.f ? (f16)0.f
+                            : f16_sat(num[e] * (gate != nullptr ? inv * fast_sigmoid((float)gv[e]) : inv));
     *(f16x4*)(z + rh * z_pitch + 4 * lane) = out;
 }
 
