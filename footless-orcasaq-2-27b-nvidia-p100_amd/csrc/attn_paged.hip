@@ -23,7 +23,6 @@ namespace {
 // ---------------------------------------------------------------------------
 constexpr int DT = 32;              // rows a tile
 constexpr int D_WAVES = 4;
-constexpr float RESCALE_LOG2 = 8.f;
 
 struct DecPart {
     int2* meta;      // [B]: a sequence's first run and its number of partials
@@ -296,12 +295,9 @@ paged_decode_f16_kernel(const f16* __restrict__ qg, int q_pitch, const char* __r
 #pragma unroll
                 for (int rr = 1; rr < 16; ++rr) mt = __builtin_elementwise_maximum(mt, sc[rr]);
                 mt = pair32_max(mt) * sl2;
-                // the running maximum only moves when the tile's is more than
-                // RESCALE_LOG2 above it: p <= 256 is exact enough in fp16, and O and l
-                // are rescaled on few tiles
-                const bool grow = mt > m_run + RESCALE_LOG2;
+                const bool grow = mt > m_run + P_TOP;
                 if (__any(grow)) {
-                    const float m_new = grow ? mt : m_run, corr = fast_exp2(m_run - m_new);
+                    const float m_new = grow ? mt - P_BELOW : m_run, corr = fast_exp2(m_run - m_new);
                     m_run = m_new;
                     l_run *= corr;
                     o0 *= corr;
@@ -370,7 +366,7 @@ paged_decode_f16_kernel(const f16* __restrict__ qg, int q_pitch, const char* __r
 //                                         + 8 g .. + 7
 //   softmax                               a lane holds column i's rows 4 g + e of both
 //                                         halves; the maximum is exchanged only when
-//                                         it moves by more than RESCALE_LOG2
+//                                         the reference moves (P_TOP)
 //   O^T (256 dims) += V^T P^T             P as it lies: k slot (g, e) is row 4 g + e of
 //                                         half e / 4; V^T by transposed LDS reads
 // K and V come as whole rows, 16 bytes a lane, non-temporal, and are turned into operands
@@ -606,13 +602,10 @@ paged_decode_q8_kernel(const f16* __restrict__ qg, int q_pitch, const char* __re
 #pragma unroll
                     for (int r = 1; r < 8; ++r) mt = __builtin_elementwise_maximum(mt, s[r]);
                     mt *= sl2;
-                    // the running maximum only moves when some score is more than
-                    // RESCALE_LOG2 above it: p <= 256 is exact enough in fp16, and O and l
-                    // are rescaled on few tiles
-                    if (__any(mt > m_run + RESCALE_LOG2)) {
+                    if (__any(mt > m_run + P_TOP)) {
                         mt = fmaxf(mt, lane_xor(mt, 16));
                         mt = pair32_max(mt);
-                        const float m_new = mt > m_run + RESCALE_LOG2 ? mt : m_run;
+                        const float m_new = mt > m_run + P_TOP ? mt - P_BELOW : m_run;
                         const float corr = fast_exp2(m_run - m_new);
                         m_run = m_new;
                         l_run *= corr;
@@ -843,10 +836,10 @@ paged_decode_q8_pairs_kernel(const f16* __restrict__ qg, int q_pitch, const char
 #pragma unroll
                         for (int r = 1; r < 8; ++r) mt = __builtin_elementwise_maximum(mt, s[r]);
                         mt *= sl2;
-                        if (__any(mt > m_run[nb] + RESCALE_LOG2)) {   // (as above; both waves alike)
+                        if (__any(mt > m_run[nb] + P_TOP)) {   // (as above; both waves alike)
                             mt = fmaxf(mt, lane_xor(mt, 16));
                             mt = pair32_max(mt);
-                            const float m_new = mt > m_run[nb] + RESCALE_LOG2 ? mt : m_run[nb];
+                            const float m_new = mt > m_run[nb] + P_TOP ? mt - P_BELOW : m_run[nb];
                             const float corr = fast_exp2(m_run[nb] - m_new);
                             m_run[nb] = m_new;
                             l_run[nb] *= corr;

@@ -22,6 +22,15 @@ using fl::PAGED_HD;
 struct Sight {
     int window, sinks;
 };
+
+// Softmax weights are held as 2^(s - m), s in log2 units, and go into the product with v in
+// fp16. A column's reference m is put P_BELOW under its running maximum and moves only when a
+// tile's maximum passes m + P_TOP, so O and l are rescaled on few tiles: weights are at most
+// 2^15 (finite in fp16), and the step of fp16's subnormals, 2^-24, is at most 2^-31 of the
+// largest weight. With m at the maximum it is 2^-24 of it, and many rows that together weigh
+// something beside a heavy first token round to nothing, or to twice their weight: 700 rows of
+// 2^-22.7 each were off by 19 %. O, l and the partials' (m, l) carry the same factor.
+constexpr float P_BELOW = 7.f, P_TOP = 15.f;
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ int uni(int x) { return __builtin_amdgcn_readfirstlane(x); }

@@ -124,8 +124,8 @@ __device__ __forceinline__ void softmax_block(f32x16& s, bool whole, uint32_t se
 #pragma unroll
     for (int r = 1; r < 16; ++r) mt = __builtin_elementwise_maximum(mt, s[r]);
     mt = pair32_max(mt) * sl2;
-    if (__any(mt > m_run + RESCALE_LOG2)) {   // always on a wave's first tile, rarely after
-        const float m_new = fmaxf(m_run, mt);
+    if (__any(mt > m_run + P_TOP)) {   // always on a wave's first tile, rarely after
+        const float m_new = fmaxf(m_run, mt - P_BELOW);
         const float corr = fast_exp2(m_run - m_new);
         m_run = m_new;
         l_run *= corr;

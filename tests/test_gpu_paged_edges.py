@@ -104,3 +104,51 @@ def test_chunk_with_some_queries_that_see_nothing(fl, dev, kv8):
     blind = torch.zeros(T, dtype=torch.bool, device="cuda")
     blind[64 + window - 1:96] = True
     assert not z[blind].any() and bool((z[~blind] != 0).flatten(1).any(1).all())
+
+
+def kernel_values(pool, n_rows, exact):
+    """A pool's rows as the kernels take them: fp16 pools as they are, int8 ones byte * scale,
+    exact or rounded to fp16."""
+    if pool.dtype != torch.int8:
+        return pool.view(n_rows, 4, 256).double()
+    v = ref.dequant(pool, n_rows, 4)
+    return v if exact else v.to(F16).double()
+
+
+@pytest.mark.parametrize("kv8", [False, True])
+@pytest.mark.parametrize("form", ["decode1", "decode4", "chunks"])
+def test_many_small_weights_beside_one_large(fl, dev, form, kv8):
+    """A first row that holds nearly all the weight and a v of 0, as first tokens do: z is what
+    the others leave, each 2^-22.7 of the largest. Weights go into the product with v as fp16
+    with a step of 2^-24 (subnormal) at the least, of the largest's reference: that is 7 octaves
+    or more above the running maximum's own 1, so a weight is off by 2^-11 of itself or 2^-32 of
+    the largest. Beside that: z to fp16 (2^-11); in 32 bits the score (22.7 in log2 units, three
+    roundings), the exponential (2 ulp) and 700 additions, numerator and denominator."""
+    g, P, L, ops = gen(3), 64, 700, fl.ops
+    pages, n_pages = ref.make_pages(g, [L], P)
+    K, V = torch.zeros(L, 4, 256), 1500 + 100 * torch.randn((L, 4, 256), generator=g)
+    K[0, :, 0], V[0] = 15.734, 0
+    kp, vp = (ops.paged_pool(n_pages, P, kv8=kv8) for _ in range(2))
+    ops.paged_kv_store(K.to(F16).cuda(), V.to(F16).cuda(), kp, vp, pages, i32(0, L), i32(0), page_size=P)
+    T = {"decode1": 1, "decode4": 4, "chunks": 40}[form]
+    B = 64 if form == "chunks" else 160          # (so many that a sequence stays in a run or two)
+    q = randn(g, B, T, 24, 512)
+    q[..., 0] = 16
+    table = pages.repeat(B, 1)
+    if form == "chunks":
+        z = ops.attention_prefill_paged(q.view(B * T, 24, 512), kp, vp, table, [T] * B, [L - T] * B, page_size=P)
+        z = z.view(B, T, 24, 256)
+    else:
+        z = ops.attn_decode_paged(q, kp, vp, table, i32(*[L - T] * B), page_size=P, gate=False)
+    rows = ref.rows_of(pages.cpu(), 0, P, torch.arange(L)).cuda()
+    K = kernel_values(kp, n_pages * P, form != "chunks")[rows]
+    V = kernel_values(vp, n_pages * P, False)[rows]
+    s = 16 * K[:, 0, 0] * SCALE                  # the same for every head
+    gap = (s[0] - s[1]).item() / torch.log(torch.tensor(2.0)).item()
+    assert 22.5 < gap < 22.9
+    rel = 2 * 2.0 ** -11 + 2.0 ** (gap - 32) + 2 * gap * 3 * 2.0 ** -24 + 2.0 ** -21 + 2 * 700 * 2.0 ** -24
+    for t in range(T):
+        n = L - T + 1 + t
+        want = (torch.softmax(s[:n], 0)[:, None, None] * V[:n]).sum(0).repeat_interleave(6, 0)
+        off = ((z[:, t].double() - want) / want).abs().max().item()
+        assert off <= rel, f"token {t}: off by {off}, {rel} allowed"
