@@ -36,3 +36,17 @@ def test_a_binding_that_does_not_say_what_it_is_of_is_not_bound(fl, monkeypatch)
     monkeypatch.setattr(fl._lib.importlib.machinery.ExtensionFileLoader, "exec_module", lambda self, m: None)
     with pytest.warns(RuntimeWarning, match="build again"):
         assert fl._lib._load_binding(fl._lib.lib()) is None
+
+
+def test_a_build_without_a_cxx_compiler_has_no_binding(fl, monkeypatch, tmp_path, capsys):
+    """The binding is optional: its build says so and takes an old one away, and the loader
+    takes its absence."""
+    import __graft_entry__ as ge
+    builder = ge._load_builder()
+    old = tmp_path / "fl355_paged.so"
+    old.write_bytes(b"of an earlier build")
+    monkeypatch.setattr(builder, "BINDING_PATH", old)
+    monkeypatch.setattr(builder.shutil, "which", lambda name: None)
+    assert builder.build_binding() is None
+    assert not old.exists() and "not built" in capsys.readouterr().out
+    assert fl._lib._load_binding(fl._lib.lib(), old) is None
