@@ -68,12 +68,6 @@ struct Args {
         return t;
     }
     const at::Tensor* dense(at::ScalarType type, int64_t dim) { return dense(next(), type, dim); }
-    // ... of these sizes
-    void* rows(at::ScalarType type, at::IntArrayRef sizes) {
-        const at::Tensor* t = dense(type, sizes.size());
-        if (!t || t->sizes() != sizes) return ok = false, nullptr;
-        return t->data_ptr();
-    }
 };
 
 // kpool, vpool, pages
