@@ -6,6 +6,7 @@ import pytest
 import torch
 
 import paged_ref as ref
+import paged_tight as tight
 
 pytestmark = pytest.mark.gpu
 
@@ -152,3 +153,114 @@ def test_many_small_weights_beside_one_large(fl, dev, form, kv8):
         want = (torch.softmax(s[:n], 0)[:, None, None] * V[:n]).sum(0).repeat_interleave(6, 0)
         off = ((z[:, t].double() - want) / want).abs().max().item()
         assert off <= rel, f"token {t}: off by {off}, {rel} allowed"
+
+
+GATES = [float("inf"), float("-inf"), 65504.0, -65504.0, 0.0, -0.0, 17.0, -17.0, 88.0, -88.0, -104.0, 2.0 ** -24]
+
+
+def small_cache(fl, g, kv8, L=300, P=32, B=1, spoil=None):
+    """Pools with B sequences of L random rows, `spoil` applied to the rows [B L, 4, 256] of k and v
+    first: (kpool, vpool, pages, a sequence's rows of the pools)."""
+    pages, n_pages = ref.make_pages(g, [L] * B, P)
+    kp, vp = (fl.ops.paged_pool(n_pages, P, kv8=kv8) for _ in range(2))
+    k, v = randn(g, B * L, 4, 256), randn(g, B * L, 4, 256)
+    if spoil:
+        spoil(k, v)
+    fl.ops.paged_kv_store(k, v, kp, vp, pages, i32(*[L * b for b in range(B + 1)]), i32(*[0] * B), page_size=P)
+    rows = [ref.rows_of(pages.cpu(), b, P, torch.arange(L)).cuda() for b in range(B)]
+    return kp, vp, pages, rows, n_pages * P
+
+
+def both_forms(fl, qg, kp, vp, pages, p0s, P=32, **args):
+    """qg [B, T, 24, 512] as decode and as chunks: [(form, z [B, T, 24, 256])]."""
+    B, T = qg.shape[:2]
+    zd = fl.ops.attn_decode_paged(qg, kp, vp, pages, i32(*p0s), page_size=P, **args)
+    zc = fl.ops.attention_prefill_paged(qg.reshape(B * T, 24, 512), kp, vp, pages, [T] * B, p0s, page_size=P,
+                                        gated=True, **args)
+    return [("decode", zd), ("chunks", zc.view(B, T, 24, 256))]
+
+
+@pytest.mark.parametrize("kv8", [False, True])
+@pytest.mark.parametrize("T", [1, 5])
+def test_gates_of_every_size(fl, dev, kv8, T):
+    """Infinite gates, the type's largest, and those whose sigmoid leaves fp16 or fp32: closed
+    ones give 0 and open ones z."""
+    g, L = gen(21), 300
+    kp, vp, pages, [rows], n = small_cache(fl, g, kv8, L)
+    qg = randn(g, 1, T, 24, 512)
+    qg[..., 256:] = torch.tensor(GATES * 22)[:256].to(F16).cuda()
+    seen = torch.arange(L, device="cuda")[None] <= torch.arange(L - T, L, device="cuda")[:, None]
+    for form, z in both_forms(fl, qg, kp, vp, pages, [L - T]):
+        K, V = kernel_values(kp, n, form == "decode")[rows], kernel_values(vp, n, False)[rows]
+        want, bound = tight.attention(qg[0, ..., :256], K, V, seen, SCALE,
+                                      tight.TWO_TERMS if kv8 and form == "decode" else tight.ONE_TERM,
+                                      qg[0, ..., 256:])
+        assert ((z[0].double() - want).abs() <= bound).all(), form
+        assert not z[0][qg[0, ..., 256:] <= -88].any()
+
+
+@pytest.mark.parametrize("value", [float("inf"), float("-inf"), float("nan")])
+def test_v_rows_that_are_not_finite(fl, dev, value):
+    """One v of a row that is in sight: the dim is not finite, or saturated, for the queries that
+    see the row; every other dim of theirs, and every other sequence, is as without it. Tokens of
+    the sequence that do not see it may have a NaN in that dim, and no more."""
+    L, T, row, dim = 300, 4, 297, 40
+
+    def spoil(k, v):
+        v[row, 2, dim] = value
+
+    clean = small_cache(fl, gen(22), False, L, B=3)
+    spoiled = small_cache(fl, gen(22), False, L, B=3, spoil=spoil)
+    qg = randn(gen(23), 3, T, 24, 512)
+    p0s = [L - T] * 3                              # token 1 of the first sequence is that row
+    for (form, want), (_, z) in zip(both_forms(fl, qg, *clean[:3], p0s), both_forms(fl, qg, *spoiled[:3], p0s)):
+        hit = z[0, 1:, 12:18, dim]
+        assert (hit.isnan() | (hit.abs() == 65504) | (hit == 0)).all(), form
+        assert hit.isnan().all() or value == value
+        before = z[0, 0, 12:18, dim]
+        assert (before.isnan() | (before == want[0, 0, 12:18, dim])).all(), form
+        z[0, :, 12:18, dim] = want[0, :, 12:18, dim]
+        assert torch.equal(z, want), form
+
+
+@pytest.mark.parametrize("kv8", [False, True])
+def test_scores_that_are_infinite(fl, dev, kv8):
+    """A k of infinity in a row in sight: minus infinity as a score leaves the row out, plus
+    infinity gives NaN (int8: the block is stored with an infinite scale, and what the row's score
+    is then is left open); queries before the row and other sequences are as without it."""
+    L, T, row = 300, 4, 298
+
+    def spoil(k, v):
+        k[row, 1, 7] = float("inf")
+
+    clean = small_cache(fl, gen(24), kv8, L, B=2)
+    spoiled = small_cache(fl, gen(24), kv8, L, B=2, spoil=spoil)
+    qg = randn(gen(25), 2, T, 24, 512)
+    qg[..., 7] = torch.where(torch.arange(24, device="cuda") % 2 == 0, 1.0, -1.0).half()
+    p0s = [L - T] * 2
+    for (form, want), (_, z) in zip(both_forms(fl, qg, *clean[:3], p0s), both_forms(fl, qg, *spoiled[:3], p0s)):
+        see = z[0, 2:, 6:12]                       # tokens 2 and 3, kv head 1's heads
+        if not kv8:
+            assert see[:, ::2].isnan().all(), form
+            K, V = kernel_values(spoiled[0], spoiled[4], True)[spoiled[3][0]], \
+                kernel_values(spoiled[1], spoiled[4], True)[spoiled[3][0]]
+            for t in (2, 3):
+                for h in (7, 9, 11):
+                    q = qg[0, t, h, :256].double()
+                    s = q @ K[:L - T + t + 1, 1].t() * SCALE
+                    out = torch.softmax(s, -1) @ V[:L - T + t + 1, 1] * torch.sigmoid(qg[0, t, h, 256:].double())
+                    # P to fp16: 2^-11 of sum w |v|, under 2 here; z: 2^-11, under 1; the rest: 2^-11
+                    assert (z[0, t, h].double() - out).abs().max() <= 2.0 ** -9, (form, t, h)
+        z[0, 2:, 6:12] = want[0, 2:, 6:12]
+        if form == "decode":
+            assert torch.equal(z, want)
+            continue
+        # In chunks the queries of a wave move their references together, each to its own maximum,
+        # so the infinite score moves where the others' weights round: not the same bits, but each
+        # within the bound of what the clean rows give.
+        seen = torch.arange(L, device="cuda")[None] <= torch.arange(L - T, L, device="cuda")[:, None]
+        K, V = (kernel_values(p, clean[4], False) for p in clean[:2])
+        for b in range(2):
+            exact, bound = tight.attention(qg[b, ..., :256], K[clean[3][b]], V[clean[3][b]], seen, SCALE,
+                                           tight.ONE_TERM, qg[b, ..., 256:])
+            assert ((z[b].double() - exact).abs() <= bound).all()
