@@ -1057,14 +1057,14 @@ int fl_attn_decode_paged(const void* qg, int q_pitch, const void* kpool, const v
     if (rc) return rc;
     const int pairs = B * T * n_q_heads;
     const f16* gate = gated ? (const f16*)qg + PAGED_HD : nullptr;
-    // Four waves a pair where a sequence has about 4 partials or more, one where it has fewer.
-    // The runs are known but over int8, where a long stream has 2^heads_lg times a short one's
-    // (Run; the lengths are on the device): twice are counted. One wave / four, us: fp16 one
-    // context of 500 11.3 / 9.6, 4 of 8k 31.5 / 28.5, 16 of 2k 28.3 / 27.9, 20 of 60 9.6 / 10.1,
-    // 96 of 60 18.1 / 19.6; int8 4 of 8k 27.0 / 23.9, 24 of 8k 83.7 / 82.5, 24 of 2k 32.0 / 32.8,
-    // 40 of 2k 46.1 / 47.1, 64 of 60 14.4 / 15.5, 64 of 8k 189.3 / 189.8; 16 of 2k with 18 rows
-    // 30.2 / 30.7, 20 of them 34.3 / 35.4.
-    const bool wide = cut.runs << (cut.heads_lg > 0) >= 4 * B;
+    // Four waves a pair where a sequence has 4 partials or more, were its stream as long as it
+    // may be (over int8 a long one has 2^heads_lg times a short one's runs, and the lengths are
+    // on the device), one where it has fewer. One wave / four, us: fp16 one context of 500 11.3 /
+    // 9.6, 4 of 8k 31.5 / 28.5, 16 of 2k 28.3 / 27.9, 20 of 60 9.6 / 10.1, 96 of 60 18.1 / 19.6;
+    // int8 4 of 8k 27.0 / 23.9, 24 of 8k 83.7 / 82.5, 40 of 100 - 32k 105.0 / 100.5 (the longest
+    // has dozens), 64 of them 147.0 / 145.3; the price, short int8 streams that count as long:
+    // 40 of 2k 46.1 / 47.1, 64 of 2k 64.3 / 65.1, 64 of 60 14.4 / 15.5.
+    const bool wide = runs >= 4 * B;
     auto merge = wide ? paged_merge_kernel<4> : paged_merge_kernel<1>;
     hipLaunchKernelGGL(merge, dim3(wide ? pairs : (pairs + 3) / 4), dim3(256), 0, (hipStream_t)stream,
                        part, (f16*)z, z_pitch, gate, q_pitch, T, n_q_heads, n_kv_heads, pairs);
