@@ -20,11 +20,11 @@
 // K, V and P are each rounded once, so z is off by about twice the rounding of z itself
 // (1.4 times over fp16 pools, where P's is the only one).
 //
-// Bound by the matrix cores: 8192 fresh tokens at 24 q and 4 kv heads 830 us, 1.0 PFLOP/s of
+// Bound by the matrix cores: 8192 fresh tokens at 24 q and 4 kv heads 842 us, 1.0 PFLOP/s of
 // the 1.3 that a large fp16 product reaches; the softmax between the two products of a tile
 // and a row tile's start and end (ITEM_COST) are the difference. Four chunks of 1024 with
-// a window 450 - 470 us (0.8: short walks), six of 1 - 1024 tokens at 0 - 60k over int8 1.25
-// ms, 117 us of it the copy (6.3 TB/s).
+// a window 450 - 470 us (0.8: short walks), six of 1 - 1024 tokens at 0 - 60k over int8 1.26 -
+// 1.31 ms, 117 us of it the copy (6.3 TB/s).
 // The wave's registers are all taken. A spill is not only slow but wrong here: the O
 // accumulators are written by inline-asm MFMAs, whose hazards the compiler does not see
 // when it stores them. Its resource report has to say 0 spilled VGPRs.
@@ -44,8 +44,8 @@ namespace {
 
 constexpr int MAX_SEQS = FL_PAGED_MAX_SEQS_PREFILL;
 constexpr int THREADS = 256;
-constexpr int OUT_ROWS = 8;    // rows whose gates are in flight when a row tile ends (4, 8, 16:
-                               // 1075, 1006, 1003 us for 8192 fresh tokens)
+constexpr int OUT_ROWS = 8;    // rows whose gates are in flight when a row tile ends (4, 8: 852,
+                               // 842 us for 8192 fresh tokens; 16 spills)
 
 // Packed chunks: sequence b's tokens are start[b] .. start[b + 1] - 1, the first at
 // position pos0[b], its row tiles tile0[b] .. tile0[b + 1] - 1; dense[b]: its first row in
@@ -561,13 +561,16 @@ int dense_rows(int T, int pos0, const Sight& sight) {
     return T == 0 ? 0 : R64_BK * make_walk(pos0, pos0 + T - 1, sight).n;
 }
 
-// The plan's costs, in tiles' time (about 1.3 us).
-constexpr int ITEM_COST = 12;   // a row tile's (Q, pipeline fill, z); 5, 8, 10, 12, 14: 1006,
-                                // 1007, 945, 926, 931 us for 8192 fresh tokens
+// The plan's costs, in tiles' time (2.0 us: 8192 fresh tokens are 387 tiles a CU and three row
+// tiles' ends). They are chosen by the plans they give, not fitted: a row tile's start and end are
+// 16 - 20 us, 448 partials' merge 34 us where the rule says 13 tiles.
+constexpr int ITEM_COST = 12;   // a row tile's (Q, pipeline fill, z); 5, 8, 10, 12, 14: 856, 845,
+                                // 842, 842, 839 us for 8192 fresh tokens, 61.6, 55.4, 60.6, 57.0,
+                                // 61.0 for 1024
 constexpr int PIECE_COST = 8;   // a piece's (its 256 KiB partial)
 constexpr int PIECE_MIN = 2;    // tiles a piece, at least
-constexpr int RUN_MIN = 6;      // a run's cost, at least; 20, 8, 6, 3: 80, 57, 57, 56 us for 1024
-                                // fresh tokens, 62, 41, 40, 38 for 37 at 3001
+constexpr int RUN_MIN = 6;      // a run's cost, at least; 20, 8, 6, 3: 70, 57, 56, 56 us for 1024
+                                // fresh tokens, 61, 41, 40, 38 for 37 at 3001
 constexpr int MERGE_COST = 2;        // the merge's launch
 constexpr int SLOTS_PER_TILE = 40;   // partials the merge reads in a tile's time
 
@@ -709,8 +712,8 @@ void make_plan(const Chunks& ch, int G, int n_kv, const Sight& sight, int n_cu, 
     const long long cut = cut_plan(n, n_kv, most, cp);
     Plan whole;
     const long long w = whole_plan(n, most, whole);
-    // (whole / cut, us: 8192 fresh tokens 826 / 895, 130 fresh 30.9 / 32.2, four chunks of 1024
-    // with a window 549 / 449, 1024 at 30000 1871 / 786, 37 at 3001 200 / 40)
+    // (whole / cut, us: 8192 fresh tokens 842 / 921, 130 fresh 31.2 / 32.4, four chunks of 1024
+    // with a window 545 / 455, 1024 at 30000 1841 / 813, 37 at 3001 197 / 40)
     cp.cut = w == 0 || cut < w;
     if (!cp.cut) {
         cp.plan = whole;

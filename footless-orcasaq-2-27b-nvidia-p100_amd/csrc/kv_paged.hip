@@ -36,10 +36,13 @@ __device__ __forceinline__ float div_near(float x, float d, float r) {
 
 // 8 halves of a 32-dim block (4 lanes) in the int8 format, q8_store_row's values. The
 // correctly rounded divisions there are most of a store's instructions and are not needed:
-// x and the scale s are fp16, so x / s (at most 127.1) is a half integer exactly or at
-// least 2^-13 away from one (|2x - (2n + 1) s| is a multiple of the smaller of their units,
-// and x >= s / 4 there), far more than div_near's error, and rint takes the same side. So
-// is absmax / 127, rounded to fp16: 127 t is no multiple of any unit near it unless exact.
+// x and the scale s are fp16, so x / s is a half integer exactly or far more than div_near's
+// error (2^-15 at most) away from one, and rint takes the same side. With s normal x / s is at
+// most 127.1, and |2x - (2n + 1) s| a multiple of the smaller of their units, and x >= s / 4
+// there: at least 2^-13 away. With s subnormal (absmax / 127 rounded to a step of 2^-24) x / s
+// is at most 190.5, clamped to 127 on both ways, and x and s are multiples of 2^-24 with s <
+// 2^-14: at least 2^-11 away. So is absmax / 127, rounded to fp16: 127 t is no multiple of any
+// unit near it unless exact.
 __device__ __forceinline__ void q8_put(f16x8 x, signed char* vals, f16* scale, bool first) {
     f16x8 m = __builtin_elementwise_abs(x);
     f16x4 m4 = __builtin_elementwise_max((f16x4){m[0], m[1], m[2], m[3]}, (f16x4){m[4], m[5], m[6], m[7]});

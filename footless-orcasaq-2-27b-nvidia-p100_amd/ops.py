@@ -780,6 +780,9 @@ def attention_prefill_paged(q, kpool, vpool, pages, Ts, pos0s, *, page_size: int
     window or r < sinks (window 0: all) on present pages; one that sees none gives
     0. gated: attn_gate applied too, the gate the second half of each head's q row.
     work: uint8 of attention_prefill_paged_work_bytes (allocated here unless given).
+    Over int8 pools k and v are rounded to fp16 once (z about twice its own rounding off;
+    attn_decode_paged takes k exactly). The last bits of a sequence's z depend on what
+    else is in the call.
     Returns z [N, n_q_heads, head_dim] fp16; rows behind the last chunk are left as
     they are (zeros in a new tensor)."""
     dev = _here()
@@ -838,8 +841,10 @@ def attn_decode_paged(qg, kpool, vpool, pages, pos0, *, page_size: int, window: 
     q | gate per head, pos0 [B] int32 on the GPU each sequence's first query
     position (read when the call runs); up to 1024 sequences. What a query sees is
     attention_prefill_paged's; one at a negative position (a padded batch's row)
-    sees nothing and gives 0. work: uint8 of attn_decode_paged_work_bytes (allocated
-    here unless given). Returns z [B, T, n_q_heads, head_dim] fp16."""
+    sees nothing and gives 0, whatever its q and gate hold. work: uint8 of
+    attn_decode_paged_work_bytes (allocated here unless given). The last bits of a
+    sequence's z depend on the batch: where its rows are cut follows all contexts.
+    Returns z [B, T, n_q_heads, head_dim] fp16."""
     dev = _here()
     if dev >= 0 and _lib.lane is not None:
         r = _lib.lane.decode(dev, _stream(), qg, kpool, vpool, pages, pos0, page_size, window, sinks, gate,

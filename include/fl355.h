@@ -401,6 +401,11 @@ int fl_attn_prep_paged(void* qg, int q_pitch, const void* k, const void* v, cons
                        int n_q_heads, int n_kv_heads, int head_dim, int rope_dim, float theta,
                        float eps, fl_stream_t stream);
 
+/* The attention entry points: a query's weights go into the product with v as fp16, 2^-11 of
+ * themselves or 2^-32 of the largest off; the rest is held in 32 bits, z rounded once. A
+ * sequence's last bits depend on what else is in the call (where its rows are cut into parts
+ * that are merged; in chunks the queries beside it as well); the same call gives the same bits. */
+
 /* Causal GQA attention of chunks of new tokens over the pages: B sequences
  * (host arrays; B <= FL_PAGED_MAX_SEQS_PREFILL), Ts[b] packed queries each (0:
  * none), the first at position pos0s[b]; their own rows are in the pool
@@ -412,7 +417,9 @@ int fl_attn_prep_paged(void* qg, int q_pitch, const void* k, const void* v, cons
  * the same arguments, 16-byte aligned, one for each call that may overlap with
  * another. pos0s[b] + Ts[b] <= max_pages * page_size. q8: the rows in sight are
  * first copied into work as f16(byte * scale), 1 KiB a row and kv head, in
- * groups of sequences that take 1 GiB together (a sequence alone: what it takes). */
+ * groups of sequences that take 1 GiB together (a sequence alone: what it takes); so
+ * k and v are rounded once, as in fl_attention_prefill_q8, and z is off by about twice its
+ * own rounding (fl_attn_decode_paged over the same rows: 1.4 times). */
 size_t fl_attention_prefill_paged_work_bytes(const int* Ts, const int* pos0s, int B, int n_q_heads,
                                              int n_kv_heads, int head_dim, int window, int sinks,
                                              int q8);
@@ -428,7 +435,8 @@ int fl_attention_prefill_paged(const void* q, int q_pitch, const void* kpool, co
  * at a negative position (a padded batch's row) sees nothing and gives 0. qg
  * [B][T][n_q_heads][q_pitch], z [B][T][n_q_heads][z_pitch], work of
  * fl_attn_decode_paged_work_bytes. Calls that overlap need a work buffer each.
- * q8: reads the bytes themselves, k with its exact scale, v as f16(byte * scale). */
+ * q8: reads the bytes themselves, k with its exact scale, v as f16(byte * scale), weights
+ * in two f16 terms. */
 size_t fl_attn_decode_paged_work_bytes(int B, int T, int n_q_heads, int n_kv_heads, int head_dim);
 int fl_attn_decode_paged(const void* qg, int q_pitch, const void* kpool, const void* vpool, int q8,
                          int n_pages, int page_size, const int* pages, int max_pages,
