@@ -15,16 +15,19 @@
 //     either a list of whole row tiles each (CUT false), or equal runs of all row tiles'
 //     walks laid end to end, cut wherever the cuts fall (CUT): an uncut row tile of a run
 //     goes to z, a cut one leaves partials that paged_piece_merge_kernel combines.
-// Over int8 pools the visible rows are first copied to fp16 (byte scale) in the work
-// buffer, absent and unwritten rows as zeros, and the same kernel walks that copy (DENSE):
-// K, V and P are each rounded once, so z is off by about twice the rounding of z itself
-// (1.4 times over fp16 pools, where P's is the only one).
+// Over int8 pools the visible rows are first copied to fp16 in the work buffer, K as the bytes
+// and V as f16(byte scale), absent and unwritten rows as zeros, and the same kernel walks that
+// copy (DENSE): K's block scales go onto the partial scores in fp32 (put_steps) and P goes in as
+// two fp16 terms, so that V's rounding is the only one of the products and z is off by 1.4 times
+// its own rounding, as over fp16 pools and in the int8 decode. (With f16(byte scale) for K as
+// well and P in one term it is 1.8 times, in two thirds of the time; K exact alone 1.7.)
 //
 // Bound by the matrix cores: 8192 fresh tokens at 24 q and 4 kv heads 842 us, 1.0 PFLOP/s of
 // the 1.3 that a large fp16 product reaches; the softmax between the two products of a tile
 // and a row tile's start and end (ITEM_COST) are the difference. Four chunks of 1024 with
-// a window 450 - 470 us (0.8: short walks), six of 1 - 1024 tokens at 0 - 60k over int8 1.26 -
-// 1.31 ms, 117 us of it the copy (6.3 TB/s).
+// a window 450 - 470 us (0.8: short walks). Over int8 pools a tile has half again the products
+// and 256 multiplications for the steps, 3.2 us where it has 2.0: 8192 fresh tokens 1300 us, six
+// of 1 - 1024 tokens at 0 - 60k 1.88 ms (0.55), 117 us of it the copy (6.3 TB/s).
 // The wave's registers are all taken. A spill is not only slow but wrong here: the O
 // accumulators are written by inline-asm MFMAs, whose hazards the compiler does not see
 // when it stores them. Its resource report has to say 0 spilled VGPRs.
@@ -36,6 +39,7 @@
 #include <new>
 #include <queue>
 #include <string.h>
+#include <type_traits>
 #include <vector>
 
 using fl::R64_BQ;
@@ -109,12 +113,43 @@ struct Parts {
 
 __device__ const u32x4 zero_row[ROW_B / 16] = {};
 
+// Over int8 pools the copy's K are the bytes, exact in fp16, and a score is formed block by block
+// in place, S <- (S + product of block b) t_b with t_b = s_b / s_(b + 1) for b < 7 and t_7 = s_7:
+// sum_b s_b q.k_b, K not rounded, in no more registers than S. t is in LDS behind the stages, for
+// this tile and the next, [tile & 1][block][row]; ahead of it the scales as they come, a stage's
+// by the waves that copy them: [wave][pair of blocks][row of its 8], a dword two blocks' scales
+// of a row (the other half of a wave's part takes what its lanes 32 - 63 copy, the same again).
+constexpr int SCALE_W = 256;                 // bytes a wave
+constexpr int SCALE_STAGE = 4 * SCALE_W;
+constexpr int STEP_AT = R64_LDS + R64_NST * SCALE_STAGE;
+constexpr int STEP_B = 8 * R64_BK * 4;
+constexpr int DENSE_LDS = STEP_AT + 2 * STEP_B;
+__device__ __forceinline__ void copy4_v(const char* vptr, uint32_t lds) {   // copy16_v, 4 bytes a lane
+    asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(vptr), "{m0}"(lds));
+}
+// t of this wave's 8 rows of a tile from its scales, a (block, row) a lane. (A scale of 0, whose
+// block's copy is 0: any other does.)
+__device__ __forceinline__ void put_steps(char* smem, int stage, int tile, int w, int lane) {
+    asm volatile("" : "+v"(lane));   // (its addresses are not worth registers across the tile loop)
+    const int blk = lane >> 3, row = lane & 7;
+    const char* sc = smem + R64_LDS + stage * SCALE_STAGE + w * SCALE_W;
+    auto scale = [&](int b) {
+        const float x = (float)*(const f16*)(sc + 32 * (b >> 1) + 4 * row + 2 * (b & 1));
+        return x == 0.f ? 0x1p-24f : x;
+    };
+    const float own = scale(blk), next = scale(min(blk + 1, 7));
+    *(float*)(smem + STEP_AT + (tile & 1) * STEP_B + 4 * (R64_BK * blk + 8 * w + row)) =
+        blk < 7 ? own * __builtin_amdgcn_rcpf(next) : own;
+}
+
 // Softmax of one 32-column block of a tile (a query column a lane pair, 16 of its 32
 // scores a lane: score r is row 8 (r / 4) + 4 hh + r % 4), `see` the column's visible rows
-// from 4 hh on; the lazy rescale of this block's O^T; P in fp16 as the PV operand.
+// from 4 hh on; the lazy rescale of this block's O^T; P in fp16 as the PV operand, TWO: and
+// what that leaves of it in another fp16 (pl).
+template <bool TWO>
 __device__ __forceinline__ void softmax_block(f32x16& s, bool whole, uint32_t see, float sl2,
                                               float& m_run, float& l_run, f32x16 (&o)[8],
-                                              f16x8 (&pk)[2]) {
+                                              f16x8 (&pk)[2], f16x8 (&pl)[2]) {
     if (!whole) {
 #pragma unroll
         for (int r = 0; r < 16; ++r)
@@ -138,10 +173,12 @@ __device__ __forceinline__ void softmax_block(f32x16& s, bool whole, uint32_t se
         psum += s[r];
     }
 #pragma unroll
-    for (int ks = 0; ks < 2; ++ks)
-        pk[ks] = __builtin_convertvector((f32x8){s[8 * ks], s[8 * ks + 1], s[8 * ks + 2], s[8 * ks + 3],
-                                                 s[8 * ks + 4], s[8 * ks + 5], s[8 * ks + 6],
-                                                 s[8 * ks + 7]}, f16x8);
+    for (int ks = 0; ks < 2; ++ks) {
+        const f32x8 p = {s[8 * ks],     s[8 * ks + 1], s[8 * ks + 2], s[8 * ks + 3],
+                         s[8 * ks + 4], s[8 * ks + 5], s[8 * ks + 6], s[8 * ks + 7]};
+        pk[ks] = __builtin_convertvector(p, f16x8);
+        if (TWO) pl[ks] = __builtin_convertvector(p - __builtin_convertvector(pk[ks], f32x8), f16x8);
+    }
     l_run += pair32_sum(psum);
 }
 
@@ -159,12 +196,13 @@ __device__ __forceinline__ void copy_rows(uint32_t d0, const char* kr, const cha
     copy16_at<R64_TILE + 6 * ROW_B>(vr, loff[3], d0);
 }
 
-// DENSE: kc and vc are the fp16 copy, [row][n_kv][256], else the pools.
+// DENSE: kc and vc are the copy, [row][n_kv][256], ksc the pool's scales of K; else the pools.
 template <bool DENSE, bool CUT>
 __global__ void __launch_bounds__(THREADS)
 paged_prefill_kernel(const f16* __restrict__ q, int q_pitch, const char* __restrict__ kc,
-                     const char* __restrict__ vc, const Pages pg, const Chunks ch,
-                     f16* __restrict__ z, int z_pitch, int gated, int n_q_heads, int n_kv, float sl2,
+                     const char* __restrict__ vc, const char* __restrict__ ksc, const Pages pg,
+                     const Chunks ch, f16* __restrict__ z, int z_pitch, int gated, int n_q_heads,
+                     int n_kv, float sl2,
                      const Sight sight, const Plan plan, Parts parts) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     // Workgroups go to the 8 XCDs round-robin, each with an L2 of its own: where the kv
@@ -196,8 +234,9 @@ paged_prefill_kernel(const f16* __restrict__ q, int q_pitch, const char* __restr
         loff[n] = r * rsb + 16 * ((lane & 31) ^ sw(8 * w + r));
     }
     const uint32_t lds_base = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)smem);
-    // K operand of k-step ks: tile row ql, chunk 16 hh + ks, at 16 hh + (ks ^ sw(ql))
-    const uint32_t koff = ql * ROW_B + 256 * hh + 16 * sw(ql);
+    // K operand of k-step ks: tile row ql, chunk 16 hh + ks, at 16 hh + (ks ^ sw(ql)); DENSE:
+    // chunk 2 ks + hh, at (2 ks) ^ hh ^ sw(ql), so that two k-steps are a 32-dim block
+    const uint32_t koff = ql * ROW_B + (DENSE ? 16 * (hh ^ sw(ql)) : 256 * hh + 16 * sw(ql));
     const int tr_r = (lane & 15) >> 2;
     const int tr_d = 16 * ((lane & 31) >> 4) + 4 * (lane & 3);
     uint32_t troff[8];
@@ -252,17 +291,22 @@ paged_prefill_kernel(const f16* __restrict__ q, int q_pitch, const char* __restr
         }
         auto ids = page_ids(pg, seq, j_lo, j_hi - 1, 0, [&](int j) { return walk.row0(j); });
         // copy tile j into the stage at dst; the pages of its halves
-        auto issue = [&](uint32_t dst, int j, int& id0, int& id1) {
-            const uint32_t d0 = uni(dst + 8 * w * ROW_B);
+        auto issue = [&](int stage, int j, int& id0, int& id1) {
+            const uint32_t d0 = uni(lds_base + stage * R64_STAGE + 8 * w * ROW_B);
             const int r0 = walk.row0(j);
             ids.at(j, id0, id1);
-            if constexpr (DENSE) {
-                const long long at = ch.dense[seq] + (r0 < dense_cut ? r0 : r0 - dense_skip) + 8 * w;
-                copy_rows(d0, kb + at * rsb, vb + at * rsb, loff);
-                return;
-            }
             const int id = w >> 1 ? id1 : id0, r = r0 + 8 * w;   // this wave's page, first row
             const long long at = ((long long)max(id, 0) << pg.shift) + (r & ((1 << pg.shift) - 1));
+            if constexpr (DENSE) {
+                const long long row = ch.dense[seq] + (r0 < dense_cut ? r0 : r0 - dense_skip) + 8 * w;
+                // (of an absent page page 0's: its scores are masked)
+                int l = lane;
+                asm volatile("" : "+v"(l));   // (as in put_steps)
+                copy4_v(uniform_ptr(ksc + (at * n_kv + h) * 16) + (16 * (l & 7) * n_kv + 4 * (l >> 3 & 3)),
+                        uni(lds_base + R64_LDS + stage * SCALE_STAGE + w * SCALE_W));
+                copy_rows(d0, kb + row * rsb, vb + row * rsb, loff);
+                return;
+            }
             const char* kr = kb + at * rsb;
             const char* vr = vb + at * rsb;
             if (id >= 0 && r + 8 <= walk.hi && (r >= walk.lo || r + 8 <= sight.sinks)) {
@@ -282,39 +326,47 @@ paged_prefill_kernel(const f16* __restrict__ q, int q_pitch, const char* __restr
         int id0[R64_NST], id1[R64_NST];
 #pragma unroll
         for (int d = 0; d < R64_DIST; ++d)
-            if (d < n_tiles) issue(lds_base + d * R64_STAGE, j_lo + d, id0[d], id1[d]);
+            if (d < n_tiles) issue(d, j_lo + d, id0[d], id1[d]);
 
-        // Q[row nb][128 hh + 8 ks + 0..7] (a lane past the rows reads token 0's; its
-        // column is never stored)
+        // Q[row nb][128 hh + 8 ks + 0..7], DENSE [16 ks + 8 hh + 0..7] (a lane past the rows
+        // reads token 0's; its column is never stored)
         f16x8 qreg[2][16];
 #pragma unroll
         for (int nb = 0; nb < 2; ++nb) {
-            const f16* qrow = q + ((size_t)(start + t[nb]) * n_q_heads + h * G + g[nb]) * q_pitch + 128 * hh;
+            const f16* qrow =
+                q + ((size_t)(start + t[nb]) * n_q_heads + h * G + g[nb]) * q_pitch + (DENSE ? 8 : 128) * hh;
 #pragma unroll
-            for (int ks = 0; ks < 16; ++ks) qreg[nb][ks] = *(const f16x8*)(qrow + 8 * ks);
+            for (int ks = 0; ks < 16; ++ks) qreg[nb][ks] = *(const f16x8*)(qrow + (DENSE ? 16 : 8) * ks);
         }
         WAIT_VMCNT(0);   // the first tiles, and Q, pinned here: a later wait would drain the copies
+        if constexpr (DENSE) {
+            asm volatile("" ::: "memory");
+            put_steps(smem, 0, 0, w, lane);
+        }
 #pragma unroll
         for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
             for (int ks = 0; ks < 16; ++ks) asm volatile("" : "+v"(qreg[nb][ks]));
 
         f32x16 o[2][8];
+        f16x8 zero = (f16x8)(0);
+        asm volatile("" : "+v"(zero));   // (not four registers across the row tiles)
 #pragma unroll
         for (int nb = 0; nb < 2; ++nb)
 #pragma unroll
-            for (int mb = 0; mb < 8; ++mb) acc_zero(o[nb][mb], (f16x8)(0));
+            for (int mb = 0; mb < 8; ++mb) acc_zero(o[nb][mb], zero);
         float m_run[2] = {-1e30f, -1e30f}, l_run[2] = {0.f, 0.f};
 
         typedef __attribute__((address_space(3))) const f16x8 lds_f16x8;
         typedef __attribute__((address_space(3))) const char lds_char;
+        constexpr int COPIES = R64_COPIES + DENSE;   // a wave's of a tile
         int st = 0;   // stage of tile j
         for (int j = 0; j < n_tiles; ++j) {
             // tile j landed: the copies of the min(DIST - 1, n_tiles - 1 - j) tiles issued
             // after it may still be in flight
             const int ahead = min(R64_DIST - 1, n_tiles - 1 - j);
-            if (ahead == 2) WAIT_VMCNT(2 * R64_COPIES);
-            else if (ahead == 1) WAIT_VMCNT(R64_COPIES);
+            if (ahead == 2) WAIT_VMCNT(2 * COPIES);
+            else if (ahead == 1) WAIT_VMCNT(COPIES);
             else WAIT_VMCNT(0);
             tile_done();   // every wave is past tile j - 1: its stage can be refilled
             const int p0 = id0[0], p1 = id1[0];
@@ -322,24 +374,67 @@ paged_prefill_kernel(const f16* __restrict__ q, int q_pitch, const char* __restr
             id0[1] = id0[2], id1[1] = id1[2];
             if (j + R64_DIST < n_tiles) {
                 const int sn = st == 0 ? R64_NST - 1 : st - 1;   // (j + DIST) % NST == (j - 1) % NST
-                issue(lds_base + sn * R64_STAGE, j_lo + j + R64_DIST, id0[2], id1[2]);
+                issue(sn, j_lo + j + R64_DIST, id0[2], id1[2]);
             }
             const int kv0 = walk.row0(j_lo + j);
             if (kv0 <= wqmax) {
                 const uint32_t kst = koff + st * R64_STAGE;
                 f32x16 s[2] = {(f32x16)(0.f), (f32x16)(0.f)};
-                constexpr int KPF = R64_KPF;
-                f16x8 ka[KPF];
+                if constexpr (DENSE) {
+                    // (the two column blocks alternate: one's products run under the other's steps)
+                    auto frag = [&](int ks) {
+                        return *(lds_f16x8*)((lds_char*)smem + (kst ^ (32 * ks)));
+                    };
+                    typedef __attribute__((address_space(3))) const f32x4 lds_f32x4;
+                    lds_char* steps = (lds_char*)smem + (STEP_AT + (j & 1) * STEP_B + 16 * hh);
+                    f16x8 ka[4] = {frag(0), frag(1), frag(2), frag(3)};
+                    f32x4 t[4];   // of rows 8 r4 + 4 hh ..
+                    auto product = [&](int nb, int ks) {
+                        s[nb] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka[ks & 3], qreg[nb][ks], s[nb], 0, 0, 0);
+                        __builtin_amdgcn_sched_barrier(0);
+                    };
+                    auto step = [&](int nb, int r4) {
 #pragma unroll
-                for (int ks = 0; ks < KPF; ++ks) ka[ks] = *(lds_f16x8*)((lds_char*)smem + (kst ^ (16 * ks)));
+                        for (int e = 0; e < 4; ++e) s[nb][4 * r4 + e] *= t[r4][e];
+                    };
+                    // one column block's products alternate with the other's steps
 #pragma unroll
-                for (int ks = 0; ks < 16; ++ks) {
-                    const f16x8 a = ka[ks % KPF];
-                    if (ks + KPF < 16)
-                        ka[ks % KPF] = *(lds_f16x8*)((lds_char*)smem + (kst ^ (16 * (ks + KPF))));
-                    s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qreg[0][ks], s[0], 0, 0, 0);
-                    s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qreg[1][ks], s[1], 0, 0, 0);
-                    __builtin_amdgcn_sched_barrier(0);   // keep the reads ahead
+                    for (int b = 0; b < 8; ++b) {
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            product(0, 2 * b + k);
+#pragma unroll
+                            for (int r4 = 2 * k; r4 < 2 * k + 2; ++r4) {   // the last block's step,
+                                if (b > 0) step(1, r4);                    // then this one's t
+                                t[r4] = *(lds_f32x4*)(steps + 4 * R64_BK * b + 32 * r4);
+                            }
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            product(1, 2 * b + k);
+                            if (b < 6) ka[(2 * b + k) & 3] = frag(2 * b + 4 + k);
+                            step(0, 2 * k), step(0, 2 * k + 1);
+                            __builtin_amdgcn_sched_barrier(0);
+                        }
+                    }
+#pragma unroll
+                    for (int r4 = 0; r4 < 4; ++r4) step(1, r4);
+                } else {
+                    constexpr int KPF = R64_KPF;
+                    f16x8 ka[KPF];
+#pragma unroll
+                    for (int ks = 0; ks < KPF; ++ks)
+                        ka[ks] = *(lds_f16x8*)((lds_char*)smem + (kst ^ (16 * ks)));
+#pragma unroll
+                    for (int ks = 0; ks < 16; ++ks) {
+                        const f16x8 a = ka[ks % KPF];
+                        if (ks + KPF < 16)
+                            ka[ks % KPF] = *(lds_f16x8*)((lds_char*)smem + (kst ^ (16 * (ks + KPF))));
+                        s[0] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qreg[0][ks], s[0], 0, 0, 0);
+                        s[1] = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, qreg[1][ks], s[1], 0, 0, 0);
+                        __builtin_amdgcn_sched_barrier(0);   // keep the reads ahead
+                    }
                 }
                 // whole: every query of the wave sees every row (uniform)
                 const TileMask mask(kv0, p0, p1, sight.sinks);
@@ -347,33 +442,71 @@ paged_prefill_kernel(const f16* __restrict__ q, int q_pitch, const char* __restr
                     return sight.window > 0 && p >= sight.window ? p - sight.window + 1 : 0;
                 };
                 const bool whole = mask.all(low(wqmax), wqmin + 1);
-                f16x8 pk[2][2];
+                f16x8 pk[2][2], pl[2][2];
 #pragma unroll
                 for (int nb = 0; nb < 2; ++nb) {
                     uint32_t see = 0;
                     if (!whole) see = mask.rows(low(qpos[nb]), qpos[nb] + 1) >> (4 * hh);
-                    softmax_block(s[nb], whole, see, sl2, m_run[nb], l_run[nb], o[nb], pk[nb]);
+                    softmax_block<DENSE>(s[nb], whole, see, sl2, m_run[nb], l_run[nb], o[nb], pk[nb], pl[nb]);
                 }
-                // O^T += V^T P^T: 4 steps (kq, dim half) of 4 fragments x 2 blocks, the next
-                // step's fragments read under this step's MFMAs
                 const char* vt = smem + st * R64_STAGE + R64_TILE;
-                s16x4 vf[2][8];
-                r64_vfrags(vf[0], vt, troff, 0);
+                auto operand = [](const s16x4& lo, const s16x4& hi) {
+                    const f16x4 lf = __builtin_bit_cast(f16x4, lo), hf = __builtin_bit_cast(f16x4, hi);
+                    return (f16x8){lf[0], lf[1], lf[2], lf[3], hf[0], hf[1], hf[2], hf[3]};
+                };
+                if constexpr (DENSE) {
+                    // O^T += V^T P^T, 16 fragments with 2 blocks x 2 terms each, VPF fragments read ahead
+                    constexpr int VPF = 4;
+                    s16x4 vf[VPF][2];
+                    auto read = [&](int i) {   // fragment i: rows 16 (i / 8) .., dim block 4 (i / 4 % 2) + i % 4
+                        const int imm = 16 * ROW_B * (i >> 3) + 256 * (i >> 2 & 1);
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
-                    if (n + 1 < 4) r64_vfrags(vf[(n + 1) & 1], vt, troff, n + 1);
+                        for (int e = 0; e < 2; ++e)
+                            vf[i % VPF][e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                (lds_s16x4*)(vt + troff[2 * (i & 3) + e] + imm));
+                    };
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const f16x4 lf = __builtin_bit_cast(f16x4, vf[n & 1][2 * u]);
-                        const f16x4 hf = __builtin_bit_cast(f16x4, vf[n & 1][2 * u + 1]);
-                        const f16x8 av = {lf[0], lf[1], lf[2], lf[3], hf[0], hf[1], hf[2], hf[3]};
-                        acc_mfma(o[0][4 * (n & 1) + u], av, pk[0][n >> 1]);
-                        acc_mfma(o[1][4 * (n & 1) + u], av, pk[1][n >> 1]);
+                    for (int i = 0; i < VPF; ++i) read(i);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const f16x8 av = operand(vf[i % VPF][0], vf[i % VPF][1]);
+                        const int mb = i & 7, kq = i >> 3;
+                        acc_mfma(o[0][mb], av, pk[0][kq]);
+                        acc_mfma(o[1][mb], av, pk[1][kq]);
+                        acc_mfma(o[0][mb], av, pl[0][kq]);
+                        acc_mfma(o[1][mb], av, pl[1][kq]);
+                        if (i + VPF < 16) read(i + VPF);
+                        __builtin_amdgcn_sched_barrier(0);
                     }
-                    __builtin_amdgcn_sched_barrier(0);
+                } else {
+                    // O^T += V^T P^T: 4 steps (kq, dim half) of 4 fragments x 2 blocks, the next
+                    // step's fragments read under this step's MFMAs
+                    s16x4 vf[2][8];
+                    r64_vfrags(vf[0], vt, troff, 0);
+#pragma unroll
+                    for (int n = 0; n < 4; ++n) {
+                        if (n + 1 < 4) r64_vfrags(vf[(n + 1) & 1], vt, troff, n + 1);
+#pragma unroll
+                        for (int u = 0; u < 4; ++u) {
+                            const f16x8 av = operand(vf[n & 1][2 * u], vf[n & 1][2 * u + 1]);
+                            acc_mfma(o[0][4 * (n & 1) + u], av, pk[0][n >> 1]);
+                            acc_mfma(o[1][4 * (n & 1) + u], av, pk[1][n >> 1]);
+                        }
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
                 }
             }
             st = st == R64_NST - 1 ? 0 : st + 1;
+            if (DENSE && j + 1 < n_tiles) {
+                // the next tile's steps: its scales were copied ahead of its rows, those of the
+                // tiles after it may still be in flight
+                const int later = min(R64_DIST - 1, n_tiles - 2 - j);
+                if (later == 2) WAIT_VMCNT(2 * COPIES + R64_COPIES);
+                else if (later == 1) WAIT_VMCNT(COPIES + R64_COPIES);
+                else WAIT_VMCNT(R64_COPIES);
+                asm volatile("" ::: "memory");
+                put_steps(smem, st, j + 1, w, lane);
+            }
         }
 
         // O leaves through LDS, a 32-row block at a time in this wave's quarter of the
@@ -396,8 +529,8 @@ paged_prefill_kernel(const f16* __restrict__ q, int q_pitch, const char* __restr
         };
         const size_t slot0 = (size_t)(slot + h * parts.n) * R64_BQ + 64 * w;
         // gates are requested OUT_ROWS rows ahead of their use (no gate: one that is open)
-        f16x4 g_next[OUT_ROWS];
-        size_t rh_next[OUT_ROWS];
+        f16x4 g_next[OUT_ROWS] = {};   // (undefined ones would hold registers through the tile loop)
+        size_t rh_next[OUT_ROWS] = {};
         auto request = [&] {
 #pragma unroll
             for (int i = 0; i < OUT_ROWS; ++i) {
@@ -801,9 +934,9 @@ int raise_lds() {
                          (const void*)paged_prefill_kernel<true, false>,
                          (const void*)paged_prefill_kernel<true, true>};
     for (const void* f : fns)
-        if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, R64_LDS) != hipSuccess) {
+        if (hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, DENSE_LDS) != hipSuccess) {
             fl::set_error("attention_prefill_paged: cannot raise the dynamic LDS limit to %d bytes",
-                          R64_LDS);
+                          DENSE_LDS);
             return FL_ELAUNCH;
         }
     done[dev].store(true);
@@ -839,14 +972,14 @@ paged_stage_kernel(const char* __restrict__ kp, const char* __restrict__ vp, con
         f16x8 kx = (f16x8)(0), vx = (f16x8)(0);
         if (row >= 0) {
             const size_t at = (size_t)row * chunks + c;
-            auto get = [&](const char* pool) {
+            auto get = [&](const char* pool, f16 s) {
                 const u32x2 b = *(const u32x2*)(pool + 8 * at);
-                const f16 s = ((const f16*)(pool + scales))[at >> 2];
                 const f16x4 lo = q8_deq4(b.x, (f16x2){s, s}), hi = q8_deq4(b.y, (f16x2){s, s});
                 return (f16x8){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
             };
-            kx = get(kp);
-            vx = get(vp);
+            // (a block of scale 0 is 0 whatever its bytes)
+            kx = get(kp, ((const f16*)(kp + scales))[at >> 2] != (f16)0.f ? (f16)1.f : (f16)0.f);
+            vx = get(vp, ((const f16*)(vp + scales))[at >> 2]);
         }
         ko[(size_t)i * chunks + c] = kx;
         vo[(size_t)i * chunks + c] = vx;
@@ -934,8 +1067,9 @@ int fl_attention_prefill_paged(const void* q, int q_pitch, const void* kpool, co
     Parts parts = {(float*)work, nullptr, nullptr, cp.slots};
     parts.pm = parts.pacc + part_rows * PF_HD;
     parts.pd = parts.pm + part_rows;
-    const char *kc = (const char*)kpool, *vc = (const char*)vpool;
+    const char *kc = (const char*)kpool, *vc = (const char*)vpool, *ksc = nullptr;
     if (q8) {
+        ksc = kc + (((size_t)n_pages << pg.shift) * n_kv_heads) * PF_HD;
         char* copy = (char*)work + part_b;
         char* copy_v = copy + dense_bytes(rows, n_kv_heads) / 2;
         hipLaunchKernelGGL(paged_stage_kernel, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, stream, kc,
@@ -950,9 +1084,9 @@ int fl_attention_prefill_paged(const void* q, int q_pitch, const void* kpool, co
     // a whole number of workgroups an XCD, so that its kv head's rows stay in one L2
     const int per = 8 % n_kv_heads == 0 ? 8 / n_kv_heads : 1;
     const int runs = (cp.plan.runs + per - 1) / per * per;
-    hipLaunchKernelGGL(kernel, dim3(runs * n_kv_heads), dim3(THREADS), R64_LDS, stream, (const f16*)q,
-                       q_pitch, kc, vc, pg, ch, (f16*)z, z_pitch, gated, n_q_heads, n_kv_heads,
-                       scale * FL_LOG2E, sight, cp.plan, parts);
+    hipLaunchKernelGGL(kernel, dim3(runs * n_kv_heads), dim3(THREADS), q8 ? DENSE_LDS : R64_LDS, stream,
+                       (const f16*)q, q_pitch, kc, vc, ksc, pg, ch, (f16*)z, z_pitch, gated, n_q_heads,
+                       n_kv_heads, scale * FL_LOG2E, sight, cp.plan, parts);
     rc = fl::check_launch("attention_prefill_paged");
     if (rc || cp.tiles.n == 0) return rc;
     hipLaunchKernelGGL(paged_piece_merge_kernel, dim3(cp.tiles.n * (R64_BQ / 4), n_kv_heads), dim3(256), 0,

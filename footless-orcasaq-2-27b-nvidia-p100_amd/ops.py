@@ -780,9 +780,7 @@ def attention_prefill_paged(q, kpool, vpool, pages, Ts, pos0s, *, page_size: int
     window or r < sinks (window 0: all) on present pages; one that sees none gives
     0. gated: attn_gate applied too, the gate the second half of each head's q row.
     work: uint8 of attention_prefill_paged_work_bytes (allocated here unless given).
-    Over int8 pools k and v are rounded to fp16 once (z about twice its own rounding off;
-    attn_decode_paged takes k exactly). The last bits of a sequence's z depend on what
-    else is in the call.
+    The last bits of a sequence's z depend on what else is in the call.
     Returns z [N, n_q_heads, head_dim] fp16; rows behind the last chunk are left as
     they are (zeros in a new tensor)."""
     dev = _here()

@@ -416,10 +416,10 @@ int fl_attn_prep_paged(void* qg, int q_pitch, const void* k, const void* v, cons
  * [sum Ts][n_q_heads][z_pitch]. work: fl_attention_prefill_paged_work_bytes of
  * the same arguments, 16-byte aligned, one for each call that may overlap with
  * another. pos0s[b] + Ts[b] <= max_pages * page_size. q8: the rows in sight are
- * first copied into work as f16(byte * scale), 1 KiB a row and kv head, in
- * groups of sequences that take 1 GiB together (a sequence alone: what it takes); so
- * k and v are rounded once, as in fl_attention_prefill_q8, and z is off by about twice its
- * own rounding (fl_attn_decode_paged over the same rows: 1.4 times). */
+ * first copied into work as fp16, 1 KiB a row and kv head, in
+ * groups of sequences that take 1 GiB together (a sequence alone: what it takes). As in
+ * the decode form k is taken with its exact scale, v as f16(byte * scale) and weights in
+ * two f16 terms. */
 size_t fl_attention_prefill_paged_work_bytes(const int* Ts, const int* pos0s, int B, int n_q_heads,
                                              int n_kv_heads, int head_dim, int window, int sinks,
                                              int q8);

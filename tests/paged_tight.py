@@ -1,9 +1,8 @@
 """Data on which a lost, repeated or swapped tile of cached rows shows, and the error that the
 paged attention kernels' roundings allow when the reference starts from the values they form.
 
-Over int8 pools the chunk kernels take K and V as fp16(byte * scale), the decode kernels K as
-byte * scale exactly and V as fp16(byte * scale): with those as the reference's K and V the
-bound needs no term for the cache's format."""
+Over int8 pools the kernels take K as byte * scale exactly and V as fp16(byte * scale): with
+those as the reference's K and V the bound needs no term for the cache's format."""
 import torch
 
 import paged_ref as ref

@@ -107,15 +107,6 @@ def test_chunk_with_some_queries_that_see_nothing(fl, dev, kv8):
     assert not z[blind].any() and bool((z[~blind] != 0).flatten(1).any(1).all())
 
 
-def kernel_values(pool, n_rows, exact):
-    """A pool's rows as the kernels take them: fp16 pools as they are, int8 ones byte * scale,
-    exact or rounded to fp16."""
-    if pool.dtype != torch.int8:
-        return pool.view(n_rows, 4, 256).double()
-    v = ref.dequant(pool, n_rows, 4)
-    return v if exact else v.to(F16).double()
-
-
 @pytest.mark.parametrize("kv8", [False, True])
 @pytest.mark.parametrize("form", ["decode1", "decode4", "chunks"])
 def test_many_small_weights_beside_one_large(fl, dev, form, kv8):
@@ -142,8 +133,8 @@ def test_many_small_weights_beside_one_large(fl, dev, form, kv8):
     else:
         z = ops.attn_decode_paged(q, kp, vp, table, i32(*[L - T] * B), page_size=P, gate=False)
     rows = ref.rows_of(pages.cpu(), 0, P, torch.arange(L)).cuda()
-    K = kernel_values(kp, n_pages * P, form != "chunks")[rows]
-    V = kernel_values(vp, n_pages * P, False)[rows]
+    K = tight.kernel_values(kp, n_pages * P, 4, True)[rows]
+    V = tight.kernel_values(vp, n_pages * P, 4, False)[rows]
     s = 16 * K[:, 0, 0] * SCALE                  # the same for every head
     gap = (s[0] - s[1]).item() / torch.log(torch.tensor(2.0)).item()
     assert 22.5 < gap < 22.9
@@ -191,10 +182,9 @@ def test_gates_of_every_size(fl, dev, kv8, T):
     qg[..., 256:] = torch.tensor(GATES * 22)[:256].to(F16).cuda()
     seen = torch.arange(L, device="cuda")[None] <= torch.arange(L - T, L, device="cuda")[:, None]
     for form, z in both_forms(fl, qg, kp, vp, pages, [L - T]):
-        K, V = kernel_values(kp, n, form == "decode")[rows], kernel_values(vp, n, False)[rows]
+        K, V = tight.kernel_values(kp, n, 4, True)[rows], tight.kernel_values(vp, n, 4, False)[rows]
         want, bound = tight.attention(qg[0, ..., :256], K, V, seen, SCALE,
-                                      tight.TWO_TERMS if kv8 and form == "decode" else tight.ONE_TERM,
-                                      qg[0, ..., 256:])
+                                      tight.TWO_TERMS if kv8 else tight.ONE_TERM, qg[0, ..., 256:])
         assert ((z[0].double() - want).abs() <= bound).all(), form
         assert not z[0][qg[0, ..., 256:] <= -88].any()
 
@@ -242,8 +232,7 @@ def test_scores_that_are_infinite(fl, dev, kv8):
         see = z[0, 2:, 6:12]                       # tokens 2 and 3, kv head 1's heads
         if not kv8:
             assert see[:, ::2].isnan().all(), form
-            K, V = kernel_values(spoiled[0], spoiled[4], True)[spoiled[3][0]], \
-                kernel_values(spoiled[1], spoiled[4], True)[spoiled[3][0]]
+            K, V = (tight.kernel_values(p, spoiled[4], 4, True)[spoiled[3][0]] for p in spoiled[:2])
             for t in (2, 3):
                 for h in (7, 9, 11):
                     q = qg[0, t, h, :256].double()
@@ -259,8 +248,29 @@ def test_scores_that_are_infinite(fl, dev, kv8):
         # so the infinite score moves where the others' weights round: not the same bits, but each
         # within the bound of what the clean rows give.
         seen = torch.arange(L, device="cuda")[None] <= torch.arange(L - T, L, device="cuda")[:, None]
-        K, V = (kernel_values(p, clean[4], False) for p in clean[:2])
+        K, V = (tight.kernel_values(p, clean[4], 4, e) for p, e in zip(clean[:2], (True, False)))
         for b in range(2):
             exact, bound = tight.attention(qg[b, ..., :256], K[clean[3][b]], V[clean[3][b]], seen, SCALE,
-                                           tight.ONE_TERM, qg[b, ..., 256:])
+                                           tight.TWO_TERMS if kv8 else tight.ONE_TERM, qg[b, ..., 256:])
             assert ((z[b].double() - exact).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("T", [1, 5])
+def test_int8_scales_of_every_size(fl, dev, T):
+    """K's block scales from 0 (whose bytes count for nothing) over subnormal ones to 0.1 side by
+    side in a row, V's likewise: the chunk kernel forms a score by the ratios of its row's scales."""
+    g, L, P = gen(31), 400, 16
+    pages, n_pages = ref.make_pages(g, [L], P)
+    sizes = torch.tensor([0.0, 2.0 ** -24, 2.0 ** -16, 1e-4, 0.003, 0.02, 0.1])
+    pools = []
+    for _ in range(2):
+        scales = sizes[torch.randint(0, 7, (n_pages * P, 4, 8), generator=g)]
+        pools.append(tight.int8_pool(torch.randint(-127, 128, (n_pages * P, 4, 256), generator=g), scales).cuda())
+    kp, vp = pools
+    rows = ref.rows_of(pages.cpu(), 0, P, torch.arange(L)).cuda()
+    K, V = tight.kernel_values(kp, n_pages * P, 4, True)[rows], tight.kernel_values(vp, n_pages * P, 4, False)[rows]
+    qg = randn(g, 1, T, 24, 512)
+    seen = torch.arange(L, device="cuda")[None] <= torch.arange(L - T, L, device="cuda")[:, None]
+    want, bound = tight.attention(qg[0, ..., :256], K, V, seen, SCALE, tight.TWO_TERMS, qg[0, ..., 256:])
+    for form, z in both_forms(fl, qg, kp, vp, pages, [L - T], P):
+        assert ((z[0].double() - want).abs() <= bound).all(), form

@@ -57,16 +57,16 @@ def check(z, want, bound, what):
     assert worst <= 1, f"{what}: {worst} of the bound"
 
 
-def of_kernel(pools, page_size, n_kv, exact_k):
+def of_kernel(pools, page_size, n_kv):
     n = pools[0].numel() // (n_kv * (272 if pools[0].dtype == torch.int8 else 256))
-    return (tight.kernel_values(pools[0], n, n_kv, exact_k), tight.kernel_values(pools[1], n, n_kv, False))
+    return (tight.kernel_values(pools[0], n, n_kv, True), tight.kernel_values(pools[1], n, n_kv, False))
 
 
 def run_decode(fl, seed, lens, page_size, kv8, T=1, window=0, sinks=0, heads=(24, 4), q_scale=1.0):
     g = gen(seed)
     n_q, n_kv = heads
     kp, vp, pages, rows = filled(fl, g, lens, page_size, kv8, n_kv)
-    K, V = of_kernel((kp, vp), page_size, n_kv, True)
+    K, V = of_kernel((kp, vp), page_size, n_kv)
     qg = randn(g, len(lens), T, n_q, 512, scale=q_scale)
     z = fl.ops.attn_decode_paged(qg, kp, vp, pages, i32(*[n - T for n in lens]), page_size=page_size,
                                  window=window, sinks=sinks, n_kv_heads=n_kv)
@@ -125,7 +125,7 @@ def test_decode_runs_that_load_their_page_ids_again(fl, dev, heads, T, B, L, pag
     assert walk > (32 if walk < 64 else 64)
     g = gen(65 + B)
     kp, vp, pages, [rows] = filled(fl, g, [L], page_size, kv8, n_kv)
-    K, V = of_kernel((kp, vp), page_size, n_kv, True)
+    K, V = of_kernel((kp, vp), page_size, n_kv)
     K, V = K[rows], V[rows]
     lens = [int(x) for x in torch.randint(L - 600, L + 1, (B,), generator=g)]
     qg = randn(g, B, T, n_q, 512)
@@ -142,7 +142,7 @@ def run_chunks(fl, seed, spans, page_size, kv8, window=0, sinks=0, heads=(24, 4)
     g = gen(seed)
     n_q, n_kv = heads
     kp, vp, pages, rows = filled(fl, g, [t + p for t, p in spans], page_size, kv8, n_kv)
-    K, V = of_kernel((kp, vp), page_size, n_kv, False)
+    K, V = of_kernel((kp, vp), page_size, n_kv)
     Ts, p0s = [t for t, _ in spans], [p for _, p in spans]
     qg = randn(g, sum(Ts), n_q, 512)
     z = fl.ops.attention_prefill_paged(qg, kp, vp, pages, Ts, p0s, page_size=page_size, window=window,
@@ -150,8 +150,8 @@ def run_chunks(fl, seed, spans, page_size, kv8, window=0, sinks=0, heads=(24, 4)
     at = 0
     for b, (t, p) in enumerate(spans):
         want, bound = tight.attention(qg[at:at + t, :, :256], K[rows[b]], V[rows[b]],
-                                      seen_mask(t, p, t + p, window, sinks), SCALE, tight.ONE_TERM,
-                                      qg[at:at + t, :, 256:])
+                                      seen_mask(t, p, t + p, window, sinks), SCALE,
+                                      tight.TWO_TERMS if kv8 else tight.ONE_TERM, qg[at:at + t, :, 256:])
         check(z[at:at + t], want, bound, f"sequence {b} ({t}@{p})")
         at += t
 
@@ -183,34 +183,45 @@ def test_int8_chunks_in_groups(fl, dev):
     run_chunks(fl, 23, [(3, 99997), (1, 98999), (20, 98480), (70, 0)], 256, True)
 
 
-@pytest.mark.parametrize("T,heads,B", [(1, (4, 1), 1), (20, (1, 1), 1), (3, (6, 1), 70)])
-def test_int8_decode_takes_k_exactly(fl, dev, T, heads, B):
-    """Scores of 100 whose differences K's rounding to fp16 would move by 5 %, up to 16 rows and
-    17 to 32 (a page each of 64 rows, shared by B sequences)."""
+@pytest.mark.parametrize("form,T,heads,B", [("decode", 1, (4, 1), 1), ("decode", 20, (1, 1), 1),
+                                            ("decode", 3, (6, 1), 70), ("chunks", 1, (4, 1), 1),
+                                            ("chunks", 50, (6, 1), 1), ("chunks", 40, (6, 1), 64)])
+def test_int8_takes_k_exactly(fl, dev, form, T, heads, B):
+    """Scores of 100 whose differences K's rounding to fp16 would move by 5 %: decode of up to 16
+    rows and of 17 to 32, chunks (a page of 64 rows, shared by B sequences)."""
     L = 64
     kp, vp, q = tight.near_ties(L)
     qg = q.cuda().expand(B, T, heads[0], 256).contiguous()
-    z = fl.ops.attn_decode_paged(qg, kp.cuda(), vp.cuda(), i32(0).view(1, 1).repeat(B, 1), i32(*[L - T] * B),
-                                 page_size=L, gate=False, n_kv_heads=1)
+    table = i32(0).view(1, 1).repeat(B, 1)
+    if form == "decode":
+        z = fl.ops.attn_decode_paged(qg, kp.cuda(), vp.cuda(), table, i32(*[L - T] * B), page_size=L, gate=False,
+                                     n_kv_heads=1)
+    else:
+        z = fl.ops.attention_prefill_paged(qg.view(B * T, heads[0], 256), kp.cuda(), vp.cuda(), table, [T] * B,
+                                           [L - T] * B, page_size=L, n_kv_heads=1).view(B, T, heads[0], 256)
     K, V = (tight.kernel_values(p, L, 1, e).cuda() for p, e in ((kp, True), (vp, False)))
     want, bound = tight.attention(qg[0], K, V, seen_mask(T, L - T, L), SCALE, tight.TWO_TERMS)
     for b in range(B):
         check(z[b], want, bound, f"sequence {b}")
 
 
-@pytest.mark.parametrize("T", [1, 20])
-def test_int8_decode_takes_weights_in_two_terms(fl, dev, T):
-    """One sequence of 64 rows beside 599 others (so that one wave or pair has them all): the mean
+@pytest.mark.parametrize("form,T", [("decode", 1), ("decode", 20), ("chunks", 30)])
+def test_int8_takes_weights_in_two_terms(fl, dev, form, T):
+    """600 sequences (60 chunks) of a page, so that one wave or pair has all its rows: the mean
     over the dims of z's relative error, whose part from z's own rounding is 2^-11 / sqrt(3 * 256),
     allowed 6 times; in one term it is more than twice that (tested on the CPU)."""
-    L, B = 32, 600
+    L, B = 32, 600 if form == "decode" else 60
     kp, vp, q, off = tight.one_term_shows(L)
     qg = q.cuda().expand(B, T, 1, 256).contiguous()
-    # (a wave's first tile holds the first row and sets the reference; the last token sees all)
-    z = fl.ops.attn_decode_paged(qg, kp.cuda(), vp.cuda(), i32(0).view(1, 1).repeat(B, 1), i32(*[L - T] * B),
-                                 page_size=L, gate=False, n_kv_heads=1)
+    table = i32(0).view(1, 1).repeat(B, 1)
+    if form == "decode":
+        z = fl.ops.attn_decode_paged(qg, kp.cuda(), vp.cuda(), table, i32(*[L - T] * B), page_size=L, gate=False,
+                                     n_kv_heads=1)
+    else:
+        z = fl.ops.attention_prefill_paged(qg.view(B * T, 1, 256), kp.cuda(), vp.cuda(), table, [T] * B,
+                                           [L - T] * B, page_size=L, n_kv_heads=1).view(B, T, 1, 256)
     K, V = (tight.kernel_values(p, L, 1, e)[:, 0].cuda() for p, e in ((kp, True), (vp, False)))
-    for t in (0, T - 1):
+    for t in (T // 2, T - 1):
         n = L - T + 1 + t
         want = torch.softmax(q.cuda().double() @ K[:n].t() * SCALE, -1) @ V[:n]
         mean = ((z[:, t, 0].double() - want) / want).mean(-1).abs().max().item()
