@@ -22,13 +22,14 @@
 // its own rounding, as over fp16 pools and in the int8 decode. (With f16(byte scale) for K as
 // well and P in one term it is 1.8 times, in two thirds of the time; K exact alone 1.7.)
 //
-// Bound by the matrix cores: 8192 fresh tokens at 24 q and 4 kv heads 842 us, 1.0 PFLOP/s of
-// the 1.3 that a large fp16 product reaches; the softmax between the two products of a tile
-// and a row tile's start and end (ITEM_COST) are the difference. Four chunks of 1024 with
-// a window 450 - 470 us (0.8: short walks). Over int8 pools a tile has half again the products
-// and 256 multiplications for the steps, 3.2 us where it has 2.0: 8192 fresh tokens 1300 us, six
-// of 1 - 1024 tokens at 0 - 60k 1.88 ms (0.55), 117 us of it the copy (6.3 TB/s).
-// The wave's registers are all taken. A spill is not only slow but wrong here: the O
+// Bound by a wave's own chain, one wave a SIMD: 8192 fresh tokens at 24 q and 4 kv heads 842 us,
+// 1.0 PFLOP/s of the 1.3 that a large fp16 product reaches, the matrix cores busy 40 % of the
+// cycles; the softmax between the two products of a tile and a row tile's start and end
+// (ITEM_COST) are the difference. Four chunks of 1024 with a window 450 - 470 us (0.8: short
+// walks). Over int8 pools a tile has half again the products and 256 multiplications for the
+// steps, 3.2 us where it has 2.0: 8192 fresh tokens 1300 us, six of 1 - 1024 tokens at 0 - 60k
+// 1.88 ms (0.55), 117 us of it the copy (6.3 TB/s).
+// The wave's registers are nearly all taken (233, over int8 pools 247 of 256, beside O's). A spill is not only slow but wrong here: the O
 // accumulators are written by inline-asm MFMAs, whose hazards the compiler does not see
 // when it stores them. Its resource report has to say 0 spilled VGPRs.
 #include "attn_paged.hpp"
@@ -948,9 +949,9 @@ int too_little_work(size_t have, size_t need) {
     return FL_ESCRATCH;
 }
 
-// The fp16 copy: row i of sequence b's part is the row of the union of its walks; a
-// wave a row, 8 dims (both of K and V) a lane and step. Rows past the sequence and of
-// absent pages are zeros.
+// The fp16 copy, K as the bytes (a block of scale 0 as zeros) and V as f16(byte scale): row i of
+// sequence b's part is the row of the union of its walks; a wave a row, 8 dims (both of K and V)
+// a lane and step. Rows past the sequence and of absent pages are zeros.
 __global__ void __launch_bounds__(256)
 paged_stage_kernel(const char* __restrict__ kp, const char* __restrict__ vp, const Pages pg,
                    const Chunks ch, const Sight sight, f16x8* __restrict__ ko, f16x8* __restrict__ vo,
