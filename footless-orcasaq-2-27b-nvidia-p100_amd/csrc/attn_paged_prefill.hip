@@ -29,9 +29,10 @@
 // walks). Over int8 pools a tile has half again the products and 256 multiplications for the
 // steps, 3.2 us where it has 2.0: 8192 fresh tokens 1300 us, six of 1 - 1024 tokens at 0 - 60k
 // 1.88 ms (0.55), 117 us of it the copy (6.3 TB/s).
-// The wave's registers are nearly all taken (233, over int8 pools 247 of 256, beside O's). A spill is not only slow but wrong here: the O
-// accumulators are written by inline-asm MFMAs, whose hazards the compiler does not see
-// when it stores them. Its resource report has to say 0 spilled VGPRs.
+// The wave's registers are nearly all taken (233, over int8 pools 247 of 256, beside O's). A
+// spill is not only slow but wrong here: the O accumulators are written by inline-asm MFMAs,
+// whose hazards the compiler does not see when it stores them. Its resource report has to say
+// 0 spilled VGPRs.
 #include "attn_paged.hpp"
 #include "attn_r64.hpp"
 
