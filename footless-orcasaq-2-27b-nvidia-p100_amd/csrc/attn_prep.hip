@@ -33,7 +33,6 @@
 
 #include <cmath>
 #include <mutex>
-#include <type_traits>
 
 // Products and sums round separately (no fma contraction), as the oracle's
 // restatement does, so the two agree bit for bit.
@@ -99,22 +98,33 @@ struct PrepPaged {
     int B, qo_pitch;
 };
 
+// ... whose rotation takes pair j's position from positions[axis[j]][i].
+struct PrepAxes : PrepPaged {
+    const int* positions;
+    int N;
+    uint8_t axis[PR_MAXPAIRS];
+};
+enum PrepKind { PLAIN, ROWS_OF, PACKED, AXES };
+template <PrepKind> struct PrepArgs { typedef PrepRows type; };
+template <> struct PrepArgs<PACKED> { typedef PrepPaged type; };
+template <> struct PrepArgs<AXES> { typedef PrepAxes type; };
+
 // flags: bit 0 norm, bit 1 rope, bit 2 KV store (k rows and their v rows),
 // bit 3 the store in the int8 format (caches of capacity max_pos); RPW rows a
-// wavefront. ROWS: token t is row t of a batched decode step, its position,
-// cache and capacity from `rows` (pos0, kc, vc and max_pos unused). PAGED: as
-// PrepPaged says, kc and vc the pools of capacity max_pos.
-template <int FLAGS, int RPW, bool ROWS = false, bool PAGED = false>
+// wavefront. ROWS_OF: token t is row t of a batched decode step, its position,
+// cache and capacity from `rows` (pos0, kc, vc and max_pos unused). PACKED, AXES: as
+// PrepPaged and PrepAxes say, kc and vc the pools of capacity max_pos.
+template <int FLAGS, int RPW, PrepKind KIND = PLAIN>
 __global__ void __launch_bounds__(64 * PR_WAVES)
 attn_prep_kernel(const f16* q, f16* qo, int q_pitch, f16* k, int k_pitch,
                  const f16* __restrict__ v, const float* __restrict__ wq,
                  const float* __restrict__ wk, void* __restrict__ kc_, void* __restrict__ vc_,
                  int n_q_heads, int n_kv_heads, int pos0, int max_pos_, int rope_dim,
-                 const RopeFreqs freqs, float eps,
-                 const typename std::conditional<PAGED, PrepPaged, PrepRows>::type rows) {
+                 const RopeFreqs freqs, float eps, const typename PrepArgs<KIND>::type rows) {
     __shared__ __attribute__((aligned(16))) float scs[PR_MAXPAIRS], ssn[PR_MAXPAIRS];
     __shared__ __attribute__((aligned(16))) f16 srow[PR_WAVES][PR_HD];
     constexpr bool NORM = FLAGS & 1, ROPE = FLAGS & 2, STORE = FLAGS & 4, Q8 = FLAGS & 8;
+    constexpr bool ROWS = KIND == ROWS_OF, PAGED = KIND == PACKED || KIND == AXES;
     const int t = blockIdx.x, hd0 = blockIdx.y * PR_WAVES * RPW;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     int pos = pos0 + t, max_pos = max_pos_;
@@ -155,7 +165,9 @@ attn_prep_kernel(const f16* q, f16* qo, int q_pitch, f16* k, int k_pitch,
     const int half_r = rope_dim >> 1;
     if (ROPE) {
         for (int j = threadIdx.x; j < half_r; j += 64 * PR_WAVES) {
-            const double ang = (double)pos * freqs.f[j];
+            int p = pos;
+            if constexpr (KIND == AXES) p = rows.positions[(size_t)rows.axis[j] * rows.N + t];
+            const double ang = (double)p * freqs.f[j];
             double sn, cs;
             sincos(ang, &sn, &cs);
             scs[j] = (float)cs;
@@ -327,6 +339,54 @@ int check_prep(const void* qg, const void* k, const void* v, const float* wq, co
     return FL_OK;
 }
 
+// The checks of packed tokens' prep, and what the kernels take of them.
+int packed_args(const void* qg, int q_pitch, const void* k, const void* v, const float* wq, const float* wk,
+                const void* q_out, int qo_pitch, const void* kpool, const void* vpool, int q8, int n_pages,
+                int page_size, const int* pages, int max_pages, long long pages_stride, const int* starts,
+                const int* pos0, int B, int N, int n_q_heads, int n_kv_heads, int head_dim, int rope_dim,
+                float eps, PrepPaged& pp) {
+    int rc = fl::make_pages(kpool, vpool, q8, n_pages, page_size, pages, max_pages, pages_stride, B,
+                            n_kv_heads, head_dim, pp.pages);
+    if (rc) return rc;
+    FL_REQUIRE(N >= 0 && starts && pos0, "null pointer");
+    rc = check_prep(qg, k, v, wq, wk, kpool, vpool, q_pitch, n_q_heads, n_kv_heads, head_dim, 0, 1, 1,
+                    rope_dim, eps);
+    if (rc) return rc;
+    FL_REQUIRE(n_q_heads <= 4096, "n_q_heads <= 4096");
+    FL_REQUIRE(q_out == nullptr || (qo_pitch >= head_dim && qo_pitch % 4 == 0 && al(q_out, 8)),
+               "q_out: pitch >= head_dim, % 4, 8-byte aligned");
+    pp.starts = starts;
+    pp.pos0 = pos0;
+    pp.B = B;
+    pp.qo_pitch = q_out ? qo_pitch : q_pitch;
+    return FL_OK;
+}
+
+template <PrepKind KIND>
+void launch_packed(void* qg, int q_pitch, const void* k, const void* v, const float* wq, const float* wk,
+                   void* q_out, void* kpool, void* vpool, int q8, int N, int n_q_heads, int n_kv_heads,
+                   int head_dim, int rope_dim, float theta, float eps,
+                   const typename PrepArgs<KIND>::type& args, fl_stream_t stream) {
+    f16* qo = (f16*)(q_out ? q_out : qg);
+    RopeFreqs freqs = {};
+    rope_freqs(theta, rope_dim, freqs);
+    const int heads = n_q_heads + n_kv_heads, capacity = args.pages.n_pages << args.pages.shift;
+    auto launch = [&](auto kernel, int rows_a_wave) {
+        hipLaunchKernelGGL(kernel,
+                           dim3(N, (heads + rows_a_wave * PR_WAVES - 1) / (rows_a_wave * PR_WAVES)),
+                           dim3(64 * PR_WAVES), 0, (hipStream_t)stream, (const f16*)qg, qo, q_pitch,
+                           (f16*)k, head_dim, (const f16*)v, wq, wk, kpool, vpool, n_q_heads,
+                           n_kv_heads, 0, capacity, rope_dim, freqs, eps, args);
+    };
+    if (N < 256) {   // launch_prep's rule
+        if (q8) launch(attn_prep_kernel<15, 1, KIND>, 1);
+        else launch(attn_prep_kernel<7, 1, KIND>, 1);
+    } else {
+        if (q8) launch(attn_prep_kernel<15, 7, KIND>, 7);
+        else launch(attn_prep_kernel<7, 7, KIND>, 7);
+    }
+}
+
 }  // namespace
 
 extern "C" {
@@ -408,12 +468,12 @@ int fl_attn_prep_rows(void* qg, int q_pitch, void* k, const void* v, const float
     rope_freqs(theta, rope_dim, freqs);
     const dim3 grid(B, (n_q_heads + n_kv_heads + PR_WAVES - 1) / PR_WAVES);
     if (q8)
-        hipLaunchKernelGGL((attn_prep_kernel<15, 1, true>), grid, dim3(64 * PR_WAVES), 0,
+        hipLaunchKernelGGL((attn_prep_kernel<15, 1, ROWS_OF>), grid, dim3(64 * PR_WAVES), 0,
                            (hipStream_t)stream, (const f16*)qg, (f16*)qg, q_pitch, (f16*)k,
                            head_dim, (const f16*)v, wq, wk, nullptr, nullptr, n_q_heads,
                            n_kv_heads, 0, 0, rope_dim, freqs, eps, rows);
     else
-        hipLaunchKernelGGL((attn_prep_kernel<7, 1, true>), grid, dim3(64 * PR_WAVES), 0,
+        hipLaunchKernelGGL((attn_prep_kernel<7, 1, ROWS_OF>), grid, dim3(64 * PR_WAVES), 0,
                            (hipStream_t)stream, (const f16*)qg, (f16*)qg, q_pitch, (f16*)k,
                            head_dim, (const f16*)v, wq, wk, nullptr, nullptr, n_q_heads,
                            n_kv_heads, 0, 0, rope_dim, freqs, eps, rows);
@@ -427,40 +487,39 @@ int fl_attn_prep_paged(void* qg, int q_pitch, const void* k, const void* v, cons
                        int n_q_heads, int n_kv_heads, int head_dim, int rope_dim, float theta,
                        float eps, fl_stream_t stream) {
     PrepPaged pp = {};
-    int rc = fl::make_pages(kpool, vpool, q8, n_pages, page_size, pages, max_pages, pages_stride, B,
-                            n_kv_heads, head_dim, pp.pages);
-    if (rc) return rc;
-    FL_REQUIRE(N >= 0 && starts && pos0, "null pointer");
-    rc = check_prep(qg, k, v, wq, wk, kpool, vpool, q_pitch, n_q_heads, n_kv_heads, head_dim, 0, 1, 1,
-                    rope_dim, eps);
-    if (rc) return rc;
-    FL_REQUIRE(n_q_heads <= 4096, "n_q_heads <= 4096");
-    FL_REQUIRE(q_out == nullptr || (qo_pitch >= head_dim && qo_pitch % 4 == 0 && al(q_out, 8)),
-               "q_out: pitch >= head_dim, % 4, 8-byte aligned");
-    if (N == 0) return FL_OK;
-    pp.starts = starts;
-    pp.pos0 = pos0;
-    pp.B = B;
-    pp.qo_pitch = q_out ? qo_pitch : q_pitch;
-    f16* qo = (f16*)(q_out ? q_out : qg);
-    RopeFreqs freqs = {};
-    rope_freqs(theta, rope_dim, freqs);
-    const int heads = n_q_heads + n_kv_heads;
-    auto launch = [&](auto kernel, int rows_a_wave) {
-        hipLaunchKernelGGL(kernel,
-                           dim3(N, (heads + rows_a_wave * PR_WAVES - 1) / (rows_a_wave * PR_WAVES)),
-                           dim3(64 * PR_WAVES), 0, (hipStream_t)stream, (const f16*)qg, qo, q_pitch,
-                           (f16*)k, head_dim, (const f16*)v, wq, wk, kpool, vpool, n_q_heads,
-                           n_kv_heads, 0, n_pages << pp.pages.shift, rope_dim, freqs, eps, pp);
-    };
-    if (N < 256) {   // launch_prep's rule
-        if (q8) launch(attn_prep_kernel<15, 1, false, true>, 1);
-        else launch(attn_prep_kernel<7, 1, false, true>, 1);
-    } else {
-        if (q8) launch(attn_prep_kernel<15, 7, false, true>, 7);
-        else launch(attn_prep_kernel<7, 7, false, true>, 7);
-    }
+    const int rc = packed_args(qg, q_pitch, k, v, wq, wk, q_out, qo_pitch, kpool, vpool, q8, n_pages,
+                               page_size, pages, max_pages, pages_stride, starts, pos0, B, N, n_q_heads,
+                               n_kv_heads, head_dim, rope_dim, eps, pp);
+    if (rc || N == 0) return rc;
+    launch_packed<PACKED>(qg, q_pitch, k, v, wq, wk, q_out, kpool, vpool, q8, N, n_q_heads, n_kv_heads,
+                          head_dim, rope_dim, theta, eps, pp, stream);
     return fl::check_launch("attn_prep_paged");
+}
+
+int fl_attn_prep_axes(void* qg, int q_pitch, const void* k, const void* v, const float* wq,
+                      const float* wk, void* q_out, int qo_pitch, void* kpool, void* vpool, int q8,
+                      int n_pages, int page_size, const int* pages, int max_pages,
+                      long long pages_stride, const int* starts, const int* pos0,
+                      const int* positions, int n_axes, const int* pair_axis, int B, int N,
+                      int n_q_heads, int n_kv_heads, int head_dim, int rope_dim, float theta,
+                      float eps, fl_stream_t stream) {
+    PrepAxes pa = {};
+    const int rc = packed_args(qg, q_pitch, k, v, wq, wk, q_out, qo_pitch, kpool, vpool, q8, n_pages,
+                               page_size, pages, max_pages, pages_stride, starts, pos0, B, N, n_q_heads,
+                               n_kv_heads, head_dim, rope_dim, eps, pa);
+    if (rc) return rc;
+    FL_REQUIRE(positions && pair_axis, "null pointer");
+    FL_REQUIRE(n_axes >= 1 && n_axes <= PR_MAXPAIRS, "1 <= n_axes <= 128");
+    for (int j = 0; j < rope_dim / 2; ++j) {
+        FL_REQUIRE(pair_axis[j] >= 0 && pair_axis[j] < n_axes, "0 <= pair_axis[j] < n_axes");
+        pa.axis[j] = (uint8_t)pair_axis[j];
+    }
+    if (N == 0) return FL_OK;
+    pa.positions = positions;
+    pa.N = N;
+    launch_packed<AXES>(qg, q_pitch, k, v, wq, wk, q_out, kpool, vpool, q8, N, n_q_heads, n_kv_heads,
+                        head_dim, rope_dim, theta, eps, pa, stream);
+    return fl::check_launch("attn_prep_axes");
 }
 
 }  // extern "C"

@@ -161,6 +161,99 @@ paged_load_kernel(const void* __restrict__ kpool, const void* __restrict__ vpool
     }
 }
 
+// ---------------------------------------------------------------------------
+// Pages and accepted rows moved inside the pools of all layers at once. A pool is 16-byte
+// units: a head row's 32 of fp16, or 16 of bytes and, behind all values, one of scales.
+// ---------------------------------------------------------------------------
+struct Pools {
+    char* p[2 * FL_POOL_MAX];   // K and V of every layer
+};
+constexpr int CP_THREADS = 256, CP_UNITS = 4;   // 16 KiB of fp16 a workgroup
+constexpr int KEEP_ROWS = 8;                    // rows of a path in flight
+
+// Unit u of run `at` (a page, a row; `units` of it are values) of a pool with `values` units of
+// values ahead of its scales.
+template <bool Q8>
+__device__ __forceinline__ u32x4* unit(char* pool, size_t at, int units, size_t values, int u) {
+    u32x4* p = (u32x4*)pool;
+    if (Q8 && u >= units) return p + values + at * (units / 16) + (u - units);
+    return p + at * units + u;
+}
+
+// A copy reads and writes each byte once: non-temporal, and a lane's units in flight together.
+template <bool Q8>
+__global__ void __launch_bounds__(CP_THREADS)
+paged_copy_kernel(const Pools pools, const int* __restrict__ src, const int* __restrict__ dst,
+                  int n_pages, int units, int parts) {
+    const int i = blockIdx.x / parts, part = blockIdx.x - i * parts;
+    const int from = src[i], to = dst[i];
+    if ((unsigned)from >= (unsigned)n_pages || (unsigned)to >= (unsigned)n_pages || from == to) return;
+    char* pool = pools.p[blockIdx.y];
+    const size_t values = (size_t)n_pages * units;
+    const int all = units + (Q8 ? units / 16 : 0);
+    const int u0 = part * CP_THREADS * CP_UNITS + threadIdx.x;
+    u32x4 x[CP_UNITS];
+#pragma unroll
+    for (int c = 0; c < CP_UNITS; ++c) {
+        const int u = u0 + c * CP_THREADS;
+        if (u < all) x[c] = __builtin_nontemporal_load(unit<Q8>(pool, from, units, values, u));
+    }
+#pragma unroll
+    for (int c = 0; c < CP_UNITS; ++c) {
+        const int u = u0 + c * CP_THREADS;
+        if (u < all) __builtin_nontemporal_store(x[c], unit<Q8>(pool, to, units, values, u));
+    }
+}
+
+// A path's entries grow, so entry d is d or more, and row pos0 + d is read for no later entry: a
+// lane moves its unit of the rows in the path's order, KEEP_ROWS of them in flight.
+template <bool Q8>
+__global__ void __launch_bounds__(128)
+paged_keep_kernel(const Pools pools, const Pages pg, const int* __restrict__ pos0,
+                  const int* __restrict__ path, int D, int units) {
+    const int b = blockIdx.x, u = blockIdx.z * 128 + threadIdx.x;
+    const int p0 = pos0[b];
+    if (p0 < 0 || u >= units + (Q8 ? units / 16 : 0)) return;
+    char* pool = pools.p[blockIdx.y];
+    const size_t values = ((size_t)pg.n_pages << pg.shift) * units;
+    auto row = [&](int i) {   // a row's run in the pool, -1: absent
+        const long long at = (long long)p0 + i;
+        return at > INT_MAX ? -1ll : fl::page_row(pg, b, (int)at);
+    };
+    int last = -1;
+    for (int d0 = 0; d0 < D; d0 += KEEP_ROWS) {
+        u32x4 x[KEEP_ROWS];
+        long long to[KEEP_ROWS];
+        bool on = true;
+#pragma unroll
+        for (int c = 0; c < KEEP_ROWS; ++c) {
+            const int d = d0 + c, i = d < D ? path[(size_t)b * D + d] : -1;
+            on = on && i > last;
+            to[c] = -1;
+            if (!on) continue;
+            last = i;
+            const long long from = i > d ? row(i) : -1;
+            if (from >= 0 && (to[c] = row(d)) >= 0) x[c] = *unit<Q8>(pool, from, units, values, u);
+        }
+#pragma unroll
+        for (int c = 0; c < KEEP_ROWS; ++c)
+            if (to[c] >= 0) *unit<Q8>(pool, to[c], units, values, u) = x[c];
+        if (!on) return;
+    }
+}
+
+int make_pools(void* const* kpools, void* const* vpools, int n_layers, Pools& out) {
+    FL_REQUIRE(kpools && vpools, "null pointer");
+    FL_REQUIRE(n_layers >= 1 && n_layers <= FL_POOL_MAX, "1 <= n_layers <= FL_POOL_MAX");
+    for (int l = 0; l < n_layers; ++l) {
+        out.p[2 * l] = (char*)kpools[l];
+        out.p[2 * l + 1] = (char*)vpools[l];
+    }
+    for (int i = 0; i < 2 * n_layers; ++i)
+        FL_REQUIRE(out.p[i] && ((uintptr_t)out.p[i] & 15) == 0, "null or unaligned pool");
+    return FL_OK;
+}
+
 int check_rows(const void* k, const void* v, long long k_stride, long long v_stride, const int* starts,
                const int* pos0, int N, int n_kv, int head_dim) {
     FL_REQUIRE(k && v && starts && pos0, "null pointer");
@@ -211,6 +304,47 @@ int fl_paged_kv_load(const void* kpool, const void* vpool, int q8, int n_pages, 
                        (hipStream_t)stream, kpool, vpool, pg, starts, pos0, (f16*)k, (f16*)v,
                        k_stride, v_stride, zero_rest, B, N, n_kv_heads);
     return fl::check_launch("paged_kv_load");
+}
+
+int fl_paged_kv_copy(void* const* kpools, void* const* vpools, int n_layers, int q8, int n_pages,
+                     int page_size, const int* src, const int* dst, int n, int n_kv_heads,
+                     int head_dim, fl_stream_t stream) {
+    Pools pools = {};
+    int rc = make_pools(kpools, vpools, n_layers, pools);
+    if (rc) return rc;
+    Pages pg;   // (the checks of the sizes; there is no table)
+    rc = fl::make_pages(kpools[0], vpools[0], q8, n_pages, page_size, (const int*)kpools[0], 1, 1, 1, n_kv_heads,
+                        head_dim, pg);
+    if (rc) return rc;
+    FL_REQUIRE(n >= 0 && (n == 0 || (src && dst)), "null pointer");
+    const long long units = (long long)page_size * n_kv_heads * (q8 ? 16 : 32);
+    const long long parts = (units + (q8 ? units / 16 : 0) + CP_THREADS * CP_UNITS - 1) / (CP_THREADS * CP_UNITS);
+    FL_REQUIRE(units * 2 <= INT_MAX && parts * n <= INT_MAX, "n * page_size * n_kv_heads < 2^36");
+    if (n == 0) return FL_OK;
+    hipLaunchKernelGGL(q8 ? paged_copy_kernel<true> : paged_copy_kernel<false>,
+                       dim3((unsigned)(parts * n), 2 * n_layers), dim3(CP_THREADS), 0, (hipStream_t)stream,
+                       pools, src, dst, n_pages, (int)units, (int)parts);
+    return fl::check_launch("paged_kv_copy");
+}
+
+int fl_paged_kv_keep(void* const* kpools, void* const* vpools, int n_layers, int q8, int n_pages,
+                     int page_size, const int* pages, int max_pages, long long pages_stride,
+                     const int* pos0, const int* path, int B, int D, int n_kv_heads, int head_dim,
+                     fl_stream_t stream) {
+    Pools pools = {};
+    int rc = make_pools(kpools, vpools, n_layers, pools);
+    if (rc) return rc;
+    Pages pg;
+    rc = fl::make_pages(kpools[0], vpools[0], q8, n_pages, page_size, pages, max_pages, pages_stride, B,
+                        n_kv_heads, head_dim, pg);
+    if (rc) return rc;
+    FL_REQUIRE(D >= 0 && pos0 && (D == 0 || path), "null pointer");
+    if (D == 0) return FL_OK;
+    const int units = n_kv_heads * (q8 ? 16 : 32), all = units + (q8 ? units / 16 : 0);
+    hipLaunchKernelGGL(q8 ? paged_keep_kernel<true> : paged_keep_kernel<false>,
+                       dim3(B, 2 * n_layers, (all + 127) / 128), dim3(128), 0, (hipStream_t)stream, pools,
+                       pg, pos0, path, D, units);
+    return fl::check_launch("paged_kv_keep");
 }
 
 }  // extern "C"

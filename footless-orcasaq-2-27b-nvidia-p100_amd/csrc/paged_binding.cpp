@@ -26,6 +26,9 @@ decltype(&fl_attention_prefill_paged_work_bytes) p_prefill_bytes;
 decltype(&fl_attention_prefill_paged) p_prefill;
 decltype(&fl_attn_decode_paged_work_bytes) p_decode_bytes;
 decltype(&fl_attn_decode_paged) p_decode;
+decltype(&fl_attn_prep_axes) p_prep_axes;
+decltype(&fl_paged_kv_copy) p_copy;
+decltype(&fl_paged_kv_keep) p_keep;
 
 constexpr int64_t HEAD_DIM = 256, KV8_ROW = HEAD_DIM + HEAD_DIM / 32 * 2;   // bytes of an int8 head row
 
@@ -207,42 +210,6 @@ PyObject* kv_load(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// (dev, stream, qg, k, v, wq, wk, q_out or None, starts, pos0, kpool, vpool, pages, page_size,
-//  n_q, n_kv, head_dim, rope_dim, theta, eps)
-PyObject* prep(PyObject*, PyObject* const* args, Py_ssize_t n) {
-    HANDLE_TH_ERRORS
-    Args a{args};
-    PLAIN(n == 20);
-    a.dev = a.integer32();
-    const auto stream = (fl_stream_t)a.integer();
-    const at::Tensor *qg = a.dense(at::kHalf, 3), *k = a.dense(at::kHalf, 3), *v = a.dense(at::kHalf, 3);
-    const at::Tensor *wq = a.dense(at::kFloat, 1), *wk = a.dense(at::kFloat, 1);
-    PyObject* qo = a.next();
-    const at::Tensor* q_out = qo == Py_None ? nullptr : a.dense(qo, at::kHalf, 3);
-    const Packed s(a);
-    Pools c(a);
-    const int64_t page_size = a.integer(), n_q = a.integer(), n_kv = a.integer(), head_dim = a.integer();
-    const int rope_dim = a.integer32();
-    const float theta = a.real(), eps = a.real();
-    PLAIN(a.ok && s.count() >= 0 && c.fit(s.count(), page_size, n_kv, head_dim));
-    const int64_t N = qg->size(0), pitch = qg->size(2);
-    PLAIN(N > 0 && N <= INT_MAX && n_q <= INT_MAX && pitch <= INT_MAX && qg->size(1) == n_q &&
-          k->sizes() == v->sizes() && k->size(0) == N && k->size(1) == n_kv && k->size(2) == head_dim &&
-          wq->numel() >= head_dim && wk->numel() >= head_dim);
-    PLAIN(!q_out || (q_out->size(0) == N && q_out->size(1) == n_q && q_out->size(2) <= INT_MAX));
-    const int rc = released([&] {
-        return p_prep(qg->data_ptr(), (int)pitch, k->data_ptr(), v->data_ptr(), (const float*)wq->data_ptr(),
-                      (const float*)wk->data_ptr(), q_out ? q_out->data_ptr() : nullptr,
-                      q_out ? (int)q_out->size(2) : 0, c.k->data_ptr(), c.v->data_ptr(), c.q8, c.n_pages,
-                      (int)page_size, (const int*)c.pages->data_ptr(), c.max_pages, c.stride,
-                      (const int*)s.starts->data_ptr(), (const int*)s.pos0->data_ptr(), (int)s.count(),
-                      (int)N, (int)n_q, (int)n_kv, (int)head_dim, rope_dim, theta, eps, stream);
-    });
-    MADE(rc);
-    Py_RETURN_TRUE;
-    END_HANDLE_TH_ERRORS
-}
-
 // host ints of a list or tuple; false where it is neither, or holds anything else
 bool ints(PyObject* o, int* out, Py_ssize_t most, Py_ssize_t& n) {
     const bool list = PyList_CheckExact(o);
@@ -258,6 +225,149 @@ bool ints(PyObject* o, int* out, Py_ssize_t most, Py_ssize_t& n) {
         out[i] = (int)v;
     }
     return true;
+}
+
+// (dev, stream, qg, k, v, wq, wk, q_out or None, starts, pos0, kpool, vpool, pages, page_size,
+//  n_q, n_kv, head_dim, rope_dim, theta, eps), AXES: and (positions, the pairs' axes)
+template <bool AXES>
+PyObject* prep_of(PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Args a{args};
+    PLAIN(n == (AXES ? 22 : 20));
+    a.dev = a.integer32();
+    const auto stream = (fl_stream_t)a.integer();
+    const at::Tensor *qg = a.dense(at::kHalf, 3), *k = a.dense(at::kHalf, 3), *v = a.dense(at::kHalf, 3);
+    const at::Tensor *wq = a.dense(at::kFloat, 1), *wk = a.dense(at::kFloat, 1);
+    PyObject* qo = a.next();
+    const at::Tensor* q_out = qo == Py_None ? nullptr : a.dense(qo, at::kHalf, 3);
+    const Packed s(a);
+    Pools c(a);
+    const int64_t page_size = a.integer(), n_q = a.integer(), n_kv = a.integer(), head_dim = a.integer();
+    const int rope_dim = a.integer32();
+    const float theta = a.real(), eps = a.real();
+    const at::Tensor* at = nullptr;
+    int axis[HEAD_DIM / 2];
+    if (AXES) {
+        at = a.dense(at::kInt, 2);
+        Py_ssize_t pairs = 0;
+        PLAIN(ints(a.next(), axis, HEAD_DIM / 2, pairs) && pairs * 2 == rope_dim);
+    }
+    PLAIN(a.ok && s.count() >= 0 && c.fit(s.count(), page_size, n_kv, head_dim));
+    const int64_t N = qg->size(0), pitch = qg->size(2);
+    PLAIN(N > 0 && N <= INT_MAX && n_q <= INT_MAX && pitch <= INT_MAX && qg->size(1) == n_q &&
+          k->sizes() == v->sizes() && k->size(0) == N && k->size(1) == n_kv && k->size(2) == head_dim &&
+          wq->numel() >= head_dim && wk->numel() >= head_dim);
+    PLAIN(!q_out || (q_out->size(0) == N && q_out->size(1) == n_q && q_out->size(2) <= INT_MAX));
+    PLAIN(!AXES || (at->size(1) == N && at->size(0) <= INT_MAX));
+    const int rc = released([&] {
+        auto call = [&](auto f, auto... more) {
+            return f(qg->data_ptr(), (int)pitch, k->data_ptr(), v->data_ptr(), (const float*)wq->data_ptr(),
+                     (const float*)wk->data_ptr(), q_out ? q_out->data_ptr() : nullptr,
+                     q_out ? (int)q_out->size(2) : 0, c.k->data_ptr(), c.v->data_ptr(), c.q8, c.n_pages,
+                     (int)page_size, (const int*)c.pages->data_ptr(), c.max_pages, c.stride,
+                     (const int*)s.starts->data_ptr(), (const int*)s.pos0->data_ptr(), more...,
+                     (int)s.count(), (int)N, (int)n_q, (int)n_kv, (int)head_dim, rope_dim, theta, eps, stream);
+        };
+        if constexpr (AXES) return call(p_prep_axes, (const int*)at->data_ptr(), (int)at->size(0), (const int*)axis);
+        else return call(p_prep);
+    });
+    MADE(rc);
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+PyObject* prep(PyObject*, PyObject* const* args, Py_ssize_t n) { return prep_of<false>(args, n); }
+PyObject* prep_axes(PyObject*, PyObject* const* args, Py_ssize_t n) { return prep_of<true>(args, n); }
+
+// The pools of several layers, alike: two lists or tuples of tensors, or two tensors.
+struct LayerPools {
+    void *k[FL_POOL_MAX], *v[FL_POOL_MAX];
+    int layers = 0, q8 = 0;
+    const at::Tensor* first = nullptr;
+
+    LayerPools(Args& a) {
+        const int nk = take(a, k), nv = take(a, v);
+        layers = nk;
+        a.ok = a.ok && nk == nv;
+    }
+    // pages of the pools, -1 where they are none of these sizes
+    int64_t pages(int64_t page_size, int64_t n_kv, int64_t head_dim) const {
+        if (page_size < 1 || n_kv < 1 || page_size > INT_MAX || n_kv > INT_MAX || head_dim != HEAD_DIM ||
+            page_size * n_kv > INT_MAX)
+            return -1;
+        if (!q8) {
+            const bool fit = first->size(1) == page_size && first->size(2) == n_kv && first->size(3) == head_dim;
+            return fit && first->size(0) <= INT_MAX ? first->size(0) : -1;
+        }
+        const int64_t unit = page_size * n_kv * KV8_ROW, n = first->numel() / unit;
+        return n * unit == first->numel() && n <= INT_MAX ? n : -1;
+    }
+
+  private:
+    int take(Args& a, void** to) {
+        PyObject* o = a.next();
+        if (THPVariable_CheckExact(o)) return one(a, o, to) ? 1 : -1;
+        const bool list = PyList_CheckExact(o);
+        const Py_ssize_t n = list ? PyList_GET_SIZE(o) : PyTuple_CheckExact(o) ? PyTuple_GET_SIZE(o) : 0;
+        if (n < 1 || n > FL_POOL_MAX) return a.ok = false, -1;
+        for (Py_ssize_t i = 0; i < n; ++i)
+            if (!one(a, list ? PyList_GET_ITEM(o, i) : PyTuple_GET_ITEM(o, i), to + i)) return -1;
+        return (int)n;
+    }
+    bool one(Args& a, PyObject* o, void** to) {
+        if (!first) q8 = THPVariable_CheckExact(o) && THPVariable_Unpack(o).scalar_type() == at::kChar;
+        const at::Tensor* t = a.dense(o, q8 ? at::kChar : at::kHalf, q8 ? 1 : 4);
+        if (!t) return false;
+        if (!first) first = t;
+        else if (t->sizes() != first->sizes()) return a.ok = false;
+        *to = t->data_ptr();
+        return true;
+    }
+};
+
+// (dev, stream, kpools, vpools, src, dst, page_size, n_kv, head_dim)
+PyObject* kv_copy(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Args a{args};
+    PLAIN(n == 9);
+    a.dev = a.integer32();
+    const auto stream = (fl_stream_t)a.integer();
+    const LayerPools c(a);
+    const at::Tensor *src = a.dense(at::kInt, 1), *dst = a.dense(at::kInt, 1);
+    const int64_t page_size = a.integer(), n_kv = a.integer(), head_dim = a.integer();
+    PLAIN(a.ok);
+    const int64_t pages = c.pages(page_size, n_kv, head_dim);
+    PLAIN(pages >= 0 && src->numel() == dst->numel() && src->numel() <= INT_MAX);
+    const int rc = released([&] {
+        return p_copy(c.k, c.v, c.layers, c.q8, (int)pages, (int)page_size, (const int*)src->data_ptr(),
+                      (const int*)dst->data_ptr(), (int)src->numel(), (int)n_kv, (int)head_dim, stream);
+    });
+    MADE(rc);
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
+// (dev, stream, kpools, vpools, pages, pos0, path, page_size, n_kv, head_dim)
+PyObject* kv_keep(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Args a{args};
+    PLAIN(n == 10);
+    a.dev = a.integer32();
+    const auto stream = (fl_stream_t)a.integer();
+    const LayerPools c(a);
+    const at::Tensor *table = a.dense(at::kInt, 2), *pos0 = a.dense(at::kInt, 1), *path = a.dense(at::kInt, 2);
+    const int64_t page_size = a.integer(), n_kv = a.integer(), head_dim = a.integer();
+    PLAIN(a.ok);
+    const int64_t pages = c.pages(page_size, n_kv, head_dim), B = pos0->numel();
+    PLAIN(pages >= 0 && B > 0 && B <= INT_MAX && table->size(0) == B && path->size(0) == B &&
+          table->size(1) <= INT_MAX && path->size(1) <= INT_MAX);
+    const int rc = released([&] {
+        return p_keep(c.k, c.v, c.layers, c.q8, (int)pages, (int)page_size, (const int*)table->data_ptr(),
+                      (int)table->size(1), table->size(1), (const int*)pos0->data_ptr(),
+                      (const int*)path->data_ptr(), (int)B, (int)path->size(1), (int)n_kv, (int)head_dim, stream);
+    });
+    MADE(rc);
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
 }
 
 // (dev, stream, q, kpool, vpool, pages, Ts, pos0s, page_size, window, sinks, gated, z or None,
@@ -364,7 +474,8 @@ PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
 // the entry points' addresses, in the order of the declarations above
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
     void** const to[] = {(void**)&p_store, (void**)&p_load, (void**)&p_prep, (void**)&p_prefill_bytes,
-                         (void**)&p_prefill, (void**)&p_decode_bytes, (void**)&p_decode};
+                         (void**)&p_prefill, (void**)&p_decode_bytes, (void**)&p_decode,
+                         (void**)&p_prep_axes, (void**)&p_copy, (void**)&p_keep};
     if (n != (Py_ssize_t)(sizeof(to) / sizeof(to[0]))) {
         PyErr_SetString(PyExc_TypeError, "bind: one address an entry point");
         return nullptr;
@@ -383,6 +494,9 @@ PyMethodDef methods[] = {
     {"prep", (PyCFunction)(void (*)())prep, METH_FASTCALL, nullptr},
     {"prefill", (PyCFunction)(void (*)())prefill, METH_FASTCALL, nullptr},
     {"decode", (PyCFunction)(void (*)())decode, METH_FASTCALL, nullptr},
+    {"prep_axes", (PyCFunction)(void (*)())prep_axes, METH_FASTCALL, nullptr},
+    {"kv_copy", (PyCFunction)(void (*)())kv_copy, METH_FASTCALL, nullptr},
+    {"kv_keep", (PyCFunction)(void (*)())kv_keep, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "fl355_paged", nullptr, -1, methods};

@@ -723,6 +723,27 @@ def paged_kv_load(kpool, vpool, pages, starts, pos0, *, T: int, page_size: int, 
     return k, v
 
 
+def _prep_args(qg, k, v, wq, wk, q_out, kpool, vpool, pages, page_size, B, n_q_heads, n_kv_heads, head_dim,
+               dev):
+    """(N, pointers, pool) of a prep of packed tokens."""
+    N, heads, q_pitch = qg.shape
+    if heads != n_q_heads or k.shape != (N, n_kv_heads, head_dim) or v.shape != k.shape:
+        raise ValueError("qg [N, n_q_heads, q_pitch], k and v [N, n_kv_heads, head_dim]")
+    qo, qo_pitch = None, 0
+    if q_out is not None:
+        if q_out.dim() != 3 or q_out.shape[0] != N or q_out.shape[1] != n_q_heads:
+            raise ValueError(f"q_out: expected [{N}, {n_q_heads}, pitch]")
+        qo_pitch = q_out.shape[2]
+        qo = _dense_ptr(q_out, F16, "q_out", N * n_q_heads * qo_pitch)
+    ptrs = (_dense_ptr(qg, F16, "qg"), q_pitch, _dense_ptr(k, F16, "k"), _dense_ptr(v, F16, "v"),
+            _dense_ptr(wq, F32, "wq", head_dim), _dense_ptr(wk, F32, "wk", head_dim), qo, qo_pitch)
+    pg = _paged(kpool, vpool, pages, page_size, B, n_kv_heads, head_dim, dev)
+    if not (qg.get_device() == k.get_device() == v.get_device() == wq.get_device()
+            == wk.get_device() == dev) or (q_out is not None and q_out.get_device() != dev):
+        _same_device(dev, qg=qg, k=k, v=v, wq=wq, wk=wk, q_out=q_out)
+    return N, ptrs, pg
+
+
 def attn_prep_paged(qg, k, v, wq, wk, kpool, vpool, pages, starts, pos0, *, page_size: int,
                     q_out=None, n_q_heads: int = N_HEADS, n_kv_heads: int = N_KV,
                     head_dim: int = HEAD_DIM, rope_dim: int = ROPE_DIM, theta: float = ROPE_THETA,
@@ -740,21 +761,8 @@ def attn_prep_paged(qg, k, v, wq, wk, kpool, vpool, pages, starts, pos0, *, page
         if r is not None:
             return _made("fl_attn_prep_paged", r, qg if q_out is None else q_out)
     sp, pp, B = _packed(starts, pos0, dev)
-    N, heads, q_pitch = qg.shape
-    if heads != n_q_heads or k.shape != (N, n_kv_heads, head_dim) or v.shape != k.shape:
-        raise ValueError("qg [N, n_q_heads, q_pitch], k and v [N, n_kv_heads, head_dim]")
-    qo, qo_pitch = None, 0
-    if q_out is not None:
-        if q_out.dim() != 3 or q_out.shape[0] != N or q_out.shape[1] != n_q_heads:
-            raise ValueError(f"q_out: expected [{N}, {n_q_heads}, pitch]")
-        qo_pitch = q_out.shape[2]
-        qo = _dense_ptr(q_out, F16, "q_out", N * n_q_heads * qo_pitch)
-    ptrs = (_dense_ptr(qg, F16, "qg"), q_pitch, _dense_ptr(k, F16, "k"), _dense_ptr(v, F16, "v"),
-            _dense_ptr(wq, F32, "wq", head_dim), _dense_ptr(wk, F32, "wk", head_dim), qo, qo_pitch)
-    pg = _paged(kpool, vpool, pages, page_size, B, n_kv_heads, head_dim, dev)
-    if not (qg.get_device() == k.get_device() == v.get_device() == wq.get_device()
-            == wk.get_device() == dev) or (q_out is not None and q_out.get_device() != dev):
-        _same_device(dev, qg=qg, k=k, v=v, wq=wq, wk=wk, q_out=q_out)
+    N, ptrs, pg = _prep_args(qg, k, v, wq, wk, q_out, kpool, vpool, pages, page_size, B, n_q_heads,
+                             n_kv_heads, head_dim, dev)
     if N:
         _lib.call("fl_attn_prep_paged", *ptrs, *pg, sp, pp, B, N, n_q_heads, n_kv_heads, head_dim,
                   rope_dim, theta, eps, _stream())
@@ -867,6 +875,161 @@ def attn_decode_paged(qg, kpool, vpool, pages, pos0, *, page_size: int, window: 
     _lib.call("fl_attn_decode_paged", qp, q_pitch, *pg, pp, B, T, n_q_heads, n_kv_heads, HEAD_DIM,
               scale, window, sinks, int(gate), zp, z.shape[3], *_prefill_work(work), _stream())
     return z
+
+
+# ---------------------------------------------------------------------------
+# Trees of drafted tokens over the paged cache (no reference counterpart: its verify
+# rounds carry a chain of 2 or 3 tokens). A drafter proposes several continuations of
+# a sequence as a tree of up to 64 tokens: parents [B, T] int32 on the GPU holds each
+# token's parent, an earlier token, or -1 (a child of the context); any other entry is
+# a place that holds no token, and so is one whose parent holds none. Token i of
+# sequence b lies in cache row pos0[b] + i, behind the context's pos0[b] rows; its
+# position is pos0[b] + its depth. A round: attn_prep_axes stores the tree's rows at its
+# positions, attn_tree_paged and gdn_tree_normed verify it, and once a path is accepted
+# (path [B, D] int32, a sequence's tokens in order, -1 behind the last) paged_kv_keep
+# moves its rows up and gdn_tree_commit forms the recurrent state behind it.
+# ---------------------------------------------------------------------------
+
+TREE_MAX, POOL_MAX = 64, 64
+
+
+@functools.lru_cache(maxsize=64)
+def _pair_axes(n_axes, sections, interleaved, rope_dim):
+    """The axis of every rotary pair."""
+    pairs = rope_dim // 2
+    if sections is None:
+        sections = (pairs,) if n_axes == 1 else ()
+    if len(sections) != n_axes or sum(sections) != pairs or min(sections, default=0) < 0:
+        raise ValueError(f"sections: {n_axes} axes' rotary pairs, {pairs} in all")
+    if not interleaved:
+        return tuple(a for a, n in enumerate(sections) for _ in range(n))
+    of = [0] * pairs
+    for a, n in enumerate(sections):
+        if a and n and a + n_axes * (n - 1) >= pairs:
+            raise ValueError(f"sections: axis {a} has no {n} pairs of every {n_axes}")
+        of[a:n_axes * n:n_axes] = [a] * len(of[a:n_axes * n:n_axes])
+    return tuple(of)
+
+
+def attn_prep_axes(qg, k, v, wq, wk, kpool, vpool, pages, starts, pos0, positions, *, page_size: int,
+                   sections=None, interleaved: bool = False, q_out=None, n_q_heads: int = N_HEADS,
+                   n_kv_heads: int = N_KV, head_dim: int = HEAD_DIM, rope_dim: int = ROPE_DIM,
+                   theta: float = ROPE_THETA, eps: float = NORM_EPS):
+    """attn_prep_paged with the rotation's positions given: positions [axes, N] int32 on
+    the GPU, one row an axis (time, height and width of images and video; a tree's
+    depths). sections: the rotary pairs of each axis, rope_dim / 2 in all (one axis: all
+    of them); axis after axis, or interleaved: pair j is axis j % axes' as far as its
+    section goes, the first axis' otherwise. The cache rows stay those that starts and
+    pos0 give. Where every axis holds those positions the values are attn_prep_paged's
+    bit for bit. Returns the tensor that holds q."""
+    dev = _here()
+    if not isinstance(positions, torch.Tensor):
+        raise TypeError("positions: expected a torch.Tensor")
+    if positions.dim() != 2 or positions.shape[0] < 1:
+        raise ValueError("positions: expected [axes, N]")
+    of = _pair_axes(positions.shape[0], None if sections is None else tuple(sections), bool(interleaved),
+                    rope_dim)
+    if dev >= 0 and _lib.lane is not None:
+        r = _lib.lane.prep_axes(dev, _stream(), qg, k, v, wq, wk, q_out, starts, pos0, kpool, vpool, pages,
+                                page_size, n_q_heads, n_kv_heads, head_dim, rope_dim, theta, eps, positions,
+                                of)
+        if r is not None:
+            return _made("fl_attn_prep_axes", r, qg if q_out is None else q_out)
+    sp, pp, B = _packed(starts, pos0, dev)
+    N, ptrs, pg = _prep_args(qg, k, v, wq, wk, q_out, kpool, vpool, pages, page_size, B, n_q_heads,
+                             n_kv_heads, head_dim, dev)
+    if positions.shape[1] != N:
+        raise ValueError(f"positions: expected [axes, {N}]")
+    at = _dense_ptr(positions, I32, "positions")
+    _same_device(dev, positions=positions)
+    if N:
+        _lib.call("fl_attn_prep_axes", *ptrs, *pg, sp, pp, at, positions.shape[0], _lib.int_array(of), B, N,
+                  n_q_heads, n_kv_heads, head_dim, rope_dim, theta, eps, _stream())
+    return qg if q_out is None else q_out
+
+
+def _layer_pools(kpools, vpools, page_size, n_kv_heads, head_dim, dev):
+    """(k pointers, v pointers, layers, q8, n_pages, page_size) of several layers' pools, alike."""
+    ks, vs = ([p] if isinstance(p, torch.Tensor) else list(p) for p in (kpools, vpools))
+    if len(ks) != len(vs) or not 1 <= len(ks) <= POOL_MAX:
+        raise ValueError(f"kpools, vpools: one of each a layer, 1 to {POOL_MAX} layers")
+    for l, (kp, vp) in enumerate(zip(ks, vs)):
+        for name, c in ((f"kpools[{l}]", kp), (f"vpools[{l}]", vp)):
+            if not isinstance(c, torch.Tensor):
+                raise TypeError(f"{name}: expected a torch.Tensor, got {type(c).__name__}")
+            if c.dtype != ks[0].dtype or c.dtype not in (F16, I8):
+                raise TypeError(f"{name}: dtype {c.dtype}, the pools are all fp16 or all int8")
+            if c.shape != ks[0].shape:
+                raise ValueError(f"{name}: shape {tuple(c.shape)}, kpools[0] has {tuple(ks[0].shape)}")
+            _contig(c, name)
+            _same_device(dev, **{name: c})
+    if page_size < 1 or n_kv_heads < 1 or head_dim != HEAD_DIM:
+        raise ValueError("page_size and n_kv_heads must be positive, head_dim 256")
+    q8, shape = ks[0].dtype == I8, tuple(ks[0].shape)
+    if q8:
+        n_pages, rest = divmod(ks[0].numel(), page_size * n_kv_heads * KV8_ROW)
+        if rest:
+            raise ValueError("kpools: not a whole number of pages")
+    else:
+        if len(shape) != 4 or shape[1:] != (page_size, n_kv_heads, head_dim):
+            raise ValueError(f"kpools: shape {shape}, expected [n_pages, {page_size}, {n_kv_heads}, {head_dim}]")
+        n_pages = shape[0]
+    ptrs = [(ctypes.c_void_p * len(t))(*(p.data_ptr() for p in t)) for t in (ks, vs)]
+    return ptrs[0], ptrs[1], len(ks), int(q8), n_pages, page_size
+
+
+def paged_kv_copy(kpools, vpools, src, dst, *, page_size: int, n_kv_heads: int = N_KV,
+                  head_dim: int = HEAD_DIM):
+    """Whole pages src[i] -> dst[i] (int32 ids on the GPU) in the pools of all layers at
+    once (lists of pools, or one K and one V pool): the private copy of the page that a
+    forked sequence goes on in (its table's row is the parent's, but for that page), pages
+    moved together. A pair with an id outside the pool is left out. No page may be written
+    twice, or written and read. (A page is freed by its table entry: -1.)"""
+    dev = _here()
+    if dev >= 0 and _lib.lane is not None:
+        r = _lib.lane.kv_copy(dev, _stream(), kpools, vpools, src, dst, page_size, n_kv_heads, head_dim)
+        if r is not None:
+            return _made("fl_paged_kv_copy", r, None)
+    if not isinstance(src, torch.Tensor) or not isinstance(dst, torch.Tensor):
+        raise TypeError("src, dst: expected torch tensors")
+    if src.dim() != 1 or src.shape != dst.shape:
+        raise ValueError("src, dst: one-dimensional, one entry a page")
+    pools = _layer_pools(kpools, vpools, page_size, n_kv_heads, head_dim, dev)
+    sp, dp = _dense_ptr(src, I32, "src"), _dense_ptr(dst, I32, "dst")
+    _same_device(dev, src=src, dst=dst)
+    if src.numel():
+        _lib.call("fl_paged_kv_copy", *pools, sp, dp, src.numel(), n_kv_heads, head_dim, _stream())
+
+
+def paged_kv_keep(kpools, vpools, pages, pos0, path, *, page_size: int, n_kv_heads: int = N_KV,
+                  head_dim: int = HEAD_DIM):
+    """The rows of accepted paths moved up behind their contexts in the pools of all
+    layers at once (lists of pools, or one K and one V pool): row pos0[b] + path[b, d] to
+    row pos0[b] + d. pos0 [B], path [B, D] int32 on the GPU; a path ends at its first
+    entry that is not larger than the one before it (-1: ends there). Rows from or to
+    absent pages, and sequences at a negative pos0, stay as they are."""
+    dev = _here()
+    if dev >= 0 and _lib.lane is not None:
+        r = _lib.lane.kv_keep(dev, _stream(), kpools, vpools, pages, pos0, path, page_size, n_kv_heads,
+                              head_dim)
+        if r is not None:
+            return _made("fl_paged_kv_keep", r, None)
+    if not isinstance(pos0, torch.Tensor) or not isinstance(path, torch.Tensor):
+        raise TypeError("pos0, path: expected torch tensors")
+    B = pos0.numel()
+    if pos0.dim() != 1 or path.dim() != 2 or path.shape[0] != B:
+        raise ValueError("pos0 [B], path [B, D]")
+    pools = _layer_pools(kpools, vpools, page_size, n_kv_heads, head_dim, dev)
+    if not isinstance(pages, torch.Tensor) or pages.dtype != I32:
+        raise TypeError(f"pages: expected a tensor of {I32}")
+    if pages.dim() != 2 or pages.shape[0] != B or (pages.stride(1) != 1 and pages.shape[1] > 1):
+        raise ValueError(f"pages: expected rows of page ids for {B} sequences")
+    pp, at = _dense_ptr(pos0, I32, "pos0"), _dense_ptr(path, I32, "path")
+    _same_device(dev, pages=pages, pos0=pos0, path=path)
+    if path.shape[1]:
+        _lib.call("fl_paged_kv_keep", *pools, pages.data_ptr(), pages.shape[1],
+                  pages.stride(0) if B > 1 else pages.shape[1], pp, at, B, path.shape[1], n_kv_heads,
+                  head_dim, _stream())
 
 
 # ---------------------------------------------------------------------------

@@ -36,6 +36,8 @@ typedef struct ihipStream_t* fl_stream_t; /* hipStream_t; NULL = default stream 
 #define FL_MAX_SEQS 16 /* sequences one batched decode call carries */
 #define FL_PAGED_MAX_SEQS 1024       /* ... one call over a paged cache */
 #define FL_PAGED_MAX_SEQS_PREFILL 64 /* ... of chunks (fl_attention_prefill_paged) */
+#define FL_TREE_MAX 64 /* drafted tokens of a sequence */
+#define FL_POOL_MAX 64 /* layers whose pools one call takes */
 
 int fl_abi_version(void);
 /* Of the fl355.h that the library was built with: the first 16 hex digits of its SHA-256
@@ -443,6 +445,48 @@ int fl_attn_decode_paged(const void* qg, int q_pitch, const void* kpool, const v
                          long long pages_stride, const int* pos0, int B, int T, int n_q_heads,
                          int n_kv_heads, int head_dim, float scale, int window, int sinks, int gated,
                          void* z, int z_pitch, void* work, size_t work_bytes, fl_stream_t stream);
+
+/* ---- trees of drafted tokens ------------------------------------------------
+ * No counterpart in the reference, whose verify rounds carry a chain of 2 or 3. A
+ * drafter proposes several continuations of a sequence as a tree of T <=
+ * FL_TREE_MAX tokens: token i has the parent parents[b][i] < i, -1 for a child of
+ * the context. Any other entry is a place that holds no token (a padded batch), and
+ * so is one whose parent holds none. Token i's cache row is pos0[b] + i, behind the
+ * context's rows [0, pos0[b]); its position is p = pos0[b] + its depth (0 for a
+ * child of the context). An accepted path is a list of tokens, path[b][0 .. D - 1],
+ * that ends at its first entry which is not larger than the one before it (-1: ends
+ * there, nothing at path[b][0] < 0) or is T or more. All of these are device arrays. */
+
+/* fl_attn_prep_paged with the rotation's positions given, on one or more axes (time,
+ * height and width of images and video; a tree's depths): pair j of token i rotates by
+ * positions[pair_axis[j]][i] * theta^(-2j / rope_dim), positions [n_axes][N] int32,
+ * pair_axis a host array of rope_dim / 2 entries in [0, n_axes). The cache rows stay
+ * pos0[b] + i - starts[b]. Where every axis holds those positions the values are
+ * fl_attn_prep_paged's bit for bit. */
+int fl_attn_prep_axes(void* qg, int q_pitch, const void* k, const void* v, const float* wq,
+                      const float* wk, void* q_out, int qo_pitch, void* kpool, void* vpool, int q8,
+                      int n_pages, int page_size, const int* pages, int max_pages,
+                      long long pages_stride, const int* starts, const int* pos0,
+                      const int* positions, int n_axes, const int* pair_axis, int B, int N,
+                      int n_q_heads, int n_kv_heads, int head_dim, int rope_dim, float theta,
+                      float eps, fl_stream_t stream);
+
+/* Whole pages src[i] -> dst[i] (device arrays of n page ids) in the K and V pools of
+ * n_layers layers (host arrays of device pointers; up to FL_POOL_MAX layers): the private
+ * copy of a forked sequence's last page, pages moved together. A pair with an entry outside
+ * [0, n_pages) is left out. No page may be written twice, or written and read: what such
+ * pages hold afterwards is undefined. */
+int fl_paged_kv_copy(void* const* kpools, void* const* vpools, int n_layers, int q8, int n_pages,
+                     int page_size, const int* src, const int* dst, int n, int n_kv_heads,
+                     int head_dim, fl_stream_t stream);
+
+/* The rows of accepted paths to behind their contexts, in the pools of n_layers layers: row
+ * pos0[b] + path[b][d] -> row pos0[b] + d. A row from or to an absent page stays as it is, and so
+ * do the sequences at a negative pos0. path [B][D] (its entries have no upper limit here). */
+int fl_paged_kv_keep(void* const* kpools, void* const* vpools, int n_layers, int q8, int n_pages,
+                     int page_size, const int* pages, int max_pages, long long pages_stride,
+                     const int* pos0, const int* path, int B, int D, int n_kv_heads, int head_dim,
+                     fl_stream_t stream);
 
 /* ---- causal conv ----------------------------------------------------------
  * conv1d_causal over `dim` channels of rows x [T][row_stride] f16: E =
