@@ -92,6 +92,10 @@ SIGNATURES = {
                                _P, _P, _I, _IP, _I, _I, _I, _I, _I, _I, _F, _F, _P]),
     "fl_paged_kv_copy": (_I, [_PP, _PP, _I, _I, _I, _I, _P, _P, _I, _I, _I, _P]),
     "fl_paged_kv_keep": (_I, [_PP, _PP, _I, _I, _I, _I, _P, _I, _LL, _P, _P, _I, _I, _I, _I, _P]),
+    "fl_gdn_tree_normed": (_I, [_P, _I, _P, _PP, _IP, _P, _P, _P, _I, _P, _P, _PP, _P, _I, _P, _P,
+                                _I, _I, _I, _I, _I, _I, _I, _F, _F, _F, _P]),
+    "fl_gdn_tree_commit": (_I, [_P, _I, _P, _PP, _PP, _IP, _P, _P, _P, _I, _P, _P, _PP, _PP, _I, _I,
+                                _I, _I, _I, _I, _I, _F, _P]),
     "fl_conv1d_causal": (_I, [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
     "fl_conv1d_causal_rows": (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _P]),
     "fl_l2norm_scaled": (_I, [_P, _P, _I, _I, _I, _F, _F, _I, _P]),
@@ -135,7 +139,7 @@ BINDING_PATH = LIB_PATH.with_name("fl355_paged.so")
 BOUND = ("fl_paged_kv_store", "fl_paged_kv_load", "fl_attn_prep_paged",
          "fl_attention_prefill_paged_work_bytes", "fl_attention_prefill_paged",
          "fl_attn_decode_paged_work_bytes", "fl_attn_decode_paged", "fl_attn_prep_axes",
-         "fl_paged_kv_copy", "fl_paged_kv_keep")
+         "fl_paged_kv_copy", "fl_paged_kv_keep", "fl_gdn_tree_normed", "fl_gdn_tree_commit")
 
 
 def _load_binding(L: ctypes.CDLL, path: Path | None = None):

@@ -13,6 +13,8 @@
 
 #include <ATen/ops/empty.h>
 
+#include <algorithm>
+
 #include <limits.h>
 
 #include "fl355.h"
@@ -29,6 +31,8 @@ decltype(&fl_attn_decode_paged) p_decode;
 decltype(&fl_attn_prep_axes) p_prep_axes;
 decltype(&fl_paged_kv_copy) p_copy;
 decltype(&fl_paged_kv_keep) p_keep;
+decltype(&fl_gdn_tree_normed) p_gdn_tree;
+decltype(&fl_gdn_tree_commit) p_gdn_commit;
 
 constexpr int64_t HEAD_DIM = 256, KV8_ROW = HEAD_DIM + HEAD_DIM / 32 * 2;   // bytes of an int8 head row
 
@@ -471,11 +475,148 @@ PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// A list or tuple of dense tensors, one a sequence: their pointers, and the fewest elements of one.
+struct Buffers {
+    void* p[FL_MAX_SEQS];
+    int n = 0;
+    int64_t least = INT64_MAX;
+
+    Buffers(Args& a, at::ScalarType type) {
+        PyObject* o = a.next();
+        const bool list = PyList_CheckExact(o);
+        const Py_ssize_t size = list ? PyList_GET_SIZE(o) : PyTuple_CheckExact(o) ? PyTuple_GET_SIZE(o) : 0;
+        if (size < 1 || size > FL_MAX_SEQS) {
+            a.ok = false;
+            return;
+        }
+        for (Py_ssize_t i = 0; i < size; ++i) {
+            PyObject* x = list ? PyList_GET_ITEM(o, i) : PyTuple_GET_ITEM(o, i);
+            const at::Tensor* t = THPVariable_CheckExact(x) ? &THPVariable_Unpack(x) : nullptr;
+            if (!t || !a.dense(x, type, t->dim())) {
+                a.ok = false;
+                return;
+            }
+            p[i] = t->data_ptr();
+            least = std::min(least, t->numel());
+        }
+        n = (int)size;
+    }
+};
+
+// What the two GDN calls of a tree round share: x, S, a, b, A_log, dt_bias
+struct GdnTree {
+    const at::Tensor* x;
+    Buffers S;
+    const at::Tensor *a, *b, *A, *dt;
+    int pos0[FL_MAX_SEQS];
+    const at::Tensor* conv_w = nullptr;
+    int64_t n_k = 0, n_v = 0, K = 0, V = 0, B = 0, T = 0;
+
+    GdnTree(Args& g)
+        : x(g.dense(at::kHalf, 3)), S(g, at::kFloat), a(g.dense(at::kFloat, 3)), b(g.dense(at::kFloat, 3)),
+          A(g.dense(at::kFloat, 1)), dt(g.dense(at::kFloat, 1)) {}
+    // pos0s, conv_w
+    void more(Args& g) {
+        Py_ssize_t n = 0;
+        g.ok = ints(g.next(), pos0, FL_MAX_SEQS, n) && g.ok && n == S.n;
+        conv_w = g.dense(at::kHalf, 2);
+    }
+    void sizes(Args& g) { n_k = g.integer(), n_v = g.integer(), K = g.integer(), V = g.integer(); }
+    bool fit(const Buffers& frames) {
+        for (int64_t d : {n_k, n_v, K, V})
+            if (d < 1 || d > 4096) return false;
+        const int64_t dim = 2 * n_k * K + n_v * V;
+        B = S.n, T = x->size(1);
+        return x->size(0) == B && T >= 1 && T <= INT_MAX && x->size(2) >= dim && x->size(2) <= INT_MAX &&
+               S.least >= n_v * V * K && a->sizes() == b->sizes() && a->size(0) == B && a->size(1) == T &&
+               a->size(2) >= n_v && a->size(2) <= INT_MAX && A->numel() >= n_v && dt->numel() >= n_v &&
+               conv_w->numel() >= 4 * dim && frames.n == S.n && frames.least >= 3 * dim;
+    }
+};
+
+// (dev, stream, x, S, a, b, A_log, dt_bias, z, norm_w, parents, y or None, pos0s, conv_w, cst_in, n_k, n_v,
+//  K, V, out_scale, l2eps, norm_eps): y
+PyObject* gdn_tree(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Args g{args};
+    PLAIN(n == 22);
+    g.dev = g.integer32();
+    const auto stream = (fl_stream_t)g.integer();
+    GdnTree c(g);
+    PyObject* zo = g.next();
+    const at::Tensor* z = THPVariable_CheckExact(zo) ? &THPVariable_Unpack(zo) : nullptr;
+    PLAIN(z && (z->dim() == 3 || z->dim() == 4));
+    z = g.dense(zo, at::kHalf, z->dim());
+    const at::Tensor *norm_w = g.dense(at::kFloat, 1), *parents = g.dense(at::kInt, 2);
+    PyObject* yo = g.next();
+    c.more(g);
+    const Buffers frames(g, at::kHalf);
+    c.sizes(g);
+    const float out_scale = g.real(), l2eps = g.real(), norm_eps = g.real();
+    PLAIN(g.ok && c.fit(frames));
+    const int64_t width = c.n_v * c.V;
+    PLAIN(z->size(0) == c.B && z->size(1) == c.T && z->numel() == c.B * c.T * width &&
+          norm_w->numel() >= c.V && parents->size(0) == c.B && parents->size(1) == c.T);
+    at::Tensor y;
+    if (yo != Py_None) {
+        const at::Tensor* t = g.dense(yo, at::kHalf, 3);
+        PLAIN(t && t->size(0) == c.B && t->size(1) == c.T && t->size(2) == width);
+        y = *t;
+    } else {
+        y = half_rows({c.B, c.T, width}, g.dev);
+    }
+    const int rc = released([&] {
+        return p_gdn_tree(c.x->data_ptr(), (int)c.x->size(2), c.conv_w->data_ptr(), frames.p, c.pos0,
+                          (const int*)parents->data_ptr(), (const float*)c.a->data_ptr(),
+                          (const float*)c.b->data_ptr(), (int)c.a->size(2), (const float*)c.A->data_ptr(),
+                          (const float*)c.dt->data_ptr(), (const float* const*)c.S.p, z->data_ptr(), (int)width,
+                          (const float*)norm_w->data_ptr(), y.data_ptr(), (int)width, (int)c.B, (int)c.T,
+                          (int)c.n_k, (int)c.n_v, (int)c.K, (int)c.V, out_scale, l2eps, norm_eps, stream);
+    });
+    MADE(rc);
+    if (yo == Py_None) return THPVariable_Wrap(std::move(y));
+    Py_INCREF(yo);
+    return yo;
+    END_HANDLE_TH_ERRORS
+}
+
+// (dev, stream, x, S, a, b, A_log, dt_bias, path, S_out, pos0s, conv_w, cst_in, cst_out, n_k, n_v, K, V, l2eps)
+PyObject* gdn_commit(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Args g{args};
+    PLAIN(n == 19);
+    g.dev = g.integer32();
+    const auto stream = (fl_stream_t)g.integer();
+    GdnTree c(g);
+    const at::Tensor* path = g.dense(at::kInt, 2);
+    const Buffers S_out(g, at::kFloat);
+    c.more(g);
+    const Buffers frames(g, at::kHalf), frames_out(g, at::kHalf);
+    c.sizes(g);
+    const float l2eps = g.real();
+    PLAIN(g.ok && c.fit(frames));
+    PLAIN(path->size(0) == c.B && path->size(1) <= INT_MAX && S_out.n == c.S.n &&
+          S_out.least >= c.n_v * c.V * c.K && frames_out.n == c.S.n &&
+          frames_out.least >= 3 * (2 * c.n_k * c.K + c.n_v * c.V));
+    const int rc = released([&] {
+        return p_gdn_commit(c.x->data_ptr(), (int)c.x->size(2), c.conv_w->data_ptr(), frames.p, frames_out.p,
+                            c.pos0, (const int*)path->data_ptr(), (const float*)c.a->data_ptr(),
+                            (const float*)c.b->data_ptr(), (int)c.a->size(2), (const float*)c.A->data_ptr(),
+                            (const float*)c.dt->data_ptr(), (const float* const*)c.S.p, (float* const*)S_out.p,
+                            (int)c.B, (int)c.T, (int)path->size(1), (int)c.n_k, (int)c.n_v, (int)c.K, (int)c.V,
+                            l2eps, stream);
+    });
+    MADE(rc);
+    Py_RETURN_TRUE;
+    END_HANDLE_TH_ERRORS
+}
+
 // the entry points' addresses, in the order of the declarations above
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
     void** const to[] = {(void**)&p_store, (void**)&p_load, (void**)&p_prep, (void**)&p_prefill_bytes,
                          (void**)&p_prefill, (void**)&p_decode_bytes, (void**)&p_decode,
-                         (void**)&p_prep_axes, (void**)&p_copy, (void**)&p_keep};
+                         (void**)&p_prep_axes, (void**)&p_copy, (void**)&p_keep, (void**)&p_gdn_tree,
+                         (void**)&p_gdn_commit};
     if (n != (Py_ssize_t)(sizeof(to) / sizeof(to[0]))) {
         PyErr_SetString(PyExc_TypeError, "bind: one address an entry point");
         return nullptr;
@@ -497,6 +638,8 @@ PyMethodDef methods[] = {
     {"prep_axes", (PyCFunction)(void (*)())prep_axes, METH_FASTCALL, nullptr},
     {"kv_copy", (PyCFunction)(void (*)())kv_copy, METH_FASTCALL, nullptr},
     {"kv_keep", (PyCFunction)(void (*)())kv_keep, METH_FASTCALL, nullptr},
+    {"gdn_tree", (PyCFunction)(void (*)())gdn_tree, METH_FASTCALL, nullptr},
+    {"gdn_commit", (PyCFunction)(void (*)())gdn_commit, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "fl355_paged", nullptr, -1, methods};

@@ -1330,6 +1330,98 @@ def gdn_prefill_layer(x, conv_w, st_in, st_out, a, b, A_log, dt_bias, S, z, norm
     return y
 
 
+# The GDN layer's part of a tree round (parents, path: "Trees of drafted tokens" above).
+
+def _tree_layer(x, S, a, b, A_log, dt_bias, conv_w, cst_in, pos0s, nodes, name, n_kheads, n_vheads, K, V, dev):
+    """(B, T, the arguments that gdn_tree_normed and gdn_tree_commit share) after their checks."""
+    for what, t in (("x", x), ("a", a), ("b", b), (name, nodes)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{what}: expected a torch.Tensor, got {type(t).__name__}")
+    B, dim = len(S), 2 * n_kheads * K + n_vheads * V
+    if x.dim() != 3 or x.shape[0] != B or x.shape[2] < dim:
+        raise ValueError(f"x: shape {tuple(x.shape)}, expected [{B}, T, {dim} or more]")
+    T = x.shape[1]
+    if a.shape != b.shape or a.dim() != 3 or tuple(a.shape[:2]) != (B, T) or a.shape[2] < n_vheads:
+        raise ValueError(f"a, b: expected [{B}, {T}, {n_vheads} or more], alike")
+    if nodes.dim() != 2 or nodes.shape[0] != B or (name == "parents" and nodes.shape[1] != T):
+        raise ValueError(f"{name}: shape {tuple(nodes.shape)}, expected {B} rows"
+                         + (f" of {T}" if name == "parents" else ""))
+    if len(cst_in) != B or len(pos0s) != B:
+        raise ValueError("cst_in, pos0s: one a sequence")
+    _same_device(dev, x=x, a=a, b=b, A_log=A_log, dt_bias=dt_bias, conv_w=conv_w, **{name: nodes})
+    for i in range(B):
+        _same_device(dev, **{f"S[{i}]": S[i], f"cst_in[{i}]": cst_in[i]})
+    state = n_vheads * V * K
+    return B, T, dict(
+        x=_dense_ptr(x, F16, "x"), x_stride=x.shape[2], conv_w=_dense_ptr(conv_w, F16, "conv_w", dim * 4),
+        cst=_lib.ptr_array([_dense_ptr(c, F16, f"cst_in[{i}]", dim * 3) for i, c in enumerate(cst_in)]),
+        pos0=_lib.int_array(pos0s), nodes=_dense_ptr(nodes, I32, name),
+        a=_dense_ptr(a, F32, "a"), b=_dense_ptr(b, F32, "b"), ab_stride=a.shape[2],
+        A=_dense_ptr(A_log, F32, "A_log", n_vheads), dt=_dense_ptr(dt_bias, F32, "dt_bias", n_vheads),
+        S=_lib.ptr_array([_dense_ptr(s, F32, f"S[{i}]", state) for i, s in enumerate(S)]))
+
+
+def gdn_tree_normed(x, S, a, b, A_log, dt_bias, z, norm_w, parents, y=None, *, pos0s, conv_w, cst_in,
+                    n_kheads: int = GDN_K_HEADS, n_vheads: int = GDN_V_HEADS, K: int = GDN_K, V: int = GDN_V,
+                    out_scale: float = Q_SCALE, l2eps: float = L2_EPS, norm_eps: float = GDN_NORM_EPS):
+    """gdn_decode_normed over trees of drafted tokens: every token's conv window, decay and
+    state follow its path from the sequence's state S[b] and frames cst_in[b] (lists of up
+    to 16, only read). x [B, T, x_stride] fp16 the raw q|k|v rows, T up to 64; a, b [B, T,
+    ab_stride] fp32; z [B, T, n_vheads * V] fp16; parents [B, T] int32 on the GPU; pos0s the
+    contexts' lengths (at 0 the frames count as zero). All in 32 bits, y rounded once: a
+    chain's values are gdn_decode_normed's but for that call's fp16 roundings between its
+    steps. Places without a token give 0. Returns y [B, T, n_vheads * V] fp16 (new unless
+    given)."""
+    dev, width = _here(), n_vheads * V
+    if dev >= 0 and _lib.lane is not None:
+        r = _lib.lane.gdn_tree(dev, _stream(), x, S, a, b, A_log, dt_bias, z, norm_w, parents, y, pos0s, conv_w,
+                               cst_in, n_kheads, n_vheads, K, V, out_scale, l2eps, norm_eps)
+        if r is not None:
+            return _made("fl_gdn_tree_normed", r, r)
+    B, T, c = _tree_layer(x, S, a, b, A_log, dt_bias, conv_w, cst_in, pos0s, parents, "parents", n_kheads,
+                          n_vheads, K, V, dev)
+    if y is None:
+        y = torch.empty((B, T, width), dtype=F16, device=x.device)
+    for name, t in (("z", z), ("y", y)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
+        if t.dim() < 3 or tuple(t.shape[:2]) != (B, T) or t.numel() != B * T * width:
+            raise ValueError(f"{name}: shape {tuple(t.shape)}, expected [{B}, {T}, {width}]")
+    _same_device(dev, z=z, y=y, norm_w=norm_w)
+    _lib.call("fl_gdn_tree_normed", *c.values(), _dense_ptr(z, F16, "z"), width,
+              _dense_ptr(norm_w, F32, "norm_w", V), _dense_ptr(y, F16, "y"), width, B, T, n_kheads, n_vheads, K,
+              V, float(out_scale), float(l2eps), float(norm_eps), _stream())
+    return y
+
+
+def gdn_tree_commit(x, S, a, b, A_log, dt_bias, path, S_out=None, *, pos0s, conv_w, cst_in, cst_out,
+                    n_kheads: int = GDN_K_HEADS, n_vheads: int = GDN_V_HEADS, K: int = GDN_K, V: int = GDN_V,
+                    l2eps: float = L2_EPS):
+    """The recurrent states and conv frames behind accepted paths, from what gdn_tree_normed
+    took: path [B, D] int32 on the GPU (it ends at its first entry that is not larger than
+    the one before it, or that is T or more; D up to 64), S_out and cst_out lists of B
+    buffers. S_out: None for S in place; no other buffers of a call may overlap. An empty
+    path leaves what was ahead of it."""
+    dev, outs = _here(), S if S_out is None else S_out
+    if dev >= 0 and _lib.lane is not None:
+        r = _lib.lane.gdn_commit(dev, _stream(), x, S, a, b, A_log, dt_bias, path, outs, pos0s, conv_w, cst_in,
+                                 cst_out, n_kheads, n_vheads, K, V, l2eps)
+        if r is not None:
+            return _made("fl_gdn_tree_commit", r, None)
+    B, T, c = _tree_layer(x, S, a, b, A_log, dt_bias, conv_w, cst_in, pos0s, path, "path", n_kheads, n_vheads, K,
+                          V, dev)
+    if len(outs) != B or len(cst_out) != B:
+        raise ValueError("S_out, cst_out: one a sequence")
+    for i in range(B):
+        _same_device(dev, **{f"S_out[{i}]": outs[i], f"cst_out[{i}]": cst_out[i]})
+    dim, state = 2 * n_kheads * K + n_vheads * V, n_vheads * V * K
+    frames = _lib.ptr_array([_dense_ptr(t, F16, f"cst_out[{i}]", dim * 3) for i, t in enumerate(cst_out)])
+    states = _lib.ptr_array([_dense_ptr(t, F32, f"S_out[{i}]", state) for i, t in enumerate(outs)])
+    _lib.call("fl_gdn_tree_commit", c["x"], c["x_stride"], c["conv_w"], c["cst"], frames, c["pos0"], c["nodes"],
+              c["a"], c["b"], c["ab_stride"], c["A"], c["dt"], c["S"], states, B, T, path.shape[1], n_kheads,
+              n_vheads, K, V, float(l2eps), _stream())
+
+
 # ---------------------------------------------------------------------------
 # A decode step's layers as the runtime calls them, one row a sequence: the
 # checks and values of attn_prep_rows + attn_decode(_q8) and of

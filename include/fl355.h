@@ -488,6 +488,31 @@ int fl_paged_kv_keep(void* const* kpools, void* const* vpools, int n_layers, int
                      const int* pos0, const int* path, int B, int D, int n_kv_heads, int head_dim,
                      fl_stream_t stream);
 
+/* A GDN layer over trees: every token's conv window, decay and state follow its path from the
+ * sequence's state S[b] and frames cst_in[b], which are only read; y[b][i] = rmsnorm_gated(o_i,
+ * z[b][i], norm_w) of the token's output o_i (fl_gdn_decode_normed's formulas; here all of it in
+ * 32 bits and y rounded once, so a chain's values are that call's but for its roundings). Places
+ * without a token give 0. An infinity or NaN of one token may reach the others of its sequence.
+ * x [B][T][x_stride] f16 the raw q|k|v rows, a, b [B][T][ab_stride] f32, z [B][T][z_pitch], y
+ * [B][T][y_pitch] f16, pos0 a host array (0: the frames are taken as zero); conv_w, S, cst_in,
+ * A_log, dt_bias, norm_w as fl_gdn_decode_normed's. K == V == 128, B <= FL_MAX_SEQS, strides and
+ * pitches of f16 rows multiples of 8, everything but a and b 16-byte aligned. */
+int fl_gdn_tree_normed(const void* x, int x_stride, const void* conv_w, const void* const* cst_in,
+                       const int* pos0, const int* parents, const float* a, const float* b, int ab_stride,
+                       const float* A_log, const float* dt_bias, const float* const* S, const void* z,
+                       int z_pitch, const float* norm_w, void* y, int y_pitch, int B, int T, int n_kheads,
+                       int n_vheads, int K, int V, float out_scale, float l2eps, float norm_eps,
+                       fl_stream_t stream);
+
+/* The state S_out[b] and the frames cst_out[b] behind the accepted path path[b][0 .. D - 1], from
+ * the tree's x, a, b and the state and frames ahead of it (an empty path: those). S_out[b] may be
+ * S[b]; apart from that no output may overlap another buffer of the call. D <= FL_TREE_MAX. */
+int fl_gdn_tree_commit(const void* x, int x_stride, const void* conv_w, const void* const* cst_in,
+                       void* const* cst_out, const int* pos0, const int* path, const float* a, const float* b,
+                       int ab_stride, const float* A_log, const float* dt_bias, const float* const* S,
+                       float* const* S_out, int B, int T, int D, int n_kheads, int n_vheads, int K, int V,
+                       float l2eps, fl_stream_t stream);
+
 /* ---- causal conv ----------------------------------------------------------
  * conv1d_causal over `dim` channels of rows x [T][row_stride] f16: E =
  * [st_in (width-1 frames, ZERO if pos0 == 0) | x], y[t][d] =

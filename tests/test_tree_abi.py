@@ -42,6 +42,35 @@ def keep(fl, **over):
     return fl._lib.lib().fl_paged_kv_keep(*a.values(), None)
 
 
+def layer(**over):
+    a = dict(x=FAKE, xs=10240, w=FAKE, cin=ptrs(FAKE, FAKE), pos0=ints(5, 5), nodes=FAKE, a=FAKE, b=FAKE, abs=48,
+             A=FAKE, dt=FAKE, S=ptrs(FAKE, FAKE))
+    return {**a, **{k: v for k, v in over.items() if k in a}}
+
+
+def gdn_tree(fl, **over):
+    a = dict(z=FAKE, zp=6144, nw=FAKE, y=FAKE, yp=6144, B=2, T=8, nk=16, nv=48, K=128, V=128, s=0.1, l2=1e-6, eps=1e-6)
+    a.update({k: v for k, v in over.items() if k in a})
+    return fl._lib.lib().fl_gdn_tree_normed(*layer(**over).values(), *a.values(), None)
+
+
+BIG = 1 << 28
+
+
+def gdn_commit(fl, **over):
+    c = layer(**{"S": ptrs(BIG, 2 * BIG), **over})
+    a = dict(cout=ptrs(3 * BIG, 4 * BIG), So=ptrs(BIG, 2 * BIG), B=2, T=8, D=4, nk=16, nv=48, K=128, V=128, l2=1e-6)
+    a.update({k: v for k, v in over.items() if k in a})
+    return fl._lib.lib().fl_gdn_tree_commit(c["x"], c["xs"], c["w"], c["cin"], a["cout"], c["pos0"], c["nodes"], c["a"],
+                                            c["b"], c["abs"], c["A"], c["dt"], c["S"], a["So"], a["B"], a["T"], a["D"],
+                                            a["nk"], a["nv"], a["K"], a["V"], a["l2"], None)
+
+
+GDN = [dict(x=None), dict(w=None), dict(cin=None), dict(pos0=None), dict(nodes=None), dict(a=None), dict(b=None),
+       dict(A=None), dict(dt=None), dict(S=None), dict(S=ptrs(FAKE, None)), dict(S=ptrs(FAKE, FAKE + 4)),
+       dict(cin=ptrs(FAKE, FAKE + 8)), dict(pos0=ints(5, -1)), dict(B=0), dict(B=17), dict(T=0), dict(T=65), dict(K=64),
+       dict(V=64), dict(nk=0), dict(nk=5), dict(nv=0), dict(xs=10232), dict(xs=10244), dict(x=FAKE + 8), dict(w=FAKE + 2),
+       dict(abs=47)]
 SIZES = [dict(q8=2), dict(hd=128), dict(kv=0), dict(page_size=8), dict(page_size=48), dict(n_pages=0),
          dict(n_pages=1 << 30)]
 TABLES = [dict(pages=None), dict(max_pages=0), dict(stride=3), dict(B=0), dict(B=1025),
@@ -57,6 +86,13 @@ LAYERS = [dict(ks=None), dict(vs=None), dict(layers=0), dict(layers=65, ks=ptrs(
         dict(qp=255), dict(nq=23), dict(q_out=FAKE, qop=128)]],
     *[(copy, o) for o in SIZES + LAYERS + [dict(n=-1), dict(n=1, src=None), dict(n=1, dst=None),
                                            dict(n=1 << 30, page_size=1 << 15)]],
+    *[(f, o) for f in (gdn_tree, gdn_commit) for o in GDN],
+    *[(gdn_tree, o) for o in (dict(z=None), dict(nw=None), dict(y=None), dict(zp=6136), dict(yp=6140), dict(y=FAKE + 8),
+                              dict(nw=FAKE + 4))],
+    *[(gdn_commit, o) for o in (
+        dict(cout=None), dict(So=None), dict(D=0), dict(D=65), dict(cout=ptrs(3 * BIG, None)), dict(So=ptrs(BIG, None)),
+        dict(cout=ptrs(FAKE, 4 * BIG)), dict(cout=ptrs(3 * BIG, FAKE + 61424)), dict(cout=ptrs(3 * BIG, 3 * BIG + 32)),
+        dict(So=ptrs(3 * BIG, 3 * BIG)), dict(So=ptrs(2 * BIG, BIG)), dict(So=ptrs(BIG + 64, 2 * BIG)))],
     *[(keep, o) for o in SIZES + TABLES + LAYERS + [dict(D=-1), dict(pos0=None), dict(D=1, path=None)]],
 ], ids=lambda x: getattr(x, "__name__", None) or str({k: v for k, v in x.items() if not isinstance(v, ctypes.Array)}))
 def test_refusals(fl, f, over):
@@ -107,6 +143,28 @@ def test_op_layer_refuses(fl):
         ops.attn_prep_axes(*x, at, page_size=16, sections=(16, 8, 8))
 
 
+def test_op_layer_refuses_gdn_trees(fl):
+    ops = fl.ops
+    x, a, A = torch.zeros((1, 3, 10240), dtype=F16), torch.zeros((1, 3, 48)), torch.zeros(48)
+    S, z, w = [torch.zeros(48, 128, 128)], torch.zeros((1, 3, 6144), dtype=F16), torch.zeros(128)
+    nodes, cw, cst = torch.zeros((1, 3), dtype=I32), torch.zeros((10240, 4), dtype=F16), [torch.zeros((10240, 3), dtype=F16)]
+    kw = dict(pos0s=[1], conv_w=cw, cst_in=cst)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.gdn_tree_normed(x, S, a, a, A, A, z, w, nodes, **kw)
+    with pytest.raises(ValueError, match="parents"):
+        ops.gdn_tree_normed(x, S, a, a, A, A, z, w, nodes[:, :2], **kw)
+    with pytest.raises(ValueError, match="x: shape"):
+        ops.gdn_tree_normed(x[..., :8192], S, a, a, A, A, z, w, nodes, **kw)
+    with pytest.raises(ValueError, match="a, b"):
+        ops.gdn_tree_normed(x, S, a, a[:, :2], A, A, z, w, nodes, **kw)
+    with pytest.raises(ValueError, match="one a sequence"):
+        ops.gdn_tree_normed(x, S, a, a, A, A, z, w, nodes, pos0s=[1, 2], conv_w=cw, cst_in=cst)
+    with pytest.raises(TypeError):
+        ops.gdn_tree_commit(x, S, a, a, A, A, [[0, 1]], cst_out=cst, **kw)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.gdn_tree_commit(x, S, a, a, A, A, nodes, cst_out=cst, **kw)
+
+
 def test_the_pairs_of_every_axis(fl):
     of = fl.ops._pair_axes
     assert of(3, (2, 1, 1), False, 8) == (0, 0, 1, 2)
@@ -131,6 +189,12 @@ def test_binding_declines_what_is_not_plain(fl):
         "kv_copy": (0, 0, [pool], [pool], ids, ids, 16, 4, 256),
         "kv_keep": (0, 0, [pool], (pool,), pages, pos0, path, 16, 4, 256),
     }
+    x, a, A = torch.zeros((1, 3, 10240), dtype=F16), torch.zeros((1, 3, 48)), torch.zeros(48)
+    layer = (0, 0, x, [torch.zeros(48, 128, 128)], a, a, A, A)
+    cw, cst = torch.zeros((10240, 4), dtype=F16), [torch.zeros((10240, 3), dtype=F16)]
+    calls["gdn_tree"] = (*layer, torch.zeros((1, 3, 6144), dtype=F16), A, pages, None, [1], cw, cst, 16, 48, 128, 128, 0.1,
+                         1e-6, 1e-6)
+    calls["gdn_commit"] = (*layer, pages, [torch.zeros(48, 128, 128)], [1], cw, cst, cst, 16, 48, 128, 128, 1e-6)
     for name, args in calls.items():
         call = getattr(lane, name)
         assert call(*args) is None and call(*args[:-1]) is None and call() is None
