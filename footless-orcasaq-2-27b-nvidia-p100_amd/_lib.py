@@ -90,6 +90,9 @@ SIGNATURES = {
                                   _I, _I, _I, _P, _I, _P, _SZ, _P]),
     "fl_attn_prep_axes": (_I, [_P, _I, _P, _P, _P, _P, _P, _I, _P, _P, _I, _I, _I, _P, _I, _LL, _P,
                                _P, _P, _I, _IP, _I, _I, _I, _I, _I, _I, _F, _F, _P]),
+    "fl_attn_tree_paged_work_bytes": (_SZ, [_I, _I, _I, _I, _I]),
+    "fl_attn_tree_paged": (_I, [_P, _I, _P, _P, _I, _I, _I, _P, _I, _LL, _P, _P, _I, _I, _I, _I, _I, _F,
+                                _I, _I, _I, _P, _I, _P, _SZ, _P]),
     "fl_paged_kv_copy": (_I, [_PP, _PP, _I, _I, _I, _I, _P, _P, _I, _I, _I, _P]),
     "fl_paged_kv_keep": (_I, [_PP, _PP, _I, _I, _I, _I, _P, _I, _LL, _P, _P, _I, _I, _I, _I, _P]),
     "fl_gdn_tree_normed": (_I, [_P, _I, _P, _PP, _IP, _P, _P, _P, _I, _P, _P, _PP, _P, _I, _P, _P,
@@ -139,7 +142,8 @@ BINDING_PATH = LIB_PATH.with_name("fl355_paged.so")
 BOUND = ("fl_paged_kv_store", "fl_paged_kv_load", "fl_attn_prep_paged",
          "fl_attention_prefill_paged_work_bytes", "fl_attention_prefill_paged",
          "fl_attn_decode_paged_work_bytes", "fl_attn_decode_paged", "fl_attn_prep_axes",
-         "fl_paged_kv_copy", "fl_paged_kv_keep", "fl_gdn_tree_normed", "fl_gdn_tree_commit")
+         "fl_paged_kv_copy", "fl_paged_kv_keep", "fl_gdn_tree_normed", "fl_gdn_tree_commit",
+         "fl_attn_tree_paged_work_bytes", "fl_attn_tree_paged")
 
 
 def _load_binding(L: ctypes.CDLL, path: Path | None = None):

@@ -40,15 +40,15 @@ HIPCC_FLAGS = [
 # accumulators are AGPRs held by inline asm); no NaNs and IEEE mode off, so
 # the score max is plain v_max / v_max3 without NaN-quieting canonicalisation
 # (scores are finite or -inf). attn_decode: its accumulators (scores read by the
-# softmax, O rescaled in place) in VGPRs as well; so attn_paged and, for its scores,
-# attn_paged_prefill. gdn_chunk, gdn_tree: the
-# products' results are split, scaled and fed back as operands by VALU code; in AGPRs
-# each would be copied out first.
+# softmax, O rescaled in place) in VGPRs as well; so attn_paged, attn_tree and, for its
+# scores, attn_paged_prefill. gdn_chunk, gdn_tree: the products' results are split, scaled
+# and fed back as operands by VALU code; in AGPRs each would be copied out first.
 FILE_FLAGS = {
     "attn_prefill": ["-mllvm", "-amdgpu-mfma-vgpr-form", "-fno-honor-nans", "-mno-amdgpu-ieee"],
     "attn_decode": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "attn_paged": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "attn_paged_prefill": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "attn_tree": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "gdn_chunk": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "gdn_tree": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }

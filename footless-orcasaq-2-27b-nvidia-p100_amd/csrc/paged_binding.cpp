@@ -33,6 +33,8 @@ decltype(&fl_paged_kv_copy) p_copy;
 decltype(&fl_paged_kv_keep) p_keep;
 decltype(&fl_gdn_tree_normed) p_gdn_tree;
 decltype(&fl_gdn_tree_commit) p_gdn_commit;
+decltype(&fl_attn_tree_paged_work_bytes) p_tree_bytes;
+decltype(&fl_attn_tree_paged) p_tree;
 
 constexpr int64_t HEAD_DIM = 256, KV8_ROW = HEAD_DIM + HEAD_DIM / 32 * 2;   // bytes of an int8 head row
 
@@ -428,17 +430,19 @@ PyObject* prefill(PyObject*, PyObject* const* args, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
-// (dev, stream, qg, kpool, vpool, pages, pos0, page_size, window, sinks, gate, z or None,
-//  work or None, n_kv, scale): z
-PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
+// (dev, stream, qg, kpool, vpool, pages, pos0, TREE: parents, page_size, window, sinks, gate, z or
+//  None, work or None, n_kv, scale): z
+template <bool TREE>
+PyObject* decode_of(PyObject* const* args, Py_ssize_t n) {
     HANDLE_TH_ERRORS
     Args a{args};
-    PLAIN(n == 15);
+    PLAIN(n == (TREE ? 16 : 15));
     a.dev = a.integer32();
     const auto stream = (fl_stream_t)a.integer();
     const at::Tensor* qg = a.dense(at::kHalf, 4);
     Pools c(a);
     const at::Tensor* pos0 = a.dense(at::kInt, 1);
+    const at::Tensor* parents = TREE ? a.dense(at::kInt, 2) : nullptr;
     const int64_t page_size = a.integer();
     const int window = a.integer32(), sinks = a.integer32(), gate = a.boolean();
     PyObject *zo = a.next(), *wo = a.next();
@@ -448,14 +452,16 @@ PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
     const int64_t B = qg->size(0), T = qg->size(1), n_q = qg->size(2), pitch = qg->size(3);
     PLAIN(B <= FL_PAGED_MAX_SEQS && T <= INT_MAX && n_q <= INT_MAX && pitch <= INT_MAX &&
           pos0->numel() == B && c.fit(B, page_size, n_kv, HEAD_DIM));
+    PLAIN(!TREE || (parents->size(0) == B && parents->size(1) == T));
     at::Tensor z;
     if (zo != Py_None) {
         const at::Tensor* t = a.dense(zo, at::kHalf, 4);
         PLAIN(t && t->size(0) == B && t->size(1) == T && t->size(2) == n_q && t->size(3) <= INT_MAX);
         z = *t;
     }
-    const size_t need =
-        wo != Py_None ? 0 : p_decode_bytes((int)B, (int)T, (int)n_q, (int)n_kv, (int)HEAD_DIM);
+    const size_t need = wo != Py_None ? 0
+                                      : (TREE ? p_tree_bytes : p_decode_bytes)((int)B, (int)T, (int)n_q, (int)n_kv,
+                                                                               (int)HEAD_DIM);
     PLAIN(wo != Py_None || need > 0);   // (sizes that the call refuses)
     at::Tensor made;
     void* work;
@@ -463,10 +469,14 @@ PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
     PLAIN(work_of(wo, a, need, made, work, bytes));
     if (zo == Py_None) z = half_rows({B, T, n_q, HEAD_DIM}, a.dev);
     const int rc = released([&] {
-        return p_decode(qg->data_ptr(), (int)pitch, c.k->data_ptr(), c.v->data_ptr(), c.q8, c.n_pages,
-                        (int)page_size, (const int*)c.pages->data_ptr(), c.max_pages, c.stride,
-                        (const int*)pos0->data_ptr(), (int)B, (int)T, (int)n_q, (int)n_kv, (int)HEAD_DIM,
-                        scale, window, sinks, gate, z.data_ptr(), (int)z.size(3), work, bytes, stream);
+        auto call = [&](auto f, auto... more) {
+            return f(qg->data_ptr(), (int)pitch, c.k->data_ptr(), c.v->data_ptr(), c.q8, c.n_pages,
+                     (int)page_size, (const int*)c.pages->data_ptr(), c.max_pages, c.stride,
+                     (const int*)pos0->data_ptr(), more..., (int)B, (int)T, (int)n_q, (int)n_kv, (int)HEAD_DIM,
+                     scale, window, sinks, gate, z.data_ptr(), (int)z.size(3), work, bytes, stream);
+        };
+        if constexpr (TREE) return call(p_tree, (const int*)parents->data_ptr());
+        else return call(p_decode);
     });
     MADE(rc);
     if (zo == Py_None) return THPVariable_Wrap(std::move(z));
@@ -474,6 +484,8 @@ PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return zo;
     END_HANDLE_TH_ERRORS
 }
+PyObject* decode(PyObject*, PyObject* const* args, Py_ssize_t n) { return decode_of<false>(args, n); }
+PyObject* tree(PyObject*, PyObject* const* args, Py_ssize_t n) { return decode_of<true>(args, n); }
 
 // A list or tuple of dense tensors, one a sequence: their pointers, and the fewest elements of one.
 struct Buffers {
@@ -616,7 +628,7 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
     void** const to[] = {(void**)&p_store, (void**)&p_load, (void**)&p_prep, (void**)&p_prefill_bytes,
                          (void**)&p_prefill, (void**)&p_decode_bytes, (void**)&p_decode,
                          (void**)&p_prep_axes, (void**)&p_copy, (void**)&p_keep, (void**)&p_gdn_tree,
-                         (void**)&p_gdn_commit};
+                         (void**)&p_gdn_commit, (void**)&p_tree_bytes, (void**)&p_tree};
     if (n != (Py_ssize_t)(sizeof(to) / sizeof(to[0]))) {
         PyErr_SetString(PyExc_TypeError, "bind: one address an entry point");
         return nullptr;
@@ -640,6 +652,7 @@ PyMethodDef methods[] = {
     {"kv_keep", (PyCFunction)(void (*)())kv_keep, METH_FASTCALL, nullptr},
     {"gdn_tree", (PyCFunction)(void (*)())gdn_tree, METH_FASTCALL, nullptr},
     {"gdn_commit", (PyCFunction)(void (*)())gdn_commit, METH_FASTCALL, nullptr},
+    {"tree", (PyCFunction)(void (*)())tree, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "fl355_paged", nullptr, -1, methods};

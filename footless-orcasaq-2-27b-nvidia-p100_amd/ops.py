@@ -948,6 +948,56 @@ def attn_prep_axes(qg, k, v, wq, wk, kpool, vpool, pages, starts, pos0, position
     return qg if q_out is None else q_out
 
 
+def attn_tree_paged_work_bytes(B: int, T: int, n_q_heads: int = N_HEADS, n_kv_heads: int = N_KV,
+                               head_dim: int = HEAD_DIM) -> int:
+    """The `work` bytes of attn_tree_paged on the current device."""
+    return _tree_paged_bytes(B, T, n_q_heads, n_kv_heads, head_dim, _here())
+
+
+@functools.lru_cache(maxsize=256)
+def _tree_paged_bytes(B, T, n_q_heads, n_kv_heads, head_dim, dev):
+    return _lib.lib().fl_attn_tree_paged_work_bytes(B, T, n_q_heads, n_kv_heads, head_dim)
+
+
+def attn_tree_paged(qg, kpool, vpool, pages, pos0, parents, *, page_size: int, window: int = 0,
+                    sinks: int = 0, gate: bool = True, z=None, work=None, n_kv_heads: int = N_KV,
+                    scale: float = ATTN_SCALE):
+    """attn_decode_paged for trees of drafted tokens: qg [B, T, n_q_heads, q_pitch] fp16 with
+    q | gate per head, T up to 64, pos0 [B] and parents [B, T] int32 on the GPU (read when the
+    call runs); up to 1024 sequences. A token sees its sequence's context and, of the tree,
+    its ancestors and itself; with a window, the rows whose positions are above p - window or
+    below sinks, p = pos0 + its depth. Places without a token, and sequences at a negative
+    pos0, give 0. work: uint8 of attn_tree_paged_work_bytes (allocated here unless given). The
+    last bits of a sequence's z depend on the batch. Returns z [B, T, n_q_heads, head_dim]
+    fp16."""
+    dev = _here()
+    if dev >= 0 and _lib.lane is not None:
+        r = _lib.lane.tree(dev, _stream(), qg, kpool, vpool, pages, pos0, parents, page_size, window, sinks, gate,
+                           z, work, n_kv_heads, scale)
+        if r is not None:
+            return _made("fl_attn_tree_paged", r, r)
+    for name, t in (("qg", qg), ("pos0", pos0), ("parents", parents)):
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name}: expected a torch.Tensor, got {type(t).__name__}")
+    B, T, n_q_heads, q_pitch = qg.shape
+    if pos0.dim() != 1 or pos0.numel() != B or tuple(parents.shape) != (B, T):
+        raise ValueError(f"pos0: expected [{B}], parents: expected [{B}, {T}]")
+    pg = _paged(kpool, vpool, pages, page_size, B, n_kv_heads, HEAD_DIM, dev)
+    qp, pp, at = _dense_ptr(qg, F16, "qg"), _dense_ptr(pos0, I32, "pos0"), _dense_ptr(parents, I32, "parents")
+    if z is None:
+        z = torch.empty((B, T, n_q_heads, HEAD_DIM), dtype=F16, device=qg.device)
+    elif z.dim() != 4 or z.shape[0] != B or z.shape[1] != T or z.shape[2] != n_q_heads:
+        raise ValueError(f"z: expected [{B}, {T}, {n_q_heads}, pitch]")
+    zp = _dense_ptr(z, F16, "z")
+    _same_device(dev, qg=qg, z=z, pos0=pos0, parents=parents, work=work)
+    if work is None:
+        work = torch.empty(_tree_paged_bytes(B, T, n_q_heads, n_kv_heads, HEAD_DIM, dev), dtype=torch.uint8,
+                           device=qg.device)
+    _lib.call("fl_attn_tree_paged", qp, q_pitch, *pg, pp, at, B, T, n_q_heads, n_kv_heads, HEAD_DIM, scale, window,
+              sinks, int(gate), zp, z.shape[3], *_prefill_work(work), _stream())
+    return z
+
+
 def _layer_pools(kpools, vpools, page_size, n_kv_heads, head_dim, dev):
     """(k pointers, v pointers, layers, q8, n_pages, page_size) of several layers' pools, alike."""
     ks, vs = ([p] if isinstance(p, torch.Tensor) else list(p) for p in (kpools, vpools))

@@ -471,6 +471,21 @@ int fl_attn_prep_axes(void* qg, int q_pitch, const void* k, const void* v, const
                       int n_q_heads, int n_kv_heads, int head_dim, int rope_dim, float theta,
                       float eps, fl_stream_t stream);
 
+/* Attention of a tree's tokens over the pages: token i sees the context's rows r < pos0[b] with r > p -
+ * window or r < sinks, and of the tree's rows those of its ancestors and its own, as far as their
+ * positions are in the same window (window 0: all), each where its page is present. Places without a
+ * token and sequences at a negative pos0 give 0. qg [B][T][n_q_heads][q_pitch], z
+ * [B][T][n_q_heads][z_pitch], the gate as fl_attn_decode_paged's; any n_q_heads / n_kv_heads. work:
+ * fl_attn_tree_paged_work_bytes on the device that runs the call, 16-byte aligned, one for each call
+ * that may overlap with another. The precision is the decode form's. */
+size_t fl_attn_tree_paged_work_bytes(int B, int T, int n_q_heads, int n_kv_heads, int head_dim);
+int fl_attn_tree_paged(const void* qg, int q_pitch, const void* kpool, const void* vpool, int q8,
+                       int n_pages, int page_size, const int* pages, int max_pages,
+                       long long pages_stride, const int* pos0, const int* parents, int B, int T,
+                       int n_q_heads, int n_kv_heads, int head_dim, float scale, int window, int sinks,
+                       int gated, void* z, int z_pitch, void* work, size_t work_bytes,
+                       fl_stream_t stream);
+
 /* Whole pages src[i] -> dst[i] (device arrays of n page ids) in the K and V pools of
  * n_layers layers (host arrays of device pointers; up to FL_POOL_MAX layers): the private
  * copy of a forked sequence's last page, pages moved together. A pair with an entry outside

@@ -42,6 +42,13 @@ def keep(fl, **over):
     return fl._lib.lib().fl_paged_kv_keep(*a.values(), None)
 
 
+def attn(fl, **over):
+    a = dict(q=FAKE, qp=512, kpool=FAKE, vpool=FAKE, **POOL, **TABLE, pos0=FAKE, parents=FAKE, B=2, T=8, nq=24, kv=4,
+             hd=256, scale=0.0625, window=0, sinks=0, gated=1, z=FAKE, zp=256, work=FAKE, wb=0)
+    a.update(over)
+    return fl._lib.lib().fl_attn_tree_paged(*a.values(), None)
+
+
 def layer(**over):
     a = dict(x=FAKE, xs=10240, w=FAKE, cin=ptrs(FAKE, FAKE), pos0=ints(5, 5), nodes=FAKE, a=FAKE, b=FAKE, abs=48,
              A=FAKE, dt=FAKE, S=ptrs(FAKE, FAKE))
@@ -84,6 +91,10 @@ LAYERS = [dict(ks=None), dict(vs=None), dict(layers=0), dict(layers=65, ks=ptrs(
         dict(kpool=None), dict(vpool=FAKE + 8), dict(positions=None), dict(of=None), dict(axes=0), dict(axes=2),
         dict(axes=129), dict(of=ints(*[-1] * 32)), dict(starts=None), dict(pos0=None), dict(N=-1), dict(rope=63),
         dict(qp=255), dict(nq=23), dict(q_out=FAKE, qop=128)]],
+    *[(attn, o) for o in SIZES + TABLES + [
+        dict(kpool=None), dict(vpool=FAKE + 8), dict(q=None), dict(z=None), dict(pos0=None), dict(parents=None), dict(T=0),
+        dict(T=65), dict(nq=0), dict(nq=23), dict(nq=4100), dict(qp=256), dict(qp=516), dict(zp=128), dict(q=FAKE + 8),
+        dict(window=-1), dict(sinks=-1), dict(scale=0.0), dict(work=FAKE + 8, wb=1 << 40)]],
     *[(copy, o) for o in SIZES + LAYERS + [dict(n=-1), dict(n=1, src=None), dict(n=1, dst=None),
                                            dict(n=1 << 30, page_size=1 << 15)]],
     *[(f, o) for f in (gdn_tree, gdn_commit) for o in GDN],
@@ -102,6 +113,14 @@ def test_refusals(fl, f, over):
 
 def test_nothing_to_do_is_ok(fl):
     assert prep_axes(fl) == copy(fl) == keep(fl) == 0
+
+
+def test_work_of_a_tree(fl):
+    """Too little is refused; it does not grow with the batch but for 8 bytes a sequence."""
+    f = fl.ops.attn_tree_paged_work_bytes
+    assert attn(fl) == 3 and attn(fl, work=None, wb=1 << 40) == 3 and b"work" in fl._lib.lib().fl_last_error()
+    assert 0 < f(1000, 26) - f(1, 26) <= 8000
+    assert f(1, 65) == f(0, 1) == f(1, 1, 23) == f(1025, 1) == 0
 
 
 def test_op_layer_refuses(fl):
@@ -141,6 +160,13 @@ def test_op_layer_refuses(fl):
         ops.attn_prep_axes(*x, None, page_size=16)
     with pytest.raises(ValueError, match="GPU"):
         ops.attn_prep_axes(*x, at, page_size=16, sections=(16, 8, 8))
+    qg, parents = torch.zeros((1, 3, 24, 512), dtype=F16), torch.zeros((1, 3), dtype=I32)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.attn_tree_paged(qg, pool, pool, pages, pos0, parents, page_size=16)
+    with pytest.raises(ValueError, match="parents"):
+        ops.attn_tree_paged(qg, pool, pool, pages, pos0, parents[:, :2], page_size=16)
+    with pytest.raises(TypeError, match="parents"):
+        ops.attn_tree_paged(qg, pool, pool, pages, pos0, [[-1, 0, 0]], page_size=16)
 
 
 def test_op_layer_refuses_gdn_trees(fl):
@@ -189,6 +215,7 @@ def test_binding_declines_what_is_not_plain(fl):
         "kv_copy": (0, 0, [pool], [pool], ids, ids, 16, 4, 256),
         "kv_keep": (0, 0, [pool], (pool,), pages, pos0, path, 16, 4, 256),
     }
+    calls["tree"] = (0, 0, q[None], pool, pool, pages, pos0, pages, 16, 0, 0, True, None, None, 4, 0.0625)
     x, a, A = torch.zeros((1, 3, 10240), dtype=F16), torch.zeros((1, 3, 48)), torch.zeros(48)
     layer = (0, 0, x, [torch.zeros(48, 128, 128)], a, a, A, A)
     cw, cst = torch.zeros((10240, 4), dtype=F16), [torch.zeros((10240, 3), dtype=F16)]
