@@ -5,8 +5,8 @@
 // whose position pos0 + depth(j) is in sight alike. The rest is the decode's:
 //   z = f16_sat(sum_r e^(scale q.k_r - m) v_r / sum_r e^(scale q.k_r - m) * sigmoid(gate)).
 //
-// The T G query rows of a kv head are columns. A workgroup has 64 CB of them, 16 CB a wave, and
-// walks tiles of 32 cache rows that its four waves share through LDS:
+// The T G query rows of a kv head are columns. A workgroup has 16 of them on each of its 4, 8 or 12
+// waves, and walks tiles of 32 cache rows that its waves share through LDS:
 //   S^T (32 rows x 16 columns) = K Q^T        16x16x32 MFMAs, Q in registers
 //   softmax                                   a lane holds column i's rows 4 g + e of both halves
 //   O^T (256 dims x 16 columns) += V^T P^T    P as it lies: k slot (g, e) is row 4 g + e of half
@@ -15,6 +15,11 @@
 // equal runs, one a workgroup, wherever the cuts fall; the runs are found from pos0 on the device, so
 // that a captured call follows it. A sequence that lies in one run is finished there; a cut one leaves
 // a partial a piece, which the merge weighs.
+//
+// Measured, from a graph: 18 us for a tree of 16 on 500 rows, 67 us for 8 of them on 8192 (4.1 TB/s),
+// 197 us for 16 of 8 tokens on 16384 (5.5 TB/s, int8 237), 291 us for 4 of 63 on 20000 to 60000 (0.8 PFLOP/s), 136 us
+// for 12 of 26 on 100 to 32768 int8 rows. Small trees are bound by the cache's bytes, large ones
+// by what a SIMD does beside its MFMAs: of 3300 clocks a tile of 32 rows and 192 columns 1540 are MFMAs.
 #include "attn_paged.hpp"
 #include "tree.hpp"
 
@@ -29,13 +34,14 @@ constexpr int TT = 32;                  // rows a tile
 constexpr int ROW_B = 2 * PAGED_HD;     // bytes a row in LDS
 constexpr int TILE_B = TT * ROW_B;
 constexpr int STAGE_B = 2 * TILE_B;     // K | V
-constexpr int W = 4;                    // waves
-constexpr int MAX_CB = 2;
 constexpr int RUN_MIN = 4;              // tiles a run, at least
 constexpr int SEQ_COST = 2;             // a further piece's fixed cost in tiles
 
-// the chunk swizzle of tile row r: 16-byte chunk c lies at c ^ sw(r)
-__device__ __forceinline__ int sw(int r) { return ((r & 3) << 2) | ((r >> 2) & 3); }
+// The chunk swizzle of tile row r: 16-byte chunk c lies at c ^ sw(r). A read of 16 bytes a lane takes
+// lanes 0 - 3, 12 - 15, 20 - 27 together, then 4 - 11, 16 - 19, 28 - 31, ...: 16 rows of K at chunk c
+// and, of other rows, at c + 1; one of V^T's 8 bytes a lane takes 8 rows' pairs of chunks together. With
+// these values both meet every bank once (with r / 4 in place of -r / 4 half of the LDS cycles are conflicts).
+__device__ __forceinline__ int sw(int r) { return ((r & 3) << 2) | (-(r >> 2) & 3); }
 
 // What a sequence's tokens see at most, as tiles: the first s ones, then those from a on, n in all.
 struct Walk {
@@ -133,18 +139,56 @@ __device__ __forceinline__ f16x8 bytes_as_ints(uint32_t a, uint32_t b) {
     return __builtin_bit_cast(f16x8, r) - (f16x8)((f16)1152.f);
 }
 
+// O^T lives in accumulation registers and is touched by the asm below alone: with the compiler's own
+// MFMAs it got a second set of registers and was moved back on every tile. What the compiler cannot see
+// in asm: an operand written by a VALU instruction right ahead of an MFMA needs two wait states (s_nop 1
+// in front of each), and a result must have left the matrix pipeline before it is read (acc_settle).
+// A spill of an accumulator would read it too early: there must be none.
+__device__ __forceinline__ void acc_mfma(f32x4& acc, const f16x8& a, const f16x8& b) {
+    asm("s_nop 1\n\tv_mfma_f32_16x16x32_f16 %0, %1, %2, %0" : "+a"(acc) : "v"(a), "v"(b));
+}
+__device__ __forceinline__ void acc_settle(f32x4 (&o)[16]) {
+    asm volatile("s_nop 7\n\ts_nop 7\n\ts_nop 7"
+                 : "+a"(o[0]), "+a"(o[1]), "+a"(o[2]), "+a"(o[3]), "+a"(o[4]), "+a"(o[5]), "+a"(o[6]), "+a"(o[7]));
+    asm volatile(""
+                 : "+a"(o[8]), "+a"(o[9]), "+a"(o[10]), "+a"(o[11]), "+a"(o[12]), "+a"(o[13]), "+a"(o[14]),
+                   "+a"(o[15]));
+}
+__device__ __forceinline__ void acc_scale(f32x4 (&o)[16], float c) {
+    acc_settle(o);
+#pragma unroll
+    for (int n = 0; n < 16; ++n) {
+        float x[4] = {o[n][0], o[n][1], o[n][2], o[n][3]}, t0, t1;
+#pragma unroll
+        for (int e = 0; e < 4; e += 2)
+            asm volatile(
+                "v_accvgpr_read_b32 %2, %0\n\t"
+                "v_accvgpr_read_b32 %3, %1\n\t"
+                "v_mul_f32 %2, %2, %4\n\t"
+                "v_mul_f32 %3, %3, %4\n\t"
+                "s_nop 2\n\t"
+                "v_accvgpr_write_b32 %0, %2\n\t"
+                "v_accvgpr_write_b32 %1, %3"
+                : "+a"(x[e]), "+a"(x[e + 1]), "=&v"(t0), "=&v"(t1)
+                : "v"(c));
+        o[n] = (f32x4){x[0], x[1], x[2], x[3]};
+    }
+}
+
 constexpr int STAGES_F16 = 4, AHEAD = STAGES_F16 - 1;   // tiles in LDS and copied ahead
-constexpr int COPIES = 8;                               // copy instructions a wave a tile
-constexpr int STAGES_Q8 = 2;
+constexpr int PLAN = 64;                                // tiles planned at a time
+constexpr int KPF = 3, VPF = 3;                         // K and V^T operands read ahead of their products
 
-// A wave's 8 rows of an int8 tile in flight: bytes [row 4 n + g][16 i .. + 15] of K and V, and the
-// scales of those 16 dims' blocks.
-struct Bytes {
-    u32x4 k[2], v[2];
-    f16 ks[2], vs[2];
-};
+// Over int8 pools a tile's bytes come to LDS as they are, RAW_AHEAD tiles ahead, a wave's rows of K, of
+// V and their scales behind each other; the same wave turns them into rows of the fp16 stage, K as the
+// integers they are and V as f16(byte scale), while the stage before it is in use.
+constexpr int STAGES_Q8 = 2, RAW_STAGES = 4, RAW_AHEAD = RAW_STAGES - 1;
+constexpr int RAW_ROW = PAGED_HD + 16;   // bytes a row and its scales
+__device__ __forceinline__ void copy4_v(const char* vptr, uint32_t dst) {   // copy16_v, 4 bytes a lane
+    asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(vptr), "{m0}"(dst));
+}
 
-template <int CB, bool Q8>
+template <int W, bool Q8>
 __global__ void __launch_bounds__(64 * W)
 tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict__ kp,
                  const char* __restrict__ vp, const Pages pg, const int* __restrict__ pos0s,
@@ -152,11 +196,21 @@ tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict
                  int run_min, float sl2, const Sight sight, f16* __restrict__ z, int z_pitch, int gated,
                  const Parts parts) {
     constexpr int STAGES = Q8 ? STAGES_Q8 : STAGES_F16;
+    constexpr int CW = W < 8 ? W : 8;                         // waves that copy
+    constexpr int ROWS = TT / CW;                             // a copying wave's rows of a tile
+    constexpr int RAW_WAVE = 2 * ROWS * RAW_ROW;
+    constexpr int COPIES = Q8 ? ROWS / 2 + 1 : ROWS;          // its copy instructions a tile
     __shared__ __attribute__((aligned(16))) char s_tile[STAGES * STAGE_B];
+    __shared__ __attribute__((aligned(16))) char s_raw[Q8 ? RAW_STAGES * CW * RAW_WAVE : 16];
     // the steps of K's blocks, [stage][block][row] (int8)
     __shared__ __attribute__((aligned(16))) float s_step[Q8 ? STAGES : 1][8][Q8 ? TT : 4];
     __shared__ uint2 s_line[TREE_MAX];   // a token's rows in sight, of the tree's
     __shared__ int s_lo[TREE_MAX];       // and the first of the context's
+    // of 64 tiles and the next 64: the pool rows of their halves (of an absent page: row 0), the rows on
+    // pages, those of them that some token sees, and the tiles that every token sees whole
+    __shared__ int2 s_rows[2 * PLAN];
+    __shared__ uint32_t s_here[2 * PLAN], s_seen[2 * PLAN];
+    __shared__ uint64_t s_whole[2];
     const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
     const int G = n_q / n_kv, R = T * G;
@@ -175,23 +229,19 @@ tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict
     TreeRun run(pos0s, B, T, run_id, runs, run_min, sight, cap);
     if (!run.any) return;   // (the whole workgroup)
 
-    // this lane's query rows: of token t[cb], or none
-    int t[CB];
-    size_t qrow[CB];
-#pragma unroll
-    for (int cb = 0; cb < CB; ++cb) {
-        const int r = (grp * W + w) * 16 * CB + 16 * cb + col;
-        t[cb] = r < R ? r / G : -1;
-        qrow[cb] = r < R ? (size_t)(r / G) * n_q + h * G + r % G : 0;
-    }
-    const bool busy = (grp * W + w) * 16 * CB < R;   // (wave-uniform)
+    // this lane's query row: of token t, or none
+    const int c0 = (grp * W + w) * 16, r_mine = c0 + col;
+    const bool busy = c0 < R;   // (wave-uniform)
+    const int t = r_mine < R ? r_mine / G : -1;
+    const int qrow = r_mine < R ? t * n_q + h * G + r_mine - t * G : 0;
     const uint32_t rsb = (Q8 ? PAGED_HD : ROW_B) * n_kv;   // bytes a pool row
     const char* kb = uniform_ptr(kp + (size_t)h * (Q8 ? PAGED_HD : ROW_B));
     const char* vb = uniform_ptr(vp + (size_t)h * (Q8 ? PAGED_HD : ROW_B));
     const size_t values = ((size_t)pg.n_pages << pg.shift) * n_kv * PAGED_HD;   // ahead of the scales
     const uint32_t lds = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)s_tile);
     // K operand of k step ks: row col (+ 16), chunk 4 ks + g, at koff ^ 64 ks; V^T operand of dims 16 n ..:
-    // this lane points at row 4 g + col / 4 (+ 16), dims 16 n + 4 (col % 4), at voff ^ 32 n
+    // this lane points at row 4 g + col / 4 (+ 16), dims 16 n + 4 (col % 4), at voff ^ 32 n (bit 8 of both
+    // is not swizzled: an immediate)
     const uint32_t koff = col * ROW_B + 16 * (g ^ sw(col));
     const int vr = 4 * g + (col >> 2);
     const uint32_t voff = vr * ROW_B + 16 * ((col >> 1 & 1) ^ sw(vr)) + 8 * (col & 1);
@@ -211,185 +261,244 @@ tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict
                                       walk.n == 0 ? -1 : count > 1 ? count : 0);
         }
         __syncthreads();   // (the last piece's reads of s_line, s_lo and the stages)
-        uint64_t present;
-        {
+        uint64_t present = 0;   // (wave 0's)
+        // Tiles j0 + 64 c ..: a tile a lane of wave 0, so that the copies and masks of one cost no more than a
+        // look at its entry (a page's lookup on the scalar unit, which a SIMD's waves share, held them all up).
+        auto row_of = [&](int c) { return walk.row0(min(j0 + PLAN * c + lane, j1 - 1)); };
+        auto ids_of = [&](int c) {   // (in the table, also behind its last page)
+            const int *row = pg.table + (size_t)b * pg.stride, r0 = row_of(c), top = pg.max_pages - 1;
+            return make_int2(row[min(r0 >> pg.shift, top)], row[min((r0 + 16) >> pg.shift, top)]);
+        };
+        auto plan = [&](int c, int2 ids) {
+            const int r0 = row_of(c), at = PLAN * (c & 1) + lane;
+            auto row = [&](int r, int id) {
+                return r < cap && (unsigned)id < (unsigned)pg.n_pages
+                           ? (id << pg.shift) + (r & ((1 << pg.shift) - 1)) : -1;
+            };
+            const int a = row(r0, ids.x), e = row(r0 + 16, ids.y);
+            const uint32_t here = (a < 0 ? 0u : 0xFFFFu) | (e < 0 ? 0u : 0xFFFF0000u);
+            uint32_t seen = low_bits(walk.ctx - r0) & (~low_bits(walk.lo0 - r0) | low_bits(sight.sinks - r0));
+            const int d = r0 - pos0;   // of the tree's
+            if (d > -TT && d < 64) seen |= (uint32_t)(d < 0 ? present << -d : present >> d) & low_bits(walk.hi - r0);
+            s_rows[at] = make_int2(max(a, 0), max(e, 0));
+            s_here[at] = here;
+            s_seen[at] = seen & here;
+            const uint64_t whole =
+                __ballot(here == ~0u && r0 + TT <= walk.ctx && (r0 >= walk.lo1 || r0 + TT <= sight.sinks));
+            if (lane == 0) s_whole[c & 1] = whole;
+        };
+        if (w == 0) {
             double none = 0.;
-            const Node node = tree_node(parents + (size_t)b * T, T, none);   // (every wave)
+            const int2 ids = j1 > j0 ? ids_of(0) : make_int2(0, 0);
+            const Node node = tree_node(parents + (size_t)b * T, T, none);
             present = __ballot(node.here());
-            if (w == 0) {
-                // a path's tokens are numbered upwards: out of the window are its first ones, but those
-                // that count as first rows of the sequence
-                uint64_t line = (uint64_t)node.hi << 32 | node.lo, kept = 0;
-                if (sight.window > 0) {
-                    const int depth = node.depth();
-                    uint64_t rest = line;
-                    for (int e = 0; __any(e <= depth - sight.window); ++e) {
-                        const uint64_t bit = rest & -rest;
-                        if (e <= depth - sight.window) {
-                            if (pos0 < sight.sinks - e) kept |= bit;
-                            rest &= ~bit;
-                        }
+            // a path's tokens are numbered upwards: out of the window are its first ones, but those
+            // that count as first rows of the sequence
+            uint64_t line = (uint64_t)node.hi << 32 | node.lo, kept = 0;
+            if (sight.window > 0) {
+                const int depth = node.depth();
+                uint64_t rest = line;
+                for (int e = 0; __any(e <= depth - sight.window); ++e) {
+                    const uint64_t bit = rest & -rest;
+                    if (e <= depth - sight.window) {
+                        if (pos0 < sight.sinks - e) kept |= bit;
+                        rest &= ~bit;
                     }
-                    line = rest | kept;
                 }
-                s_line[lane] = make_uint2((uint32_t)line, (uint32_t)(line >> 32));
-                s_lo[lane] = node.here() ? window_from(pos0, node.depth(), sight.window) : INT_MAX;
+                line = rest | kept;
             }
+            s_line[lane] = make_uint2((uint32_t)line, (uint32_t)(line >> 32));
+            s_lo[lane] = node.here() ? window_from(pos0, node.depth(), sight.window) : INT_MAX;
+            if (j1 > j0) plan(0, ids);
         }
         __syncthreads();
         if (j1 > j0) {
-            f16x8 q[CB][8];
-            f32x4 o[CB][16];
-            float m_run[CB], l_run[CB];
-            int lo[CB];
-            uint2 line[CB];
+            f16x8 q[8];
+            f32x4 o[16];
+            float m_run, l_run;
+            auto begin = [&] {   // (with the first tiles' copies under way)
+                const f16* row = qg + ((size_t)b * T * n_q + qrow) * q_pitch + 8 * g;
 #pragma unroll
-            for (int cb = 0; cb < CB; ++cb) {
-                const f16* row = qg + ((size_t)b * T * n_q + qrow[cb]) * q_pitch + 8 * g;
+                for (int ks = 0; ks < 8; ++ks) q[ks] = t >= 0 ? *(const f16x8*)(row + 32 * ks) : (f16x8)(0);
+                WAIT_VMCNT(0);   // Q is here: a wait for it later would drain the copies
 #pragma unroll
-                for (int ks = 0; ks < 8; ++ks) q[cb][ks] = t[cb] >= 0 ? *(const f16x8*)(row + 32 * ks) : (f16x8)(0);
+                for (int ks = 0; ks < 8; ++ks) {   // (beside O, as far as there is room at three waves a SIMD)
+                    if (ks < 5) asm volatile("" : "+a"(q[ks]));
+                    else asm volatile("" : "+v"(q[ks]));
+                }
 #pragma unroll
-                for (int n = 0; n < 16; ++n) o[cb][n] = (f32x4)(0.f);
-                m_run[cb] = -1e30f, l_run[cb] = 0.f;
-                lo[cb] = t[cb] >= 0 ? s_lo[t[cb]] : INT_MAX;
-                line[cb] = t[cb] >= 0 ? s_line[t[cb]] : make_uint2(0, 0);
-            }
-            auto ids = page_ids(pg, b, j0, j1 - 1, 0, [&](int j) { return walk.row0(j); });
-            // the rows of [r, r + 32) that some token sees, were their pages there
-            auto seen_rows = [&](int r) {
-                uint32_t m = low_bits(walk.ctx - r) & (~low_bits(walk.lo0 - r) | low_bits(sight.sinks - r));
-                const int d = r - pos0;   // of the tree's
-                if (d > -32 && d < 64) m |= (uint32_t)(d < 0 ? present << -d : present >> d) & low_bits(walk.hi - r);
-                return m;
+                for (int n = 0; n < 16; ++n) {
+                    o[n] = (f32x4)(0.f);
+                    asm volatile("" : "+a"(o[n]));
+                }
+                m_run = -1e30f, l_run = 0.f;
             };
             auto tree_bits = [&](uint2 l, int r) {
                 const int d = r - pos0;
                 const uint64_t x = (uint64_t)l.y << 32 | l.x;
                 return d <= -32 || d >= 64 ? 0u : (uint32_t)(d < 0 ? x << -d : x >> d);
             };
-            // scores, softmax and product with V of the tile at row r0 in a stage; here: rows on pages
-            auto tile = [&](int stage, int r0, uint32_t here) {
+            uint64_t whole_bits = 0;
+            // scores, softmax and product with V of tile j0 + j, in a stage
+            auto tile = [&](int stage, int j) {
                 if (!busy) return;
-                const char *kt = s_tile + stage * STAGE_B, *vt = kt + TILE_B;
-                f32x4 s[CB][2];
+                if ((j & (PLAN - 1)) == 0) {
+                    const uint64_t x = s_whole[j / PLAN & 1];
+                    whole_bits = (uint64_t)(uint32_t)uni((int)(x >> 32)) << 32 | (uint32_t)uni((int)x);
+                }
+                uint32_t ko = koff, vo = voff;
+                asm volatile("" : "+v"(ko), "+v"(vo));   // (its swizzled forms are not worth registers across tiles)
+                auto k_frag = [&](int i) {   // k step i % 8 of rows 16 (i / 8) ..
+                    return *(const f16x8*)(s_tile + stage * STAGE_B + (ko ^ (64 * (i & 3))) + 256 * (i >> 2 & 1) +
+                                           16 * ROW_B * (i >> 3));
+                };
+                s16x4 vf[VPF][2];
+                auto v_frag = [&](int n) {
+                    const char* at = s_tile + stage * STAGE_B + TILE_B + (vo ^ (32 * (n & 7))) + 256 * (n >> 3);
+                    vf[n % VPF][0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at);
+                    vf[n % VPF][1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 16 * ROW_B));
+                };
+                f32x4 s[2];
+                f16x8 ka[KPF];
+                // the two halves' products alternate: one's are a chain
+                auto product = [&](int i, f32x4 c) {
+                    return __builtin_amdgcn_mfma_f32_16x16x32_f16(ka[i % KPF], q[i >> 1], c, 0, 0, 0);
+                };
+                auto frag_of = [](int i) { return (i & 1) << 3 | i >> 1; };
 #pragma unroll
-                for (int rb = 0; rb < 2; ++rb) {
+                for (int i = 0; i < KPF; ++i) ka[i] = k_frag(frag_of(i));
+                if constexpr (Q8) {
+                    // a k step is a block: its step goes onto its product, under the next one
+                    f32x4 p[2], step[2];
+                    auto block = [&](int i) {
+                        step[i & 1] = *(const f32x4*)&s_step[stage][i >> 1][16 * (i & 1) + 4 * g];
+                        p[i & 1] = product(i, (f32x4)(0.f));
+                        if (i + KPF < 16) ka[i % KPF] = k_frag(frag_of(i + KPF));
+                        __builtin_amdgcn_sched_barrier(0);
+                    };
+                    block(0);
 #pragma unroll
-                    for (int cb = 0; cb < CB; ++cb) s[cb][rb] = (f32x4)(0.f);
+                    for (int i = 0; i < 16; ++i) {
+                        if (i + 1 < 16) block(i + 1);
 #pragma unroll
-                    for (int ks = 0; ks < 8; ++ks) {
-                        const f16x8 a = *(const f16x8*)(kt + 16 * rb * ROW_B + (koff ^ (64 * ks)));
-                        if constexpr (Q8) {
-                            const f32x4 step = *(const f32x4*)&s_step[stage][ks][16 * rb + 4 * g];
+                        for (int e = 0; e < 4; ++e)
+                            s[i & 1][e] = i < 2 ? step[i & 1][e] * p[i & 1][e]
+                                                : fmaf(step[i & 1][e], p[i & 1][e], s[i & 1][e]);
+                        asm volatile("" : "+v"(s[i & 1]));   // (here: sunk behind the masks, all products would be held)
+                        __builtin_amdgcn_sched_barrier(0);
+                    }
+                } else {
 #pragma unroll
-                            for (int cb = 0; cb < CB; ++cb) {
-                                const f32x4 p = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q[cb][ks], (f32x4)(0.f), 0, 0, 0);
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) s[cb][rb][e] = fmaf(step[e], p[e], s[cb][rb][e]);
-                            }
-                        } else {
-#pragma unroll
-                            for (int cb = 0; cb < CB; ++cb)
-                                s[cb][rb] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, q[cb][ks], s[cb][rb], 0, 0, 0);
-                        }
+                    for (int i = 0; i < 16; ++i) {
+                        s[i & 1] = product(i, i < 2 ? (f32x4)(0.f) : s[i & 1]);
+                        if (i + KPF < 16) ka[i % KPF] = k_frag(frag_of(i + KPF));
+                        __builtin_amdgcn_sched_barrier(0);   // (keeps the reads ahead)
                     }
                 }
-                // whole: every token sees every row (uniform)
-                const bool whole = here == ~0u && r0 + TT <= walk.ctx && (r0 >= walk.lo1 || r0 + TT <= sight.sinks);
-                f16x8 p_hi[CB], p_lo[CB];
 #pragma unroll
-                for (int cb = 0; cb < CB; ++cb) {
-                    float x[8];
+                for (int n = 0; n < VPF; ++n) v_frag(n);
+                __builtin_amdgcn_sched_barrier(0);
+                if (!(whole_bits >> (j & (PLAN - 1)) & 1)) {   // (uniform)
+                    int mine = t;
+                    asm volatile("" : "+v"(mine));   // (nor are the entries' addresses)
+                    const int lo = mine >= 0 ? s_lo[mine] : INT_MAX, r0 = walk.row0(j0 + j);
+                    const uint2 line = mine >= 0 ? s_line[mine] : make_uint2(0, 0);
+                    uint32_t see = low_bits(walk.ctx - r0) & (~low_bits(lo - r0) | low_bits(sight.sinks - r0));
+                    see = lo == INT_MAX ? 0u : see | (tree_bits(line, r0) & low_bits(walk.hi - r0));
+                    see = (see & s_here[j & (2 * PLAN - 1)]) >> (4 * g);
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) x[e] = s[cb][e >> 2][e & 3];
-                    if (!whole) {
-                        uint32_t see = low_bits(walk.ctx - r0) & (~low_bits(lo[cb] - r0) | low_bits(sight.sinks - r0));
-                        see = lo[cb] == INT_MAX ? 0u : here & (see | (tree_bits(line[cb], r0) & low_bits(walk.hi - r0)));
-                        see >>= 4 * g;
+                    for (int e = 0; e < 8; ++e)
+                        s[e >> 2][e & 3] = see & (1u << (16 * (e >> 2) + (e & 3))) ? s[e >> 2][e & 3] : -INFINITY;
+                }
+                f32x8 p;
+                float sum;
+                auto weights = [&] {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) x[e] = see & (1u << (16 * (e >> 2) + (e & 3))) ? x[e] : -INFINITY;
-                    }
-                    float mt = x[0];
+                    for (int e = 0; e < 8; ++e) p[e] = fast_exp2(fmaf(s[e >> 2][e & 3], sl2, -m_run));
+                    sum = ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+                };
+                weights();
+                // A sum past 2^P_TOP: a score may be that far above the column's reference. On a piece's first
+                // tile, rarely after, so the maximum is looked for only then.
+                if (__any(sum > 32768.f)) {
+                    float mt = s[0][0];
 #pragma unroll
-                    for (int e = 1; e < 8; ++e) mt = __builtin_elementwise_maximum(mt, x[e]);
+                    for (int e = 1; e < 8; ++e) mt = __builtin_elementwise_maximum(mt, s[e >> 2][e & 3]);
                     mt *= sl2;
-                    if (__any(mt > m_run[cb] + P_TOP)) {
-                        mt = fmaxf(mt, lane_xor(mt, 16));
-                        mt = pair32_max(mt);
-                        const float m_new = mt > m_run[cb] + P_TOP ? mt - P_BELOW : m_run[cb];
-                        const float corr = fast_exp2(m_run[cb] - m_new);
-                        m_run[cb] = m_new;
-                        l_run[cb] *= corr;
-#pragma unroll
-                        for (int n = 0; n < 16; ++n) o[cb][n] *= corr;
-                    }
-                    f32x8 p;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        p[e] = fast_exp2(fmaf(x[e], sl2, -m_run[cb]));
-                        l_run[cb] += p[e];
-                    }
-                    p_hi[cb] = __builtin_convertvector(p, f16x8);
-                    if (Q8) p_lo[cb] = __builtin_convertvector(p - __builtin_convertvector(p_hi[cb], f32x8), f16x8);
+                    mt = fmaxf(mt, lane_xor(mt, 16));
+                    mt = pair32_max(mt);
+                    const float m_new = mt > m_run + P_TOP ? mt - P_BELOW : m_run;
+                    const float corr = fast_exp2(m_run - m_new);
+                    m_run = m_new;
+                    l_run *= corr;
+                    acc_scale(o, corr);
+                    weights();
                 }
+                l_run += sum;
+                const f16x8 p_hi = __builtin_convertvector(p, f16x8);
+                f16x8 p_lo;
+                if (Q8) p_lo = __builtin_convertvector(p - __builtin_convertvector(p_hi, f32x8), f16x8);
 #pragma unroll
                 for (int n = 0; n < 16; ++n) {
-                    const char* at = vt + (voff ^ (32 * n));
-                    const f16x4 va = __builtin_bit_cast(f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)at));
-                    const f16x4 vc = __builtin_bit_cast(
-                        f16x4, __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s16x4*)(at + 16 * ROW_B)));
+                    const f16x4 va = __builtin_bit_cast(f16x4, vf[n % VPF][0]);
+                    const f16x4 vc = __builtin_bit_cast(f16x4, vf[n % VPF][1]);
                     const f16x8 a = {va[0], va[1], va[2], va[3], vc[0], vc[1], vc[2], vc[3]};
-#pragma unroll
-                    for (int cb = 0; cb < CB; ++cb) {
-                        o[cb][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p_hi[cb], o[cb][n], 0, 0, 0);
-                        if (Q8) o[cb][n] = __builtin_amdgcn_mfma_f32_16x16x32_f16(a, p_lo[cb], o[cb][n], 0, 0, 0);
-                    }
+                    acc_mfma(o[n], a, p_hi);
+                    if (Q8) acc_mfma(o[n], a, p_lo);
+                    if (n + VPF < 16) v_frag(n + VPF);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
             };
             const int n_tiles = j1 - j0;
-            auto pages_here = [](int id0, int id1) { return (id0 < 0 ? 0u : 0xFFFFu) | (id1 < 0 ? 0u : 0xFFFF0000u); };
-            // the pool row of this wave's first row of a tile (of an absent page: page 0's)
-            auto pool_row = [&](int r0, int id0, int id1) {
-                const int id = w >> 1 ? id1 : id0;
-                return ((long long)max(id, 0) << pg.shift) + ((r0 + 8 * w) & ((1 << pg.shift) - 1));
+            // a copying wave's entry of the tile that it copies next: its first row in the pool, and those of the
+            // tile's rows that some token sees
+            int e_row = 0;
+            uint32_t e_seen = 0;
+            auto look = [&](int j) {
+                if (w >= CW) return;
+                const int at = min(j, n_tiles - 1) & (2 * PLAN - 1);
+                e_row = ROWS * w >= 16 ? s_rows[at].y : s_rows[at].x;
+                e_seen = s_seen[at];
+            };
+            auto pool_row = [&] { return (long long)uni(e_row) + (ROWS * w & 15); };
+            // between two tiles: the plan of the next 64
+            auto ahead = [&](int j) {
+                if (w == 0 && (j & (PLAN - 1)) == 0 && j + PLAN < n_tiles) plan(j / PLAN + 1, ids_of(j / PLAN + 1));
             };
             if constexpr (!Q8) {
-                uint32_t loff[4];
+                uint32_t loff[ROWS / 2];
 #pragma unroll
-                for (int n = 0; n < 4; ++n) {
+                for (int n = 0; n < ROWS / 2; ++n) {
                     const int r = 2 * n + (lane >> 5);
-                    loff[n] = r * rsb + 16 * ((lane & 31) ^ sw(8 * w + r));
+                    loff[n] = r * rsb + 16 * ((lane & 31) ^ sw(ROWS * w + r));
                 }
-                auto issue = [&](int stage, int j, uint32_t& here) {
-                    int id0, id1;
-                    ids.at(j, id0, id1);
-                    const int r0 = walk.row0(j);
-                    here = pages_here(id0, id1);
-                    const long long at = pool_row(r0, id0, id1) * rsb;
+                auto issue = [&](int j) {   // tile j0 + j, whose entry look() fetched
+                    if (w >= CW) return;
+                    const long long at = pool_row() * rsb;
                     const char *kr = uniform_ptr(kb + at), *vr = uniform_ptr(vb + at);
-                    const uint32_t d0 = uni(lds + stage * STAGE_B + 8 * w * ROW_B);
+                    const uint32_t d0 = uni(lds + (j & 3) * STAGE_B + ROWS * w * ROW_B);
                     // rows that no token sees may hold anything, and 0 x NaN is a NaN: zeros
-                    const uint32_t on = (seen_rows(r0) & here) >> (8 * w) & 0xFF;
-                    if (on == 0xFF) {
+                    const uint32_t on = (uint32_t)uni((int)e_seen) >> (ROWS * w);
+                    look(j + 1);
+                    if ((on & ((1u << ROWS) - 1)) == (1u << ROWS) - 1) {
 #pragma unroll
-                        for (int n = 0; n < 4; ++n) copy16(kr, loff[n], d0 + 2 * n * ROW_B);
+                        for (int n = 0; n < ROWS / 2; ++n) copy16(kr, loff[n], d0 + 2 * n * ROW_B);
 #pragma unroll
-                        for (int n = 0; n < 4; ++n) copy16(vr, loff[n], d0 + TILE_B + 2 * n * ROW_B);
+                        for (int n = 0; n < ROWS / 2; ++n) copy16(vr, loff[n], d0 + TILE_B + 2 * n * ROW_B);
                     } else {
                         const char* zero = (const char*)zero_row + 16 * (lane & 31);
 #pragma unroll
-                        for (int n = 0; n < 4; ++n) {
+                        for (int n = 0; n < ROWS / 2; ++n) {
                             const bool ok = on >> (2 * n + (lane >> 5)) & 1;
                             copy16_v(ok ? kr + loff[n] : zero, d0 + 2 * n * ROW_B);
                             copy16_v(ok ? vr + loff[n] : zero, d0 + TILE_B + 2 * n * ROW_B);
                         }
                     }
                 };
-                uint32_t here[STAGES_F16] = {};
-#pragma unroll
-                for (int d = 0; d < AHEAD; ++d)
-                    if (d < n_tiles) issue(d, j0 + d, here[d]);
-                int st = 0;
+                look(0);
+#pragma unroll 1
+                for (int d = 0; d < min(AHEAD, n_tiles); ++d) issue(d);
+                begin();
                 for (int j = 0; j < n_tiles; ++j) {
                     // tile j landed; those issued after it may still be in flight
                     const int later = min(AHEAD - 1, n_tiles - 1 - j);
@@ -397,100 +506,111 @@ tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict
                     else if (later == 1) WAIT_VMCNT(COPIES);
                     else WAIT_VMCNT(0);
                     tile_done();   // every wave is past tile j - 1: its stage can be refilled
-                    const uint32_t now = here[0];
-                    here[0] = here[1], here[1] = here[2];
-                    if (j + AHEAD < n_tiles) issue(st == 0 ? STAGES_F16 - 1 : st - 1, j0 + j + AHEAD, here[2]);
-                    tile(st, walk.row0(j0 + j), now);
-                    st = st == STAGES_F16 - 1 ? 0 : st + 1;
+                    if (j + AHEAD < n_tiles) issue(j + AHEAD);
+                    ahead(j);
+                    tile(j & 3, j);
                 }
             } else {
-                const uint32_t xo = g * rsb + 16 * col, so = (g * rsb >> 4) + (col & ~1);
-                auto load = [&](Bytes& x, int j, uint32_t& here) {
-                    int id0, id1;
-                    ids.at(j, id0, id1);
-                    here = pages_here(id0, id1);
-                    const long long at = pool_row(walk.row0(j), id0, id1);
-                    const gptr k0 = uni_global(kb + at * rsb), v0 = uni_global(vb + at * rsb);
-                    const gptr k1 = uni_global(kp + values + (at * n_kv + h) * 16), v1 = uni_global(vp + values + (at * n_kv + h) * 16);
+                const uint32_t raw0 = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)s_raw) + w * RAW_WAVE;
+                auto issue = [&](int j) {   // tile j0 + j, whose entry look() fetched
+                    if (w >= CW) return;
+                    const long long at = pool_row();
+                    look(j + 1);
+                    int l = lane;
+                    asm volatile("" : "+v"(l));   // (what follows is not worth registers across tiles)
+                    const uint32_t xo = (l >> 4) * rsb + 16 * (l & 15);
+                    // scales: a row's on 4 lanes, K's rows on the first 4 ROWS lanes, V's on the next
+                    const uint32_t so = ((l >> 2) & (ROWS - 1)) * (rsb >> 4) + 4 * (l & 3);
+                    const char *kr = uniform_ptr(kb + at * rsb), *vr = uniform_ptr(vb + at * rsb);
+                    const uint32_t d0 = uni(raw0 + (j % RAW_STAGES) * (CW * RAW_WAVE));
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        x.k[n] = load_g<u32x4>(k0, xo + 4 * n * rsb);
-                        x.v[n] = load_g<u32x4>(v0, xo + 4 * n * rsb);
-                        x.ks[n] = load_g<f16>(k1, so + 4 * n * (rsb >> 4));
-                        x.vs[n] = load_g<f16>(v1, so + 4 * n * (rsb >> 4));
+                    for (int n = 0; n < ROWS / 4; ++n) {
+                        copy16(kr, xo + 4 * n * rsb, d0 + 4 * n * PAGED_HD);
+                        copy16(vr, xo + 4 * n * rsb, d0 + (ROWS + 4 * n) * PAGED_HD);
                     }
+                    const char* scales = ((l & (4 * ROWS)) == 0 ? kp : vp) + values + (at * n_kv + h) * 16;
+                    if (lane < 8 * ROWS) copy4_v(scales + so, d0 + 2 * ROWS * PAGED_HD);
                 };
-                auto put = [&](const Bytes& x, int stage, int r0, uint32_t here) {
-                    const uint32_t on = seen_rows(r0) & here;
+                auto convert = [&](int j) {   // this wave's rows of tile j0 + j to its stage
+                    if (w >= CW) return;
+                    const char* raw = s_raw + (j % RAW_STAGES) * (CW * RAW_WAVE) + w * RAW_WAVE;
+                    const uint32_t on = s_seen[j & (2 * PLAN - 1)];
+                    const int stage = j & 1;
+                    int l = lane;
+                    asm volatile("" : "+v"(l));   // (as in issue)
+                    const int g = l >> 4, col = l & 15;
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        const int r = 8 * w + 4 * n + g;
+                    for (int n = 0; n < ROWS / 4; ++n) {
+                        const f16* sc = (const f16*)(raw + 2 * ROWS * PAGED_HD) + 8 * (4 * n + g) + (col >> 1);
+                        const u32x4 kx = *(const u32x4*)(raw + 1024 * n + 16 * l);
+                        const u32x4 vx = *(const u32x4*)(raw + ROWS * PAGED_HD + 1024 * n + 16 * l);
+                        const f16 ks = sc[0], vs = sc[8 * ROWS];
+                        const int r = ROWS * w + 4 * n + g;
                         // rows that no token sees may hold any scale: theirs is 0
-                        const bool ok = on >> r & 1;
-                        const f16 vs = ok ? x.vs[n] : (f16)0.f;
+                        const f16 v = on >> r & 1 ? vs : (f16)0.f;
                         char* at = s_tile + stage * STAGE_B + r * ROW_B;
-                        const int c0 = 16 * ((2 * col) ^ sw(r)), c1 = 16 * ((2 * col + 1) ^ sw(r));
-                        *(f16x8*)(at + c0) = bytes_as_ints(x.k[n].x, x.k[n].y);
-                        *(f16x8*)(at + c1) = bytes_as_ints(x.k[n].z, x.k[n].w);
-                        const f16x4 a = q8_deq4(x.v[n].x, (f16x2){vs, vs}), c = q8_deq4(x.v[n].y, (f16x2){vs, vs});
-                        const f16x4 e = q8_deq4(x.v[n].z, (f16x2){vs, vs}), f = q8_deq4(x.v[n].w, (f16x2){vs, vs});
-                        *(f16x8*)(at + TILE_B + c0) = (f16x8){a[0], a[1], a[2], a[3], c[0], c[1], c[2], c[3]};
-                        *(f16x8*)(at + TILE_B + c1) = (f16x8){e[0], e[1], e[2], e[3], f[0], f[1], f[2], f[3]};
-                        if ((col & 1) == 0) s_step[stage][col >> 1][r] = (float)x.ks[n];
+                        const int a0 = 16 * ((2 * col) ^ sw(r)), a1 = 16 * ((2 * col + 1) ^ sw(r));
+                        auto values8 = [&](uint32_t x, uint32_t y) {
+                            const f16x4 a = q8_deq4(x, (f16x2){v, v}), c = q8_deq4(y, (f16x2){v, v});
+                            return (f16x8){a[0], a[1], a[2], a[3], c[0], c[1], c[2], c[3]};
+                        };
+                        *(f16x8*)(at + a0) = bytes_as_ints(kx.x, kx.y);
+                        *(f16x8*)(at + a1) = bytes_as_ints(kx.z, kx.w);
+                        *(f16x8*)(at + TILE_B + a0) = values8(vx.x, vx.y);
+                        *(f16x8*)(at + TILE_B + a1) = values8(vx.z, vx.w);
+                        if ((col & 1) == 0) s_step[stage][col >> 1][r] = (float)ks;
                     }
                 };
-                Bytes x[2];
-                uint32_t here[2];
-                load(x[0], j0, here[0]);
-                put(x[0], 0, walk.row0(j0), here[0]);
-                uint32_t now = here[0];
-                load(x[0], min(j0 + 1, j1 - 1), here[0]);
-                load(x[1], min(j0 + 2, j1 - 1), here[1]);
-                __syncthreads();
-                auto body = [&](int j, int buf) {
-                    tile(j & 1, walk.row0(j0 + j), now);
-                    if (j + 1 < n_tiles) {
-                        put(x[buf], (j + 1) & 1, walk.row0(j0 + j + 1), here[buf]);
-                        now = here[buf];
-                        load(x[buf], min(j0 + j + 3, j1 - 1), here[buf]);
-                    }
+                look(0);
+#pragma unroll 1
+                for (int d = 0; d < min(RAW_AHEAD, n_tiles); ++d) issue(d);
+                begin();
+                asm volatile("" ::: "memory");
+                convert(0);
+                for (int j = 0; j < n_tiles; ++j) {
+                    // stage j % 2 is written, and the other one done with
                     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-                };
-                for (int j = 0; j < n_tiles; j += 2) {
-                    body(j, 0);
-                    if (j + 1 < n_tiles) body(j + 1, 1);
+                    if (j + RAW_AHEAD < n_tiles) issue(j + RAW_AHEAD);
+                    ahead(j);
+                    tile(j & 1, j);
+                    if (j + 1 < n_tiles) {
+                        const int later = min(RAW_AHEAD - 1, n_tiles - 2 - j);   // tiles issued after j + 1
+                        if (later == 2) WAIT_VMCNT(2 * COPIES);
+                        else if (later == 1) WAIT_VMCNT(COPIES);
+                        else WAIT_VMCNT(0);
+                        asm volatile("" ::: "memory");
+                        convert(j + 1);
+                    }
                 }
             }
             if (busy) {
-#pragma unroll
-                for (int cb = 0; cb < CB; ++cb) {
-                    float l = l_run[cb];
-                    l += lane_xor(l, 16);
-                    l = pair32_sum(l);
-                    if (t[cb] < 0) continue;
-                    if (lo[cb] == INT_MAX) l = 0.f;   // (a place without a token, in tiles that all others see)
-                    const int r = (grp * W + w) * 16 * CB + 16 * cb + col;
+                acc_settle(o);
+                float l = l_run;
+                l += lane_xor(l, 16);
+                l = pair32_sum(l);
+                if (t >= 0) {
+                    if (s_lo[t] == INT_MAX) l = 0.f;   // (a place without a token, in tiles that all others see)
                     if (!whole_seq) {
-                        const size_t part = ((size_t)slot * n_kv + h) * R + r;
+                        const size_t part = ((size_t)slot * n_kv + h) * R + r_mine;
                         float* dst = parts.pacc + part * PAGED_HD + 4 * g;
 #pragma unroll
-                        for (int n = 0; n < 16; ++n) *(f32x4*)(dst + 16 * n) = o[cb][n];
-                        if (g == 0) parts.pm[part] = m_run[cb], parts.pd[part] = l;
-                        continue;
-                    }
-                    const size_t rh = (size_t)b * T * n_q + qrow[cb];
-                    const f16* gate = qg + rh * q_pitch + PAGED_HD + 4 * g;
-                    const float inv = 1.f / l;
+                        for (int n = 0; n < 16; ++n) *(f32x4*)(dst + 16 * n) = o[n];
+                        if (g == 0) parts.pm[part] = m_run, parts.pd[part] = l;
+                    } else {
+                        const size_t rh = (size_t)b * T * n_q + qrow;
+                        const f16* gate = qg + rh * q_pitch + PAGED_HD + 4 * g;
+                        const float inv = 1.f / l;
 #pragma unroll
-                    for (int n = 0; n < 16; ++n) {
-                        f32x4 v = o[cb][n] * inv;
-                        if (gated) {
-                            const f16x4 gv = *(const f16x4*)(gate + 16 * n);
+                        for (int n = 0; n < 16; ++n) {
+                            f32x4 v = o[n] * inv;
+                            if (gated) {
+                                const f16x4 gv = *(const f16x4*)(gate + 16 * n);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) v[e] *= fast_sigmoid((float)gv[e]);
+                                for (int e = 0; e < 4; ++e) v[e] *= fast_sigmoid((float)gv[e]);
+                            }
+                            // (no row seen: 0, whatever the gate holds)
+                            *(f16x4*)(z + rh * z_pitch + 16 * n + 4 * g) = l == 0.f ? (f16x4)(0) : f16_sat4(v);
                         }
-                        // (no row seen: 0, whatever the gate holds)
-                        *(f16x4*)(z + rh * z_pitch + 16 * n + 4 * g) = l == 0.f ? (f16x4)(0) : f16_sat4(v);
                     }
                 }
             }
@@ -565,15 +685,15 @@ tree_merge_kernel(const Parts in, f16* __restrict__ z, int z_pitch, const f16* _
     *(f16x4*)out = v;
 }
 
-// How a call is cut: groups of 64 CB columns, runs a kv head and group.
+// How a call is cut: groups of 16 `waves` columns, runs a kv head and group.
 struct TreeCut {
-    int cb, groups, runs, run_min;
+    int waves, groups, runs, run_min;
 };
 TreeCut tree_cut(int T, int n_q, int n_kv) {
     const int R = T * (n_q / n_kv);
     TreeCut c;
-    c.groups = (R + 64 * MAX_CB - 1) / (64 * MAX_CB);
-    c.cb = ((R + c.groups - 1) / c.groups + 63) / 64;
+    c.waves = R <= 64 ? 4 : R <= 128 ? 8 : 12;
+    c.groups = (R + 16 * c.waves - 1) / (16 * c.waves);
     c.runs = std::max(1, cu_count() / (n_kv * c.groups));
     c.run_min = RUN_MIN;
     return c;
@@ -621,9 +741,10 @@ int fl_attn_tree_paged(const void* qg, int q_pitch, const void* kpool, const voi
         return FL_ESCRATCH;
     }
     FL_REQUIRE(aligned16(work), "16-byte aligned work");
-    auto kernel = cut.cb == 1 ? (q8 ? tree_attn_kernel<1, true> : tree_attn_kernel<1, false>)
-                              : (q8 ? tree_attn_kernel<2, true> : tree_attn_kernel<2, false>);
-    hipLaunchKernelGGL(kernel, dim3(cut.runs * n_kv_heads * cut.groups), dim3(64 * W), 0, (hipStream_t)stream,
+    auto kernel = cut.waves == 4 ? (q8 ? tree_attn_kernel<4, true> : tree_attn_kernel<4, false>)
+                  : cut.waves == 8 ? (q8 ? tree_attn_kernel<8, true> : tree_attn_kernel<8, false>)
+                                   : (q8 ? tree_attn_kernel<12, true> : tree_attn_kernel<12, false>);
+    hipLaunchKernelGGL(kernel, dim3(cut.runs * n_kv_heads * cut.groups), dim3(64 * cut.waves), 0, (hipStream_t)stream,
                        (const f16*)qg, q_pitch, (const char*)kpool, (const char*)vpool, pg, pos0, parents, B, T,
                        n_q_heads, n_kv_heads, cut.groups, cut.runs, cut.run_min, scale * FL_LOG2E,
                        Sight{window, sinks}, (f16*)z, z_pitch, gated, parts);
