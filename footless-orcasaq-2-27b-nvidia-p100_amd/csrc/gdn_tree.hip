@@ -27,11 +27,14 @@
 
 namespace {
 
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+
 constexpr int GT_K = 128;                // K = V
 constexpr int GT_WAVES = 8;
 constexpr int GT_THREADS = 64 * GT_WAVES;
-constexpr int ROW_P = GT_K + 4;          // floats a row of k, q, v in LDS
-constexpr int GT_SLOTS = GT_THREADS / 48;   // tokens whose conv is formed at a time, 8 channels a thread
+constexpr int ROW_P = GT_K + 4;          // floats a row of v and o in LDS
+constexpr int ROW_H = GT_K + 8;          // terms a row of k and q
+constexpr float QK_SCALE = 16384.f;      // of q and k, whose norms are at most 1
 constexpr int INV_P = 20;                // floats a row of an inverse block
 
 // Sum over the 16 lanes of a DPP row, on every one of them.
@@ -104,6 +107,22 @@ struct TreeSeqs {
     int pos0[FL_MAX_SEQS];
 };
 
+// x as two fp16 terms: 22 bits of it, and what lies 2^-24 below 1 (so x is scaled up first)
+__device__ __forceinline__ void split(f32x8 x, f16x8& hi, f16x8& lo) {
+    hi = __builtin_convertvector(x, f16x8);
+    lo = __builtin_convertvector(x - __builtin_convertvector(hi, f32x8), f16x8);
+}
+__device__ __forceinline__ int ilogb_bits(float x) { return (int)(__float_as_uint(x) >> 23 & 255) - 127; }
+__device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+struct Terms {
+    f16x8 hi, lo;
+};
+// c + a b without the product of the two low terms (2^-22 of a b)
+__device__ __forceinline__ f32x4 mfma_terms(const Terms& a, const Terms& b, f32x4 c) {
+    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.lo, b.hi, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.hi, b.lo, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.hi, b.hi, c, 0, 0, 0);
+}
 __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
@@ -117,13 +136,16 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
                 f16* __restrict__ y, int y_pitch, int T, int n_kheads, int n_vheads, float out_scale,
                 float l2eps, float norm_eps) {
     constexpr int TP = 16 * NB, MAT_P = TP + 4;
-    __shared__ __attribute__((aligned(16))) float s_q[TP][ROW_P], s_k[TP][ROW_P], s_v[TP][ROW_P];
+    // q and k (hi, lo each); v and then o take q's place
+    __shared__ __attribute__((aligned(16))) f16 s_q[2][TP][ROW_H], s_k[2][TP][ROW_H];
+    float(*s_v)[ROW_P] = (float(*)[ROW_P])s_q;
+    static_assert(sizeof(float) * TP * ROW_P <= sizeof(s_q), "v over q");
     __shared__ __attribute__((aligned(16))) float s_a[TP][MAT_P], s_p[TP][MAT_P];   // -A; the q.k side
     __shared__ __attribute__((aligned(16))) float s_inv[NB][16][INV_P];
     __shared__ double s_log[64];
     __shared__ uint2 s_line[64];
     __shared__ int4 s_up[64];            // the three tokens before it on its path (-1 -n: a frame), here
-    __shared__ float s_beta[64], s_gain[64], s_nq[TP], s_nk[TP];
+    __shared__ float s_beta[64], s_gain[64];
     __shared__ int s_n;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
@@ -136,17 +158,19 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
     }
     const int hk = hv / (n_vheads / n_kheads);
 
-    // S0: row 16 w + col, columns 16 c + 4 g .. + 3
-    f32x4 s0[8];
-    const float* srow = seqs.S[b] + ((size_t)hv * GT_K + 16 * w + col) * GT_K + 4 * g;
+    // S0: row 16 w + col, columns 32 c + 8 g .. + 7
+    f32x8 s0[4];
+    const float* srow = seqs.S[b] + ((size_t)hv * GT_K + 16 * w + col) * GT_K + 8 * g;
 #pragma unroll
-    for (int c = 0; c < 8; ++c) s0[c] = *(const f32x4*)(srow + 16 * c);
+    for (int c = 0; c < 4; ++c) s0[c] = *(const f32x8*)(srow + 32 * c);
 
-    // the conv's thread: 8 channels of q, k or v (a DPP row each), tokens slot, slot + GT_SLOTS, ...
-    const int slot = tid / 48, part = tid % 48 >> 4, ch8 = 8 * (tid & 15);
-    const int ch = (part == 0 ? hk : part == 1 ? n_kheads + hk : 2 * n_kheads + hv) * GT_K + ch8;
+    // the conv: a thread forms 8 channels of q or k, later of v, of tokens slot, slot + 16 (32), ...
+    const bool fresh = seqs.pos0[b] == 0;
+    const int part = tid >> 4 & 1, ch8 = 8 * (tid & 15);
+    const f16* xb = x + (size_t)b * T * x_stride;
+    const int ch_qk = (part == 0 ? hk : n_kheads + hk) * GT_K + ch8, ch_v = (2 * n_kheads + hv) * GT_K + ch8;
     Conv8 conv;
-    if (slot < GT_SLOTS) conv.load(conv_w, seqs.frames[b], seqs.pos0[b] == 0, ch);
+    conv.load(conv_w, seqs.frames[b], fresh, ch_qk);
 
     if (w == 0) {
         double sum = 0.;
@@ -174,50 +198,50 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
     __syncthreads();
     const int n = __builtin_amdgcn_readfirstlane(s_n), nb = (n + 15) >> 4;   // tokens, blocks of them
 
-    if (slot < GT_SLOTS)
-        for (int i = slot; i < n; i += GT_SLOTS) {
-            const int4 up = s_up[i];
-            const f16* xb = x + (size_t)b * T * x_stride + ch;
-            const f16x8 f0 = conv.f0, f1 = conv.f1, f2 = conv.f2;
-            const f16x8 x0 = *(const f16x8*)(xb + (size_t)i * x_stride);
-            const f16x8 x1 = token(-1 - up.x, xb + (size_t)max(up.x, 0) * x_stride, f0, f1, f2);
-            const f16x8 x2 = token(-1 - up.y, xb + (size_t)max(up.y, 0) * x_stride, f0, f1, f2);
-            const f16x8 x3 = token(-1 - up.z, xb + (size_t)max(up.z, 0) * x_stride, f0, f1, f2);
-            f32x4 lo, hi;
-            conv.apply(lo, hi, x3, x2, x1, x0);
-            float* dst = (part == 0 ? s_q[i] : part == 1 ? s_k[i] : s_v[i]) + ch8;
-            *(f32x4*)dst = lo;
-            *(f32x4*)(dst + 4) = hi;
-            if (part < 2) {   // 1 / |q|, 1 / |k|
-                const float ss = row16_sum(sum_sq(lo, hi));
-                if ((tid & 15) == 0) (part == 0 ? s_nq : s_nk)[i] = 1.f / sqrtf(ss + l2eps);
-            }
-        }
+    auto conv_of = [&](const Conv8& cv, int i, int ch, f32x4& lo, f32x4& hi) {
+        const int4 up = s_up[i];
+        const f16* at = xb + ch;
+        const f16x8 f0 = cv.f0, f1 = cv.f1, f2 = cv.f2;
+        const f16x8 x0 = *(const f16x8*)(at + (size_t)i * x_stride);
+        const f16x8 x1 = token(-1 - up.x, at + (size_t)max(up.x, 0) * x_stride, f0, f1, f2);
+        const f16x8 x2 = token(-1 - up.y, at + (size_t)max(up.y, 0) * x_stride, f0, f1, f2);
+        const f16x8 x3 = token(-1 - up.z, at + (size_t)max(up.z, 0) * x_stride, f0, f1, f2);
+        cv.apply(lo, hi, x3, x2, x1, x0);
+    };
+    for (int i = tid >> 5; i < n; i += GT_THREADS / 32) {
+        f32x4 lo, hi;
+        conv_of(conv, i, ch_qk, lo, hi);
+        const float inv = QK_SCALE / sqrtf(row16_sum(sum_sq(lo, hi)) + l2eps);
+        f16x8 h, l;
+        split(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7) * inv, h, l);
+        f16(*dst)[TP][ROW_H] = part == 0 ? s_q : s_k;
+        *(f16x8*)(dst[0][i] + ch8) = h;
+        *(f16x8*)(dst[1][i] + ch8) = l;
+    }
+    conv.load(conv_w, seqs.frames[b], fresh, ch_v);
     __syncthreads();
+    auto terms = [&](const f16 (*m)[TP][ROW_H], int row, int c) {
+        return Terms{*(const f16x8*)(m[0][row] + 32 * c + 8 * g), *(const f16x8*)(m[1][row] + 32 * c + 8 * g)};
+    };
 
     // -A and the q.k side, 16 x 16 blocks on and below the diagonal
     for (int job = w; job < nb * (nb + 1); job += GT_WAVES) {
         const bool qk = job & 1;
         int r = 0, c = job >> 1;
         while (c > r) c -= ++r;
-        const float *ra = (qk ? s_q : s_k)[16 * r + col] + 4 * g, *rb = s_k[16 * c + col] + 4 * g;
         f32x4 acc = (f32x4)(0.f);
 #pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            const f32x4 av = *(const f32x4*)(ra + 16 * s), bv = *(const f32x4*)(rb + 16 * s);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) acc = mfma4(av[e], bv[e], acc);
-        }
+        for (int s = 0; s < 4; ++s)
+            acc = mfma_terms(terms(qk ? s_q : s_k, 16 * r + col, s), terms(s_k, 16 * c + col, s), acc);
         const int j = 16 * c + col;
         const double lj = s_log[j];
-        const float nj = s_nk[j];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const int i = 16 * r + 4 * g + e;
             const uint2 line = s_line[i];
             const bool anc = ((j < 32 ? line.x : line.y) >> (j & 31) & 1) && (qk || j != i);
-            const float m = acc[e] * nj * ratio(s_log[i] - lj);
-            (qk ? s_p : s_a)[i][j] = anc ? m * (qk ? s_nq[i] : -s_beta[i] * s_nk[i]) : 0.f;
+            const float m = acc[e] * (1.f / (QK_SCALE * QK_SCALE)) * ratio(s_log[i] - lj);
+            (qk ? s_p : s_a)[i][j] = anc ? m * (qk ? 1.f : -s_beta[i]) : 0.f;
         }
     }
     __syncthreads();
@@ -236,23 +260,40 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
 #pragma unroll
             for (int i = 0; i < 16; ++i) s_inv[w][i][col] = xi[i];
     }
-    // S0 k_i and S0 q_i: row 16 r + 4 g + e, state row 16 w + col
+    // S0 k_i and S0 q_i: row 16 r + 4 g + e, state row 16 w + col. S0's terms are those of its rows with
+    // their largest entries brought to [2^14, 2^15).
+    float top = 0.f;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(s0[c][e]));
+    top = fmaxf(top, lane_xor(top, 16));
+    top = fmaxf(top, lane_xor(top, 32));
+    const int up = 14 - min(max(ilogb_bits(top), -100), 100);
+    Terms st[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) split(s0[c] * pow2(up), st[c].hi, st[c].lo);
+    const float down = pow2(-up) * (1.f / QK_SCALE);
     f32x4 wk[NB], wq[NB];
 #pragma unroll
     for (int r = 0; r < NB; ++r) {
         wk[r] = wq[r] = (f32x4)(0.f);
         if (r < nb) {
 #pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                const f32x4 kv = *(const f32x4*)(s_k[16 * r + col] + 16 * c + 4 * g);
-                const f32x4 qv = *(const f32x4*)(s_q[16 * r + col] + 16 * c + 4 * g);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    wk[r] = mfma4(kv[e], s0[c][e], wk[r]);
-                    wq[r] = mfma4(qv[e], s0[c][e], wq[r]);
-                }
+            for (int c = 0; c < 4; ++c) {
+                wk[r] = mfma_terms(terms(s_k, 16 * r + col, c), st[c], wk[r]);
+                wq[r] = mfma_terms(terms(s_q, 16 * r + col, c), st[c], wq[r]);
             }
+            wk[r] *= down;
+            wq[r] *= down;
         }
+    }
+    __syncthreads();
+    for (int i = tid >> 4; i < n; i += GT_THREADS / 16) {
+        f32x4 lo, hi;
+        conv_of(conv, i, ch_v, lo, hi);
+        *(f32x4*)(s_v[i] + ch8) = lo;
+        *(f32x4*)(s_v[i] + ch8 + 4) = hi;
     }
     __syncthreads();
 
@@ -268,8 +309,8 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
                 // (a place without a token adds nothing to others, whatever lies there)
                 const bool here = s_up[i].w;
                 const float gain = s_gain[i];
-                rhs[e] = here ? s_beta[i] * (s_v[i][16 * w + col] - gain * s_nk[i] * wk[r][e]) : 0.f;
-                o[e] = here ? gain * s_nq[i] * wq[r][e] : 0.f;
+                rhs[e] = here ? s_beta[i] * (s_v[i][16 * w + col] - gain * wk[r][e]) : 0.f;
+                o[e] = here ? gain * wq[r][e] : 0.f;
             }
 #pragma unroll
             for (int c = 0; c < NB; ++c)
