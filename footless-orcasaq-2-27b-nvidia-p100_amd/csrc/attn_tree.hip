@@ -289,8 +289,9 @@ tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict
         };
         if (w == 0) {
             double none = 0.;
+            const int parent = parents[(size_t)b * T + min(lane, T - 1)];
             const int2 ids = j1 > j0 ? ids_of(0) : make_int2(0, 0);
-            const Node node = tree_node(parents + (size_t)b * T, T, none);
+            const Node node = tree_node(parent, T, none);
             present = __ballot(node.here());
             // a path's tokens are numbered upwards: out of the window are its first ones, but those
             // that count as first rows of the sequence

@@ -30,12 +30,10 @@ namespace {
 typedef float f32x8 __attribute__((ext_vector_type(8)));
 
 constexpr int GT_K = 128;                // K = V
-constexpr int GT_WAVES = 8;
-constexpr int GT_THREADS = 64 * GT_WAVES;
-constexpr int ROW_P = GT_K + 4;          // floats a row of v and o in LDS
 constexpr int ROW_H = GT_K + 8;          // terms a row of k and q
 constexpr float QK_SCALE = 16384.f;      // of q and k, whose norms are at most 1
-constexpr int INV_P = 20;                // floats a row of an inverse block
+constexpr int GT_MANY = 256;             // heads from which a workgroup takes several
+constexpr int BLOCK_P = 20;              // floats a row of a 16 x 16 block
 
 // Sum over the 16 lanes of a DPP row, on every one of them.
 __device__ __forceinline__ float row16_sum(float v) {
@@ -53,38 +51,52 @@ __device__ __forceinline__ float log_decay(float a_dt, float A) {
     const float l = -hw_expf(A) * sp;
     return l < -1000.f ? -1000.f : l;
 }
-// e^x of a difference of such sums
-__device__ __forceinline__ float ratio(double x) { return fast_exp2((float)(x * 1.4426950408889634)); }
+// The product of the decays of which x is such a sum, or a difference of two, in log2 units
+__device__ __forceinline__ float decayed(double x) { return fast_exp2((float)x); }
 
-// Eight channels' conv: the taps and the sequence's last three frames ([channel][frame], oldest
-// first; zero for a fresh sequence).
-struct Conv8 {
-    f16x8 w0, w1, w2, w3;   // a tap of all channels each, the newest last
-    f16x8 f0, f1, f2;
-    __device__ __forceinline__ void load(const f16* conv_w, const f16* frames, bool fresh, int ch) {
-        const f16x8 *t = (const f16x8*)(conv_w + 4 * ch), *x = (const f16x8*)(frames + 3 * ch);
-        const f16x8 a = t[0], b = t[1], c = t[2], d = t[3], x0 = x[0], x1 = x[1], x2 = x[2];
+// Eight channels' conv: the taps, the newest last.
+struct Taps8 {
+    f16x8 w0, w1, w2, w3;   // a tap of all channels each
+    __device__ __forceinline__ void load(const f16* conv_w, int ch) {
+        const f16x8* t = (const f16x8*)(conv_w + 4 * ch);
+        const f16x8 a = t[0], b = t[1], c = t[2], d = t[3];
         w0 = (f16x8){a[0], a[4], b[0], b[4], c[0], c[4], d[0], d[4]};
         w1 = (f16x8){a[1], a[5], b[1], b[5], c[1], c[5], d[1], d[5]};
         w2 = (f16x8){a[2], a[6], b[2], b[6], c[2], c[6], d[2], d[6]};
         w3 = (f16x8){a[3], a[7], b[3], b[7], c[3], c[7], d[3], d[7]};
-        f0 = (f16x8){x0[0], x0[3], x0[6], x1[1], x1[4], x1[7], x2[2], x2[5]};
-        f1 = (f16x8){x0[1], x0[4], x0[7], x1[2], x1[5], x2[0], x2[3], x2[6]};
-        f2 = (f16x8){x0[2], x0[5], x1[0], x1[3], x1[6], x2[1], x2[4], x2[7]};
-        if (fresh) f0 = f1 = f2 = (f16x8)(0);
     }
     // silu of the taps over x0 (the token's) and the three before it
-    __device__ __forceinline__ float channel(int c, f16x8 x3, f16x8 x2, f16x8 x1, f16x8 x0) const {
-        float s = (float)w0[c] * (float)x3[c];
+    __device__ __forceinline__ float channel(int c, f16x8 x3, f16x8 x2, f16x8 x1, f16x8 x0, float zero) const {
+        float s = fmaf((float)w0[c], (float)x3[c], zero);
         s = fmaf((float)w1[c], (float)x2[c], s);
         s = fmaf((float)w2[c], (float)x1[c], s);
         s = fmaf((float)w3[c], (float)x0[c], s);
         return s * __builtin_amdgcn_rcpf(1.f + hw_expf(-s));
     }
     __device__ __forceinline__ void apply(f32x4& lo, f32x4& hi, f16x8 x3, f16x8 x2, f16x8 x1, f16x8 x0) const {
-        auto y = [&](int c) { return channel(c, x3, x2, x1, x0); };
+        float zero = 0.f;
+        asm("" : "+v"(zero));   // (a mixed fma takes both halves as they are, a product would convert them)
+        auto y = [&](int c) { return channel(c, x3, x2, x1, x0, zero); };
         lo = (f32x4){y(0), y(1), y(2), y(3)};
         hi = (f32x4){y(4), y(5), y(6), y(7)};
+    }
+};
+// The sequence's last three frames ([channel][frame], oldest first; zero for a fresh sequence).
+struct Frames8 {
+    f16x8 f0, f1, f2;
+    __device__ __forceinline__ void load(const f16* frames, bool fresh, int ch) {
+        const f16x8* x = (const f16x8*)(frames + 3 * ch);
+        const f16x8 x0 = x[0], x1 = x[1], x2 = x[2];
+        f0 = (f16x8){x0[0], x0[3], x0[6], x1[1], x1[4], x1[7], x2[2], x2[5]};
+        f1 = (f16x8){x0[1], x0[4], x0[7], x1[2], x1[5], x2[0], x2[3], x2[6]};
+        f2 = (f16x8){x0[2], x0[5], x1[0], x1[3], x1[6], x2[1], x2[4], x2[7]};
+        if (fresh) f0 = f1 = f2 = (f16x8)(0);
+    }
+};
+struct Conv8 : Taps8, Frames8 {
+    __device__ __forceinline__ void load(const f16* conv_w, const f16* frames, bool fresh, int ch) {
+        Taps8::load(conv_w, ch);
+        Frames8::load(frames, fresh, ch);
     }
 };
 // The row at `row`, or the frame n > 0 tokens ahead of a path's first: n = 1 is the newest. (By
@@ -107,9 +119,13 @@ struct TreeSeqs {
     int pos0[FL_MAX_SEQS];
 };
 
-// x as two fp16 terms: 22 bits of it, and what lies 2^-24 below 1 (so x is scaled up first)
+// x as two fp16 terms: 21 bits of it, and what lies 2^-24 below 1 (so x is scaled up first)
 __device__ __forceinline__ void split(f32x8 x, f16x8& hi, f16x8& lo) {
-    hi = __builtin_convertvector(x, f16x8);
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {   // (cut off: the rest is lo's)
+        const auto p = __builtin_amdgcn_cvt_pkrtz(x[e], x[e + 1]);
+        hi[e] = p[0], hi[e + 1] = p[1];
+    }
     lo = __builtin_convertvector(x - __builtin_convertvector(hi, f32x8), f16x8);
 }
 __device__ __forceinline__ int ilogb_bits(float x) { return (int)(__float_as_uint(x) >> 23 & 255) - 127; }
@@ -117,115 +133,222 @@ __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)
 struct Terms {
     f16x8 hi, lo;
 };
-// c + a b without the product of the two low terms (2^-22 of a b)
+// The exponent that brings the largest of a column's entries to [2^14, 2^15): the four lanes of a column
+// have some each, the largest of which is `top`.
+__device__ __forceinline__ int lift(float top) {
+    top = fmaxf(top, lane_xor(top, 16));
+    top = pair32_max(top);
+    return 14 - min(max(ilogb_bits(top), -100), 100);
+}
+struct Terms4 {
+    f16x4 hi, lo;
+};
+__device__ __forceinline__ Terms4 split4(f32x4 x) {
+    const f16x4 hi = __builtin_convertvector(x, f16x4);
+    return {hi, __builtin_convertvector(x - __builtin_convertvector(hi, f32x4), f16x4)};
+}
+__device__ __forceinline__ f32x4 mfma_terms4(const Terms4& a, const Terms4& b, f32x4 c) {
+    c = __builtin_amdgcn_mfma_f32_16x16x16f16(a.lo, b.hi, c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x16f16(a.hi, b.lo, c, 0, 0, 0);
+    return __builtin_amdgcn_mfma_f32_16x16x16f16(a.hi, b.hi, c, 0, 0, 0);
+}
+// c + a b without the product of the two low terms (2^-21 of a b)
 __device__ __forceinline__ f32x4 mfma_terms(const Terms& a, const Terms& b, f32x4 c) {
     c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.lo, b.hi, c, 0, 0, 0);
     c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.hi, b.lo, c, 0, 0, 0);
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a.hi, b.hi, c, 0, 0, 0);
 }
-__device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+// What a wave wrote to LDS for itself, in another order.
+__device__ __forceinline__ void wave_sync() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
-template <int NB>
-__global__ void __launch_bounds__(GT_THREADS)
+// A number of at most 1 (as all of A, its inverses and the q.k side are) in a row of 16 high and 16 low terms.
+__device__ __forceinline__ void put_term(float* row, int at, float a) {
+    const float x = a * QK_SCALE;
+    const f16 hi = (f16)x;
+    ((f16*)row)[at] = hi;
+    ((f16*)row)[16 + at] = (f16)(x - (float)hi);
+}
+
+// NB blocks of 16 tokens, HP v heads of one k head, TL tiles of 16 state rows a wave.
+template <int NB, int HP, int TL>
+__global__ void __launch_bounds__(512 * HP / TL)
 gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__ conv_w, const TreeSeqs seqs,
                 const int* __restrict__ parents, const float* __restrict__ ga, const float* __restrict__ gb,
                 int ab_stride, const float* __restrict__ A_log, const float* __restrict__ dt_bias,
                 const f16* __restrict__ z, int z_pitch, const float* __restrict__ norm_w,
                 f16* __restrict__ y, int y_pitch, int T, int n_kheads, int n_vheads, float out_scale,
                 float l2eps, float norm_eps) {
-    constexpr int TP = 16 * NB, MAT_P = TP + 4;
-    // q and k (hi, lo each); v and then o take q's place
-    __shared__ __attribute__((aligned(16))) f16 s_q[2][TP][ROW_H], s_k[2][TP][ROW_H];
-    float(*s_v)[ROW_P] = (float(*)[ROW_P])s_q;
-    static_assert(sizeof(float) * TP * ROW_P <= sizeof(s_q), "v over q");
-    __shared__ __attribute__((aligned(16))) float s_a[TP][MAT_P], s_p[TP][MAT_P];   // -A; the q.k side
-    __shared__ __attribute__((aligned(16))) float s_inv[NB][16][INV_P];
-    __shared__ double s_log[64];
+    constexpr int HW = 8 / TL, WAVES = HP * HW, THREADS = 64 * WAVES;   // a head's waves
+    constexpr int TP = 16 * NB, BLOCKS = NB * (NB + 1) / 2;
+    constexpr int COLS = 16 * TL;                       // a wave's state rows
+    constexpr int LT = 64 / (2 * TL), VR = (TP + LT - 1) / LT;   // its tokens at a time, 8 columns a lane
+    constexpr int QT = THREADS / 32, QR = (TP + QT - 1) / QT;    // all waves' tokens of q and k at a time
+    constexpr int RAW_P = COLS + 8, OUT_P = COLS + 4, OUT_ROWS = LT < TP ? LT : TP;
+    constexpr int OWN_B = 4 * OUT_ROWS * OUT_P > 2 * (TP + 3) * RAW_P ? 4 * OUT_ROWS * OUT_P : 2 * (TP + 3) * RAW_P;
+    typedef f16 Rows[TP][ROW_H];
+    // (of a row 16 high and 16 low terms; transposed and in fp32 while it waits to be inverted)
+    typedef float Block[16][BLOCK_P];
+    constexpr int MATS_B = 2 * HP * BLOCKS * sizeof(Block);
+    constexpr int RAW_ROWS = TP + 3, RAW_B = 2 * RAW_ROWS * ROW_H * sizeof(f16);
+    __shared__ __attribute__((aligned(16))) Rows s_q[2], s_k[2];   // hi, lo
+    // q's and k's input rows behind three frames, then the heads' -A (inverses of I + A on the diagonal)
+    // and q.k sides
+    __shared__ __attribute__((aligned(16))) char s_mats[MATS_B > RAW_B ? MATS_B : RAW_B];
+    // a wave's own: its columns' frames and input rows, later v and o on the way between two layouts
+    __shared__ __attribute__((aligned(16))) char s_own[WAVES][OWN_B];
+    __shared__ __attribute__((aligned(16))) float s_ss[HP][TP][HW];
+    __shared__ double s_log[HP][64];
+    __shared__ __attribute__((aligned(16))) float s_beta[HP][64], s_gain[HP][64];
     __shared__ uint2 s_line[64];
-    __shared__ int4 s_up[64];            // the three tokens before it on its path (-1 -n: a frame), here
-    __shared__ float s_beta[64], s_gain[64];
+    __shared__ int4 s_up[64];            // the rows of the three tokens before it on its path; here
     __shared__ int s_n;
+    auto s_raw = (f16(*)[RAW_ROWS][ROW_H])s_mats;
+    auto s_a = (Block(*)[BLOCKS])s_mats, s_p = s_a + HP;
     const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 15, g = lane >> 4;
-    // Workgroups go to the 8 XCDs round-robin: a k head's v heads to one of them.
-    int hv = blockIdx.x % n_vheads, b = blockIdx.x / n_vheads;
-    if (n_vheads % 8 == 0) {
-        const int per = n_vheads / 8, r = blockIdx.x >> 3;
-        hv = (blockIdx.x & 7) * per + r % per;
+    // Workgroups go to the 8 XCDs round-robin: neighbouring heads to one of them.
+    const int group = n_vheads / n_kheads, units = n_vheads / HP;
+    int unit = blockIdx.x % units, b = blockIdx.x / units;
+    if (units % 8 == 0) {
+        const int per = units / 8, r = blockIdx.x >> 3;
+        unit = (blockIdx.x & 7) * per + r % per;
         b = r / per;
     }
-    const int hk = hv / (n_vheads / n_kheads);
-
-    // S0: row 16 w + col, columns 32 c + 8 g .. + 7
-    f32x8 s0[4];
-    const float* srow = seqs.S[b] + ((size_t)hv * GT_K + 16 * w + col) * GT_K + 8 * g;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) s0[c] = *(const f32x8*)(srow + 32 * c);
-
-    // the conv: a thread forms 8 channels of q or k, later of v, of tokens slot, slot + 16 (32), ...
+    const int h = w / HW, hv = unit * HP + h, hk = unit * HP / group;   // the wave's head
+    const int c0 = (w - h * HW) * COLS;                                 // and first state row
     const bool fresh = seqs.pos0[b] == 0;
-    const int part = tid >> 4 & 1, ch8 = 8 * (tid & 15);
-    const f16* xb = x + (size_t)b * T * x_stride;
-    const int ch_qk = (part == 0 ? hk : n_kheads + hk) * GT_K + ch8, ch_v = (2 * n_kheads + hv) * GT_K + ch8;
-    Conv8 conv;
-    conv.load(conv_w, seqs.frames[b], fresh, ch_qk);
 
-    if (w == 0) {
-        double sum = 0.;
-        float beta = 0.f;
-        if (lane < T) {
-            const size_t at = ((size_t)b * T + lane) * ab_stride + hv;
-            sum = (double)log_decay(ga[at] + dt_bias[hv], A_log[hv]);
-            beta = gdn_beta(gb[at]);
+    // Asked for first: what the tokens' conv needs. S0, which takes longest, follows once that is here.
+    const int head = unit * HP + (w < HP ? w : 0), token0 = min(lane, T - 1);   // (the gates of head w)
+    const size_t at_ab = ((size_t)b * T + token0) * ab_stride + head;
+    const int parent = parents[(size_t)b * T + token0];
+    const float a_in = ga[at_ab], b_in = gb[at_ab], dt = dt_bias[head], A = A_log[head];
+    const f16* xb = x + (size_t)b * T * x_stride;
+    const int part = tid >> 4 & 1, ch8 = 8 * (tid & 15), v8 = 8 * (lane & (2 * TL - 1));
+    const int ch_qk = (part == 0 ? hk : n_kheads + hk) * GT_K + ch8;
+    const int ch_v = (2 * n_kheads + hv) * GT_K + c0 + v8;
+    f16x8 x_qk[QR], x_v[VR];
+#pragma unroll
+    for (int n = 0; n < QR; ++n) x_qk[n] = *(const f16x8*)(xb + (size_t)min(tid / 32 + n * QT, T - 1) * x_stride + ch_qk);
+#pragma unroll
+    for (int n = 0; n < VR; ++n)
+        x_v[n] = *(const f16x8*)(xb + (size_t)min(lane / (2 * TL) + n * LT, T - 1) * x_stride + ch_v);
+    Taps8 conv, conv_v;
+    Frames8 old, old_v;
+    conv.load(conv_w, ch_qk);
+    conv_v.load(conv_w, ch_v);
+    if (tid < 32) old.load(seqs.frames[b], fresh, ch_qk);
+    if (lane < 2 * TL) old_v.load(seqs.frames[b], fresh, ch_v);
+    if (w < HP) {
+        double sum = lane < T ? (double)log_decay(a_in + dt, A) : 0.;
+        const Node n = tree_node(parent, T, sum);
+        // a place without a token has zeros everywhere: nothing of it reaches the others
+        s_log[w][lane] = sum *= 1.4426950408889634;
+        s_beta[w][lane] = n.here() ? gdn_beta(b_in) : 0.f;
+        s_gain[w][lane] = n.here() ? decayed(sum) : 0.f;
+        if (w == 0) {
+            // (the n-th token ahead of the context: frame n, as -1 - n)
+            const int p1 = n.parent < 0 ? -2 : n.parent;
+            const int up1 = lane_of(n.parent, max(p1, 0));
+            const int p2 = p1 < 0 ? p1 - 1 : up1 < 0 ? -2 : up1;
+            const int up2 = lane_of(n.parent, max(p2, 0));
+            const int p3 = p2 < 0 ? p2 - 1 : up2 < 0 ? -2 : up2;
+            auto row = [](int p) { return p < 0 ? p + 4 : p + 3; };
+            s_up[lane] = make_int4(row(p1), row(p2), row(p3), n.here());
+            s_line[lane] = make_uint2(n.lo, n.hi);
+            const uint64_t here = __ballot(n.here());
+            if (lane == 0) s_n = here ? 64 - __builtin_clzll(here) : 0;
         }
-        const Node n = tree_node(parents + (size_t)b * T, T, sum);
-        // (the n-th token ahead of the context: frame n, as -1 - n)
-        const int p1 = n.parent < 0 ? -2 : n.parent;
-        const int up1 = lane_of(n.parent, max(p1, 0));
-        const int p2 = p1 < 0 ? p1 - 1 : up1 < 0 ? -2 : up1;
-        const int up2 = lane_of(n.parent, max(p2, 0));
-        const int p3 = p2 < 0 ? p2 - 1 : up2 < 0 ? -2 : up2;
-        s_up[lane] = make_int4(p1, p2, p3, n.here());
-        s_line[lane] = make_uint2(n.lo, n.hi);
-        s_log[lane] = sum;
-        s_beta[lane] = beta;
-        s_gain[lane] = ratio(sum);
-        const uint64_t here = __ballot(n.here());
-        if (lane == 0) s_n = here ? 64 - __builtin_clzll(here) : 0;
+    }
+    f16(*own_x)[RAW_P] = (f16(*)[RAW_P])s_own[w];
+    float(*own)[OUT_P] = (float(*)[OUT_P])s_own[w];
+#pragma unroll
+    for (int n = 0; n < QR; ++n)
+        if (QR * QT == TP || tid / 32 + n * QT < TP) *(f16x8*)(s_raw[part][3 + tid / 32 + n * QT] + ch8) = x_qk[n];
+#pragma unroll
+    for (int n = 0; n < VR; ++n)
+        if (VR * LT == TP || lane / (2 * TL) + n * LT < TP) *(f16x8*)(own_x[3 + lane / (2 * TL) + n * LT] + v8) = x_v[n];
+    if (tid < 32) {
+        *(f16x8*)(s_raw[part][0] + ch8) = old.f0;
+        *(f16x8*)(s_raw[part][1] + ch8) = old.f1;
+        *(f16x8*)(s_raw[part][2] + ch8) = old.f2;
+    }
+    if (lane < 2 * TL) {
+        *(f16x8*)(own_x[0] + v8) = old_v.f0;
+        *(f16x8*)(own_x[1] + v8) = old_v.f1;
+        *(f16x8*)(own_x[2] + v8) = old_v.f2;
     }
     __syncthreads();
     const int n = __builtin_amdgcn_readfirstlane(s_n), nb = (n + 15) >> 4;   // tokens, blocks of them
-
-    auto conv_of = [&](const Conv8& cv, int i, int ch, f32x4& lo, f32x4& hi) {
-        const int4 up = s_up[i];
-        const f16* at = xb + ch;
-        const f16x8 f0 = cv.f0, f1 = cv.f1, f2 = cv.f2;
-        const f16x8 x0 = *(const f16x8*)(at + (size_t)i * x_stride);
-        const f16x8 x1 = token(-1 - up.x, at + (size_t)max(up.x, 0) * x_stride, f0, f1, f2);
-        const f16x8 x2 = token(-1 - up.y, at + (size_t)max(up.y, 0) * x_stride, f0, f1, f2);
-        const f16x8 x3 = token(-1 - up.z, at + (size_t)max(up.z, 0) * x_stride, f0, f1, f2);
-        cv.apply(lo, hi, x3, x2, x1, x0);
+    // S0: rows c0 + 16 t + col, columns 32 c + 8 g .. + 7. (A wave waits while its loads are taken: half ahead
+    // of the conv.)
+    f32x8 s0[TL][4];
+    const float* srow = seqs.S[b] + ((size_t)hv * GT_K + c0 + col) * GT_K + 8 * g;
+    auto load_s0 = [&](int t) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s0[t][c] = *(const f32x8*)(srow + 16 * t * GT_K + 32 * c);
     };
-    for (int i = tid >> 5; i < n; i += GT_THREADS / 32) {
+    load_s0(0);
+
+    auto conv_of = [&](const Taps8& taps, const f16* at, int pitch, int i, f32x4& lo, f32x4& hi) {
+        const int4 up = s_up[i];
+        taps.apply(lo, hi, *(const f16x8*)(at + up.z * pitch), *(const f16x8*)(at + up.y * pitch),
+                   *(const f16x8*)(at + up.x * pitch), *(const f16x8*)(at + (i + 3) * pitch));
+    };
+    for (int i = tid >> 5; i < 16 * nb; i += QT) {
         f32x4 lo, hi;
-        conv_of(conv, i, ch_qk, lo, hi);
+        const bool here = s_up[i].w;
+        conv_of(conv, s_raw[part][0] + ch8, ROW_H, i, lo, hi);
         const float inv = QK_SCALE / sqrtf(row16_sum(sum_sq(lo, hi)) + l2eps);
-        f16x8 h, l;
-        split(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7) * inv, h, l);
-        f16(*dst)[TP][ROW_H] = part == 0 ? s_q : s_k;
-        *(f16x8*)(dst[0][i] + ch8) = h;
-        *(f16x8*)(dst[1][i] + ch8) = l;
+        f16x8 t_hi, t_lo;
+        split(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7) * inv, t_hi, t_lo);
+        if (!here) t_hi = t_lo = (f16x8)(0);
+        Rows* dst = part == 0 ? s_q : s_k;
+        *(f16x8*)(dst[0][i] + ch8) = t_hi;
+        *(f16x8*)(dst[1][i] + ch8) = t_lo;
     }
-    conv.load(conv_w, seqs.frames[b], fresh, ch_v);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int t = 1; t < TL; ++t) load_s0(t);
+    // v: token 16 r + 4 g + e, state row c0 + 16 t + col
+    f32x4 v[NB][TL];
+    {
+        f32x4 lo[VR], hi[VR];
+#pragma unroll
+        for (int k = 0; k < VR; ++k)
+            if (k * LT < n) {
+                const int i = VR * LT == TP ? lane / (2 * TL) + k * LT : min(lane / (2 * TL) + k * LT, TP - 1);
+                conv_of(conv_v, own_x[0] + v8, RAW_P, i, lo[k], hi[k]);
+                if (!s_up[i].w) lo[k] = hi[k] = (f32x4)(0.f);
+            } else {
+                lo[k] = hi[k] = (f32x4)(0.f);
+            }
+#pragma unroll
+        for (int k = 0; k < VR; ++k) {
+            wave_sync();
+            if (OUT_ROWS == LT || lane / (2 * TL) < OUT_ROWS) {
+                *(f32x4*)(own[lane / (2 * TL)] + v8) = lo[k];
+                *(f32x4*)(own[lane / (2 * TL)] + v8 + 4) = hi[k];
+            }
+            wave_sync();
+#pragma unroll
+            for (int r = k * LT / 16; r < (k + 1) * LT / 16 && r < NB; ++r)
+#pragma unroll
+                for (int t = 0; t < TL; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[r][t][e] = own[16 * r - k * LT + 4 * g + e][16 * t + col];
+        }
+    }
     __syncthreads();
-    auto terms = [&](const f16 (*m)[TP][ROW_H], int row, int c) {
+    auto terms = [&](const Rows* m, int row, int c) {
         return Terms{*(const f16x8*)(m[0][row] + 32 * c + 8 * g), *(const f16x8*)(m[1][row] + 32 * c + 8 * g)};
     };
 
     // -A and the q.k side, 16 x 16 blocks on and below the diagonal
-    for (int job = w; job < nb * (nb + 1); job += GT_WAVES) {
+    for (int job = w; job < nb * (nb + 1); job += WAVES) {
         const bool qk = job & 1;
         int r = 0, c = job >> 1;
         while (c > r) c -= ++r;
@@ -233,129 +356,192 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
 #pragma unroll
         for (int s = 0; s < 4; ++s)
             acc = mfma_terms(terms(qk ? s_q : s_k, 16 * r + col, s), terms(s_k, 16 * c + col, s), acc);
-        const int j = 16 * c + col;
-        const double lj = s_log[j];
+        const int j = 16 * c + col, i0 = 16 * r + 4 * g;
+        float f[4];
+        bool anc[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            const int i = 16 * r + 4 * g + e;
-            const uint2 line = s_line[i];
-            const bool anc = ((j < 32 ? line.x : line.y) >> (j & 31) & 1) && (qk || j != i);
-            const float m = acc[e] * (1.f / (QK_SCALE * QK_SCALE)) * ratio(s_log[i] - lj);
-            (qk ? s_p : s_a)[i][j] = anc ? m * (qk ? 1.f : -s_beta[i]) : 0.f;
+            const uint2 line = s_line[i0 + e];
+            anc[e] = ((j < 32 ? line.x : line.y) >> (j & 31) & 1) && (qk || j != i0 + e);
+            f[e] = anc[e] ? acc[e] * (1.f / (QK_SCALE * QK_SCALE)) : 0.f;
+        }
+#pragma unroll
+        for (int m = 0; m < HP; ++m) {
+            f32x4 beta = (f32x4)(1.f);
+            if (!qk) beta = -*(const f32x4*)&s_beta[m][i0];
+            const double lj = s_log[m][j];
+            float a[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)   // (others' decays may be anything)
+                a[e] = f[e] * beta[e] * decayed(anc[e] ? s_log[m][i0 + e] - lj : 0.);
+            Block& to = (qk ? s_p : s_a)[m][job >> 1];
+            if (!qk && r == c) {
+                *(f32x4*)&to[col][4 * g] = (f32x4){a[0], a[1], a[2], a[3]};
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) put_term(to[4 * g + e], col, a[e]);
+            }
         }
     }
     __syncthreads();
-
     // the inverse of a diagonal block I + A, a column a lane
-    if (w < nb) {
+    if (w < HP * nb) {
+        Block& m = s_a[w / nb][(w % nb) * (w % nb + 3) / 2];
         float xi[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-            float s = i == col ? 1.f : 0.f;
+        for (int i = 0; i < 16; ++i) xi[i] = i == col ? 1.f : 0.f;
 #pragma unroll
-            for (int m = 0; m < i; ++m) s = fmaf(s_a[16 * w + i][16 * w + m], xi[m], s);
-            xi[i] = s;
+        for (int i = 0; i < 15; ++i) {   // (a row of m is a column of -A: no chain but over the rows)
+            f32x4 a[4];
+#pragma unroll
+            for (int q = (i + 1) / 4; q < 4; ++q) a[q] = *(const f32x4*)&m[i][4 * q];
+#pragma unroll
+            for (int q = i + 1; q < 16; ++q) xi[q] = fmaf(a[q >> 2][q & 3], xi[i], xi[q]);
         }
         if (g == 0)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) s_inv[w][i][col] = xi[i];
+            for (int i = 0; i < 16; ++i) put_term(m[i], col, xi[i]);
     }
-    // S0 k_i and S0 q_i: row 16 r + 4 g + e, state row 16 w + col. S0's terms are those of its rows with
+    // The right side and o's first part, from S0 k_i and S0 q_i. S0's terms are those of its rows with
     // their largest entries brought to [2^14, 2^15).
-    float top = 0.f;
+    Terms st[TL][4];
+    float f_k[TL], f_v[TL];   // the units of u's columns over those of the product, and over 1
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
+    for (int t = 0; t < TL; ++t) {
+        float top = 0.f, top_v = 0.f;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(s0[c][e]));
-    top = fmaxf(top, lane_xor(top, 16));
-    top = fmaxf(top, lane_xor(top, 32));
-    const int up = 14 - min(max(ilogb_bits(top), -100), 100);
-    Terms st[4];
+        for (int c = 0; c < 4; ++c)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) split(s0[c] * pow2(up), st[c].hi, st[c].lo);
-    const float down = pow2(-up) * (1.f / QK_SCALE);
-    f32x4 wk[NB], wq[NB];
+            for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(s0[t][c][e]));
+#pragma unroll
+        for (int r = 0; r < NB; ++r)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) top_v = fmaxf(top_v, fabsf(v[r][t][e]));
+        const int up = lift(top);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) split(s0[t][c] * pow2(up), st[t][c].hi, st[t][c].lo);
+        // A step contracts: a column's u are at most 64 |v| + |S0's row|, their sums in a block's right side
+        // at most 17 of them. With all of those below 2^15, what lies 2^-25 below 1 is far below u.
+        const int up_u = lift(32.f * (64.f * top_v + 12.f * top));
+        f_v[t] = pow2(up_u);
+        f_k[t] = pow2(up_u - up) * (1.f / QK_SCALE);
+    }
+    f32x4 u[NB][TL], o[NB][TL];   // scaled by f_v QK_SCALE
 #pragma unroll
     for (int r = 0; r < NB; ++r) {
-        wk[r] = wq[r] = (f32x4)(0.f);
-        if (r < nb) {
+        if (r >= nb) continue;
+        f32x4 wk[TL], wq[TL];
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                wk[r] = mfma_terms(terms(s_k, 16 * r + col, c), st[c], wk[r]);
-                wq[r] = mfma_terms(terms(s_q, 16 * r + col, c), st[c], wq[r]);
+        for (int t = 0; t < TL; ++t) wk[t] = wq[t] = (f32x4)(0.f);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+            const Terms k = terms(s_k, 16 * r + col, c), q = terms(s_q, 16 * r + col, c);
+#pragma unroll
+            for (int t = 0; t < TL; ++t) {
+                wk[t] = mfma_terms(k, st[t][c], wk[t]);
+                wq[t] = mfma_terms(q, st[t][c], wq[t]);
             }
-            wk[r] *= down;
-            wq[r] *= down;
         }
-    }
-    __syncthreads();
-    for (int i = tid >> 4; i < n; i += GT_THREADS / 16) {
-        f32x4 lo, hi;
-        conv_of(conv, i, ch_v, lo, hi);
-        *(f32x4*)(s_v[i] + ch8) = lo;
-        *(f32x4*)(s_v[i] + ch8 + 4) = hi;
-    }
-    __syncthreads();
-
-    f32x4 u[NB];
+        const f32x4 beta = *(const f32x4*)&s_beta[h][16 * r + 4 * g] * QK_SCALE;
+        const f32x4 gain = *(const f32x4*)&s_gain[h][16 * r + 4 * g];
 #pragma unroll
-    for (int r = 0; r < NB; ++r) {
-        u[r] = (f32x4)(0.f);
-        if (r < nb) {
-            f32x4 rhs, o;
+        for (int t = 0; t < TL; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                const int i = 16 * r + 4 * g + e;
-                // (a place without a token adds nothing to others, whatever lies there)
-                const bool here = s_up[i].w;
-                const float gain = s_gain[i];
-                rhs[e] = here ? s_beta[i] * (s_v[i][16 * w + col] - gain * wk[r][e]) : 0.f;
-                o[e] = here ? gain * wq[r][e] : 0.f;
+                u[r][t][e] = beta[e] * fmaf(-gain[e], wk[t][e] * f_k[t], v[r][t][e] * f_v[t]);
+                o[r][t][e] = gain[e] * QK_SCALE * (wq[t][e] * f_k[t]);
             }
-#pragma unroll
-            for (int c = 0; c < NB; ++c)
-                if (c < r) {
-                    const f32x4 av = *(const f32x4*)&s_a[16 * r + col][16 * c + 4 * g];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) rhs = mfma4(av[e], u[c][e], rhs);
-                }
-            const f32x4 iv = *(const f32x4*)&s_inv[r][col][4 * g];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) u[r] = mfma4(iv[e], rhs[e], u[r]);
-#pragma unroll
-            for (int c = 0; c < NB; ++c)
-                if (c <= r) {
-                    const f32x4 pv = *(const f32x4*)&s_p[16 * r + col][16 * c + 4 * g];
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) o = mfma4(pv[e], u[c][e], o);
-                }
-            // (this wave's columns of v, which no other wave reads)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) s_v[16 * r + 4 * g + e][16 * w + col] = o[e] * out_scale;
-        }
     }
+    // the output's gates, a token a row of 2 TL lanes (whose places are not worth registers until here)
+    int l = lane;
+    asm volatile("" : "+v"(l));
+    const int row0 = l / (2 * TL), out8 = 8 * (l & (2 * TL - 1));
+    f16x8 gate[VR];
+#pragma unroll
+    for (int k = 0; k < VR; ++k)
+        gate[k] = *(const f16x8*)(z + ((size_t)b * T + min(row0 + k * LT, T - 1)) * z_pitch + hv * GT_K + c0 + out8);
     __syncthreads();
 
-    // the gated norm of a row, 8 dims a lane of a DPP row
-    const f32x4 w0 = *(const f32x4*)(norm_w + ch8), w1 = *(const f32x4*)(norm_w + ch8 + 4);
-    for (int i = tid >> 4; i < T; i += GT_THREADS / 16) {
-        const size_t row = (size_t)b * T + i;
-        f16x8 out = (f16x8)(0);
-        if (i < n && s_up[i].w) {
-            const f16x8 gate = *(const f16x8*)(z + row * z_pitch + hv * GT_K + ch8);
-            const f32x4 a = *(const f32x4*)(s_v[i] + ch8), c = *(const f32x4*)(s_v[i] + ch8 + 4);
-            float o[8] = {a[0], a[1], a[2], a[3], c[0], c[1], c[2], c[3]}, ss = 0.f;
+    // block by block of tokens
+    Terms4 ut[NB][TL];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) ss = fmaf(o[e], o[e], ss);
-            const float inv = 1.f / sqrtf(row16_sum(ss) / (float)GT_K + norm_eps);
+    for (int r = 0; r < NB; ++r) {
+        if (r >= nb) continue;
+        auto at = [&](const Block* m, int c) {
+            const f16* row = (const f16*)m[r * (r + 1) / 2 + c][col] + 4 * g;
+            return Terms4{*(const f16x4*)row, *(const f16x4*)(row + 16)};
+        };
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float gz = (float)gate[e];
-                o[e] *= inv * (e < 4 ? w0[e] : w1[e - 4]) * (gz * __builtin_amdgcn_rcpf(1.f + hw_expf(-gz)));
-            }
-            out = f16_sat8(o);
+        for (int c = 0; c < r; ++c) {
+            const Terms4 a = at(s_a[h], c);
+#pragma unroll
+            for (int t = 0; t < TL; ++t) u[r][t] = mfma_terms4(a, ut[c][t], u[r][t]);
         }
-        *(f16x8*)(y + row * y_pitch + hv * GT_K + ch8) = out;
+        const Terms4 inv = at(s_a[h], r);
+        Terms4 rhs[TL];
+#pragma unroll
+        for (int t = 0; t < TL; ++t) rhs[t] = split4(u[r][t] * (1.f / QK_SCALE));
+#pragma unroll
+        for (int t = 0; t < TL; ++t) u[r][t] = mfma_terms4(inv, rhs[t], (f32x4)(0.f));
+#pragma unroll
+        for (int t = 0; t < TL; ++t) ut[r][t] = split4(u[r][t] * (1.f / QK_SCALE));
+#pragma unroll
+        for (int c = 0; c <= r; ++c) {
+            const Terms4 p = at(s_p[h], c);
+#pragma unroll
+            for (int t = 0; t < TL; ++t) o[r][t] = mfma_terms4(p, ut[c][t], o[r][t]);
+        }
+    }
+    // o in true units; squares of a row over this wave's columns, then over the head's waves
+    float f_o[TL];
+#pragma unroll
+    for (int t = 0; t < TL; ++t) f_o[t] = out_scale / QK_SCALE / f_v[t];
+#pragma unroll
+    for (int r = 0; r < NB; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            float ss = 0.f;
+#pragma unroll
+            for (int t = 0; t < TL; ++t) {
+                o[r][t][e] = r < nb ? o[r][t][e] * f_o[t] : 0.f;
+                ss = fmaf(o[r][t][e], o[r][t][e], ss);
+            }
+            ss = row16_sum(ss);
+            if (col == 0) s_ss[h][16 * r + 4 * g + e][w - h * HW] = ss;
+        }
+    __syncthreads();
+    const f32x4 w0 = *(const f32x4*)(norm_w + c0 + out8), w1 = *(const f32x4*)(norm_w + c0 + out8 + 4);
+#pragma unroll
+    for (int k = 0; k < VR; ++k) {
+        wave_sync();
+#pragma unroll
+        for (int r = k * LT / 16; r < (k + 1) * LT / 16 && r < NB; ++r)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int t = 0; t < TL; ++t) own[16 * r - k * LT + 4 * g + e][16 * t + col] = o[r][t][e];
+        wave_sync();
+        const int i = row0 + k * LT;
+        if (i < T) {
+            f16x8 out = (f16x8)(0);
+            if (s_up[i].w) {
+                const f32x4 a = *(const f32x4*)(own[row0] + out8), c = *(const f32x4*)(own[row0] + out8 + 4);
+                float t[8] = {a[0], a[1], a[2], a[3], c[0], c[1], c[2], c[3]}, ss = 0.f;
+#pragma unroll
+                for (int m = 0; m < HW; m += 4) {
+                    const f32x4 p = *(const f32x4*)&s_ss[h][i][m];
+                    ss += (p[0] + p[1]) + (p[2] + p[3]);
+                }
+                const float inv = 1.f / sqrtf(ss / (float)GT_K + norm_eps);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float gz = (float)gate[k][e];
+                    t[e] *= inv * (e < 4 ? w0[e] : w1[e - 4]) * (gz * __builtin_amdgcn_rcpf(1.f + hw_expf(-gz)));
+                }
+                out = f16_sat8(t);
+            }
+            *(f16x8*)(y + ((size_t)b * T + i) * y_pitch + hv * GT_K + c0 + out8) = out;
+        }
     }
 }
 
@@ -534,12 +720,24 @@ int fl_gdn_tree_normed(const void* x, int x_stride, const void* conv_w, const vo
         seqs.frames[i] = (const f16*)cst_in[i];
         seqs.pos0[i] = pos0[i];
     }
-    auto kernel = T <= 16 ? gdn_tree_kernel<1> : T <= 32 ? gdn_tree_kernel<2> : T <= 48 ? gdn_tree_kernel<3>
-                                                                                       : gdn_tree_kernel<4>;
-    hipLaunchKernelGGL(kernel, dim3(B * n_vheads), dim3(GT_THREADS), 0, (hipStream_t)stream, (const f16*)x,
-                       x_stride, (const f16*)conv_w, seqs, parents, a, b, ab_stride, A_log, dt_bias,
-                       (const f16*)z, z_pitch, norm_w, (f16*)y, y_pitch, T, n_kheads, n_vheads, out_scale, l2eps,
-                       norm_eps);
+    const int group = n_vheads / n_kheads;
+    auto launch = [&](auto kernel, int heads, int threads) {
+        hipLaunchKernelGGL(kernel, dim3(B * (n_vheads / heads)), dim3(threads), 0, (hipStream_t)stream, (const f16*)x,
+                           x_stride, (const f16*)conv_w, seqs, parents, a, b, ab_stride, A_log, dt_bias,
+                           (const f16*)z, z_pitch, norm_w, (f16*)y, y_pitch, T, n_kheads, n_vheads, out_scale,
+                           l2eps, norm_eps);
+    };
+    const int nb = (T + 15) / 16;
+    const bool many = B * n_vheads > GT_MANY;
+    if (nb <= 3 && many && group % 3 == 0)
+        launch(nb == 1 ? gdn_tree_kernel<1, 3, 2> : nb == 2 ? gdn_tree_kernel<2, 3, 2> : gdn_tree_kernel<3, 3, 2>, 3, 768);
+    else if (nb <= 3 && many && group % 2 == 0)
+        launch(nb == 1 ? gdn_tree_kernel<1, 2, 2> : nb == 2 ? gdn_tree_kernel<2, 2, 2> : gdn_tree_kernel<3, 2, 2>, 2, 512);
+    else
+        launch(nb == 1   ? gdn_tree_kernel<1, 1, 1>
+               : nb == 2 ? gdn_tree_kernel<2, 1, 1>
+               : nb == 3 ? gdn_tree_kernel<3, 1, 1>
+                         : gdn_tree_kernel<4, 1, 1>, 1, 512);
     return fl::check_launch("gdn_tree_normed");
 }
 

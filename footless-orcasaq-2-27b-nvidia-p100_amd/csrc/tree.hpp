@@ -35,9 +35,9 @@ struct Node {
 // Of a whole wave. Every round a token takes over what the token `up` has gathered and that
 // one's own `up`: 2^r ancestors after r rounds, as many rounds as the tree is deep in bits.
 // `sum` becomes its sum over the path to the token, itself included.
-__device__ __forceinline__ Node tree_node(const int* parents, int T, double& sum) {
+__device__ __forceinline__ Node tree_node(int p, int T, double& sum) {   // p: lane i's parents[i]
     const int i = threadIdx.x & 63;
-    const int p = i < T ? parents[i] : -2;
+    if (i >= T) p = -2;
     const bool ok = p >= -1 && p < i;
     Node n = {ok ? p : -1, i < 32 ? 1u << i : 0u, i < 32 ? 0u : 1u << (i - 32)};
     int up = n.parent, lost = !ok;

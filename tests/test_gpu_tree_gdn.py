@@ -74,6 +74,19 @@ def test_other_head_counts_and_strides(fl, n_k, n_v):
     check(y, want, bound, f"{n_k} / {n_v} heads")
 
 
+@pytest.mark.parametrize("n_k,n_v,B,T", [(16, 48, 6, 16), (16, 48, 7, 19), (16, 48, 6, 41), (16, 48, 6, 64),
+                                         (16, 32, 9, 9), (8, 32, 16, 32), (16, 32, 12, 48), (3, 18, 15, 33),
+                                         (5, 25, 11, 20)])
+def test_batches_of_several_heads_a_workgroup(fl, n_k, n_v, B, T):
+    g = gen(100 * B + T)
+    d = ref.gdn_layer(g, B, T, n_k, n_v)
+    parents = [tree(g, int(torch.randint(0, T + 1, (1,), generator=g)), T) for _ in range(B)]
+    parents[0] = tree(g, T, T, "binary")
+    pos0 = [b % 3 for b in range(B)]
+    want, bound = ref.gdn_tree(d, parents, [p == 0 for p in pos0])
+    check(run(fl, d, parents, pos0), want, bound, f"{n_k} / {n_v} heads, B {B} T {T}")
+
+
 def test_places_without_a_token_do_not_matter(fl):
     """Whatever they hold: parents out of order or range, descendants of such places, NaN rows."""
     g = gen(8)
