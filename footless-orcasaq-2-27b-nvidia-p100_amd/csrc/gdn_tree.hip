@@ -119,20 +119,21 @@ struct TreeSeqs {
     int pos0[FL_MAX_SEQS];
 };
 
-// x as two fp16 terms: 21 bits of it, and what lies 2^-24 below 1 (so x is scaled up first)
-__device__ __forceinline__ void split(f32x8 x, f16x8& hi, f16x8& lo) {
-#pragma unroll
-    for (int e = 0; e < 8; e += 2) {   // (cut off: the rest is lo's)
-        const auto p = __builtin_amdgcn_cvt_pkrtz(x[e], x[e + 1]);
-        hi[e] = p[0], hi[e + 1] = p[1];
-    }
-    lo = __builtin_convertvector(x - __builtin_convertvector(hi, f32x8), f16x8);
-}
 __device__ __forceinline__ int ilogb_bits(float x) { return (int)(__float_as_uint(x) >> 23 & 255) - 127; }
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
+// x s as two fp16 terms: 22 bits of it, down to 2^-24 (so s scales up). Two mixed fmas a number.
 struct Terms {
     f16x8 hi, lo;
 };
+__device__ __forceinline__ Terms split8(f32x8 x, float s) {
+    Terms r;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r.hi[e] = (f16)fmaf(x[e], s, 0.f);
+    asm("" : "+v"(r.hi));   // (as it is packed: it would be formed twice)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) r.lo[e] = (f16)fmaf(x[e], s, -(float)r.hi[e]);
+    return r;
+}
 // The exponent that brings the largest of a column's entries to [2^14, 2^15): the four lanes of a column
 // have some each, the largest of which is `top`.
 __device__ __forceinline__ int lift(float top) {
@@ -143,16 +144,21 @@ __device__ __forceinline__ int lift(float top) {
 struct Terms4 {
     f16x4 hi, lo;
 };
-__device__ __forceinline__ Terms4 split4(f32x4 x) {
-    const f16x4 hi = __builtin_convertvector(x, f16x4);
-    return {hi, __builtin_convertvector(x - __builtin_convertvector(hi, f32x4), f16x4)};
+__device__ __forceinline__ Terms4 split4(f32x4 x, float s) {
+    Terms4 r;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r.hi[e] = (f16)fmaf(x[e], s, 0.f);
+    asm("" : "+v"(r.hi));   // (as it is packed: it would be formed twice)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) r.lo[e] = (f16)fmaf(x[e], s, -(float)r.hi[e]);
+    return r;
 }
 __device__ __forceinline__ f32x4 mfma_terms4(const Terms4& a, const Terms4& b, f32x4 c) {
     c = __builtin_amdgcn_mfma_f32_16x16x16f16(a.lo, b.hi, c, 0, 0, 0);
     c = __builtin_amdgcn_mfma_f32_16x16x16f16(a.hi, b.lo, c, 0, 0, 0);
     return __builtin_amdgcn_mfma_f32_16x16x16f16(a.hi, b.hi, c, 0, 0, 0);
 }
-// c + a b without the product of the two low terms (2^-21 of a b)
+// c + a b without the product of the two low terms (2^-22 of a b)
 __device__ __forceinline__ f32x4 mfma_terms(const Terms& a, const Terms& b, f32x4 c) {
     c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.lo, b.hi, c, 0, 0, 0);
     c = __builtin_amdgcn_mfma_f32_16x16x32_f16(a.hi, b.lo, c, 0, 0, 0);
@@ -166,10 +172,9 @@ __device__ __forceinline__ void wave_sync() {
 
 // A number of at most 1 (as all of A, its inverses and the q.k side are) in a row of 16 high and 16 low terms.
 __device__ __forceinline__ void put_term(float* row, int at, float a) {
-    const float x = a * QK_SCALE;
-    const f16 hi = (f16)x;
+    const f16 hi = (f16)(a * QK_SCALE);
     ((f16*)row)[at] = hi;
-    ((f16*)row)[16 + at] = (f16)(x - (float)hi);
+    ((f16*)row)[16 + at] = (f16)fmaf(a, QK_SCALE, -(float)hi);
 }
 
 // NB blocks of 16 tokens, HP v heads of one k head, TL tiles of 16 state rows a wave.
@@ -211,21 +216,26 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
     const int col = lane & 15, g = lane >> 4;
     // Workgroups go to the 8 XCDs round-robin: neighbouring heads to one of them.
     const int group = n_vheads / n_kheads, units = n_vheads / HP;
-    int unit = blockIdx.x % units, b = blockIdx.x / units;
+    int at = blockIdx.x % units, b = blockIdx.x / units;
     if (units % 8 == 0) {
         const int per = units / 8, r = blockIdx.x >> 3;
-        unit = (blockIdx.x & 7) * per + r % per;
+        at = (blockIdx.x & 7) * per + r % per;
         b = r / per;
     }
-    const int h = w / HW, hv = unit * HP + h, hk = unit * HP / group;   // the wave's head
+    const int h = w / HW, hv = at * HP + h, hk = at * HP / group;   // the wave's head
     const int c0 = (w - h * HW) * COLS;                                 // and first state row
     const bool fresh = seqs.pos0[b] == 0;
 
     // Asked for first: what the tokens' conv needs. S0, which takes longest, follows once that is here.
-    const int head = unit * HP + (w < HP ? w : 0), token0 = min(lane, T - 1);   // (the gates of head w)
-    const size_t at_ab = ((size_t)b * T + token0) * ab_stride + head;
-    const int parent = parents[(size_t)b * T + token0];
-    const float a_in = ga[at_ab], b_in = gb[at_ab], dt = dt_bias[head], A = A_log[head];
+    int parent = -2;
+    float a_in = 0.f, b_in = 0.f, dt = 0.f, A = 0.f;
+    if (w < HP) {   // the gates of head w
+        const size_t token = (size_t)b * T + min(lane, T - 1);
+        const int head = at * HP + w;
+        parent = parents[token];
+        a_in = ga[token * ab_stride + head], b_in = gb[token * ab_stride + head];
+        dt = dt_bias[head], A = A_log[head];
+    }
     const f16* xb = x + (size_t)b * T * x_stride;
     const int part = tid >> 4 & 1, ch8 = 8 * (tid & 15), v8 = 8 * (lane & (2 * TL - 1));
     const int ch_qk = (part == 0 ? hk : n_kheads + hk) * GT_K + ch8;
@@ -237,11 +247,29 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
     for (int n = 0; n < VR; ++n)
         x_v[n] = *(const f16x8*)(xb + (size_t)min(lane / (2 * TL) + n * LT, T - 1) * x_stride + ch_v);
     Taps8 conv, conv_v;
-    Frames8 old, old_v;
     conv.load(conv_w, ch_qk);
     conv_v.load(conv_w, ch_v);
-    if (tid < 32) old.load(seqs.frames[b], fresh, ch_qk);
-    if (lane < 2 * TL) old_v.load(seqs.frames[b], fresh, ch_v);
+    // the frames ahead of the rows, by two waves that have no gates to form
+    Frames8 old;
+    if (w == WAVES - 1 && lane < 32) {
+        old.load(seqs.frames[b], fresh, ch_qk);
+        f16* to = s_raw[part][0] + ch8;
+        *(f16x8*)to = old.f0, *(f16x8*)(to + ROW_H) = old.f1, *(f16x8*)(to + 2 * ROW_H) = old.f2;
+    }
+    if (w == WAVES - 2 && lane < 16 * HP) {
+        old.load(seqs.frames[b], fresh, (2 * n_kheads + at * HP) * GT_K + 8 * lane);
+        f16* to = (f16*)s_own[8 * lane / COLS] + 8 * lane % COLS;
+        *(f16x8*)to = old.f0, *(f16x8*)(to + RAW_P) = old.f1, *(f16x8*)(to + 2 * RAW_P) = old.f2;
+    }
+    // S0: rows c0 + 16 t + col, columns 32 c + 8 g .. + 7
+    f32x8 s0[TL][4];
+    const float* srow = seqs.S[b] + ((size_t)hv * GT_K + c0 + col) * GT_K + 8 * g;
+    auto load_s0 = [&](int t) {
+#pragma unroll
+        for (int c = 0; c < 4; ++c) s0[t][c] = *(const f32x8*)(srow + 16 * t * GT_K + 32 * c);
+    };
+    load_s0(0);
+
     if (w < HP) {
         double sum = lane < T ? (double)log_decay(a_in + dt, A) : 0.;
         const Node n = tree_node(parent, T, sum);
@@ -271,27 +299,10 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
 #pragma unroll
     for (int n = 0; n < VR; ++n)
         if (VR * LT == TP || lane / (2 * TL) + n * LT < TP) *(f16x8*)(own_x[3 + lane / (2 * TL) + n * LT] + v8) = x_v[n];
-    if (tid < 32) {
-        *(f16x8*)(s_raw[part][0] + ch8) = old.f0;
-        *(f16x8*)(s_raw[part][1] + ch8) = old.f1;
-        *(f16x8*)(s_raw[part][2] + ch8) = old.f2;
-    }
-    if (lane < 2 * TL) {
-        *(f16x8*)(own_x[0] + v8) = old_v.f0;
-        *(f16x8*)(own_x[1] + v8) = old_v.f1;
-        *(f16x8*)(own_x[2] + v8) = old_v.f2;
-    }
     __syncthreads();
     const int n = __builtin_amdgcn_readfirstlane(s_n), nb = (n + 15) >> 4;   // tokens, blocks of them
-    // S0: rows c0 + 16 t + col, columns 32 c + 8 g .. + 7. (A wave waits while its loads are taken: half ahead
-    // of the conv.)
-    f32x8 s0[TL][4];
-    const float* srow = seqs.S[b] + ((size_t)hv * GT_K + c0 + col) * GT_K + 8 * g;
-    auto load_s0 = [&](int t) {
 #pragma unroll
-        for (int c = 0; c < 4; ++c) s0[t][c] = *(const f32x8*)(srow + 16 * t * GT_K + 32 * c);
-    };
-    load_s0(0);
+    for (int t = 1; t < TL; ++t) load_s0(t);
 
     auto conv_of = [&](const Taps8& taps, const f16* at, int pitch, int i, f32x4& lo, f32x4& hi) {
         const int4 up = s_up[i];
@@ -303,16 +314,12 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
         const bool here = s_up[i].w;
         conv_of(conv, s_raw[part][0] + ch8, ROW_H, i, lo, hi);
         const float inv = QK_SCALE / sqrtf(row16_sum(sum_sq(lo, hi)) + l2eps);
-        f16x8 t_hi, t_lo;
-        split(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7) * inv, t_hi, t_lo);
-        if (!here) t_hi = t_lo = (f16x8)(0);
+        Terms t = split8(__builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7), inv);
+        if (!here) t.hi = t.lo = (f16x8)(0);
         Rows* dst = part == 0 ? s_q : s_k;
-        *(f16x8*)(dst[0][i] + ch8) = t_hi;
-        *(f16x8*)(dst[1][i] + ch8) = t_lo;
+        *(f16x8*)(dst[0][i] + ch8) = t.hi;
+        *(f16x8*)(dst[1][i] + ch8) = t.lo;
     }
-    __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-    for (int t = 1; t < TL; ++t) load_s0(t);
     // v: token 16 r + 4 g + e, state row c0 + 16 t + col
     f32x4 v[NB][TL];
     {
@@ -402,10 +409,11 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
 #pragma unroll
             for (int i = 0; i < 16; ++i) put_term(m[i], col, xi[i]);
     }
-    // The right side and o's first part, from S0 k_i and S0 q_i. S0's terms are those of its rows with
-    // their largest entries brought to [2^14, 2^15).
+    // The right side and o's first part, from S0 k_i and S0 q_i. A step contracts: the u of a state row are at
+    // most 64 |v| + |S0's row|, and a block's right side 17 of them. In units that keep those below 2^15 the
+    // terms' 2^-25 is 2^-29 of the largest v, or less than 2^-31 of S0's row.
     Terms st[TL][4];
-    float f_k[TL], f_v[TL];   // the units of u's columns over those of the product, and over 1
+    float unit[TL];
 #pragma unroll
     for (int t = 0; t < TL; ++t) {
         float top = 0.f, top_v = 0.f;
@@ -417,16 +425,12 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
         for (int r = 0; r < NB; ++r)
 #pragma unroll
             for (int e = 0; e < 4; ++e) top_v = fmaxf(top_v, fabsf(v[r][t][e]));
-        const int up = lift(top);
+        unit[t] = pow2(lift(32.f * (64.f * top_v + 12.f * top)));
 #pragma unroll
-        for (int c = 0; c < 4; ++c) split(s0[t][c] * pow2(up), st[t][c].hi, st[t][c].lo);
-        // A step contracts: a column's u are at most 64 |v| + |S0's row|, their sums in a block's right side
-        // at most 17 of them. With all of those below 2^15, what lies 2^-25 below 1 is far below u.
-        const int up_u = lift(32.f * (64.f * top_v + 12.f * top));
-        f_v[t] = pow2(up_u);
-        f_k[t] = pow2(up_u - up) * (1.f / QK_SCALE);
+        for (int c = 0; c < 4; ++c) st[t][c] = split8(s0[t][c], unit[t]);
+        unit[t] *= QK_SCALE;
     }
-    f32x4 u[NB][TL], o[NB][TL];   // scaled by f_v QK_SCALE
+    f32x4 u[NB][TL], o[NB][TL];   // times unit
 #pragma unroll
     for (int r = 0; r < NB; ++r) {
         if (r >= nb) continue;
@@ -442,14 +446,14 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
                 wq[t] = mfma_terms(q, st[t][c], wq[t]);
             }
         }
-        const f32x4 beta = *(const f32x4*)&s_beta[h][16 * r + 4 * g] * QK_SCALE;
+        const f32x4 beta = *(const f32x4*)&s_beta[h][16 * r + 4 * g];
         const f32x4 gain = *(const f32x4*)&s_gain[h][16 * r + 4 * g];
 #pragma unroll
         for (int t = 0; t < TL; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                u[r][t][e] = beta[e] * fmaf(-gain[e], wk[t][e] * f_k[t], v[r][t][e] * f_v[t]);
-                o[r][t][e] = gain[e] * QK_SCALE * (wq[t][e] * f_k[t]);
+                u[r][t][e] = beta[e] * fmaf(-gain[e], wk[t][e], v[r][t][e] * unit[t]);
+                o[r][t][e] = gain[e] * wq[t][e];
             }
     }
     // the output's gates, a token a row of 2 TL lanes (whose places are not worth registers until here)
@@ -480,11 +484,11 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
         const Terms4 inv = at(s_a[h], r);
         Terms4 rhs[TL];
 #pragma unroll
-        for (int t = 0; t < TL; ++t) rhs[t] = split4(u[r][t] * (1.f / QK_SCALE));
+        for (int t = 0; t < TL; ++t) rhs[t] = split4(u[r][t], 1.f / QK_SCALE);
 #pragma unroll
         for (int t = 0; t < TL; ++t) u[r][t] = mfma_terms4(inv, rhs[t], (f32x4)(0.f));
 #pragma unroll
-        for (int t = 0; t < TL; ++t) ut[r][t] = split4(u[r][t] * (1.f / QK_SCALE));
+        for (int t = 0; t < TL; ++t) ut[r][t] = split4(u[r][t], 1.f / QK_SCALE);
 #pragma unroll
         for (int c = 0; c <= r; ++c) {
             const Terms4 p = at(s_p[h], c);
@@ -495,7 +499,7 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
     // o in true units; squares of a row over this wave's columns, then over the head's waves
     float f_o[TL];
 #pragma unroll
-    for (int t = 0; t < TL; ++t) f_o[t] = out_scale / QK_SCALE / f_v[t];
+    for (int t = 0; t < TL; ++t) f_o[t] = out_scale / unit[t];
 #pragma unroll
     for (int r = 0; r < NB; ++r)
 #pragma unroll
