@@ -33,6 +33,7 @@ constexpr int GT_K = 128;                // K = V
 constexpr int ROW_H = GT_K + 8;          // terms a row of k and q
 constexpr float QK_SCALE = 16384.f;      // of q and k, whose norms are at most 1
 constexpr int GT_MANY = 256;             // heads from which a workgroup takes several
+constexpr int GC_ROWS = 32;              // state rows that a workgroup moves on
 constexpr int BLOCK_P = 20;              // floats a row of a 16 x 16 block
 
 // Sum over the 16 lanes of a DPP row, on every one of them.
@@ -550,12 +551,10 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
 }
 
 // ---------------------------------------------------------------------------
-// The state and the conv frames behind an accepted path, token by token: 32 state rows a
-// workgroup, a row on 8 lanes (columns 4 l + 32 j .. + 3) in registers throughout, k and v of
-// the path's tokens formed first. Reads and writes a state once: bound by that for a batch.
+// The state and the conv frames behind an accepted path, token by token: ROWS state rows a workgroup,
+// a row on 8 lanes (columns 4 l + 32 j .. + 3) in registers throughout, k and v of the path's tokens
+// formed first. Reads and writes a state once: bound by that for a batch.
 // ---------------------------------------------------------------------------
-constexpr int GC_ROWS = 32, GC_THREADS = 256;
-
 struct CommitSeqs {
     const float* S[FL_MAX_SEQS];
     float* S_out[FL_MAX_SEQS];
@@ -570,25 +569,26 @@ __device__ __forceinline__ float row8_sum(float v) {
     return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x141, 0xF, 0xF, true));   // half mirror
 }
 
-__global__ void __launch_bounds__(GC_THREADS)
+// A token's conv input: its own row and the three before it.
+struct Window8 {
+    f16x8 x3, x2, x1, x0;
+};
+
+__global__ void __launch_bounds__(8 * GC_ROWS)
 gdn_commit_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__ conv_w, const CommitSeqs seqs,
                   const int* __restrict__ path, const float* __restrict__ ga, const float* __restrict__ gb,
                   int ab_stride, const float* __restrict__ A_log, const float* __restrict__ dt_bias, int T, int D,
                   int n_kheads, int n_vheads, float l2eps) {
-    __shared__ __attribute__((aligned(16))) float s_k[TREE_MAX][GT_K], s_v[TREE_MAX][GC_ROWS];
+    constexpr int ROWS = GC_ROWS, THREADS = 8 * ROWS, PARTS = GT_K / ROWS, VL = ROWS / 8;   // lanes a token's v takes
+    extern __shared__ __attribute__((aligned(16))) float s_kv[];            // [D][128] of k, [D][ROWS] of v
     __shared__ float s_beta[TREE_MAX], s_alpha[TREE_MAX];
     __shared__ int s_at[TREE_MAX], s_n;
+    float(*s_k)[GT_K] = (float(*)[GT_K])s_kv;
+    float(*s_v)[ROWS] = (float(*)[ROWS])(s_kv + D * GT_K);
     const int tid = threadIdx.x;
-    constexpr int PARTS = GT_K / GC_ROWS;
     const int part = blockIdx.x % PARTS, hv = blockIdx.x / PARTS % n_vheads, b = blockIdx.x / PARTS / n_vheads;
     const int group = n_vheads / n_kheads, hk = hv / group;
     const bool fresh = seqs.pos0[b] == 0;
-
-    // the state: row part GC_ROWS + tid / 8
-    const size_t srow = ((size_t)hv * GT_K + part * GC_ROWS + (tid >> 3)) * GT_K + 4 * (tid & 7);
-    f32x4 s[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) s[j] = *(const f32x4*)(seqs.S[b] + srow + 32 * j);
 
     if (tid < 64) {   // the path's tokens, and their gates
         const int i = tid < D ? path[(size_t)b * D + tid] : -1;
@@ -603,6 +603,11 @@ gdn_commit_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict
             s_beta[tid] = gdn_beta(gb[at]);
         }
     }
+    const int k8 = 8 * (tid & 15), v8 = 8 * (tid & (VL - 1));   // k: a token on 16 lanes
+    const int ch_k = (n_kheads + hk) * GT_K + k8, ch_v = (2 * n_kheads + hv) * GT_K + part * ROWS + v8;
+    Conv8 ck, cv;
+    ck.load(conv_w, seqs.frames[b], fresh, ch_k);
+    cv.load(conv_w, seqs.frames[b], fresh, ch_v);
     __syncthreads();
     const int n = s_n;
 
@@ -617,52 +622,51 @@ gdn_commit_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict
         to[1] = (f16x8){z[2], x[3], y[3], z[3], x[4], y[4], z[4], x[5]};
         to[2] = (f16x8){y[5], z[5], x[6], y[6], z[6], x[7], y[7], z[7]};
     };
-    {   // k, a token on a DPP row
-        const int ch8 = 8 * (tid & 15), ch = (n_kheads + hk) * GT_K + ch8;
-        Conv8 c;
-        c.load(conv_w, seqs.frames[b], fresh, ch);
-        for (int d = tid >> 4; d < n; d += GC_THREADS / 16) {
-            f32x4 lo, hi;
-            const f16x8 x3 = token(3 - d, row(d - 3, ch), c.f0, c.f1, c.f2);
-            const f16x8 x2 = token(2 - d, row(d - 2, ch), c.f0, c.f1, c.f2);
-            const f16x8 x1 = token(1 - d, row(d - 1, ch), c.f0, c.f1, c.f2);
-            c.apply(lo, hi, x3, x2, x1, *(const f16x8*)row(d, ch));
-            const float inv = 1.f / sqrtf(row16_sum(sum_sq(lo, hi)) + l2eps);
-            *(f32x4*)(s_k[d] + ch8) = lo * inv;
-            *(f32x4*)(s_k[d] + ch8 + 4) = hi * inv;
-        }
-        if (hv == hk * group && part == 0 && tid < 32) {   // the frames of q and k, once a k head
-            if (tid < 16) {
-                put_frames(c.f0, c.f1, c.f2, ch);
-            } else {
-                c.load(conv_w, seqs.frames[b], fresh, hk * GT_K + ch8);
-                put_frames(c.f0, c.f1, c.f2, hk * GT_K + ch8);
-            }
-        }
-    }
-    {   // this part's v, a token on 4 lanes
-        const int ch8 = 8 * (tid & 3), ch = (2 * n_kheads + hv) * GT_K + part * GC_ROWS + ch8;
-        Conv8 c;
-        c.load(conv_w, seqs.frames[b], fresh, ch);
-        for (int d = tid >> 2; d < n; d += GC_THREADS / 4) {
-            f32x4 lo, hi;
-            const f16x8 x3 = token(3 - d, row(d - 3, ch), c.f0, c.f1, c.f2);
-            const f16x8 x2 = token(2 - d, row(d - 2, ch), c.f0, c.f1, c.f2);
-            const f16x8 x1 = token(1 - d, row(d - 1, ch), c.f0, c.f1, c.f2);
-            c.apply(lo, hi, x3, x2, x1, *(const f16x8*)row(d, ch));
-            *(f32x4*)(s_v[d] + ch8) = lo;
-            *(f32x4*)(s_v[d] + ch8 + 4) = hi;
-        }
-        if (tid < 4) put_frames(c.f0, c.f1, c.f2, ch);
+    auto window = [&](int d, int ch, f16x8 f0, f16x8 f1, f16x8 f2) {
+        return Window8{token(3 - d, row(d - 3, ch), f0, f1, f2), token(2 - d, row(d - 2, ch), f0, f1, f2),
+                       token(1 - d, row(d - 1, ch), f0, f1, f2), *(const f16x8*)row(d, ch)};
+    };
+    auto form_k = [&](int d, const Window8& m) {
+        f32x4 lo, hi;
+        ck.apply(lo, hi, m.x3, m.x2, m.x1, m.x0);
+        const float inv = 1.f / sqrtf(row16_sum(sum_sq(lo, hi)) + l2eps);
+        *(f32x4*)(s_k[d] + k8) = lo * inv;
+        *(f32x4*)(s_k[d] + k8 + 4) = hi * inv;
+    };
+    auto form_v = [&](int d, const Window8& m) {
+        f32x4 lo, hi;
+        cv.apply(lo, hi, m.x3, m.x2, m.x1, m.x0);
+        *(f32x4*)(s_v[d] + v8) = lo;
+        *(f32x4*)(s_v[d] + v8 + 4) = hi;
+    };
+    // the first tokens' rows, then the state (row part ROWS + tid / 8): loads return in order
+    int dk = tid >> 4, dv = tid / VL;
+    Window8 mk, mv;
+    if (dk < n) mk = window(dk, ch_k, ck.f0, ck.f1, ck.f2);
+    if (dv < n) mv = window(dv, ch_v, cv.f0, cv.f1, cv.f2);
+    const size_t srow = ((size_t)hv * GT_K + part * ROWS + (tid >> 3)) * GT_K + 4 * (tid & 7);
+    f32x4 s[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] = *(const f32x4*)(seqs.S[b] + srow + 32 * j);
+    if (dk < n) form_k(dk, mk);
+    if (dv < n) form_v(dv, mv);
+    while ((dk += THREADS / 16) < n) form_k(dk, window(dk, ch_k, ck.f0, ck.f1, ck.f2));
+    while ((dv += THREADS / VL) < n) form_v(dv, window(dv, ch_v, cv.f0, cv.f1, cv.f2));
+    if (tid < VL) put_frames(cv.f0, cv.f1, cv.f2, ch_v);
+    if (hv == hk * group && part == 0 && tid < 32) {   // the frames of q and k, once a k head
+        const int ch = tid < 16 ? ch_k : hk * GT_K + k8;
+        if (tid >= 16) ck.load(conv_w, seqs.frames[b], fresh, ch);
+        put_frames(ck.f0, ck.f1, ck.f2, ch);
     }
     __syncthreads();
     for (int d = 0; d < n; ++d) {
         f32x4 k[4];
+        const float alpha = s_alpha[d];
         float m = 0.f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             k[j] = *(const f32x4*)(s_k[d] + 4 * (tid & 7) + 32 * j);
-            s[j] *= s_alpha[d];
+            s[j] *= alpha;
 #pragma unroll
             for (int e = 0; e < 4; ++e) m = fmaf(s[j][e], k[j][e], m);
         }
@@ -773,9 +777,10 @@ int fl_gdn_tree_commit(const void* x, int x_stride, const void* conv_w, const vo
         seqs.frames_out[i] = (f16*)cst_out[i];
         seqs.pos0[i] = pos0[i];
     }
-    hipLaunchKernelGGL(gdn_commit_kernel, dim3(B * n_vheads * (GT_K / GC_ROWS)), dim3(GC_THREADS), 0,
-                       (hipStream_t)stream, (const f16*)x, x_stride, (const f16*)conv_w, seqs, path, a, b,
-                       ab_stride, A_log, dt_bias, T, D, n_kheads, n_vheads, l2eps);
+    hipLaunchKernelGGL(gdn_commit_kernel, dim3(B * n_vheads * (GT_K / GC_ROWS)), dim3(8 * GC_ROWS),
+                       D * (GT_K + GC_ROWS) * sizeof(float), (hipStream_t)stream, (const f16*)x,
+                       x_stride, (const f16*)conv_w, seqs, path, a, b, ab_stride, A_log, dt_bias, T, D, n_kheads,
+                       n_vheads, l2eps);
     return fl::check_launch("gdn_tree_commit");
 }
 
