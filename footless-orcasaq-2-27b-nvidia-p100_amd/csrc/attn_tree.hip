@@ -16,10 +16,13 @@
 // that a captured call follows it. A sequence that lies in one run is finished there; a cut one leaves
 // a partial a piece, which the merge weighs.
 //
-// Measured, from a graph: 18 us for a tree of 16 on 500 rows, 67 us for 8 of them on 8192 (4.1 TB/s),
-// 197 us for 16 of 8 tokens on 16384 (5.5 TB/s, int8 237), 291 us for 4 of 63 on 20000 to 60000 (0.8 PFLOP/s), 136 us
-// for 12 of 26 on 100 to 32768 int8 rows. Small trees are bound by the cache's bytes, large ones
-// by what a SIMD does beside its MFMAs: of 3300 clocks a tile of 32 rows and 192 columns 1540 are MFMAs.
+// Measured, from a graph: 17 us for a tree of 16 on 500 rows, 61 us for 8 of them on 8192 (4.5 TB/s),
+// 193 us for 16 of 8 tokens on 16384 (5.6 TB/s, int8 227), 283 us for 4 of 63 on 20000 to 60000 (0.8 PFLOP/s),
+// 121 us for 12 of 26 on 100 to 32768 int8 rows. Small trees are bound by the cache's bytes; a large one's tile
+// of 32 rows and 192 columns takes 3100 clocks (int8 5000), of which MFMAs are 1540 (2300) and as many LDS
+// reads: the waves of a tile are in step, so that their softmaxes (and conversions) find no MFMAs to hide them.
+// Scores of the next tile under the softmax, two tiles a barrier and conversion under the product with V were
+// all built, and none was faster.
 #include "attn_paged.hpp"
 #include "tree.hpp"
 
@@ -34,8 +37,13 @@ constexpr int TT = 32;                  // rows a tile
 constexpr int ROW_B = 2 * PAGED_HD;     // bytes a row in LDS
 constexpr int TILE_B = TT * ROW_B;
 constexpr int STAGE_B = 2 * TILE_B;     // K | V
-constexpr int RUN_MIN = 4;              // tiles a run, at least
-constexpr int SEQ_COST = 2;             // a further piece's fixed cost in tiles
+// Tiles a run, at least: with one a tree of 16 on 2000 rows takes 25 us in place of 23 (more partials), with
+// six 4 trees of 32 on 1000 rows 42 us in place of 34 (CUs without work).
+constexpr int RUN_MIN = 3;
+// What a sequence's start costs in tiles, where there are several (its tree, plan, Q and first rows come one
+// behind another): counted as 2, 8 trees of 16 on 8192 rows take 68 us in place of 61, and 12 of 26 on ragged
+// int8 rows 141 us in place of 121; 12 is no better.
+constexpr int SEQ_COST = 8;
 
 // The chunk swizzle of tile row r: 16-byte chunk c lies at c ^ sw(r). A read of 16 bytes a lane takes
 // lanes 0 - 3, 12 - 15, 20 - 27 together, then 4 - 11, 16 - 19, 28 - 31, ...: 16 rows of K at chunk c
@@ -690,10 +698,14 @@ tree_merge_kernel(const Parts in, f16* __restrict__ z, int z_pitch, const f16* _
 struct TreeCut {
     int waves, groups, runs, run_min;
 };
-TreeCut tree_cut(int T, int n_q, int n_kv) {
+// Waves, of 16 columns each: as many as share a tile's copies without more registers than there are. (4 of
+// 63 on 20000 to 60000 rows: 287 us with twelve, 325 with eight; 12 of 26 on int8 rows: 142 and 189. 96 columns
+// on eight: 67 us, on twelve 75. 48 on four: 192, on eight 206, but over int8 pools, where the waves that copy
+// a tile convert it, 242 and 226.)
+TreeCut tree_cut(int T, int n_q, int n_kv, bool q8) {
     const int R = T * (n_q / n_kv);
     TreeCut c;
-    c.waves = R <= 64 ? 4 : R <= 128 ? 8 : 12;
+    c.waves = R <= 64 && !q8 ? 4 : R <= 128 ? 8 : 12;
     c.groups = (R + 16 * c.waves - 1) / (16 * c.waves);
     c.runs = std::max(1, cu_count() / (n_kv * c.groups));
     c.run_min = RUN_MIN;
@@ -718,7 +730,7 @@ extern "C" {
 size_t fl_attn_tree_paged_work_bytes(int B, int T, int n_q_heads, int n_kv_heads, int head_dim) {
     if (!tree_sizes(B, T, n_q_heads, n_kv_heads, head_dim)) return 0;
     Parts p;
-    return tree_parts(B, T, n_q_heads, tree_cut(T, n_q_heads, n_kv_heads).runs, nullptr, p);
+    return tree_parts(B, T, n_q_heads, tree_cut(T, n_q_heads, n_kv_heads, false).runs, nullptr, p);
 }
 
 int fl_attn_tree_paged(const void* qg, int q_pitch, const void* kpool, const void* vpool, int q8, int n_pages,
@@ -734,19 +746,19 @@ int fl_attn_tree_paged(const void* qg, int q_pitch, const void* kpool, const voi
     if (rc) return rc;
     FL_REQUIRE(pos0 && parents, "null pointer");
     FL_REQUIRE(tree_sizes(B, T, n_q_heads, n_kv_heads, head_dim), "1 <= T <= FL_TREE_MAX");
-    FL_REQUIRE((((long long)max_pages << pg.shift) / TT + 8) * B < INT_MAX, "B * max_pages * page_size < 2^36");
-    const TreeCut cut = tree_cut(T, n_q_heads, n_kv_heads);
+    FL_REQUIRE((((long long)max_pages << pg.shift) / TT + 16) * B < INT_MAX, "B * max_pages * page_size < 2^36");
+    const TreeCut cut = tree_cut(T, n_q_heads, n_kv_heads, q8);   // (as many runs either way)
     Parts parts;
     if (tree_parts(B, T, n_q_heads, cut.runs, (char*)work, parts) > work_bytes || !work) {
         fl::set_error("work: smaller than fl_attn_tree_paged_work_bytes");
         return FL_ESCRATCH;
     }
     FL_REQUIRE(aligned16(work), "16-byte aligned work");
-    auto kernel = cut.waves == 4 ? (q8 ? tree_attn_kernel<4, true> : tree_attn_kernel<4, false>)
+    auto kernel = cut.waves == 4   ? tree_attn_kernel<4, false>
                   : cut.waves == 8 ? (q8 ? tree_attn_kernel<8, true> : tree_attn_kernel<8, false>)
                                    : (q8 ? tree_attn_kernel<12, true> : tree_attn_kernel<12, false>);
-    hipLaunchKernelGGL(kernel, dim3(cut.runs * n_kv_heads * cut.groups), dim3(64 * cut.waves), 0, (hipStream_t)stream,
-                       (const f16*)qg, q_pitch, (const char*)kpool, (const char*)vpool, pg, pos0, parents, B, T,
+    hipLaunchKernelGGL(kernel, dim3(cut.runs * n_kv_heads * cut.groups), dim3(64 * cut.waves), 0,
+                       (hipStream_t)stream, (const f16*)qg, q_pitch, (const char*)kpool, (const char*)vpool, pg, pos0, parents, B, T,
                        n_q_heads, n_kv_heads, cut.groups, cut.runs, cut.run_min, scale * FL_LOG2E,
                        Sight{window, sinks}, (f16*)z, z_pitch, gated, parts);
     rc = fl::check_launch("attn_tree_paged");
