@@ -520,7 +520,8 @@ tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict
                     tile(j & 3, j);
                 }
             } else {
-                const uint32_t raw0 = (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)s_raw) + w * RAW_WAVE;
+                const uint32_t raw0 =
+                    (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)s_raw) + w * RAW_WAVE;
                 auto issue = [&](int j) {   // tile j0 + j, whose entry look() fetched
                     if (w >= CW) return;
                     const long long at = pool_row();
@@ -758,8 +759,8 @@ int fl_attn_tree_paged(const void* qg, int q_pitch, const void* kpool, const voi
                   : cut.waves == 8 ? (q8 ? tree_attn_kernel<8, true> : tree_attn_kernel<8, false>)
                                    : (q8 ? tree_attn_kernel<12, true> : tree_attn_kernel<12, false>);
     hipLaunchKernelGGL(kernel, dim3(cut.runs * n_kv_heads * cut.groups), dim3(64 * cut.waves), 0,
-                       (hipStream_t)stream, (const f16*)qg, q_pitch, (const char*)kpool, (const char*)vpool, pg, pos0, parents, B, T,
-                       n_q_heads, n_kv_heads, cut.groups, cut.runs, cut.run_min, scale * FL_LOG2E,
+                       (hipStream_t)stream, (const f16*)qg, q_pitch, (const char*)kpool, (const char*)vpool, pg, pos0,
+                       parents, B, T, n_q_heads, n_kv_heads, cut.groups, cut.runs, cut.run_min, scale * FL_LOG2E,
                        Sight{window, sinks}, (f16*)z, z_pitch, gated, parts);
     rc = fl::check_launch("attn_tree_paged");
     if (rc) return rc;

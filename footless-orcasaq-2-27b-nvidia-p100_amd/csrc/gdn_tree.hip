@@ -10,15 +10,21 @@
 //   o_i = s (G_i S0 q_i + sum_{j anc-or-self i} (G_i / G_j) (q_i . k_j) u_j),
 // so no token's state is ever formed: the first line is (I + A) U = R with A strictly lower
 // triangular, both need S0 only in products with all k_i and q_i. y_i is rmsnorm_gated of o_i.
-// Everything is fp32 (fp64: the sums of log alpha, whose differences are the logarithms of
+// Everything is held in fp32 (fp64: the sums of log alpha, whose differences are the logarithms of
 // G_i / G_j) and y is rounded once, where gdn_decode_normed rounds the conv's output, q, k and o to
-// fp16 as the reference does.
+// fp16 as the reference does. The products' operands are two scaled fp16 terms each, 22 bits: three
+// 16x16x32 MFMAs of 16 clocks take the place of eight fp32 ones of 32.
 //
-// A workgroup is a (sequence, v head); wave w has state rows 16 w .. + 15, held as the B operand of
-// 16x16x4 fp32 MFMAs whose accumulators are in turn the B operands of the next product: D's
-// register e of lane (g, c) is row 4 g + e of column c, and a k step takes k = 4 g + e from lane
-// group g on both sides. The 16-row diagonal blocks of I + A are inverted by substitution, a
-// column a lane; U is then a product a block.
+// A workgroup has the v heads of a k head, up to three: their q, k and products are formed once. A wave
+// has 16 or 32 of a head's state rows as the B operand, a row a column; the accumulators (register e of lane
+// (g, c) is token 4 g + e of column c) are in turn B operands of the 16x16x16 products with A and the
+// q.k side. The 16-row diagonal blocks of I + A are inverted by substitution, a column a lane.
+//
+// Measured, from a graph, 16 k and 48 v heads: a tree of 16 9.2 us, 4 of 37 15.5, 16 of 16 17, 16 of 9 to 37
+// 28, 8 of 64 36 us; a path of 4 committed 6.2 us, 16 of 7 26.5 us (3.9 TB/s of states read and written). The
+// trees are bound by instructions: of a workgroup's 44000 clocks (3 heads, 37 tokens) 10000 go by until the
+// first loads are here, and the rest is within a fifth of what its VALU and MFMA instructions take, three waves
+// a SIMD. S0's 50 MB alone would be 9 us.
 #include "tree.hpp"
 
 #include "gdn_gates.hpp"
@@ -32,8 +38,13 @@ typedef float f32x8 __attribute__((ext_vector_type(8)));
 constexpr int GT_K = 128;                // K = V
 constexpr int ROW_H = GT_K + 8;          // terms a row of k and q
 constexpr float QK_SCALE = 16384.f;      // of q and k, whose norms are at most 1
-constexpr int GT_MANY = 256;             // heads from which a workgroup takes several
-constexpr int GC_ROWS = 32;              // state rows that a workgroup moves on
+// Heads up to which a workgroup takes one, with 16 state rows a wave: a round of workgroups is the shorter one
+// then (240 heads of 16 tokens 9.5 us, by threes 14.9; of 37 tokens 16.0 and 25.4), two rounds are not
+// (288 heads 16.9 and 15.1; 29.4 and 25.6; 768 heads of 37: 44 and 27).
+constexpr int GT_MANY = 256;
+// State rows that a workgroup moves on (16 paths of 7: 26 to 27 us with 16 or 32, 28 with 64 or 128; 2 of 40
+// 16.0, 14.7, 13.4 and 18.8; one of 4 6.1, 6.2, 6.8 and 8.2)
+constexpr int GC_ROWS = 32;
 constexpr int BLOCK_P = 20;              // floats a row of a 16 x 16 block
 
 // Sum over the 16 lanes of a DPP row, on every one of them.
@@ -135,12 +146,12 @@ __device__ __forceinline__ Terms split8(f32x8 x, float s) {
     for (int e = 0; e < 8; ++e) r.lo[e] = (f16)fmaf(x[e], s, -(float)r.hi[e]);
     return r;
 }
-// The exponent that brings the largest of a column's entries to [2^14, 2^15): the four lanes of a column
-// have some each, the largest of which is `top`.
+// The exponent that brings the largest of a column's entries to [2^14, 2^15) (to less where all are below
+// 2^-60): the four lanes of a column have some each, the largest of which is `top`.
 __device__ __forceinline__ int lift(float top) {
     top = fmaxf(top, lane_xor(top, 16));
     top = pair32_max(top);
-    return 14 - min(max(ilogb_bits(top), -100), 100);
+    return 14 - min(max(ilogb_bits(top), -60), 126);
 }
 struct Terms4 {
     f16x4 hi, lo;
@@ -736,11 +747,15 @@ int fl_gdn_tree_normed(const void* x, int x_stride, const void* conv_w, const vo
                            l2eps, norm_eps);
     };
     const int nb = (T + 15) / 16;
-    const bool many = B * n_vheads > GT_MANY;
+    const bool many = B * n_vheads > GT_MANY;   // (beyond 48 tokens LDS holds one head's)
     if (nb <= 3 && many && group % 3 == 0)
-        launch(nb == 1 ? gdn_tree_kernel<1, 3, 2> : nb == 2 ? gdn_tree_kernel<2, 3, 2> : gdn_tree_kernel<3, 3, 2>, 3, 768);
+        launch(nb == 1   ? gdn_tree_kernel<1, 3, 2>
+               : nb == 2 ? gdn_tree_kernel<2, 3, 2>
+                         : gdn_tree_kernel<3, 3, 2>, 3, 768);
     else if (nb <= 3 && many && group % 2 == 0)
-        launch(nb == 1 ? gdn_tree_kernel<1, 2, 2> : nb == 2 ? gdn_tree_kernel<2, 2, 2> : gdn_tree_kernel<3, 2, 2>, 2, 512);
+        launch(nb == 1   ? gdn_tree_kernel<1, 2, 2>
+               : nb == 2 ? gdn_tree_kernel<2, 2, 2>
+                         : gdn_tree_kernel<3, 2, 2>, 2, 512);
     else
         launch(nb == 1   ? gdn_tree_kernel<1, 1, 1>
                : nb == 2 ? gdn_tree_kernel<2, 1, 1>

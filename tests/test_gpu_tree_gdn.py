@@ -87,6 +87,23 @@ def test_batches_of_several_heads_a_workgroup(fl, n_k, n_v, B, T):
     check(run(fl, d, parents, pos0), want, bound, f"{n_k} / {n_v} heads, B {B} T {T}")
 
 
+@pytest.mark.parametrize("state,values", [(0.0, 0.0), (0.0, 1.0), (1e-30, 0.0), (1e-30, 1e-3), (1e-6, 1.0),
+                                          (1e6, 1.0), (1e15, 0.0), (1e15, 1.0)])
+@pytest.mark.parametrize("B,T", [(1, 37), (6, 18)])
+def test_states_and_values_of_other_sizes(fl, B, T, state, values):
+    """Also rows of the state whose values are all 0 beside others: the scales of the terms are a row's."""
+    g = gen(B)
+    d = ref.gdn_layer(g, B, T)
+    for s in d["S"]:
+        s *= state * 20
+        s[:, ::5] = 0
+    d["conv_w"][2 * 16 * 128:] *= values
+    d["conv_w"][2 * 16 * 128::3] = 0
+    parents = [tree(g, T - b, T) for b in range(B)]
+    want, bound = ref.gdn_tree(d, parents, [False] * B)
+    check(run(fl, d, parents, [7] * B), want, bound, f"states {state}, values {values}")
+
+
 def test_places_without_a_token_do_not_matter(fl):
     """Whatever they hold: parents out of order or range, descendants of such places, NaN rows."""
     g = gen(8)
