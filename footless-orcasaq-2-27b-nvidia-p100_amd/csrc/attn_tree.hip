@@ -296,10 +296,9 @@ tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict
             if (lane == 0) s_whole[c & 1] = whole;
         };
         if (w == 0) {
-            double none = 0.;
             const int parent = parents[(size_t)b * T + min(lane, T - 1)];
             const int2 ids = j1 > j0 ? ids_of(0) : make_int2(0, 0);
-            const Node node = tree_node(parent, T, none);
+            const Node node = tree_node<false>(parent, T);
             present = __ballot(node.here());
             // a path's tokens are numbered upwards: out of the window are its first ones, but those
             // that count as first rows of the sequence
@@ -440,7 +439,7 @@ tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict
                     const float corr = fast_exp2(m_run - m_new);
                     m_run = m_new;
                     l_run *= corr;
-                    acc_scale(o, corr);
+                    if (j > 0) acc_scale(o, corr);   // (O is 0 till then)
                     weights();
                 }
                 l_run += sum;

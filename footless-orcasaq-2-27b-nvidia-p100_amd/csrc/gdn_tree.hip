@@ -284,7 +284,7 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
 
     if (w < HP) {
         double sum = lane < T ? (double)log_decay(a_in + dt, A) : 0.;
-        const Node n = tree_node(parent, T, sum);
+        const Node n = tree_node<true>(parent, T, &sum);
         // a place without a token has zeros everywhere: nothing of it reaches the others
         s_log[w][lane] = sum *= 1.4426950408889634;
         s_beta[w][lane] = n.here() ? gdn_beta(b_in) : 0.f;

@@ -34,8 +34,9 @@ struct Node {
 
 // Of a whole wave. Every round a token takes over what the token `up` has gathered and that
 // one's own `up`: 2^r ancestors after r rounds, as many rounds as the tree is deep in bits.
-// `sum` becomes its sum over the path to the token, itself included.
-__device__ __forceinline__ Node tree_node(int p, int T, double& sum) {   // p: lane i's parents[i]
+// `sum`, if there is one, becomes its sum over the path to the token, itself included.
+template <bool SUM>
+__device__ __forceinline__ Node tree_node(int p, int T, double* sum = nullptr) {   // p: lane i's parents[i]
     const int i = threadIdx.x & 63;
     if (i >= T) p = -2;
     const bool ok = p >= -1 && p < i;
@@ -45,8 +46,12 @@ __device__ __forceinline__ Node tree_node(int p, int T, double& sum) {   // p: l
         const int from = up >= 0 ? up : i;
         const uint32_t lo = lane_of((int)n.lo, from), hi = lane_of((int)n.hi, from);
         const int l = lane_of(lost, from), u = lane_of(up, from);
-        const double s = lane_of(sum, from);
-        if (up >= 0) n.lo |= lo, n.hi |= hi, lost |= l, sum += s, up = u;
+        double s = 0.;
+        if constexpr (SUM) s = lane_of(*sum, from);
+        if (up >= 0) {
+            n.lo |= lo, n.hi |= hi, lost |= l, up = u;
+            if constexpr (SUM) *sum += s;
+        }
     }
     if (lost) n.lo = n.hi = 0, n.parent = -1;
     return n;
