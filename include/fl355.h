@@ -477,7 +477,8 @@ int fl_attn_prep_axes(void* qg, int q_pitch, const void* k, const void* v, const
  * token and sequences at a negative pos0 give 0. qg [B][T][n_q_heads][q_pitch], z
  * [B][T][n_q_heads][z_pitch], the gate as fl_attn_decode_paged's; any n_q_heads / n_kv_heads. work:
  * fl_attn_tree_paged_work_bytes on the device that runs the call, 16-byte aligned, one for each call
- * that may overlap with another. The precision is the decode form's. */
+ * that may overlap with another. The precision is the decode form's. Rows that no token of a sequence sees
+ * may hold anything; an infinity or NaN in one that some token sees may reach the others. */
 size_t fl_attn_tree_paged_work_bytes(int B, int T, int n_q_heads, int n_kv_heads, int head_dim);
 int fl_attn_tree_paged(const void* qg, int q_pitch, const void* kpool, const void* vpool, int q8,
                        int n_pages, int page_size, const int* pages, int max_pages,
@@ -506,8 +507,10 @@ int fl_paged_kv_keep(void* const* kpools, void* const* vpools, int n_layers, int
 /* A GDN layer over trees: every token's conv window, decay and state follow its path from the
  * sequence's state S[b] and frames cst_in[b], which are only read; y[b][i] = rmsnorm_gated(o_i,
  * z[b][i], norm_w) of the token's output o_i (fl_gdn_decode_normed's formulas; here all of it in
- * 32 bits and y rounded once, so a chain's values are that call's but for its roundings). Places
- * without a token give 0. An infinity or NaN of one token may reach the others of its sequence.
+ * 32 bits, products from numbers of 22 bits, and y rounded once, so a chain's values are that call's
+ * but for its roundings). Places without a token give 0. An infinity or NaN of one token may reach the
+ * others of its sequence. The values do not depend on the other sequences, the number of them may move
+ * their last bits. y may not overlap another buffer of the call.
  * x [B][T][x_stride] f16 the raw q|k|v rows, a, b [B][T][ab_stride] f32, z [B][T][z_pitch], y
  * [B][T][y_pitch] f16, pos0 a host array (0: the frames are taken as zero); conv_w, S, cst_in,
  * A_log, dt_bias, norm_w as fl_gdn_decode_normed's. K == V == 128, B <= FL_MAX_SEQS, strides and
