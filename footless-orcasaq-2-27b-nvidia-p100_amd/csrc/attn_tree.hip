@@ -196,7 +196,8 @@ __device__ __forceinline__ void copy4_v(const char* vptr, uint32_t dst) {   // c
     asm volatile("s_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(vptr), "{m0}"(dst));
 }
 
-template <int W, bool Q8>
+// W waves, of which COPY only copy and convert tiles (0: the first ones do, beside their columns).
+template <int W, bool Q8, int COPY = 0>
 __global__ void __launch_bounds__(64 * W)
 tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict__ kp,
                  const char* __restrict__ vp, const Pages pg, const int* __restrict__ pos0s,
@@ -204,7 +205,9 @@ tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict
                  int run_min, float sl2, const Sight sight, f16* __restrict__ z, int z_pitch, int gated,
                  const Parts parts) {
     constexpr int STAGES = Q8 ? STAGES_Q8 : STAGES_F16;
-    constexpr int CW = W < 8 ? W : 8;                         // waves that copy
+    constexpr int COLW = W - COPY;                            // waves with columns
+    constexpr int CW = COPY ? COPY : W < 8 ? W : 8;           // waves that copy: C0 ..
+    constexpr int C0 = COPY ? COLW : 0;
     constexpr int ROWS = TT / CW;                             // a copying wave's rows of a tile
     constexpr int RAW_WAVE = 2 * ROWS * RAW_ROW;
     constexpr int COPIES = Q8 ? ROWS / 2 + 1 : ROWS;          // its copy instructions a tile
@@ -220,7 +223,8 @@ tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict
     __shared__ uint32_t s_here[2 * PLAN], s_seen[2 * PLAN];
     __shared__ uint64_t s_whole[2];
     const int tid = threadIdx.x, lane = tid & 63, w = uni(tid >> 6);
-    const int col = lane & 15, g = lane >> 4;
+    const int col = lane & 15, g = lane >> 4, cw = w - C0;
+    const bool copies = cw >= 0 && cw < CW;
     const int G = n_q / n_kv, R = T * G;
     const int cap = pg.max_pages << pg.shift;
     // Workgroups go to the 8 XCDs round-robin: the groups and kv heads of a run go to one of them, for
@@ -238,8 +242,7 @@ tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict
     if (!run.any) return;   // (the whole workgroup)
 
     // this lane's query row: of token t, or none
-    const int c0 = (grp * W + w) * 16, r_mine = c0 + col;
-    const bool busy = c0 < R;   // (wave-uniform)
+    const int c0 = w < COLW ? (grp * COLW + w) * 16 : R, r_mine = c0 + col;
     const int t = r_mine < R ? r_mine / G : -1;
     const int qrow = r_mine < R ? t * n_q + h * G + r_mine - t * G : 0;
     const uint32_t rsb = (Q8 ? PAGED_HD : ROW_B) * n_kv;   // bytes a pool row
@@ -320,6 +323,8 @@ tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict
             if (j1 > j0) plan(0, ids);
         }
         __syncthreads();
+        // (a padded batch's waves without a token have no products; wave-uniform)
+        const bool busy = __any(t >= 0 && s_lo[max(t, 0)] != INT_MAX);
         if (j1 > j0) {
             f16x8 q[8];
             f32x4 o[16];
@@ -463,12 +468,12 @@ tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict
             int e_row = 0;
             uint32_t e_seen = 0;
             auto look = [&](int j) {
-                if (w >= CW) return;
+                if (!copies) return;
                 const int at = min(j, n_tiles - 1) & (2 * PLAN - 1);
-                e_row = ROWS * w >= 16 ? s_rows[at].y : s_rows[at].x;
+                e_row = ROWS * cw >= 16 ? s_rows[at].y : s_rows[at].x;
                 e_seen = s_seen[at];
             };
-            auto pool_row = [&] { return (long long)uni(e_row) + (ROWS * w & 15); };
+            auto pool_row = [&] { return (long long)uni(e_row) + (ROWS * cw & 15); };
             // between two tiles: the plan of the next 64
             auto ahead = [&](int j) {
                 if (w == 0 && (j & (PLAN - 1)) == 0 && j + PLAN < n_tiles) plan(j / PLAN + 1, ids_of(j / PLAN + 1));
@@ -478,15 +483,15 @@ tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict
 #pragma unroll
                 for (int n = 0; n < ROWS / 2; ++n) {
                     const int r = 2 * n + (lane >> 5);
-                    loff[n] = r * rsb + 16 * ((lane & 31) ^ sw(ROWS * w + r));
+                    loff[n] = r * rsb + 16 * ((lane & 31) ^ sw(ROWS * cw + r));
                 }
                 auto issue = [&](int j) {   // tile j0 + j, whose entry look() fetched
-                    if (w >= CW) return;
+                    if (!copies) return;
                     const long long at = pool_row() * rsb;
                     const char *kr = uniform_ptr(kb + at), *vr = uniform_ptr(vb + at);
-                    const uint32_t d0 = uni(lds + (j & 3) * STAGE_B + ROWS * w * ROW_B);
+                    const uint32_t d0 = uni(lds + (j & 3) * STAGE_B + ROWS * cw * ROW_B);
                     // rows that no token sees may hold anything, and 0 x NaN is a NaN: zeros
-                    const uint32_t on = (uint32_t)uni((int)e_seen) >> (ROWS * w);
+                    const uint32_t on = (uint32_t)uni((int)e_seen) >> (ROWS * cw);
                     look(j + 1);
                     if ((on & ((1u << ROWS) - 1)) == (1u << ROWS) - 1) {
 #pragma unroll
@@ -520,9 +525,9 @@ tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict
                 }
             } else {
                 const uint32_t raw0 =
-                    (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)s_raw) + w * RAW_WAVE;
+                    (uint32_t)(uintptr_t)((__attribute__((address_space(3))) char*)s_raw) + cw * RAW_WAVE;
                 auto issue = [&](int j) {   // tile j0 + j, whose entry look() fetched
-                    if (w >= CW) return;
+                    if (!copies) return;
                     const long long at = pool_row();
                     look(j + 1);
                     int l = lane;
@@ -541,8 +546,8 @@ tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict
                     if (lane < 8 * ROWS) copy4_v(scales + so, d0 + 2 * ROWS * PAGED_HD);
                 };
                 auto convert = [&](int j) {   // this wave's rows of tile j0 + j to its stage
-                    if (w >= CW) return;
-                    const char* raw = s_raw + (j % RAW_STAGES) * (CW * RAW_WAVE) + w * RAW_WAVE;
+                    if (!copies) return;
+                    const char* raw = s_raw + (j % RAW_STAGES) * (CW * RAW_WAVE) + cw * RAW_WAVE;
                     const uint32_t on = s_seen[j & (2 * PLAN - 1)];
                     const int stage = j & 1;
                     int l = lane;
@@ -554,7 +559,7 @@ tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict
                         const u32x4 kx = *(const u32x4*)(raw + 1024 * n + 16 * l);
                         const u32x4 vx = *(const u32x4*)(raw + ROWS * PAGED_HD + 1024 * n + 16 * l);
                         const f16 ks = sc[0], vs = sc[8 * ROWS];
-                        const int r = ROWS * w + 4 * n + g;
+                        const int r = ROWS * cw + 4 * n + g;
                         // rows that no token sees may hold any scale: theirs is 0
                         const f16 v = on >> r & 1 ? vs : (f16)0.f;
                         char* at = s_tile + stage * STAGE_B + r * ROW_B;
@@ -592,7 +597,7 @@ tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict
                     }
                 }
             }
-            if (busy) {
+            if (c0 < R) {
                 acc_settle(o);
                 float l = l_run;
                 l += lane_xor(l, 16);
@@ -699,13 +704,12 @@ struct TreeCut {
     int waves, groups, runs, run_min;
 };
 // Waves, of 16 columns each: as many as share a tile's copies without more registers than there are. (4 of
-// 63 on 20000 to 60000 rows: 287 us with twelve, 325 with eight; 12 of 26 on int8 rows: 142 and 189. 96 columns
-// on eight: 67 us, on twelve 75. 48 on four: 192, on eight 206, but over int8 pools, where the waves that copy
-// a tile convert it, 242 and 226.)
-TreeCut tree_cut(int T, int n_q, int n_kv, bool q8) {
+// 63 on 20000 to 60000 rows: 287 us with twelve, 325 with eight; 96 columns on eight: 67 us, on twelve 75; 48 on
+// four: 192, on eight 206.) Over int8 pools four more waves copy and convert where there is room for them.
+TreeCut tree_cut(int T, int n_q, int n_kv) {
     const int R = T * (n_q / n_kv);
     TreeCut c;
-    c.waves = R <= 64 && !q8 ? 4 : R <= 128 ? 8 : 12;
+    c.waves = R <= 64 ? 4 : R <= 128 ? 8 : 12;
     c.groups = (R + 16 * c.waves - 1) / (16 * c.waves);
     c.runs = std::max(1, cu_count() / (n_kv * c.groups));
     c.run_min = RUN_MIN;
@@ -730,7 +734,7 @@ extern "C" {
 size_t fl_attn_tree_paged_work_bytes(int B, int T, int n_q_heads, int n_kv_heads, int head_dim) {
     if (!tree_sizes(B, T, n_q_heads, n_kv_heads, head_dim)) return 0;
     Parts p;
-    return tree_parts(B, T, n_q_heads, tree_cut(T, n_q_heads, n_kv_heads, false).runs, nullptr, p);
+    return tree_parts(B, T, n_q_heads, tree_cut(T, n_q_heads, n_kv_heads).runs, nullptr, p);
 }
 
 int fl_attn_tree_paged(const void* qg, int q_pitch, const void* kpool, const void* vpool, int q8, int n_pages,
@@ -747,17 +751,18 @@ int fl_attn_tree_paged(const void* qg, int q_pitch, const void* kpool, const voi
     FL_REQUIRE(pos0 && parents, "null pointer");
     FL_REQUIRE(tree_sizes(B, T, n_q_heads, n_kv_heads, head_dim), "1 <= T <= FL_TREE_MAX");
     FL_REQUIRE((((long long)max_pages << pg.shift) / TT + 16) * B < INT_MAX, "B * max_pages * page_size < 2^36");
-    const TreeCut cut = tree_cut(T, n_q_heads, n_kv_heads, q8);   // (as many runs either way)
+    const TreeCut cut = tree_cut(T, n_q_heads, n_kv_heads);
     Parts parts;
     if (tree_parts(B, T, n_q_heads, cut.runs, (char*)work, parts) > work_bytes || !work) {
         fl::set_error("work: smaller than fl_attn_tree_paged_work_bytes");
         return FL_ESCRATCH;
     }
     FL_REQUIRE(aligned16(work), "16-byte aligned work");
-    auto kernel = cut.waves == 4   ? tree_attn_kernel<4, false>
-                  : cut.waves == 8 ? (q8 ? tree_attn_kernel<8, true> : tree_attn_kernel<8, false>)
+    const int copy = q8 && cut.waves < 12 ? 4 : 0;
+    auto kernel = cut.waves == 4   ? (q8 ? tree_attn_kernel<8, true, 4> : tree_attn_kernel<4, false>)
+                  : cut.waves == 8 ? (q8 ? tree_attn_kernel<12, true, 4> : tree_attn_kernel<8, false>)
                                    : (q8 ? tree_attn_kernel<12, true> : tree_attn_kernel<12, false>);
-    hipLaunchKernelGGL(kernel, dim3(cut.runs * n_kv_heads * cut.groups), dim3(64 * cut.waves), 0,
+    hipLaunchKernelGGL(kernel, dim3(cut.runs * n_kv_heads * cut.groups), dim3(64 * (cut.waves + copy)), 0,
                        (hipStream_t)stream, (const f16*)qg, q_pitch, (const char*)kpool, (const char*)vpool, pg, pos0,
                        parents, B, T, n_q_heads, n_kv_heads, cut.groups, cut.runs, cut.run_min, scale * FL_LOG2E,
                        Sight{window, sinks}, (f16*)z, z_pitch, gated, parts);
