@@ -16,13 +16,14 @@
 // that a captured call follows it. A sequence that lies in one run is finished there; a cut one leaves
 // a partial a piece, which the merge weighs.
 //
-// Measured, from a graph: 17 us for a tree of 16 on 500 rows, 61 us for 8 of them on 8192 (4.5 TB/s),
-// 193 us for 16 of 8 tokens on 16384 (5.6 TB/s, int8 227), 283 us for 4 of 63 on 20000 to 60000 (0.8 PFLOP/s),
-// 121 us for 12 of 26 on 100 to 32768 int8 rows. Small trees are bound by the cache's bytes; a large one's tile
-// of 32 rows and 192 columns takes 3100 clocks (int8 5000), of which MFMAs are 1540 (2300) and as many LDS
-// reads: the waves of a tile are in step, so that their softmaxes (and conversions) find no MFMAs to hide them.
-// Scores of the next tile under the softmax, two tiles a barrier and conversion under the product with V were
-// all built, and none was faster.
+// Measured, from a graph: a tree of 16 on 500 rows 17 us, 8 of them on 8192 62 us (4.4 TB/s, int8 73 us), 16 of 8
+// tokens on 16384 196 us (5.5 TB/s, int8 174), 4 of 63 on 20000 to 60000 281 us (0.83 PFLOP/s), 12 of 5 to 26 on
+// 100 to 32768 int8 rows 117 us. Small trees are bound by the cache's bytes, and by what comes ahead of the first
+// tile and behind the last (a sequence's tree, plan and first rows 10 us one behind another, the partials' merge
+// 4 to 12); a large one's tile of 32 rows and 192 columns takes 3100 clocks (int8 5000), of which MFMAs are 1540
+// (2300) and LDS reads as many: a tile's waves are in step and use both at once. Scores of the next tile under the
+// softmax, two tiles a barrier, an int8 tile's conversion under the products with V, and waves that convert
+// ahead of their products beside waves that do behind them were all built, and none was faster.
 #include "attn_paged.hpp"
 #include "tree.hpp"
 
@@ -705,7 +706,8 @@ struct TreeCut {
 };
 // Waves, of 16 columns each: as many as share a tile's copies without more registers than there are. (4 of
 // 63 on 20000 to 60000 rows: 287 us with twelve, 325 with eight; 96 columns on eight: 67 us, on twelve 75; 48 on
-// four: 192, on eight 206.) Over int8 pools four more waves copy and convert where there is room for them.
+// four: 192, on eight 206.) Over int8 pools four more waves copy and convert where there is room for them (48
+// columns on 16384 rows: 174 us, with waves that do both 227, with eight more 183; 96 on 8192: 73, 85).
 TreeCut tree_cut(int T, int n_q, int n_kv) {
     const int R = T * (n_q / n_kv);
     TreeCut c;

@@ -7,6 +7,8 @@ import paged_tight as tight
 import tree_ref
 from test_gpu_paged import SCALE, filled, gen, i32, randn
 from test_gpu_tree_attention import check as check_z, run as run_attention, seen_by
+from test_gpu_tree_cache import (test_axes_that_hold_the_sequences_positions_give_the_plain_prep as plain_prep,
+                                 test_every_pair_turns_by_its_own_axis as every_pair)
 from test_gpu_tree_gdn import check, commit, run as run_gdn, tree
 
 pytestmark = pytest.mark.gpu
@@ -43,6 +45,16 @@ def test_other_trees_over_one_context(fl, dev, kv8):
         want, bound = tight.attention(q[b][here][..., :256], K[idx], V[idx], seen_by(trees[b], c)[here], SCALE,
                                       tight.TWO_TERMS if kv8 else tight.ONE_TERM, q[b][here][..., 256:])
         check_z(z[b][here], want, bound, f"tree {b}")
+
+
+@pytest.mark.parametrize("N", [511, 512, 1001])
+def test_many_tokens_turn_by_several_axes(fl, N):
+    every_pair(fl, N, (11, 11, 10), True)
+
+
+@pytest.mark.parametrize("kv8", [False, True])
+def test_axes_prep_of_many_tokens_is_the_plain_one(fl, kv8):
+    plain_prep(fl, [(300, 0), (255, 17), (400, 1000)], 3, (12, 10, 10), False, kv8)
 
 
 def gdn_batch(seed, B, T):
