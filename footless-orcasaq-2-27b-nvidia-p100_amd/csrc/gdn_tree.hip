@@ -22,9 +22,10 @@
 //
 // Measured, from a graph, 16 k and 48 v heads: a tree of 16 9.2 us, 4 of 37 15.5, 16 of 16 17, 16 of 9 to 37
 // 28, 8 of 64 36 us; a path of 4 committed 6.2 us, 16 of 7 26.5 us (3.9 TB/s of states read and written). The
-// trees are bound by instructions: of a workgroup's 44000 clocks (3 heads, 37 tokens) 10000 go by until the
-// first loads are here, and the rest is within a fifth of what its VALU and MFMA instructions take, three waves
-// a SIMD. S0's 50 MB alone would be 9 us.
+// trees are bound by a workgroup's chain of phases, each between two barriers: of 43000 clocks (3 heads, 9 to 37
+// tokens) 14000 until the tokens' rows are here and half of S0 is on its way, 9000 the conv, 4000 A and the q.k
+// side, 10000 the products with S0, 4500 the system, 2000 the norm; VALU instructions are a quarter of it, MFMAs
+// less than a tenth. S0's 50 MB alone would be 10 us.
 #include "tree.hpp"
 
 #include "gdn_gates.hpp"
