@@ -65,4 +65,4 @@ def test_nothing_reads_an_accumulator_ahead_of_its_waits(tmp_path):
             if not app and not settled and any(agprs(x) & O for x in reads):
                 raise AssertionError(f"{name}: {op} {', '.join(ops)} reads an accumulator that may be in flight")
         found += 1
-    assert found == 5
+    assert found >= 5
