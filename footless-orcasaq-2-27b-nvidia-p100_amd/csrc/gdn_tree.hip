@@ -106,12 +106,6 @@ struct Frames8 {
         if (fresh) f0 = f1 = f2 = (f16x8)(0);
     }
 };
-struct Conv8 : Taps8, Frames8 {
-    __device__ __forceinline__ void load(const f16* conv_w, const f16* frames, bool fresh, int ch) {
-        Taps8::load(conv_w, ch);
-        Frames8::load(frames, fresh, ch);
-    }
-};
 // The row at `row`, or the frame n > 0 tokens ahead of a path's first: n = 1 is the newest. (By
 // value: with the frames behind a reference the choice becomes one of addresses, in scratch.)
 __device__ __forceinline__ f16x8 token(int n, const f16* row, f16x8 f0, f16x8 f1, f16x8 f2) {
@@ -581,22 +575,19 @@ __device__ __forceinline__ float row8_sum(float v) {
     return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x141, 0xF, 0xF, true));   // half mirror
 }
 
-// A token's conv input: its own row and the three before it.
-struct Window8 {
-    f16x8 x3, x2, x1, x0;
-};
-
 __global__ void __launch_bounds__(8 * GC_ROWS)
 gdn_commit_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__ conv_w, const CommitSeqs seqs,
                   const int* __restrict__ path, const float* __restrict__ ga, const float* __restrict__ gb,
                   int ab_stride, const float* __restrict__ A_log, const float* __restrict__ dt_bias, int T, int D,
                   int n_kheads, int n_vheads, float l2eps) {
     constexpr int ROWS = GC_ROWS, THREADS = 8 * ROWS, PARTS = GT_K / ROWS, VL = ROWS / 8;   // lanes a token's v takes
-    extern __shared__ __attribute__((aligned(16))) float s_kv[];            // [D][128] of k, [D][ROWS] of v
-    __shared__ float s_beta[TREE_MAX], s_alpha[TREE_MAX];
+    extern __shared__ __attribute__((aligned(16))) float s_kv[];            // [D][128] of k, [D][ROWS] of v,
+    __shared__ float s_beta[TREE_MAX], s_alpha[TREE_MAX];                   // and their input's rows
     __shared__ int s_at[TREE_MAX], s_n;
     float(*s_k)[GT_K] = (float(*)[GT_K])s_kv;
     float(*s_v)[ROWS] = (float(*)[ROWS])(s_kv + D * GT_K);
+    f16(*x_k)[GT_K] = (f16(*)[GT_K])(s_kv + D * (GT_K + ROWS));   // three frames, then the path's tokens
+    f16(*x_v)[ROWS] = (f16(*)[ROWS])(x_k + D + 3);
     const int tid = threadIdx.x;
     const int part = blockIdx.x % PARTS, hv = blockIdx.x / PARTS % n_vheads, b = blockIdx.x / PARTS / n_vheads;
     const int group = n_vheads / n_kheads, hk = hv / group;
@@ -617,58 +608,75 @@ gdn_commit_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict
     }
     const int k8 = 8 * (tid & 15), v8 = 8 * (tid & (VL - 1));   // k: a token on 16 lanes
     const int ch_k = (n_kheads + hk) * GT_K + k8, ch_v = (2 * n_kheads + hv) * GT_K + part * ROWS + v8;
-    Conv8 ck, cv;
-    ck.load(conv_w, seqs.frames[b], fresh, ch_k);
-    cv.load(conv_w, seqs.frames[b], fresh, ch_v);
+    if (tid >= 64 && tid < 80) {
+        Frames8 old;
+        old.load(seqs.frames[b], fresh, ch_k);
+        *(f16x8*)(x_k[0] + k8) = old.f0, *(f16x8*)(x_k[1] + k8) = old.f1, *(f16x8*)(x_k[2] + k8) = old.f2;
+    }
+    if (tid >= 128 && tid < 128 + VL) {
+        Frames8 old;
+        old.load(seqs.frames[b], fresh, ch_v);
+        *(f16x8*)(x_v[0] + v8) = old.f0, *(f16x8*)(x_v[1] + v8) = old.f1, *(f16x8*)(x_v[2] + v8) = old.f2;
+    }
+    Taps8 tk, tv;
+    tk.load(conv_w, ch_k);
+    tv.load(conv_w, ch_v);
     __syncthreads();
     const int n = s_n;
 
-    // Token d of the frames and the path as one row of tokens: d < 0 are frames.
+    // the tokens' rows, then the state (row part ROWS + tid / 8): loads return in order
     const f16* xb = x + (size_t)b * T * x_stride;
-    auto row = [&](int d, int ch) { return xb + (size_t)s_at[max(d, 0)] * x_stride + ch; };
-    auto put_frames = [&](f16x8 f0, f16x8 f1, f16x8 f2, int ch) {   // [channel][frame] of the last three
-        const f16x8 x = token(3 - n, row(n - 3, ch), f0, f1, f2);
-        const f16x8 y = token(2 - n, row(n - 2, ch), f0, f1, f2), z = token(1 - n, row(n - 1, ch), f0, f1, f2);
+    auto row_k = [&](int d) { return *(const f16x8*)(xb + (size_t)s_at[d] * x_stride + ch_k); };
+    auto row_v = [&](int d) { return *(const f16x8*)(xb + (size_t)s_at[d] * x_stride + ch_v); };
+    int dk = tid >> 4, dv = tid / VL;
+    f16x8 rk, rv;
+    if (dk < n) rk = row_k(dk);
+    if (dv < n) rv = row_v(dv);
+    const size_t srow = ((size_t)hv * GT_K + part * ROWS + (tid >> 3)) * GT_K + 4 * (tid & 7);
+    f32x4 s[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) s[j] = *(const f32x4*)(seqs.S[b] + srow + 32 * j);
+    if (dk < n) *(f16x8*)(x_k[dk + 3] + k8) = rk;
+    if (dv < n) *(f16x8*)(x_v[dv + 3] + v8) = rv;
+    while ((dk += THREADS / 16) < n) *(f16x8*)(x_k[dk + 3] + k8) = row_k(dk);
+    while ((dv += THREADS / VL) < n) *(f16x8*)(x_v[dv + 3] + v8) = row_v(dv);
+    __syncthreads();
+
+    auto put_frames = [&](f16x8 x, f16x8 y, f16x8 z, int ch) {   // [channel][frame] of the last three
         f16x8* to = (f16x8*)(seqs.frames_out[b] + 3 * ch);
         to[0] = (f16x8){x[0], y[0], z[0], x[1], y[1], z[1], x[2], y[2]};
         to[1] = (f16x8){z[2], x[3], y[3], z[3], x[4], y[4], z[4], x[5]};
         to[2] = (f16x8){y[5], z[5], x[6], y[6], z[6], x[7], y[7], z[7]};
     };
-    auto window = [&](int d, int ch, f16x8 f0, f16x8 f1, f16x8 f2) {
-        return Window8{token(3 - d, row(d - 3, ch), f0, f1, f2), token(2 - d, row(d - 2, ch), f0, f1, f2),
-                       token(1 - d, row(d - 1, ch), f0, f1, f2), *(const f16x8*)row(d, ch)};
-    };
-    auto form_k = [&](int d, const Window8& m) {
+    for (int d = tid >> 4; d < n; d += THREADS / 16) {
         f32x4 lo, hi;
-        ck.apply(lo, hi, m.x3, m.x2, m.x1, m.x0);
+        auto at = [&](int r) { return *(const f16x8*)(x_k[d + r] + k8); };
+        tk.apply(lo, hi, at(0), at(1), at(2), at(3));
         const float inv = 1.f / sqrtf(row16_sum(sum_sq(lo, hi)) + l2eps);
         *(f32x4*)(s_k[d] + k8) = lo * inv;
         *(f32x4*)(s_k[d] + k8 + 4) = hi * inv;
-    };
-    auto form_v = [&](int d, const Window8& m) {
+    }
+    for (int d = tid / VL; d < n; d += THREADS / VL) {
         f32x4 lo, hi;
-        cv.apply(lo, hi, m.x3, m.x2, m.x1, m.x0);
+        auto at = [&](int r) { return *(const f16x8*)(x_v[d + r] + v8); };
+        tv.apply(lo, hi, at(0), at(1), at(2), at(3));
         *(f32x4*)(s_v[d] + v8) = lo;
         *(f32x4*)(s_v[d] + v8 + 4) = hi;
-    };
-    // the first tokens' rows, then the state (row part ROWS + tid / 8): loads return in order
-    int dk = tid >> 4, dv = tid / VL;
-    Window8 mk, mv;
-    if (dk < n) mk = window(dk, ch_k, ck.f0, ck.f1, ck.f2);
-    if (dv < n) mv = window(dv, ch_v, cv.f0, cv.f1, cv.f2);
-    const size_t srow = ((size_t)hv * GT_K + part * ROWS + (tid >> 3)) * GT_K + 4 * (tid & 7);
-    f32x4 s[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) s[j] = *(const f32x4*)(seqs.S[b] + srow + 32 * j);
-    if (dk < n) form_k(dk, mk);
-    if (dv < n) form_v(dv, mv);
-    while ((dk += THREADS / 16) < n) form_k(dk, window(dk, ch_k, ck.f0, ck.f1, ck.f2));
-    while ((dv += THREADS / VL) < n) form_v(dv, window(dv, ch_v, cv.f0, cv.f1, cv.f2));
-    if (tid < VL) put_frames(cv.f0, cv.f1, cv.f2, ch_v);
-    if (hv == hk * group && part == 0 && tid < 32) {   // the frames of q and k, once a k head
-        const int ch = tid < 16 ? ch_k : hk * GT_K + k8;
-        if (tid >= 16) ck.load(conv_w, seqs.frames[b], fresh, ch);
-        put_frames(ck.f0, ck.f1, ck.f2, ch);
+    }
+    auto last = [&](int r) { return *(const f16x8*)(x_v[n + r] + v8); };
+    if (tid < VL) put_frames(last(0), last(1), last(2), ch_v);
+    if (hv == hk * group && part == 0) {   // the frames of q and k, once a k head
+        auto last = [&](int r) { return *(const f16x8*)(x_k[n + r] + k8); };
+        if (tid >= 64 && tid < 80) put_frames(last(0), last(1), last(2), ch_k);
+        if (tid >= 128 && tid < 144) {
+            const int ch = hk * GT_K + k8;
+            Frames8 old;
+            old.load(seqs.frames[b], fresh, ch);
+            auto row = [&](int d) { return xb + (size_t)s_at[max(d, 0)] * x_stride + ch; };
+            put_frames(token(3 - n, row(n - 3), old.f0, old.f1, old.f2),
+                       token(2 - n, row(n - 2), old.f0, old.f1, old.f2),
+                       token(1 - n, row(n - 1), old.f0, old.f1, old.f2), ch);
+        }
     }
     __syncthreads();
     for (int d = 0; d < n; ++d) {
@@ -794,7 +802,7 @@ int fl_gdn_tree_commit(const void* x, int x_stride, const void* conv_w, const vo
         seqs.pos0[i] = pos0[i];
     }
     hipLaunchKernelGGL(gdn_commit_kernel, dim3(B * n_vheads * (GT_K / GC_ROWS)), dim3(8 * GC_ROWS),
-                       D * (GT_K + GC_ROWS) * sizeof(float), (hipStream_t)stream, (const f16*)x,
+                       (D * 6 + 6) * (GT_K + GC_ROWS), (hipStream_t)stream, (const f16*)x,
                        x_stride, (const f16*)conv_w, seqs, path, a, b, ab_stride, A_log, dt_bias, T, D, n_kheads,
                        n_vheads, l2eps);
     return fl::check_launch("gdn_tree_commit");
