@@ -21,7 +21,7 @@
 // q.k side. The 16-row diagonal blocks of I + A are inverted by substitution, a column a lane.
 //
 // Measured, from a graph, 16 k and 48 v heads: a tree of 16 9.2 us, 4 of 37 15.5, 16 of 16 17, 16 of 9 to 37
-// 28, 8 of 64 36 us; a path of 4 committed 6.2 us, 16 of 7 26.5 us (3.9 TB/s of states read and written). The
+// 28, 8 of 64 36 us; a path of 4 committed 5.4 us, 16 of 7 22.6 us (4.6 TB/s of states read and written). The
 // trees are bound by a workgroup's chain of phases, each between two barriers: of 43000 clocks (3 heads, 9 to 37
 // tokens) 14000 until the tokens' rows are here and half of S0 is on its way, 9000 the conv, 4000 A and the q.k
 // side, 10000 the products with S0, 4500 the system, 2000 the norm; VALU instructions are a quarter of it, MFMAs
@@ -43,8 +43,8 @@ constexpr float QK_SCALE = 16384.f;      // of q and k, whose norms are at most 
 // then (240 heads of 16 tokens 9.5 us, by threes 14.9; of 37 tokens 16.0 and 25.4), two rounds are not
 // (288 heads 16.9 and 15.1; 29.4 and 25.6; 768 heads of 37: 44 and 27).
 constexpr int GT_MANY = 256;
-// State rows that a workgroup moves on (16 paths of 7: 26 to 27 us with 16 or 32, 28 with 64 or 128; 2 of 40
-// 16.0, 14.7, 13.4 and 18.8; one of 4 6.1, 6.2, 6.8 and 8.2)
+// State rows that a workgroup moves on (measured with the conv's input in registers yet, 16, 32, 64 and 128
+// rows: 16 paths of 7 25.9, 26.9, 28.4 and 28.4 us; 2 of 40 16.0, 14.7, 13.4 and 18.8; one of 4 6.1, 6.2, 6.8, 8.2)
 constexpr int GC_ROWS = 32;
 constexpr int BLOCK_P = 20;              // floats a row of a 16 x 16 block
 
@@ -79,17 +79,18 @@ struct Taps8 {
         w3 = (f16x8){a[3], a[7], b[3], b[7], c[3], c[7], d[3], d[7]};
     }
     // silu of the taps over x0 (the token's) and the three before it
-    __device__ __forceinline__ float channel(int c, f16x8 x3, f16x8 x2, f16x8 x1, f16x8 x0, float zero) const {
-        float s = fmaf((float)w0[c], (float)x3[c], zero);
-        s = fmaf((float)w1[c], (float)x2[c], s);
-        s = fmaf((float)w2[c], (float)x1[c], s);
-        s = fmaf((float)w3[c], (float)x0[c], s);
-        return s * __builtin_amdgcn_rcpf(1.f + hw_expf(-s));
-    }
     __device__ __forceinline__ void apply(f32x4& lo, f32x4& hi, f16x8 x3, f16x8 x2, f16x8 x1, f16x8 x0) const {
+        // (a mixed fma takes its halves as they are: they are neither converted here nor ahead of a loop)
+        f16x8 v0 = w0, v1 = w1, v2 = w2, v3 = w3;
         float zero = 0.f;
-        asm("" : "+v"(zero));   // (a mixed fma takes both halves as they are, a product would convert them)
-        auto y = [&](int c) { return channel(c, x3, x2, x1, x0, zero); };
+        asm("" : "+v"(v0), "+v"(v1), "+v"(v2), "+v"(v3), "+v"(zero));
+        auto y = [&](int c) {
+            float s = fmaf((float)v0[c], (float)x3[c], zero);
+            s = fmaf((float)v1[c], (float)x2[c], s);
+            s = fmaf((float)v2[c], (float)x1[c], s);
+            s = fmaf((float)v3[c], (float)x0[c], s);
+            return s * __builtin_amdgcn_rcpf(1.f + hw_expf(-s));
+        };
         lo = (f32x4){y(0), y(1), y(2), y(3)};
         hi = (f32x4){y(4), y(5), y(6), y(7)};
     }
@@ -575,7 +576,8 @@ __device__ __forceinline__ float row8_sum(float v) {
     return v + __int_as_float(__builtin_amdgcn_mov_dpp(__float_as_int(v), 0x141, 0xF, 0xF, true));   // half mirror
 }
 
-__global__ void __launch_bounds__(8 * GC_ROWS)
+// (five waves a SIMD: 22.6 us for 16 paths of 7, with the registers of four 23.5, six spill)
+__global__ void __launch_bounds__(8 * GC_ROWS, 5)
 gdn_commit_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__ conv_w, const CommitSeqs seqs,
                   const int* __restrict__ path, const float* __restrict__ ga, const float* __restrict__ gb,
                   int ab_stride, const float* __restrict__ A_log, const float* __restrict__ dt_bias, int T, int D,
