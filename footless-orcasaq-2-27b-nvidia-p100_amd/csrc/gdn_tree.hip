@@ -20,8 +20,8 @@
 // (g, c) is token 4 g + e of column c) are in turn B operands of the 16x16x16 products with A and the
 // q.k side. The 16-row diagonal blocks of I + A are inverted by substitution, a column a lane.
 //
-// Measured, from a graph, 16 k and 48 v heads: a tree of 16 9.2 us, 4 of 37 15.5, 16 of 16 17, 16 of 9 to 37
-// 28, 8 of 64 36 us; a path of 4 committed 5.4 us, 16 of 7 22.6 us (4.6 TB/s of states read and written). The
+// Measured, from a graph, 16 k and 48 v heads: a tree of 16 8.5 us, 4 of 37 15, 16 of 16 17, 16 of 9 to 37
+// 28, 8 of 64 35 us; a path of 4 committed 5.4 us, 16 of 7 22.6 us (4.6 TB/s of states read and written). The
 // trees are bound by a workgroup's chain of phases, each between two barriers: of 43000 clocks (3 heads, 9 to 37
 // tokens) 14000 until the tokens' rows are here and half of S0 is on its way, 9000 the conv, 4000 A and the q.k
 // side, 10000 the products with S0, 4500 the system, 2000 the norm; VALU instructions are a quarter of it, MFMAs
@@ -276,7 +276,9 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
 #pragma unroll
         for (int c = 0; c < 4; ++c) s0[t][c] = *(const f32x8*)(srow + 16 * t * GT_K + 32 * c);
     };
-    load_s0(0);
+    // (half of it now where there is much of it: 16 trees of 16 17.0 us in place of 18.3; by one head a workgroup the
+    // rows come sooner without, one tree of 16 8.5 us in place of 9.2)
+    if (TL > 1) load_s0(0);
 
     if (w < HP) {
         double sum = lane < T ? (double)log_decay(a_in + dt, A) : 0.;
@@ -310,7 +312,7 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
     __syncthreads();
     const int n = __builtin_amdgcn_readfirstlane(s_n), nb = (n + 15) >> 4;   // tokens, blocks of them
 #pragma unroll
-    for (int t = 1; t < TL; ++t) load_s0(t);
+    for (int t = TL > 1; t < TL; ++t) load_s0(t);
 
     auto conv_of = [&](const Taps8& taps, const f16* at, int pitch, int i, f32x4& lo, f32x4& hi) {
         const int4 up = s_up[i];
