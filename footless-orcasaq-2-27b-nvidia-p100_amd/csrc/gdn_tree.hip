@@ -20,8 +20,8 @@
 // (g, c) is token 4 g + e of column c) are in turn B operands of the 16x16x16 products with A and the
 // q.k side. The 16-row diagonal blocks of I + A are inverted by substitution, a column a lane.
 //
-// Measured, from a graph, 16 k and 48 v heads: a tree of 16 8.5 us, 4 of 37 15, 16 of 16 17, 16 of 9 to 37
-// 28, 8 of 64 35 us; a path of 4 committed 5.4 us, 16 of 7 22.6 us (4.6 TB/s of states read and written). The
+// Measured, from a graph, 16 k and 48 v heads: a tree of 16 8.3 us, 4 of 37 14, 16 of 16 17, 16 of 9 to 37
+// 27, 8 of 64 34 us; a path of 4 committed 5.2 us, 16 of 7 22.3 us (4.7 TB/s of states read and written). The
 // trees are bound by a workgroup's chain of phases, each between two barriers: of 43000 clocks (3 heads, 9 to 37
 // tokens) 14000 until the tokens' rows are here and half of S0 is on its way, 9000 the conv, 4000 A and the q.k
 // side, 10000 the products with S0, 4500 the system, 2000 the norm; VALU instructions are a quarter of it, MFMAs
@@ -67,28 +67,25 @@ __device__ __forceinline__ float log_decay(float a_dt, float A) {
 // The product of the decays of which x is such a sum, or a difference of two, in log2 units
 __device__ __forceinline__ float decayed(double x) { return fast_exp2((float)x); }
 
-// Eight channels' conv: the taps, the newest last.
+// Eight channels' conv: their taps, a channel's newest last.
 struct Taps8 {
-    f16x8 w0, w1, w2, w3;   // a tap of all channels each
+    f16x8 t[4];   // of two channels each
     __device__ __forceinline__ void load(const f16* conv_w, int ch) {
-        const f16x8* t = (const f16x8*)(conv_w + 4 * ch);
-        const f16x8 a = t[0], b = t[1], c = t[2], d = t[3];
-        w0 = (f16x8){a[0], a[4], b[0], b[4], c[0], c[4], d[0], d[4]};
-        w1 = (f16x8){a[1], a[5], b[1], b[5], c[1], c[5], d[1], d[5]};
-        w2 = (f16x8){a[2], a[6], b[2], b[6], c[2], c[6], d[2], d[6]};
-        w3 = (f16x8){a[3], a[7], b[3], b[7], c[3], c[7], d[3], d[7]};
+        const f16x8* w = (const f16x8*)(conv_w + 4 * ch);
+        t[0] = w[0], t[1] = w[1], t[2] = w[2], t[3] = w[3];
     }
     // silu of the taps over x0 (the token's) and the three before it
-    __device__ __forceinline__ void apply(f32x4& lo, f32x4& hi, f16x8 x3, f16x8 x2, f16x8 x1, f16x8 x0) const {
+    __device__ __forceinline__ void apply(f32x4& lo, f32x4& hi, f16x8 x3, f16x8 x2, f16x8 x1, f16x8 x0) {
         // (a mixed fma takes its halves as they are: they are neither converted here nor ahead of a loop)
-        f16x8 v0 = w0, v1 = w1, v2 = w2, v3 = w3;
         float zero = 0.f;
-        asm("" : "+v"(v0), "+v"(v1), "+v"(v2), "+v"(v3), "+v"(zero));
-        auto y = [&](int c) {
-            float s = fmaf((float)v0[c], (float)x3[c], zero);
-            s = fmaf((float)v1[c], (float)x2[c], s);
-            s = fmaf((float)v2[c], (float)x1[c], s);
-            s = fmaf((float)v3[c], (float)x0[c], s);
+        asm("" : "+v"(t[0]), "+v"(t[1]), "+v"(t[2]), "+v"(t[3]), "+v"(zero));
+        auto y = [&](int i) {
+            const f16x8 w = t[i >> 1];
+            const int at = 4 * (i & 1);
+            float s = fmaf((float)w[at], (float)x3[i], zero);
+            s = fmaf((float)w[at + 1], (float)x2[i], s);
+            s = fmaf((float)w[at + 2], (float)x1[i], s);
+            s = fmaf((float)w[at + 3], (float)x0[i], s);
             return s * __builtin_amdgcn_rcpf(1.f + hw_expf(-s));
         };
         lo = (f32x4){y(0), y(1), y(2), y(3)};
@@ -314,7 +311,7 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
 #pragma unroll
     for (int t = TL > 1; t < TL; ++t) load_s0(t);
 
-    auto conv_of = [&](const Taps8& taps, const f16* at, int pitch, int i, f32x4& lo, f32x4& hi) {
+    auto conv_of = [&](Taps8& taps, const f16* at, int pitch, int i, f32x4& lo, f32x4& hi) {
         const int4 up = s_up[i];
         taps.apply(lo, hi, *(const f16x8*)(at + up.z * pitch), *(const f16x8*)(at + up.y * pitch),
                    *(const f16x8*)(at + up.x * pitch), *(const f16x8*)(at + (i + 3) * pitch));
@@ -388,9 +385,13 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
             if (!qk) beta = -*(const f32x4*)&s_beta[m][i0];
             const double lj = s_log[m][j];
             float a[4];
+            double li[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) li[e] = s_log[m][i0 + e];
+            asm("" : "+v"(li[0]), "+v"(li[1]), "+v"(li[2]), "+v"(li[3]));   // (here: a branch a number otherwise)
 #pragma unroll
             for (int e = 0; e < 4; ++e)   // (others' decays may be anything)
-                a[e] = f[e] * beta[e] * decayed(anc[e] ? s_log[m][i0 + e] - lj : 0.);
+                a[e] = f[e] * beta[e] * decayed(anc[e] ? li[e] - lj : 0.);
             Block& to = (qk ? s_p : s_a)[m][job >> 1];
             if (!qk && r == c) {
                 *(f32x4*)&to[col][4 * g] = (f32x4){a[0], a[1], a[2], a[3]};
@@ -405,13 +406,16 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
     if (w < HP * nb) {
         Block& m = s_a[w / nb][(w % nb) * (w % nb + 3) / 2];
         float xi[16];
+        uint32_t at_m = 0;
 #pragma unroll
         for (int i = 0; i < 16; ++i) xi[i] = i == col ? 1.f : 0.f;
 #pragma unroll
         for (int i = 0; i < 15; ++i) {   // (a row of m is a column of -A: no chain but over the rows)
+            // (no column before the sixth-last number is known: all at once are too many registers)
+            if (i >= 6) asm("" : "+v"(at_m) : "v"(xi[i - 5]));
             f32x4 a[4];
 #pragma unroll
-            for (int q = (i + 1) / 4; q < 4; ++q) a[q] = *(const f32x4*)&m[i][4 * q];
+            for (int q = (i + 1) / 4; q < 4; ++q) a[q] = *(const f32x4*)((const char*)&m[i][4 * q] + at_m);
 #pragma unroll
             for (int q = i + 1; q < 16; ++q) xi[q] = fmaf(a[q >> 2][q & 3], xi[i], xi[q]);
         }
