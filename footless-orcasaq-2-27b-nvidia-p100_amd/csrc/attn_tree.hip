@@ -273,6 +273,11 @@ tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict
                                       walk.n == 0 ? -1 : count > 1 ? count : 0);
         }
         __syncthreads();   // (the last piece's reads of s_line, s_lo and the stages)
+        // Q, ahead of the tree and the plan: a wait for it later would drain the copies
+        f16x8 q[8];
+        const f16* q_row = qg + ((size_t)b * T * n_q + qrow) * q_pitch + 8 * g;
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) q[ks] = t >= 0 ? *(const f16x8*)(q_row + 32 * ks) : (f16x8)(0);
         uint64_t present = 0;   // (wave 0's)
         // Tiles j0 + 64 c ..: a tile a lane of wave 0, so that the copies and masks of one cost no more than a
         // look at its entry (a page's lookup on the scalar unit, which a SIMD's waves share, held them all up).
@@ -327,26 +332,18 @@ tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict
         // (a padded batch's waves without a token have no products; wave-uniform)
         const bool busy = __any(t >= 0 && s_lo[max(t, 0)] != INT_MAX);
         if (j1 > j0) {
-            f16x8 q[8];
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks) {   // (beside O, as far as there is room at three waves a SIMD)
+                if (ks < 5) asm volatile("" : "+a"(q[ks]));
+                else asm volatile("" : "+v"(q[ks]));
+            }
             f32x4 o[16];
-            float m_run, l_run;
-            auto begin = [&] {   // (with the first tiles' copies under way)
-                const f16* row = qg + ((size_t)b * T * n_q + qrow) * q_pitch + 8 * g;
 #pragma unroll
-                for (int ks = 0; ks < 8; ++ks) q[ks] = t >= 0 ? *(const f16x8*)(row + 32 * ks) : (f16x8)(0);
-                WAIT_VMCNT(0);   // Q is here: a wait for it later would drain the copies
-#pragma unroll
-                for (int ks = 0; ks < 8; ++ks) {   // (beside O, as far as there is room at three waves a SIMD)
-                    if (ks < 5) asm volatile("" : "+a"(q[ks]));
-                    else asm volatile("" : "+v"(q[ks]));
-                }
-#pragma unroll
-                for (int n = 0; n < 16; ++n) {
-                    o[n] = (f32x4)(0.f);
-                    asm volatile("" : "+a"(o[n]));
-                }
-                m_run = -1e30f, l_run = 0.f;
-            };
+            for (int n = 0; n < 16; ++n) {
+                o[n] = (f32x4)(0.f);
+                asm volatile("" : "+a"(o[n]));
+            }
+            float m_run = -1e30f, l_run = 0.f;
             auto tree_bits = [&](uint2 l, int r) {
                 const int d = r - pos0;
                 const uint64_t x = (uint64_t)l.y << 32 | l.x;
@@ -512,7 +509,6 @@ tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict
                 look(0);
 #pragma unroll 1
                 for (int d = 0; d < min(AHEAD, n_tiles); ++d) issue(d);
-                begin();
                 for (int j = 0; j < n_tiles; ++j) {
                     // tile j landed; those issued after it may still be in flight
                     const int later = min(AHEAD - 1, n_tiles - 1 - j);
@@ -579,8 +575,14 @@ tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict
                 look(0);
 #pragma unroll 1
                 for (int d = 0; d < min(RAW_AHEAD, n_tiles); ++d) issue(d);
-                begin();
-                asm volatile("" ::: "memory");
+                auto landed = [&](int j) {   // tile j did; those issued after it may still be in flight
+                    const int later = min(RAW_AHEAD - 1, n_tiles - 1 - j);
+                    if (later == 2) WAIT_VMCNT(2 * COPIES);
+                    else if (later == 1) WAIT_VMCNT(COPIES);
+                    else WAIT_VMCNT(0);
+                    asm volatile("" ::: "memory");
+                };
+                landed(0);
                 convert(0);
                 for (int j = 0; j < n_tiles; ++j) {
                     // stage j % 2 is written, and the other one done with
@@ -589,11 +591,7 @@ tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict
                     ahead(j);
                     tile(j & 1, j);
                     if (j + 1 < n_tiles) {
-                        const int later = min(RAW_AHEAD - 1, n_tiles - 2 - j);   // tiles issued after j + 1
-                        if (later == 2) WAIT_VMCNT(2 * COPIES);
-                        else if (later == 1) WAIT_VMCNT(COPIES);
-                        else WAIT_VMCNT(0);
-                        asm volatile("" ::: "memory");
+                        landed(j + 1);
                         convert(j + 1);
                     }
                 }
