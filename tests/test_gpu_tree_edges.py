@@ -110,3 +110,41 @@ def test_sequences_that_share_a_state(fl, B):
     for b, (want, bound, f) in enumerate(tree_ref.gdn_commit(d, [[0, 3, 5]] * B, [False] * B)):
         check(S[b], want, bound, f"fork {b}")
         assert torch.equal(frames[b], f)
+
+
+@pytest.mark.parametrize("kv8", [False, True])
+@pytest.mark.parametrize("ctxs,T", [([1000], 16), ([40, 0, 900, 5], 33), ([20000, 300], 64), ([64] * 70, 2)])
+def test_nothing_behind_the_buffers_is_written(fl, dev, ctxs, T, kv8):
+    """The work buffer exactly as large as asked for, z with a wider pitch, both in the middle of others."""
+    g, B = gen(T), len(ctxs)
+    kp, vp, pages, _ = filled(fl, g, [c + T for c in ctxs], 16, kv8)
+    q, parents = randn(g, B, T, 24, 512), torch.tensor([tree(g, T, T)] * B, dtype=I32).cuda()
+    need = fl.ops.attn_tree_paged_work_bytes(B, T)
+    work = torch.full((need + 8192,), 0x5A, dtype=torch.uint8, device="cuda")
+    z = torch.full((B + 2, T, 24, 264), 7.0, dtype=F16, device="cuda")
+    call = lambda **kw: fl.ops.attn_tree_paged(q, kp, vp, pages, i32(*ctxs), parents, page_size=16, **kw)
+    call(work=work[4096:4096 + need], z=z[1:-1])
+    assert torch.equal(z[1:-1, ..., :256], call())
+    assert (z[1:-1, ..., 256:] == 7).all() and (z[0] == 7).all() and (z[-1] == 7).all()
+    assert (work[:4096] == 0x5A).all() and (work[4096 + need:] == 0x5A).all()
+
+
+@pytest.mark.parametrize("B,T", [(1, 3), (2, 64), (6, 40), (16, 17)])
+def test_gdn_trees_write_their_outputs_alone(fl, B, T):
+    _, d, parents = gdn_batch(B, B, T)
+    wide = 48 * 128
+    y = torch.full((B * T + 2, wide), 7.0, dtype=F16, device="cuda")
+    out = y[1:-1].view(B, T, wide)
+    S = torch.full((B + 2, 48, 128, 128), 7.0, device="cuda")
+    frames = torch.full((B + 2, 10240, 3), 7.0, dtype=F16, device="cuda")
+    at = torch.tensor(parents, dtype=I32).cuda()
+    fl.ops.gdn_tree_normed(d["x"], d["S"], d["a"], d["b"], d["A_log"], d["dt_bias"], d["z"], d["norm_w"], at, out,
+                           pos0s=[4] * B, conv_w=d["conv_w"], cst_in=d["cst"])
+    assert torch.equal(out, run_gdn(fl, d, parents, [4] * B))
+    path = torch.tensor([[0, 1, 2, -1]] * B, dtype=I32).cuda()
+    fl.ops.gdn_tree_commit(d["x"], d["S"], d["a"], d["b"], d["A_log"], d["dt_bias"], path, list(S[1:-1]),
+                           pos0s=[4] * B, conv_w=d["conv_w"], cst_in=d["cst"], cst_out=list(frames[1:-1]))
+    torch.cuda.synchronize()
+    for t in (y, S, frames):
+        assert (t[0] == 7).all() and (t[-1] == 7).all()
+    assert (S[1:-1] != 7).any(-1).all() and (frames[1:-1] != 7).any(-1).all()
