@@ -602,7 +602,9 @@ tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict
                 l += lane_xor(l, 16);
                 l = pair32_sum(l);
                 if (t >= 0) {
-                    if (s_lo[t] == INT_MAX) l = 0.f;   // (a place without a token, in tiles that all others see)
+                    // a place without a token, in tiles that all others see: its partial weighs nothing, whatever
+                    // its q made of m (an infinite one would be the merge's maximum)
+                    if (s_lo[t] == INT_MAX) l = 0.f, m_run = -1e30f;
                     if (!whole_seq) {
                         const size_t part = ((size_t)slot * n_kv + h) * R + r_mine;
                         float* dst = parts.pacc + part * PAGED_HD + 4 * g;
