@@ -12,16 +12,19 @@
 // triangular, both need S0 only in products with all k_i and q_i. y_i is rmsnorm_gated of o_i.
 // Everything is held in fp32 (fp64: the sums of log alpha, whose differences are the logarithms of
 // G_i / G_j) and y is rounded once, where gdn_decode_normed rounds the conv's output, q, k and o to
-// fp16 as the reference does. The products' operands are two scaled fp16 terms each, 22 bits: three
-// 16x16x32 MFMAs of 16 clocks take the place of eight fp32 ones of 32.
+// fp16 as the reference does. The operands of the products with S0 and among keys are two scaled fp16
+// terms each, 22 bits: three 16x16x32 MFMAs of 16 clocks take the place of eight fp32 ones of 32. Their
+// scales are a row's of S0 and a constant (|q|, |k| <= 1). The system's products are in fp32: a scale
+// that tokens share would cost a small one its bits beside a large one that is not on its path.
 //
 // A workgroup has the v heads of a k head, up to three: their q, k and products are formed once. A wave
 // has 16 or 32 of a head's state rows as the B operand, a row a column; the accumulators (register e of lane
-// (g, c) is token 4 g + e of column c) are in turn B operands of the 16x16x16 products with A and the
-// q.k side. The 16-row diagonal blocks of I + A are inverted by substitution, a column a lane.
+// (g, c) is token 4 g + e of column c) are in turn B operands of the products with A and the q.k side,
+// whose k slot g of step e is token 4 g + e. The 16-row diagonal blocks of I + A are inverted by
+// substitution, a column a lane.
 //
-// Measured, from a graph, 16 k and 48 v heads: a tree of 16 8.3 us, 4 of 37 14, 16 of 16 17, 16 of 9 to 37
-// 27, 8 of 64 34 us; a path of 4 committed 5.2 us, 16 of 7 22.3 us (4.7 TB/s of states read and written). The
+// Measured, from a graph, 16 k and 48 v heads: a tree of 16 8.2 us, 4 of 37 14.7, 16 of 16 16.4, 16 of 9 to 37
+// 28.5, 8 of 64 34.9 us; a path of 4 committed 5.2 us, 16 of 7 22.3 us (4.7 TB/s of states read and written). The
 // trees are bound by a workgroup's chain of phases, each between two barriers: of 43000 clocks (3 heads, 9 to 37
 // tokens) 14000 until the tokens' rows are here and half of S0 is on its way, 9000 the conv, 4000 A and the q.k
 // side, 10000 the products with S0, 4500 the system, 2000 the norm; VALU instructions are a quarter of it, MFMAs
@@ -140,28 +143,17 @@ __device__ __forceinline__ Terms split8(f32x8 x, float s) {
     return r;
 }
 // The exponent that brings the largest of a column's entries to [2^14, 2^15) (to less where all are below
-// 2^-60): the four lanes of a column have some each, the largest of which is `top`.
+// 2^-98): the four lanes of a column have some each, the largest of which is `top`.
 __device__ __forceinline__ int lift(float top) {
     top = fmaxf(top, lane_xor(top, 16));
     top = pair32_max(top);
-    return 14 - min(max(ilogb_bits(top), -60), 126);
+    return 14 - min(max(ilogb_bits(top), -98), 127);
 }
-struct Terms4 {
-    f16x4 hi, lo;
-};
-__device__ __forceinline__ Terms4 split4(f32x4 x, float s) {
-    Terms4 r;
+// c + a b for a 16 x 16 block: this lane has a's row `col`, columns 4 g .. + 3, and b's rows 4 g .. + 3.
+__device__ __forceinline__ f32x4 mfma_block(f32x4 a, f32x4 b, f32x4 c) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) r.hi[e] = (f16)fmaf(x[e], s, 0.f);
-    asm("" : "+v"(r.hi));   // (as it is packed: it would be formed twice)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) r.lo[e] = (f16)fmaf(x[e], s, -(float)r.hi[e]);
-    return r;
-}
-__device__ __forceinline__ f32x4 mfma_terms4(const Terms4& a, const Terms4& b, f32x4 c) {
-    c = __builtin_amdgcn_mfma_f32_16x16x16f16(a.lo, b.hi, c, 0, 0, 0);
-    c = __builtin_amdgcn_mfma_f32_16x16x16f16(a.hi, b.lo, c, 0, 0, 0);
-    return __builtin_amdgcn_mfma_f32_16x16x16f16(a.hi, b.hi, c, 0, 0, 0);
+    for (int e = 0; e < 4; ++e) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], b[e], c, 0, 0, 0);
+    return c;
 }
 // c + a b without the product of the two low terms (2^-22 of a b)
 __device__ __forceinline__ f32x4 mfma_terms(const Terms& a, const Terms& b, f32x4 c) {
@@ -173,13 +165,6 @@ __device__ __forceinline__ f32x4 mfma_terms(const Terms& a, const Terms& b, f32x
 __device__ __forceinline__ void wave_sync() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
-}
-
-// A number of at most 1 (as all of A, its inverses and the q.k side are) in a row of 16 high and 16 low terms.
-__device__ __forceinline__ void put_term(float* row, int at, float a) {
-    const f16 hi = (f16)(a * QK_SCALE);
-    ((f16*)row)[at] = hi;
-    ((f16*)row)[16 + at] = (f16)fmaf(a, QK_SCALE, -(float)hi);
 }
 
 // NB blocks of 16 tokens, HP v heads of one k head, TL tiles of 16 state rows a wave.
@@ -199,7 +184,7 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
     constexpr int RAW_P = COLS + 8, OUT_P = COLS + 4, OUT_ROWS = LT < TP ? LT : TP;
     constexpr int OWN_B = 4 * OUT_ROWS * OUT_P > 2 * (TP + 3) * RAW_P ? 4 * OUT_ROWS * OUT_P : 2 * (TP + 3) * RAW_P;
     typedef f16 Rows[TP][ROW_H];
-    // (of a row 16 high and 16 low terms; transposed and in fp32 while it waits to be inverted)
+    // (transposed while it waits to be inverted)
     typedef float Block[16][BLOCK_P];
     constexpr int MATS_B = 2 * HP * BLOCKS * sizeof(Block);
     constexpr int RAW_ROWS = TP + 3, RAW_B = 2 * RAW_ROWS * ROW_H * sizeof(f16);
@@ -397,7 +382,7 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
                 *(f32x4*)&to[col][4 * g] = (f32x4){a[0], a[1], a[2], a[3]};
             } else {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) put_term(to[4 * g + e], col, a[e]);
+                for (int e = 0; e < 4; ++e) to[4 * g + e][col] = a[e];
             }
         }
     }
@@ -421,30 +406,26 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
         }
         if (g == 0)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) put_term(m[i], col, xi[i]);
+            for (int i = 0; i < 16; ++i) m[i][col] = xi[i];
     }
-    // The right side and o's first part, from S0 k_i and S0 q_i. A step contracts: the u of a state row are at
-    // most 64 |v| + |S0's row|, and a block's right side 17 of them. In units that keep those below 2^15 the
-    // terms' 2^-25 is 2^-29 of the largest v, or less than 2^-31 of S0's row.
+    // The right side and o's first part, from S0 k_i and S0 q_i. With the largest number of a state row at
+    // 2^14 or more the terms' 2^-25 is 2^-39 of it.
     Terms st[TL][4];
-    float unit[TL];
+    float back[TL];   // from the products' units
 #pragma unroll
     for (int t = 0; t < TL; ++t) {
-        float top = 0.f, top_v = 0.f;
+        float top = 0.f;
 #pragma unroll
         for (int c = 0; c < 4; ++c)
 #pragma unroll
             for (int e = 0; e < 8; ++e) top = fmaxf(top, fabsf(s0[t][c][e]));
+        const int up = lift(top);
+        const float unit = pow2(up);
 #pragma unroll
-        for (int r = 0; r < NB; ++r)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) top_v = fmaxf(top_v, fabsf(v[r][t][e]));
-        unit[t] = pow2(lift(32.f * (64.f * top_v + 12.f * top)));
-#pragma unroll
-        for (int c = 0; c < 4; ++c) st[t][c] = split8(s0[t][c], unit[t]);
-        unit[t] *= QK_SCALE;
+        for (int c = 0; c < 4; ++c) st[t][c] = split8(s0[t][c], unit);
+        back[t] = pow2(-up) * (1.f / QK_SCALE);
     }
-    f32x4 u[NB][TL], o[NB][TL];   // times unit
+    f32x4 u[NB][TL], o[NB][TL];
 #pragma unroll
     for (int r = 0; r < NB; ++r) {
         if (r >= nb) continue;
@@ -466,8 +447,8 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
         for (int t = 0; t < TL; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                u[r][t][e] = beta[e] * fmaf(-gain[e], wk[t][e], v[r][t][e] * unit[t]);
-                o[r][t][e] = gain[e] * wq[t][e];
+                u[r][t][e] = beta[e] * fmaf(-gain[e], wk[t][e] * back[t], v[r][t][e]);
+                o[r][t][e] = gain[e] * (wq[t][e] * back[t]);
             }
     }
     // the output's gates, a token a row of 2 TL lanes (whose places are not worth registers until here)
@@ -481,39 +462,27 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
     __syncthreads();
 
     // block by block of tokens
-    Terms4 ut[NB][TL];
 #pragma unroll
     for (int r = 0; r < NB; ++r) {
         if (r >= nb) continue;
-        auto at = [&](const Block* m, int c) {
-            const f16* row = (const f16*)m[r * (r + 1) / 2 + c][col] + 4 * g;
-            return Terms4{*(const f16x4*)row, *(const f16x4*)(row + 16)};
-        };
+        auto at = [&](const Block* m, int c) { return *(const f32x4*)&m[r * (r + 1) / 2 + c][col][4 * g]; };
 #pragma unroll
         for (int c = 0; c < r; ++c) {
-            const Terms4 a = at(s_a[h], c);
+            const f32x4 a = at(s_a[h], c);
 #pragma unroll
-            for (int t = 0; t < TL; ++t) u[r][t] = mfma_terms4(a, ut[c][t], u[r][t]);
+            for (int t = 0; t < TL; ++t) u[r][t] = mfma_block(a, u[c][t], u[r][t]);
         }
-        const Terms4 inv = at(s_a[h], r);
-        Terms4 rhs[TL];
+        const f32x4 inv = at(s_a[h], r);
 #pragma unroll
-        for (int t = 0; t < TL; ++t) rhs[t] = split4(u[r][t], 1.f / QK_SCALE);
-#pragma unroll
-        for (int t = 0; t < TL; ++t) u[r][t] = mfma_terms4(inv, rhs[t], (f32x4)(0.f));
-#pragma unroll
-        for (int t = 0; t < TL; ++t) ut[r][t] = split4(u[r][t], 1.f / QK_SCALE);
+        for (int t = 0; t < TL; ++t) u[r][t] = mfma_block(inv, u[r][t], (f32x4)(0.f));
 #pragma unroll
         for (int c = 0; c <= r; ++c) {
-            const Terms4 p = at(s_p[h], c);
+            const f32x4 p = at(s_p[h], c);
 #pragma unroll
-            for (int t = 0; t < TL; ++t) o[r][t] = mfma_terms4(p, ut[c][t], o[r][t]);
+            for (int t = 0; t < TL; ++t) o[r][t] = mfma_block(p, u[c][t], o[r][t]);
         }
     }
-    // o in true units; squares of a row over this wave's columns, then over the head's waves
-    float f_o[TL];
-#pragma unroll
-    for (int t = 0; t < TL; ++t) f_o[t] = out_scale / unit[t];
+    // o scaled; squares of a row over this wave's columns, then over the head's waves
 #pragma unroll
     for (int r = 0; r < NB; ++r)
 #pragma unroll
@@ -521,7 +490,7 @@ gdn_tree_kernel(const f16* __restrict__ x, int x_stride, const f16* __restrict__
             float ss = 0.f;
 #pragma unroll
             for (int t = 0; t < TL; ++t) {
-                o[r][t][e] = r < nb ? o[r][t][e] * f_o[t] : 0.f;
+                o[r][t][e] = r < nb ? o[r][t][e] * out_scale : 0.f;
                 ss = fmaf(o[r][t][e], o[r][t][e], ss);
             }
             ss = row16_sum(ss);

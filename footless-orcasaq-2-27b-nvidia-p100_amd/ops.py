@@ -1418,9 +1418,10 @@ def gdn_tree_normed(x, S, a, b, A_log, dt_bias, z, norm_w, parents, y=None, *, p
     state follow its path from the sequence's state S[b] and frames cst_in[b] (lists of up
     to 16, only read). x [B, T, x_stride] fp16 the raw q|k|v rows, T up to 64; a, b [B, T,
     ab_stride] fp32; z [B, T, n_vheads * V] fp16; parents [B, T] int32 on the GPU; pos0s the
-    contexts' lengths (at 0 the frames count as zero). All is held in 32 bits (products from
-    numbers of 22) and y rounded once: a chain's values are gdn_decode_normed's but for that
-    call's fp16 roundings between its steps. Places without a token give 0. A sequence's last
+    contexts' lengths (at 0 the frames count as zero). All is held in 32 bits (the products
+    with S and between keys from numbers of 22) and y rounded once: a chain's values are
+    gdn_decode_normed's but for that call's fp16 roundings between its steps. Places without a
+    token give 0; an infinity or NaN of one token may make others of its sequence NaN. A sequence's last
     bits depend on the number of sequences. Returns y [B, T, n_vheads * V] fp16 (new unless
     given; it may not overlap an input)."""
     dev, width = _here(), n_vheads * V

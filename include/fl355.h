@@ -507,10 +507,12 @@ int fl_paged_kv_keep(void* const* kpools, void* const* vpools, int n_layers, int
 /* A GDN layer over trees: every token's conv window, decay and state follow its path from the
  * sequence's state S[b] and frames cst_in[b], which are only read; y[b][i] = rmsnorm_gated(o_i,
  * z[b][i], norm_w) of the token's output o_i (fl_gdn_decode_normed's formulas; here all of it in
- * 32 bits, products from numbers of 22 bits, and y rounded once, so a chain's values are that call's
- * but for its roundings). Places without a token give 0. An infinity or NaN of one token may reach the
- * others of its sequence. The values do not depend on the other sequences, the number of them may move
- * their last bits. y may not overlap another buffer of the call.
+ * 32 bits, the products with S and between keys from numbers of 22 bits, and y rounded once, so a
+ * chain's values are that call's but for its roundings). Places without a token give 0. A token's error
+ * is measured by its own path's terms, whatever the others hold; an infinity or NaN of one token may
+ * make others of its sequence NaN, not wrong numbers. The values do not depend on the other
+ * sequences, the number of them may move their last bits. y may not overlap another buffer of the
+ * call.
  * x [B][T][x_stride] f16 the raw q|k|v rows, a, b [B][T][ab_stride] f32, z [B][T][z_pitch], y
  * [B][T][y_pitch] f16, pos0 a host array (0: the frames are taken as zero); conv_w, S, cst_in,
  * A_log, dt_bias, norm_w as fl_gdn_decode_normed's. K == V == 128, B <= FL_MAX_SEQS, strides and
