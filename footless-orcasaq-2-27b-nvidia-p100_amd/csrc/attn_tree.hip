@@ -752,7 +752,9 @@ int fl_attn_tree_paged(const void* qg, int q_pitch, const void* kpool, const voi
     if (rc) return rc;
     FL_REQUIRE(pos0 && parents, "null pointer");
     FL_REQUIRE(tree_sizes(B, T, n_q_heads, n_kv_heads, head_dim), "1 <= T <= FL_TREE_MAX");
-    FL_REQUIRE((((long long)max_pages << pg.shift) / TT + 16) * B < INT_MAX, "B * max_pages * page_size < 2^36");
+    // (tiles and starts of all sequences in 32 bits, with TreeRun's 1.0001)
+    FL_REQUIRE((((long long)max_pages << pg.shift) / TT + 16) * B <= INT_MAX - INT_MAX / 1024,
+               "B * max_pages * page_size < 0.999 * 2^36");
     const TreeCut cut = tree_cut(T, n_q_heads, n_kv_heads);
     Parts parts;
     if (tree_parts(B, T, n_q_heads, cut.runs, (char*)work, parts) > work_bytes || !work) {
