@@ -698,10 +698,6 @@ int check_layer(const void* x, int x_stride, const void* conv_w, const void* con
     return FL_OK;
 }
 
-bool meet(const void* p, size_t np, const void* q, size_t nq) {
-    return (uintptr_t)p < (uintptr_t)q + nq && (uintptr_t)q < (uintptr_t)p + np;
-}
-
 }  // namespace
 
 extern "C" {
@@ -719,6 +715,24 @@ int fl_gdn_tree_normed(const void* x, int x_stride, const void* conv_w, const vo
     FL_REQUIRE(z_pitch >= n_vheads * V && y_pitch >= n_vheads * V && z_pitch % 8 == 0 && y_pitch % 8 == 0 &&
                    al16(z) && al16(y) && al16(norm_w) && norm_eps >= 0.f,
                "z, y: pitch >= n_vheads V, % 8, 16-byte aligned; norm_w 16-byte aligned, eps >= 0");
+    const size_t rows = (size_t)B * T, width = (size_t)n_vheads * V, dim = 2 * (size_t)n_kheads * K + width;
+    const RowsOf out = {y, rows, 2 * (size_t)y_pitch, 2 * width};
+    bool apart = true;
+    for (const RowsOf& in : {RowsOf{x, rows, 2 * (size_t)x_stride, 2 * dim}, RowsOf{z, rows, 2 * (size_t)z_pitch, 2 * width},
+                             RowsOf{a, rows, 4 * (size_t)ab_stride, 4 * (size_t)n_vheads},
+                             RowsOf{b, rows, 4 * (size_t)ab_stride, 4 * (size_t)n_vheads}})
+        apart = apart && !meet(out, in);
+    auto clear_of = [&](const void* p, size_t n) { apart = apart && !meet(y, out.bytes(), p, n); };
+    clear_of(conv_w, 8 * dim);
+    clear_of(parents, 4 * rows);
+    clear_of(A_log, 4 * (size_t)n_vheads);
+    clear_of(dt_bias, 4 * (size_t)n_vheads);
+    clear_of(norm_w, 4 * (size_t)V);
+    for (int i = 0; i < B; ++i) {
+        clear_of(S[i], 4 * width * K);
+        clear_of(cst_in[i], 6 * dim);
+    }
+    FL_REQUIRE(apart, "y overlaps an input");
     TreeSeqs seqs = {};
     for (int i = 0; i < B; ++i) {
         seqs.S[i] = S[i];

@@ -57,4 +57,22 @@ __device__ __forceinline__ Node tree_node(int p, int T, double* sum = nullptr) {
     return n;
 }
 
+// Do np bytes at p and nq bytes at q have any in common? (on the host)
+inline bool meet(const void* p, size_t np, const void* q, size_t nq) {
+    return (uintptr_t)p < (uintptr_t)q + nq && (uintptr_t)q < (uintptr_t)p + np;
+}
+// Rows: n of `width` bytes, `pitch` apart. Rows of one pitch may lie between each other.
+struct RowsOf {
+    const void* p;
+    size_t n, pitch, width;
+    size_t bytes() const { return (n - 1) * pitch + width; }
+};
+inline bool meet(const RowsOf& a, const RowsOf& b) {
+    if (!meet(a.p, a.bytes(), b.p, b.bytes())) return false;
+    if (a.pitch != b.pitch) return true;
+    const RowsOf &lo = (uintptr_t)a.p <= (uintptr_t)b.p ? a : b, &hi = &lo == &a ? b : a;
+    const size_t at = ((uintptr_t)hi.p - (uintptr_t)lo.p) % lo.pitch;
+    return at < lo.width || at + hi.width > lo.pitch;
+}
+
 }  // namespace

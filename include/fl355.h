@@ -511,8 +511,8 @@ int fl_paged_kv_keep(void* const* kpools, void* const* vpools, int n_layers, int
  * chain's values are that call's but for its roundings). Places without a token give 0. A token's error
  * is measured by its own path's terms, whatever the others hold; an infinity or NaN of one token may
  * make others of its sequence NaN, not wrong numbers. The values do not depend on the other
- * sequences, the number of them may move their last bits. y may not overlap another buffer of the
- * call.
+ * sequences, the number of them may move their last bits. y overlaps no other buffer of the call (it
+ * may be columns of rows whose other columns are x or z).
  * x [B][T][x_stride] f16 the raw q|k|v rows, a, b [B][T][ab_stride] f32, z [B][T][z_pitch], y
  * [B][T][y_pitch] f16, pos0 a host array (0: the frames are taken as zero); conv_w, S, cst_in,
  * A_log, dt_bias, norm_w as fl_gdn_decode_normed's. K == V == 128, B <= FL_MAX_SEQS, strides and

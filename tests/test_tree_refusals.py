@@ -1,7 +1,7 @@
 """Calls of the tree operators that are refused on the host for what a kernel would do with them."""
 import pytest
 
-from test_tree_abi import FAKE, attn
+from test_tree_abi import BIG, FAKE, attn, gdn_tree, ptrs
 
 
 @pytest.mark.parametrize("B,pages,page_size,rc", [
@@ -14,3 +14,38 @@ def test_a_batch_of_more_tiles_than_a_run_can_count(fl, B, pages, page_size, rc)
     assert attn(fl, B=B, max_pages=pages, stride=pages, page_size=page_size, n_pages=8) == rc
     if rc == 1:
         assert b"max_pages" in fl._lib.lib().fl_last_error()
+
+
+WIDTH, DIM, STATE = 6144, 10240, 48 * 128 * 128
+
+
+def gdn(fl, **over):
+    """gdn_tree of 2 sequences of 8 tokens, every buffer BIG bytes behind the one before it."""
+    at = {name: (i + 1) * BIG for i, name in enumerate(
+        ("x", "w", "nodes", "a", "b", "A", "dt", "z", "nw", "y", "S0", "S1", "c0", "c1"))}
+    at.update({k: v for k, v in over.items() if k in at})
+    args = {k: v for k, v in at.items() if k not in ("S0", "S1", "c0", "c1")}
+    args.update({k: v for k, v in over.items() if k not in at})
+    rc = gdn_tree(fl, S=ptrs(at["S0"], at["S1"]), cin=ptrs(at["c0"], at["c1"]), **args)
+    return rc, fl._lib.lib().fl_last_error()
+
+
+@pytest.mark.parametrize("name,bytes_", [
+    ("x", 16 * DIM * 2), ("w", DIM * 8), ("nodes", 16 * 4), ("a", 16 * 48 * 4), ("b", 16 * 48 * 4), ("A", 48 * 4),
+    ("dt", 48 * 4), ("z", 16 * WIDTH * 2), ("nw", 128 * 4), ("S0", STATE * 4), ("S1", STATE * 4), ("c0", DIM * 6),
+    ("c1", DIM * 6)])
+def test_y_over_an_input_of_the_gdn_layer(fl, name, bytes_):
+    """Its first and its last 16 bytes: a workgroup that is done writes what another has yet to read."""
+    for y in (BIG * 20 - 16 * WIDTH * 2 + 16, BIG * 20 + (bytes_ - 16) // 16 * 16):
+        rc, error = gdn(fl, y=y, **{name: BIG * 20})
+        assert rc == 1 and b"overlap" in error, (name, rc, error)
+
+
+@pytest.mark.parametrize("over", [
+    dict(z=BIG * 20, zp=WIDTH * 2, y=BIG * 20 + WIDTH * 2 - 16, yp=WIDTH * 2),
+    dict(z=BIG * 20, zp=WIDTH * 2, y=BIG * 20 + WIDTH * 2 + 16, yp=WIDTH * 2),
+    dict(z=BIG * 20, zp=WIDTH * 2, y=BIG * 20 + WIDTH * 2, yp=WIDTH * 2 + 8),
+    dict(x=BIG * 20, xs=20480, y=BIG * 20 - WIDTH * 2 + 16, yp=20480)])
+def test_y_in_the_rows_of_an_input(fl, over):
+    rc, error = gdn(fl, **over)
+    assert rc == 1 and b"overlap" in error, (rc, error)
