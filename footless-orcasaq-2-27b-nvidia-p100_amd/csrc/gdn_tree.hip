@@ -698,6 +698,18 @@ int check_layer(const void* x, int x_stride, const void* conv_w, const void* con
     return FL_OK;
 }
 
+// Does an output overlap one of a layer's inputs (`nodes`: parents or path; the states and frames apart)?
+bool meet_layer(const RowsOf& out, const void* x, int x_stride, const void* conv_w, const int* nodes, size_t n_nodes,
+                const float* a, const float* b, int ab_stride, const float* A_log, const float* dt_bias, size_t rows,
+                int n_kheads, int n_vheads) {
+    const size_t dim = (2 * (size_t)n_kheads + n_vheads) * GT_K, gates = 4 * (size_t)n_vheads;
+    auto flat = [&](const void* p, size_t n) { return meet(out.p, out.bytes(), p, n); };
+    return meet(out, RowsOf{x, rows, 2 * (size_t)x_stride, 2 * dim}) ||
+           meet(out, RowsOf{a, rows, 4 * (size_t)ab_stride, gates}) ||
+           meet(out, RowsOf{b, rows, 4 * (size_t)ab_stride, gates}) || flat(conv_w, 8 * dim) || flat(nodes, 4 * n_nodes) ||
+           flat(A_log, gates) || flat(dt_bias, gates);
+}
+
 }  // namespace
 
 extern "C" {
@@ -715,23 +727,14 @@ int fl_gdn_tree_normed(const void* x, int x_stride, const void* conv_w, const vo
     FL_REQUIRE(z_pitch >= n_vheads * V && y_pitch >= n_vheads * V && z_pitch % 8 == 0 && y_pitch % 8 == 0 &&
                    al16(z) && al16(y) && al16(norm_w) && norm_eps >= 0.f,
                "z, y: pitch >= n_vheads V, % 8, 16-byte aligned; norm_w 16-byte aligned, eps >= 0");
-    const size_t rows = (size_t)B * T, width = (size_t)n_vheads * V, dim = 2 * (size_t)n_kheads * K + width;
+    const size_t rows = (size_t)B * T, width = (size_t)n_vheads * V;
     const RowsOf out = {y, rows, 2 * (size_t)y_pitch, 2 * width};
-    bool apart = true;
-    for (const RowsOf& in : {RowsOf{x, rows, 2 * (size_t)x_stride, 2 * dim}, RowsOf{z, rows, 2 * (size_t)z_pitch, 2 * width},
-                             RowsOf{a, rows, 4 * (size_t)ab_stride, 4 * (size_t)n_vheads},
-                             RowsOf{b, rows, 4 * (size_t)ab_stride, 4 * (size_t)n_vheads}})
-        apart = apart && !meet(out, in);
-    auto clear_of = [&](const void* p, size_t n) { apart = apart && !meet(y, out.bytes(), p, n); };
-    clear_of(conv_w, 8 * dim);
-    clear_of(parents, 4 * rows);
-    clear_of(A_log, 4 * (size_t)n_vheads);
-    clear_of(dt_bias, 4 * (size_t)n_vheads);
-    clear_of(norm_w, 4 * (size_t)V);
-    for (int i = 0; i < B; ++i) {
-        clear_of(S[i], 4 * width * K);
-        clear_of(cst_in[i], 6 * dim);
-    }
+    bool apart = !meet_layer(out, x, x_stride, conv_w, parents, rows, a, b, ab_stride, A_log, dt_bias, rows, n_kheads,
+                             n_vheads) &&
+                 !meet(out, RowsOf{z, rows, 2 * (size_t)z_pitch, 2 * width}) && !meet(y, out.bytes(), norm_w, 4 * (size_t)V);
+    for (int i = 0; i < B; ++i)
+        apart = apart && !meet(y, out.bytes(), S[i], 4 * width * K) &&
+                !meet(y, out.bytes(), cst_in[i], 6 * (2 * (size_t)n_kheads * K + width));
     FL_REQUIRE(apart, "y overlaps an input");
     TreeSeqs seqs = {};
     for (int i = 0; i < B; ++i) {
@@ -785,7 +788,14 @@ int fl_gdn_tree_commit(const void* x, int x_stride, const void* conv_w, const vo
                        "two sequences' S_out or cst_out overlap");
             FL_REQUIRE(!meet(S_out[i], state, S[j], state) || (i == j && S_out[i] == S[i]),
                        "S_out overlaps an S other than its own");
+            FL_REQUIRE(!meet(S_out[i], state, cst_in[j], ring) && !meet(S_out[i], state, cst_out[j], ring) &&
+                           !meet(cst_out[i], ring, S[j], state),
+                       "states and frames overlap");
         }
+        for (const RowsOf& out : {RowsOf{S_out[i], 1, state, state}, RowsOf{cst_out[i], 1, ring, ring}})
+            FL_REQUIRE(!meet_layer(out, x, x_stride, conv_w, path, (size_t)B * D, a, b, ab_stride, A_log, dt_bias,
+                                   (size_t)B * T, n_kheads, n_vheads),
+                       "S_out or cst_out overlaps an input");
         seqs.S[i] = S[i];
         seqs.S_out[i] = S_out[i];
         seqs.frames[i] = (const f16*)cst_in[i];

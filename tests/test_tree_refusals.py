@@ -1,7 +1,7 @@
 """Calls of the tree operators that are refused on the host for what a kernel would do with them."""
 import pytest
 
-from test_tree_abi import BIG, FAKE, attn, gdn_tree, ptrs
+from test_tree_abi import BIG, attn, gdn_commit, gdn_tree, ptrs
 
 
 @pytest.mark.parametrize("B,pages,page_size,rc", [
@@ -49,3 +49,26 @@ def test_y_over_an_input_of_the_gdn_layer(fl, name, bytes_):
 def test_y_in_the_rows_of_an_input(fl, over):
     rc, error = gdn(fl, **over)
     assert rc == 1 and b"overlap" in error, (rc, error)
+
+
+def commit(fl, **over):
+    at = {name: (i + 1) * BIG for i, name in enumerate(
+        ("x", "w", "nodes", "a", "b", "A", "dt", "S0", "S1", "So0", "So1", "c0", "c1", "co0", "co1"))}
+    at.update(over)
+    pairs = dict(S="S", So="So", cin="c", cout="co")
+    args = {k: v for k, v in at.items() if k.rstrip("01") not in pairs.values()}
+    rc = gdn_commit(fl, **args, **{k: ptrs(at[v + "0"], at[v + "1"]) for k, v in pairs.items()})
+    return rc, fl._lib.lib().fl_last_error()
+
+
+@pytest.mark.parametrize("out,size", [("So0", STATE * 4), ("So1", STATE * 4), ("co0", DIM * 6), ("co1", DIM * 6)])
+@pytest.mark.parametrize("name,bytes_", [
+    ("x", 16 * DIM * 2), ("w", DIM * 8), ("nodes", 8 * 4), ("a", 16 * 48 * 4), ("b", 16 * 48 * 4), ("A", 48 * 4),
+    ("dt", 48 * 4), ("S0", STATE * 4), ("S1", STATE * 4), ("c0", DIM * 6), ("c1", DIM * 6), ("So0", STATE * 4),
+    ("So1", STATE * 4), ("co0", DIM * 6), ("co1", DIM * 6)])
+def test_outputs_of_a_commit_over_other_buffers(fl, out, size, name, bytes_):
+    if name == out:
+        return
+    for p in (BIG * 20 - size + 16, BIG * 20 + (bytes_ - 16) // 16 * 16):
+        rc, error = commit(fl, **{out: p, name: BIG * 20})
+        assert rc == 1 and b"overlap" in error, (rc, error)
