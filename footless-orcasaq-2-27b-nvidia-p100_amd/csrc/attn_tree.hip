@@ -762,6 +762,17 @@ int fl_attn_tree_paged(const void* qg, int q_pitch, const void* kpool, const voi
         return FL_ESCRATCH;
     }
     FL_REQUIRE(aligned16(work), "16-byte aligned work");
+    const int rows = B * T * n_q_heads;
+    const size_t need = tree_parts(B, T, n_q_heads, cut.runs, (char*)work, parts);
+    const size_t pool = ((size_t)n_pages << pg.shift) * n_kv_heads * (q8 ? PAGED_HD + PAGED_HD / 16 : 2 * PAGED_HD);
+    const RowsOf out = {z, (size_t)rows, 2 * (size_t)z_pitch, ROW_B};
+    const RowsOf in = {qg, (size_t)rows, 2 * (size_t)q_pitch, (gated ? 2u : 1u) * ROW_B};
+    auto clear_of = [&](const void* p, size_t n) { return !meet(z, out.bytes(), p, n) && !meet(work, need, p, n); };
+    FL_REQUIRE(!meet(out, in) && !meet(work, need, qg, in.bytes()) && !meet(work, need, z, out.bytes()) &&
+                   clear_of(kpool, pool) && clear_of(vpool, pool) && clear_of(pos0, 4 * (size_t)B) &&
+                   clear_of(parents, 4 * (size_t)B * T) &&
+                   clear_of(pages, 4 * ((B - 1) * (size_t)pages_stride + max_pages)),
+               "z or work overlaps another buffer");
     const int copy = q8 && cut.waves < 12 ? 4 : 0;
     auto kernel = cut.waves == 4   ? (q8 ? tree_attn_kernel<8, true, 4> : tree_attn_kernel<4, false>)
                   : cut.waves == 8 ? (q8 ? tree_attn_kernel<12, true, 4> : tree_attn_kernel<8, false>)
@@ -772,7 +783,6 @@ int fl_attn_tree_paged(const void* qg, int q_pitch, const void* kpool, const voi
                        Sight{window, sinks}, (f16*)z, z_pitch, gated, parts);
     rc = fl::check_launch("attn_tree_paged");
     if (rc) return rc;
-    const int rows = B * T * n_q_heads;
     hipLaunchKernelGGL(tree_merge_kernel, dim3((rows + 3) / 4), dim3(256), 0, (hipStream_t)stream, parts, (f16*)z,
                        z_pitch, gated ? (const f16*)qg + PAGED_HD : nullptr, q_pitch, T, n_q_heads, n_kv_heads, rows);
     return fl::check_launch("attn_tree_paged merge");

@@ -967,9 +967,9 @@ def attn_tree_paged(qg, kpool, vpool, pages, pos0, parents, *, page_size: int, w
     call runs); up to 1024 sequences. A token sees its sequence's context and, of the tree,
     its ancestors and itself; with a window, the rows whose positions are above p - window or
     below sinks, p = pos0 + its depth. Places without a token, and sequences at a negative
-    pos0, give 0. work: uint8 of attn_tree_paged_work_bytes (allocated here unless given). The
-    last bits of a sequence's z depend on the batch. Returns z [B, T, n_q_heads, head_dim]
-    fp16."""
+    pos0, give 0. work: uint8 of attn_tree_paged_work_bytes (allocated here unless given);
+    neither z nor work may overlap another buffer. The last bits of a sequence's z depend on the
+    batch. Returns z [B, T, n_q_heads, head_dim] fp16."""
     dev = _here()
     if dev >= 0 and _lib.lane is not None:
         r = _lib.lane.tree(dev, _stream(), qg, kpool, vpool, pages, pos0, parents, page_size, window, sinks, gate,

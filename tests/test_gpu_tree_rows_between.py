@@ -3,6 +3,7 @@ import pytest
 import torch
 
 import tree_ref
+from test_gpu_paged import filled, gen as randn_gen, randn
 from test_gpu_tree_gdn import gen, i32, run, tree
 
 pytestmark = pytest.mark.gpu
@@ -29,3 +30,19 @@ def test_y_of_the_gdn_layer_beside_z(fl, B, T, first):
         torch.cuda.current_stream().cuda_stream)
     assert rc == 0, lib.lib().fl_last_error()
     assert torch.equal(y, want) and torch.equal(z, d["z"])
+
+
+@pytest.mark.parametrize("kv8", [False, True])
+def test_z_of_the_attention_in_place_of_a_gate_that_is_not_used(fl, dev, kv8):
+    g, T, ctxs = randn_gen(3), 9, [70, 900]
+    kp, vp, pages, _ = filled(fl, g, [c + T for c in ctxs], 16, kv8)
+    qg, at, pos0 = randn(g, 2, T, 24, 512), i32([tree(g, T, T)] * 2), i32(ctxs)
+    want = fl.ops.attn_tree_paged(qg, kp, vp, pages, pos0, at, page_size=16, gate=False)
+    before, work = qg.clone(), torch.empty(fl.ops.attn_tree_paged_work_bytes(2, T), dtype=torch.uint8, device="cuda")
+    n_pages = kp.numel() // (16 * 4 * 272) if kv8 else kp.shape[0]
+    rc = fl._lib.lib().fl_attn_tree_paged(
+        qg.data_ptr(), 512, kp.data_ptr(), vp.data_ptr(), int(kv8), n_pages, 16, pages.data_ptr(), pages.shape[1],
+        pages.shape[1], pos0.data_ptr(), at.data_ptr(), 2, T, 24, 4, 256, 256 ** -0.5, 0, 0, 0, qg.data_ptr() + 512, 512,
+        work.data_ptr(), work.numel(), torch.cuda.current_stream().cuda_stream)
+    assert rc == 0, fl._lib.lib().fl_last_error()
+    assert torch.equal(qg[..., 256:], want) and torch.equal(qg[..., :256], before[..., :256])

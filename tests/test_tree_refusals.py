@@ -72,3 +72,34 @@ def test_outputs_of_a_commit_over_other_buffers(fl, out, size, name, bytes_):
     for p in (BIG * 20 - size + 16, BIG * 20 + (bytes_ - 16) // 16 * 16):
         rc, error = commit(fl, **{out: p, name: BIG * 20})
         assert rc == 1 and b"overlap" in error, (rc, error)
+
+
+def attention(fl, **over):
+    """attn_tree_paged of 2 sequences of 8 tokens, every buffer BIG bytes behind the one before it."""
+    names = ("q", "kpool", "vpool", "pages", "pos0", "parents", "z", "work")
+    at = {name: (i + 1) * BIG for i, name in enumerate(names)}
+    at["wb"] = fl.ops.attn_tree_paged_work_bytes(2, 8)
+    at.update(over)
+    return attn(fl, **at), fl._lib.lib().fl_last_error()
+
+
+@pytest.mark.parametrize("q8", [0, 1])
+@pytest.mark.parametrize("out", ["z", "work"])
+@pytest.mark.parametrize("name", ["q", "kpool", "vpool", "pages", "pos0", "parents", "z", "work"])
+def test_outputs_of_the_attention_over_other_buffers(fl, out, name, q8):
+    work = fl.ops.attn_tree_paged_work_bytes(2, 8)
+    sizes = dict(q=16 * 24 * 1024, kpool=8 * 16 * 4 * (272 if q8 else 512), vpool=8 * 16 * 4 * (272 if q8 else 512),
+                 pages=8 * 4, pos0=2 * 4, parents=16 * 4, z=16 * 24 * 512, work=work)
+    if name == out:
+        return
+    first = BIG * 20 - sizes[out] + 16
+    for p in (first - first % 16, BIG * 20 + (sizes[name] - 4) // 16 * 16):
+        rc, error = attention(fl, **{out: p, name: BIG * 20}, q8=q8)
+        assert rc == 1 and b"overlap" in error, (rc, error)
+
+
+@pytest.mark.parametrize("over", [dict(z=BIG * 20 + 512, zp=512), dict(z=BIG * 20, zp=512, gated=0),
+                                  dict(z=BIG * 20 + 1016, zp=512, gated=0), dict(z=BIG * 20 + 1024, zp=520)])
+def test_z_in_the_rows_of_q(fl, over):
+    rc, error = attention(fl, q=BIG * 20, **over)
+    assert rc == 1 and b"overlap" in error, (rc, error)
