@@ -16,6 +16,8 @@
 // 3 us for 48, the rows' own loads running meanwhile.
 #include "kv_pages.hpp"
 
+#include <algorithm>
+
 #include <math.h>
 
 using fl::Pages;
@@ -341,6 +343,11 @@ int fl_paged_kv_keep(void* const* kpools, void* const* vpools, int n_layers, int
     FL_REQUIRE(D >= 0 && pos0 && (D == 0 || path), "null pointer");
     if (D == 0) return FL_OK;
     const int units = n_kv_heads * (q8 ? 16 : 32), all = units + (q8 ? units / 16 : 0);
+    // (a pool that is there twice would have its rows moved twice, the second time from where they are no more)
+    Pools sorted = pools;
+    std::sort(sorted.p, sorted.p + 2 * n_layers);
+    for (int i = 1; i < 2 * n_layers; ++i)
+        FL_REQUIRE((size_t)(sorted.p[i] - sorted.p[i - 1]) >= ((size_t)n_pages << pg.shift) * all * 16, "two pools overlap");
     hipLaunchKernelGGL(q8 ? paged_keep_kernel<true> : paged_keep_kernel<false>,
                        dim3(B, 2 * n_layers, (all + 127) / 128), dim3(128), 0, (hipStream_t)stream, pools,
                        pg, pos0, path, D, units);

@@ -1057,7 +1057,8 @@ def paged_kv_keep(kpools, vpools, pages, pos0, path, *, page_size: int, n_kv_hea
     layers at once (lists of pools, or one K and one V pool): row pos0[b] + path[b, d] to
     row pos0[b] + d. pos0 [B], path [B, D] int32 on the GPU; a path ends at its first
     entry that is not larger than the one before it (-1: ends there). Rows from or to
-    absent pages, and sequences at a negative pos0, stay as they are."""
+    absent pages, and sequences at a negative pos0, stay as they are. Every pool once, and
+    the rows behind a context on pages of its own (paged_kv_copy)."""
     dev = _here()
     if dev >= 0 and _lib.lane is not None:
         r = _lib.lane.kv_keep(dev, _stream(), kpools, vpools, pages, pos0, path, page_size, n_kv_heads,

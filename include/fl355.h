@@ -499,7 +499,9 @@ int fl_paged_kv_copy(void* const* kpools, void* const* vpools, int n_layers, int
 
 /* The rows of accepted paths to behind their contexts, in the pools of n_layers layers: row
  * pos0[b] + path[b][d] -> row pos0[b] + d. A row from or to an absent page stays as it is, and so
- * do the sequences at a negative pos0. path [B][D] (its entries have no upper limit here). */
+ * do the sequences at a negative pos0. path [B][D] (its entries have no upper limit here). Pools that
+ * overlap are refused; what a row holds that two sequences write, or one writes and another reads, is
+ * undefined (a fork has its own copy of the page that it goes on in). */
 int fl_paged_kv_keep(void* const* kpools, void* const* vpools, int n_layers, int q8, int n_pages,
                      int page_size, const int* pages, int max_pages, long long pages_stride,
                      const int* pos0, const int* path, int B, int D, int n_kv_heads, int head_dim,

@@ -1,7 +1,7 @@
 """Calls of the tree operators that are refused on the host for what a kernel would do with them."""
 import pytest
 
-from test_tree_abi import BIG, attn, gdn_commit, gdn_tree, ptrs
+from test_tree_abi import BIG, attn, gdn_commit, gdn_tree, keep, ptrs
 
 
 @pytest.mark.parametrize("B,pages,page_size,rc", [
@@ -103,3 +103,16 @@ def test_outputs_of_the_attention_over_other_buffers(fl, out, name, q8):
 def test_z_in_the_rows_of_q(fl, over):
     rc, error = attention(fl, q=BIG * 20, **over)
     assert rc == 1 and b"overlap" in error, (rc, error)
+
+
+@pytest.mark.parametrize("q8,bytes_", [(0, 8 * 16 * 4 * 512), (1, 8 * 16 * 4 * 272)])
+@pytest.mark.parametrize("ks,vs", [((1, 1), (2, 3)), ((1, 2), (1, 3)), ((3, 2), (1, 2))])
+def test_accepted_rows_of_a_pool_that_is_there_twice(fl, ks, vs, q8, bytes_):
+    """Two workgroups would move its rows, one of them from where the other has written."""
+    for shift in (0, bytes_ - 16):      # the second time it comes
+        at, seen = [], set()
+        for n in (*ks, *vs):
+            at.append(BIG * n + (shift if n in seen else 0))
+            seen.add(n)
+        assert keep(fl, ks=ptrs(*at[:2]), vs=ptrs(*at[2:]), q8=q8, D=1) == 1
+        assert b"overlap" in fl._lib.lib().fl_last_error()
