@@ -477,9 +477,10 @@ int fl_attn_prep_axes(void* qg, int q_pitch, const void* k, const void* v, const
  * token and sequences at a negative pos0 give 0. qg [B][T][n_q_heads][q_pitch], z
  * [B][T][n_q_heads][z_pitch], the gate as fl_attn_decode_paged's; any n_q_heads / n_kv_heads. work:
  * fl_attn_tree_paged_work_bytes on the device that runs the call, 16-byte aligned, one for each call
- * that may overlap with another. Neither z nor work overlaps another buffer of the call (ungated z may be
- * the unused columns of q's rows). The precision is the decode form's. Rows that no token of a sequence sees
- * may hold anything; an infinity or NaN in one that some token sees may reach the others. */
+ * that may overlap with another. Neither z nor work overlaps another buffer of the call (ungated z may
+ * be the unused columns of q's rows). The precision is the decode form's. Rows that no token of a
+ * sequence sees may hold anything; an infinity or NaN in a K row reaches the tokens that see it, in a V
+ * row it may make that dim NaN for others of its sequence as well, not wrong. */
 size_t fl_attn_tree_paged_work_bytes(int B, int T, int n_q_heads, int n_kv_heads, int head_dim);
 int fl_attn_tree_paged(const void* qg, int q_pitch, const void* kpool, const void* vpool, int q8,
                        int n_pages, int page_size, const int* pages, int max_pages,
