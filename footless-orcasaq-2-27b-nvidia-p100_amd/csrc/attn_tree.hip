@@ -17,8 +17,8 @@
 // a partial a piece, which the merge weighs.
 //
 // Measured, from a graph: a tree of 16 on 500 rows 17 us, 8 of them on 8192 62 us (4.4 TB/s, int8 73 us), 16 of 8
-// tokens on 16384 196 us (5.5 TB/s, int8 174), 4 of 63 on 20000 to 60000 281 us (0.83 PFLOP/s), 12 of 5 to 26 on
-// 100 to 32768 int8 rows 117 us. Small trees are bound by the cache's bytes, and by what comes ahead of the first
+// tokens on 16384 195 us (5.5 TB/s, int8 175), 4 of 63 on 20000 to 60000 282 us (0.82 PFLOP/s; 291 on another card),
+// 12 of 5 to 26 on 100 to 32768 int8 rows 117 us. Small trees are bound by the cache's bytes, and by what comes ahead of the first
 // tile and behind the last (a sequence's tree, plan and first rows 10 us one behind another, the partials' merge
 // 4 to 12); a large one's tile of 32 rows and 192 columns takes 3100 clocks (int8 5000), of which MFMAs are 1540
 // (2300) and LDS reads as many: a tile's waves are in step and use both at once. Scores of the next tile under the
@@ -446,6 +446,8 @@ tree_attn_kernel(const f16* __restrict__ qg, int q_pitch, const char* __restrict
                     weights();
                 }
                 l_run += sum;
+                // Into the product with V in fp16, as in the decode: over fp16 pools one term (z 2.9e-4 off, 2.1e-4 of it
+                // its own rounding; a second term, 2.1e-4, takes 343 us for 282, 4 trees of 63 on 20000 to 60000)
                 const f16x8 p_hi = __builtin_convertvector(p, f16x8);
                 f16x8 p_lo;
                 if (Q8) p_lo = __builtin_convertvector(p - __builtin_convertvector(p_hi, f32x8), f16x8);
@@ -707,7 +709,8 @@ struct TreeCut {
 // Waves, of 16 columns each: as many as share a tile's copies without more registers than there are. (4 of
 // 63 on 20000 to 60000 rows: 287 us with twelve, 325 with eight; 96 columns on eight: 67 us, on twelve 75; 48 on
 // four: 192, on eight 206.) Over int8 pools four more waves copy and convert where there is room for them (48
-// columns on 16384 rows: 174 us, with waves that do both 227, with eight more 183; 96 on 8192: 73, 85).
+// columns on 16384 rows: 174 us, with waves that do both 227, with eight more 183; 96 on 8192: 73, 85). Of 193 to 256
+// columns (two groups of twelve: 198 on 20000 rows 133 us, 192 in one group 107) two groups of eight were not timed.
 TreeCut tree_cut(int T, int n_q, int n_kv) {
     const int R = T * (n_q / n_kv);
     TreeCut c;

@@ -24,11 +24,11 @@
 // substitution, a column a lane.
 //
 // Measured, from a graph, 16 k and 48 v heads: a tree of 16 8.2 us, 4 of 37 14.7, 16 of 16 16.4, 16 of 9 to 37
-// 28.5, 8 of 64 34.9 us; a path of 4 committed 5.2 us, 16 of 7 22.3 us (4.7 TB/s of states read and written). The
+// 28.5, 8 of 64 34.9 us; a path of 4 committed 5.2 us, 16 of 7 22.3 us (4.5 TB/s of states read and written). The
 // trees are bound by a workgroup's chain of phases, each between two barriers: of 43000 clocks (3 heads, 9 to 37
-// tokens) 14000 until the tokens' rows are here and half of S0 is on its way, 9000 the conv, 4000 A and the q.k
-// side, 10000 the products with S0, 4500 the system, 2000 the norm; VALU instructions are a quarter of it, MFMAs
-// less than a tenth. S0's 50 MB alone would be 10 us.
+// tokens) 14000 until the tokens' rows are here and half of S0 is on its way, 9000 the conv, 2700 A and the q.k
+// side, 9300 the products with S0, 2400 the system, 5600 the norm and the stores; VALU instructions are a fifth of
+// it, MFMAs a tenth. S0's 50 MB alone would be 10 us.
 #include "tree.hpp"
 
 #include "gdn_gates.hpp"
@@ -43,8 +43,9 @@ constexpr int GT_K = 128;                // K = V
 constexpr int ROW_H = GT_K + 8;          // terms a row of k and q
 constexpr float QK_SCALE = 16384.f;      // of q and k, whose norms are at most 1
 // Heads up to which a workgroup takes one, with 16 state rows a wave: a round of workgroups is the shorter one
-// then (240 heads of 16 tokens 9.5 us, by threes 14.9; of 37 tokens 16.0 and 25.4), two rounds are not
-// (288 heads 16.9 and 15.1; 29.4 and 25.6; 768 heads of 37: 44 and 27).
+// then (240 heads of 16 tokens 8.7 us, by threes 14.0; of 37 tokens 15.2 and 26.0), several are not (288 heads of 37
+// tokens 27.9 and 26.2; 768 heads of 16 18.4 and 16.6, of 9 to 37 33.3 and 28.8) unless little LDS lets a CU have
+// two at a time (288 heads of 16 tokens 12.4 and 14.2, which this number leaves at 14.2).
 constexpr int GT_MANY = 256;
 // State rows that a workgroup moves on (measured with the conv's input in registers yet, 16, 32, 64 and 128
 // rows: 16 paths of 7 25.9, 26.9, 28.4 and 28.4 us; 2 of 40 16.0, 14.7, 13.4 and 18.8; one of 4 6.1, 6.2, 6.8, 8.2)
